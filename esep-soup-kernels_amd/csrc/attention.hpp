@@ -72,6 +72,46 @@ hipError_t launch_attn_fwd(const AttnArgs& a, int dt, int D, int max_seqlen, hip
 hipError_t launch_attn_bwd(const AttnBwdArgs& a, int dt, int D, int max_seqlen, hipStream_t s,
                            bool* supported);
 
+// Windowed attention (attention_window.hip): query i of a sequence sees key j <= i if i - j < window
+// or j < sinks (positions within the sequence). f / b as above; lse is [HQ, T] too.
+struct AttnWinArgs {
+  AttnBwdArgs b;     // the forward uses b.f alone
+  int window;        // >= 1
+  int sinks;         // >= 0, at most max_seqlen
+  int zero_rest;     // the forward writes o = 0 behind the last sequence
+  int far;           // some sequence may be long enough for the separate pass over sink keys
+  int far_split;     // blocks per kv head in that pass (a divisor of HQ / HK)
+  float* sink_main;  // [T / (window + kWinFar) + 1][split][HK][2][sinks][D]
+  float* sink_far;   // [win_far_slots][far_split][HK][2][sinks][D]
+  int n_main;        // dK / dV blocks before the far ones
+};
+
+// Queries of a far block, and the length past the window from which a sequence has them.
+constexpr int kWinFar = 512;
+inline int64_t win_main_slots(int64_t T, int window) { return T / ((int64_t)window + kWinFar) + 1; }
+inline int64_t win_far_slots(int64_t T, int window) {
+  return T / kWinFar + win_main_slots(T, window);
+}
+// The separate pass over sink keys runs only where the bound on the lengths admits a long sequence.
+inline bool win_has_far(int window, int sinks, int max_seqlen) {
+  return sinks > 0 && (int64_t)max_seqlen > (int64_t)window + kWinFar;
+}
+// Blocks per kv head of that pass: enough of them for two rounds of its two blocks per CU, short of one
+// head per block.
+inline int win_far_split(int64_t T, int HQ, int HK, int window, int sinks) {
+  const int G = HQ / HK;
+  const int64_t blocks = win_far_slots(T, window) * HK * ((sinks + 127) / 128);
+  int s = 1;
+  while (blocks * s < 1024 && s < G) {
+    ++s;
+    while (G % s) ++s;
+  }
+  return s;
+}
+
+hipError_t launch_attn_win_fwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
+hipError_t launch_attn_win_bwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
+
 // ---------------------------------------------------------------------------------------
 // Device helpers shared by the attention kernels
 // ---------------------------------------------------------------------------------------

@@ -25,79 +25,10 @@
 #include <cmath>
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_tiles.hpp"
 
 namespace esep {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-// 32 keys of the dQ walk for a wavefront's 32 queries: keys kh .. kh + 31, held in 32 rows of the
-// swizzled LDS tiles at ks / vs (attention.hpp: SwzFill, swz_row_base, SwzTr). S^T = K Q^T and
-// dP^T = V dO^T with the wave's Q and dO as B operands, dS^T = P^T * (dP^T - delta), then
-// dQ^T += K^T dS^T with K^T read transposed out of ks and dS^T in the permuted key order. K and V
-// operands are read three ahead of their MFMAs and the first two K^T ones before the exponentials
-// (config 5 bwd 7.11 -> 6.97 ms).
-template <typename T, int D>
-__device__ __forceinline__ void dq_tile_swz(const char* ks, const char* vs, int kh, int qw0, int qi,
-                                            int lane, float scale_log2, float lse2, float delta,
-                                            const typename Mfma<T>::v8 (&qb)[D / 16],
-                                            const typename Mfma<T>::v8 (&db)[D / 16],
-                                            f32x16 (&dqa)[D / 32]) {
-  constexpr int RB = 2 * D;
-  using V8 = typename Mfma<T>::v8;
-  const int hi = lane >> 5;
-  __builtin_amdgcn_s_setprio(1);  // MFMA runs at raised priority, as in the forward
-  f32x16 s = f32x16{}, dp = f32x16{};
-  const uint32_t r0 = swz_row_base<RB>(lane);
-  constexpr int KA = 3;
-  V8 kbuf[KA], vbuf[KA];
-#pragma unroll
-  for (int c = 0; c < KA; ++c) {
-    kbuf[c] = ld16<V8>(ks + (r0 ^ (32u * c)));
-    vbuf[c] = ld16<V8>(vs + (r0 ^ (32u * c)));
-  }
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    s = Mfma<T>::run(kbuf[c % KA], qb[c], s);
-    dp = Mfma<T>::run(vbuf[c % KA], db[c], dp);
-    if (c + KA < D / 16) {
-      kbuf[c % KA] = ld16<V8>(ks + (r0 ^ (32u * (c + KA))));
-      vbuf[c % KA] = ld16<V8>(vs + (r0 ^ (32u * (c + KA))));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  const SwzTr<RB> kt(lane);
-  constexpr int TA = 2;
-  V8 tbuf[TA];
-#pragma unroll
-  for (int j = 0; j < TA; ++j) tbuf[j] = kt.template read<V8>(ks, 16 * (j & 1), j >> 1);
-  __builtin_amdgcn_sched_barrier(0);
-  if (kh + 31 > qw0) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int kj = kh + 8 * (i / 4) + 4 * hi + (i % 4);
-      if (kj > qi) s[i] = -INFINITY;
-    }
-  }
-  __builtin_amdgcn_s_setprio(0);
-  V8 dsb[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float p = exp2_fast(fmaf(s[i], scale_log2, -lse2));
-    dsb[i / 8][i % 8] = (T)(p * (dp[i] - delta));
-  }
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    dqa[j / 2] = Mfma<T>::run(tbuf[j % TA], dsb[j % 2], dqa[j / 2]);
-    if (j + TA < D / 16) tbuf[j % TA] = kt.template read<V8>(ks, 16 * ((j + TA) & 1), (j + TA) >> 1);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __builtin_amdgcn_s_setprio(0);
-}
 
 // dQ with the K / V tiles moved as the forward moves them: swizzled BN-key tiles filled by dwordx4
 // LDS DMA through a ring of two buffers (tile t + 1 in flight while tile t is consumed, one
@@ -189,8 +120,9 @@ __global__ __launch_bounds__(64 * NW, kDqPerCU<D>) void k_attn_bwd_dq_dma(const 
 #pragma unroll
     for (int h = 0; h < BN / 32; ++h) {
       if (!wave_live || kt + 32 * h > wq_last) return;
-      dq_tile_swz<T, D>(kv[B][0] + 32 * RB * h, kv[B][1] + 32 * RB * h, kt + 32 * h, qw0, qi, lane,
-                        a.scale_log2, lse2, delta, qb, db, dqa);
+      const int kh = kt + 32 * h;
+      dq_tile_swz<T, D>(kv[B][0] + 32 * RB * h, kv[B][1] + 32 * RB * h, lane, a.scale_log2, lse2, delta,
+                        qb, db, dqa, [&](f32x16& s) __attribute__((always_inline)) { mask_future(s, kh, qw0, qi, hi); });
     }
   };
   int t = 0;

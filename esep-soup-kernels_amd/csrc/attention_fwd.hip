@@ -2,101 +2,10 @@
 #include <cmath>
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_tiles.hpp"
 
 namespace esep {
 namespace {
-
-// 32 keys of the online softmax for a wavefront's 32 queries: keys kh .. kh + 31, held in 32 rows of
-// the swizzled LDS tiles at ks / vs (the layout, its DMA and its readers are in attention.hpp).
-// Lane (lq, hi) gets the scores of its query qi against keys kh + 8 (i / 4) + 4 hi + i % 4, i < 16,
-// from S^T = K Q^T (K rows from LDS as the A operand, the wave's Q^T in registers as B), then
-// updates (m, l) and O^T += V^T P^T, the contraction in the permuted key order of pb (element e of
-// chunk c2 is key kh + 16 c2 + 8 (e / 4) + 4 hi + e % 4).
-//
-// Online softmax (base 2) with a lazy reference: the lane's m moves only when the 32 keys' maximum
-// exceeds it by more than 8, so p <= 2^8 (exact in bf16 / fp16 relative terms) and O, l are
-// rescaled only where some lane's m moved. Operands are read ahead of their MFMAs (K three, V^T two,
-// the first V^T ones before the softmax, whose VALU work hides their latency), pinned by
-// scheduling barriers: the compiler sinks each read to just before its use (config 5 forward
-// 2.03 -> 1.93 ms).
-template <typename T, int D>
-__device__ __forceinline__ void fwd_tile_swz(const char* ks, const char* vs, int kh, int qw0,
-                                             int qi, int lane, float scale_log2,
-                                             const typename Mfma<T>::v8 (&qb)[D / 16],
-                                             f32x16 (&oacc)[D / 32], float& m, float& l) {
-  constexpr int RB = 2 * D;
-  using V8 = typename Mfma<T>::v8;
-  const int lq = lane & 31, hi = lane >> 5;
-  // The MFMA runs go at raised wave priority, the softmax between them at the normal one: with
-  // several wavefronts per SIMD the arbiter then feeds the matrix core from a wavefront in its
-  // MFMA run ahead of another's vector work (all three kernels; config 5: forward 1.44 -> 1.43
-  // ms, backward 5.00 -> 4.91 ms).
-  __builtin_amdgcn_s_setprio(1);
-  f32x16 acc = f32x16{};
-  const uint32_t k0 = swz_row_base<RB>(lane);
-  constexpr int KA = 3;
-  V8 kbuf[KA];
-#pragma unroll
-  for (int c = 0; c < KA; ++c) kbuf[c] = ld16<V8>(ks + (k0 ^ (32u * c)));
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    acc = Mfma<T>::run(kbuf[c % KA], qb[c], acc);
-    if (c + KA < D / 16) kbuf[c % KA] = ld16<V8>(ks + (k0 ^ (32u * (c + KA))));
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  // V^T operand j: rows 16 (j & 1) .., columns 32 (j >> 1) .. of the V tile
-  const SwzTr<RB> vt(lane);
-  auto ldv = [&](int j) { return vt.template read<V8>(vs, 16 * (j & 1), j >> 1); };
-  constexpr int VA = 2;
-  V8 vbuf[VA];
-#pragma unroll
-  for (int j = 0; j < VA; ++j) vbuf[j] = ldv(j);
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_setprio(0);
-  if (kh + 31 > qw0) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int kj = kh + 8 * (i / 4) + 4 * hi + (i % 4);
-      if (kj > qi) acc[i] = -INFINITY;
-    }
-  }
-  float mx = acc[0];
-#pragma unroll
-  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[i]);
-  mx = pair_max(mx) * scale_log2;
-  const bool grow = mx > m + 8.f;
-  float alpha = 1.f;
-  if (grow) {
-    alpha = exp2_fast(m - mx);
-    m = mx;
-  }
-  const float nm = m == -INFINITY ? 0.f : -m;
-  float ps = 0.f;
-  V8 pb[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float p = exp2_fast(fmaf(acc[i], scale_log2, nm));
-    ps += p;
-    pb[i / 8][i % 8] = (T)p;
-  }
-  ps = pair_sum(ps);
-  l = fmaf(l, alpha, ps);
-  if (__any(grow)) {
-#pragma unroll
-    for (int md = 0; md < D / 32; ++md) oacc[md] *= alpha;
-  }
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    oacc[j / 2] = Mfma<T>::run(vbuf[j % VA], pb[j % 2], oacc[j / 2]);
-    if (j + VA < D / 16) vbuf[j % VA] = ldv(j + VA);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __builtin_amdgcn_s_setprio(0);
-}
 
 // The forward kernel: blocks of 4 wavefronts own 128 queries of one (sequence, query head) with the
 // online softmax in registers; the BN-key K / V tiles go through a ring of NBUF = 2 swizzled LDS
@@ -181,8 +90,9 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_fwd_swz(con
 #pragma unroll
     for (int h = 0; h < BN / 32; ++h) {
       if (!wave_live || kt + 32 * h > wq_last) return;
-      fwd_tile_swz<T, D>(kv[B][0] + 32 * RB * h, kv[B][1] + 32 * RB * h, kt + 32 * h, qw0, qi, lane,
-                         a.scale_log2, qb, oacc, m, l);
+      const int kh = kt + 32 * h;
+      fwd_tile_swz<T, D>(kv[B][0] + 32 * RB * h, kv[B][1] + 32 * RB * h, lane, a.scale_log2, qb, oacc,
+                         m, l, [&](f32x16& acc) __attribute__((always_inline)) { mask_future(acc, kh, qw0, qi, hi); });
     }
   };
   int t = 0;

@@ -109,6 +109,147 @@ int attn_split(int64_t T, int HQ, int HK) {
   return s;
 }
 
+int window_ok(const char* what, int window, int sinks) {
+  if (window < 1 || sinks < 0)
+    return fail(ESEP_ESHAPE, "%s: window=%d sinks=%d (a window of 1 or more, 0 or more sinks)", what,
+                window, sinks);
+  return 0;
+}
+
+// The windowed backward's workspace in floats: delta [HQ, T], the split's dK / dV partials, the sink rows'
+// near and far ones.
+struct WinLayout {
+  int split, sinks, far, far_split;
+  int64_t main_at, far_at, total;
+};
+WinLayout win_layout(int64_t T, int HQ, int HK, int D, int max_seqlen, int window, int sinks) {
+  WinLayout w{};
+  w.split = attn_split(T, HQ, HK);
+  w.sinks = sinks < max_seqlen ? sinks : max_seqlen;
+  w.far = esep::win_has_far(window, w.sinks, max_seqlen);
+  w.far_split = w.far ? esep::win_far_split(T, HQ, HK, window, w.sinks) : 1;
+  const int64_t row = (int64_t)HK * 2 * w.sinks * D;
+  w.main_at = (((int64_t)HQ * T + 3) & ~(int64_t)3) + (w.split > 1 ? 2 * w.split * T * HK * D : 0);
+  w.far_at = w.main_at + (w.far ? esep::win_main_slots(T, window) * w.split * row : 0);
+  w.total = w.far_at + (w.far ? esep::win_far_slots(T, window) * w.far_split * row : 0);
+  return w;
+}
+
+// Token strides of the attention tensors, in elements, at most 2^22 (8 MiB of 16-bit
+// elements): the LDS-DMA tile fills address a wavefront's rows with 32-bit per-lane byte
+// offsets of up to 39 strides from an SGPR base (64-key tiles: row groups 32 rows apart, 8 rows each).
+constexpr int64_t kAttnMaxStride = int64_t{1} << 22;
+
+// Checks and fills the arguments of an attention forward. 0 with out->T = 0 where there is nothing to do.
+int attn_fwd_args(const char* what, const void* q, int64_t q_rs, const void* k, int64_t k_rs,
+                  const void* v, int64_t v_rs, void* o, int64_t o_rs, float* lse, int dt, int64_t T,
+                  int HQ, int HK, int D, const int32_t* cu_seqlens, int n_seq, int max_seqlen,
+                  float scale, esep::AttnArgs* out) {
+  if (dt != ESEP_F16 && dt != ESEP_BF16)
+    return fail(ESEP_EINVAL, "%s: dtype %d is not fp16 / bf16", what, dt);
+  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "%s: D=%d not in {64, 128}", what, D);
+  if (T < 0 || T > 0x7fffffff || HQ < 1 || HK < 1 || HQ % HK != 0 || n_seq < 0 || max_seqlen < 0)
+    return fail(ESEP_ESHAPE, "%s: bad sizes T=%lld HQ=%d HK=%d n_seq=%d max_seqlen=%d", what,
+                (long long)T, HQ, HK, n_seq, max_seqlen);
+  if (q_rs < (int64_t)HQ * D || o_rs < (int64_t)HQ * D || k_rs < (int64_t)HK * D ||
+      v_rs < (int64_t)HK * D)
+    return fail(ESEP_ESHAPE, "%s: token stride smaller than heads * D", what);
+  if (q_rs > kAttnMaxStride || o_rs > kAttnMaxStride || k_rs > kAttnMaxStride ||
+      v_rs > kAttnMaxStride)
+    return fail(ESEP_ESHAPE, "%s: token stride above %lld elements", what, (long long)kAttnMaxStride);
+  if (T == 0 || n_seq == 0 || max_seqlen == 0) return 0;
+  if (q == nullptr || k == nullptr || v == nullptr || o == nullptr || cu_seqlens == nullptr)
+    return fail(ESEP_EINVAL, "%s: q, k, v, o and cu_seqlens are required", what);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (q_rs & 7) ||
+      (k_rs & 7) || (v_rs & 7) || (o_rs & 7))
+    return fail(ESEP_EALIGN, "%s: q, k, v, o need 16-byte alignment and token strides "
+                             "that are multiples of 8 elements", what);
+  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "%s: scale must be positive", what);
+  esep::AttnArgs& a = *out;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.lse = lse;
+  a.cu = cu_seqlens;
+  a.q_rs = q_rs;
+  a.k_rs = k_rs;
+  a.v_rs = v_rs;
+  a.o_rs = o_rs;
+  a.T = T;
+  a.n_seq = n_seq;
+  a.HQ = HQ;
+  a.HK = HK;
+  a.scale = scale;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return 0;
+}
+
+// Checks and fills the arguments of an attention backward, but for the split and the partials behind
+// delta. 0 with out->f.T = 0 where there is nothing to do.
+int attn_bwd_args(const char* what, const void* q, int64_t q_rs, const void* k, int64_t k_rs,
+                  const void* v, int64_t v_rs, const void* o, int64_t o_rs, const void* dout,
+                  int64_t do_rs, const float* lse, float* workspace, void* dq, int64_t dq_rs, void* dk,
+                  int64_t dk_rs, void* dv, int64_t dv_rs, int dt, int64_t T, int HQ, int HK, int D,
+                  const int32_t* cu_seqlens, int n_seq, int max_seqlen, float scale,
+                  esep::AttnBwdArgs* out) {
+  if (dt != ESEP_F16 && dt != ESEP_BF16)
+    return fail(ESEP_EINVAL, "%s: dtype %d is not fp16 / bf16", what, dt);
+  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "%s: D=%d not in {64, 128}", what, D);
+  if (T < 0 || T > 0x7fffffff || HQ < 1 || HK < 1 || HQ % HK != 0 || n_seq < 0 || max_seqlen < 0)
+    return fail(ESEP_ESHAPE, "%s: bad sizes T=%lld HQ=%d HK=%d n_seq=%d max_seqlen=%d", what,
+                (long long)T, HQ, HK, n_seq, max_seqlen);
+  const int64_t wq = (int64_t)HQ * D, wk = (int64_t)HK * D;
+  if (q_rs < wq || o_rs < wq || do_rs < wq || dq_rs < wq || k_rs < wk || v_rs < wk ||
+      dk_rs < wk || dv_rs < wk)
+    return fail(ESEP_ESHAPE, "%s: token stride smaller than heads * D", what);
+  for (int64_t rs : {q_rs, o_rs, do_rs, dq_rs, k_rs, v_rs, dk_rs, dv_rs})
+    if (rs > kAttnMaxStride)
+      return fail(ESEP_ESHAPE, "%s: token stride above %lld elements", what,
+                  (long long)kAttnMaxStride);
+  if (T == 0 || n_seq == 0 || max_seqlen == 0) return 0;
+  const void* ptrs[] = {q, k, v, o, dout, dq, dk, dv};
+  for (const void* p : ptrs)
+    if (p == nullptr) return fail(ESEP_EINVAL, "%s: q, k, v, o, dout, dq, dk, dv are required", what);
+  if (lse == nullptr || workspace == nullptr || cu_seqlens == nullptr)
+    return fail(ESEP_EINVAL, "%s: lse, the workspace and cu_seqlens are required", what);
+  if (!aligned16(workspace)) return fail(ESEP_EALIGN, "%s: workspace needs 16-byte alignment", what);
+  const int64_t rss[] = {q_rs, k_rs, v_rs, o_rs, do_rs, dq_rs, dk_rs, dv_rs};
+  for (int i = 0; i < 8; ++i)
+    if (!aligned16(ptrs[i]) || (rss[i] & 7))
+      return fail(ESEP_EALIGN, "%s: tensors need 16-byte alignment and token strides "
+                               "that are multiples of 8 elements", what);
+  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "%s: scale must be positive", what);
+  esep::AttnBwdArgs& b = *out;
+  b.f.q = q;
+  b.f.k = k;
+  b.f.v = v;
+  b.f.o = const_cast<void*>(o);
+  b.f.lse = const_cast<float*>(lse);
+  b.f.cu = cu_seqlens;
+  b.f.q_rs = q_rs;
+  b.f.k_rs = k_rs;
+  b.f.v_rs = v_rs;
+  b.f.o_rs = o_rs;
+  b.f.T = T;
+  b.f.n_seq = n_seq;
+  b.f.HQ = HQ;
+  b.f.HK = HK;
+  b.f.scale = scale;
+  b.f.scale_log2 = scale * 1.4426950408889634f;
+  b.dout = dout;
+  b.delta = workspace;
+  b.part = workspace + (((int64_t)HQ * T + 3) & ~(int64_t)3);  // behind delta
+  b.dq = dq;
+  b.dk = dk;
+  b.dv = dv;
+  b.do_rs = do_rs;
+  b.dq_rs = dq_rs;
+  b.dk_rs = dk_rs;
+  b.dv_rs = dv_rs;
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -523,53 +664,15 @@ int esep_rope(const void* q, const int64_t q_strides[3], const void* q_delta,
   return 0;
 }
 
-// Token strides of the attention tensors, in elements, at most 2^22 (8 MiB of 16-bit
-// elements): the LDS-DMA tile fills address a wavefront's rows with 32-bit per-lane byte
-// offsets of up to 39 strides from an SGPR base (64-key tiles: row groups 32 rows apart, 8 rows each).
-constexpr int64_t kAttnMaxStride = int64_t{1} << 22;
-
 int esep_attn_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
                   int64_t v_rs, void* o, int64_t o_rs, float* lse, int dt, int64_t T, int HQ,
                   int HK, int D, const int32_t* cu_seqlens, int n_seq, int max_seqlen,
                   float scale, void* stream) {
   g_err[0] = 0;
-  if (dt != ESEP_F16 && dt != ESEP_BF16)
-    return fail(ESEP_EINVAL, "attn_fwd: dtype %d is not fp16 / bf16", dt);
-  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "attn_fwd: D=%d not in {64, 128}", D);
-  if (T < 0 || T > 0x7fffffff || HQ < 1 || HK < 1 || HQ % HK != 0 || n_seq < 0 || max_seqlen < 0)
-    return fail(ESEP_ESHAPE, "attn_fwd: bad sizes T=%lld HQ=%d HK=%d n_seq=%d max_seqlen=%d",
-                (long long)T, HQ, HK, n_seq, max_seqlen);
-  if (q_rs < (int64_t)HQ * D || o_rs < (int64_t)HQ * D || k_rs < (int64_t)HK * D ||
-      v_rs < (int64_t)HK * D)
-    return fail(ESEP_ESHAPE, "attn_fwd: token stride smaller than heads * D");
-  if (q_rs > kAttnMaxStride || o_rs > kAttnMaxStride || k_rs > kAttnMaxStride ||
-      v_rs > kAttnMaxStride)
-    return fail(ESEP_ESHAPE, "attn_fwd: token stride above %lld elements", (long long)kAttnMaxStride);
-  if (T == 0 || n_seq == 0 || max_seqlen == 0) return 0;
-  if (q == nullptr || k == nullptr || v == nullptr || o == nullptr || cu_seqlens == nullptr)
-    return fail(ESEP_EINVAL, "attn_fwd: q, k, v, o and cu_seqlens are required");
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (q_rs & 7) ||
-      (k_rs & 7) || (v_rs & 7) || (o_rs & 7))
-    return fail(ESEP_EALIGN, "attn_fwd: q, k, v, o need 16-byte alignment and token strides "
-                             "that are multiples of 8 elements");
-  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "attn_fwd: scale must be positive");
   esep::AttnArgs a{};
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.o = o;
-  a.lse = lse;
-  a.cu = cu_seqlens;
-  a.q_rs = q_rs;
-  a.k_rs = k_rs;
-  a.v_rs = v_rs;
-  a.o_rs = o_rs;
-  a.T = T;
-  a.n_seq = n_seq;
-  a.HQ = HQ;
-  a.HK = HK;
-  a.scale = scale;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  const int rc = attn_fwd_args("attn_fwd", q, q_rs, k, k_rs, v, v_rs, o, o_rs, lse, dt, T, HQ, HK, D,
+                               cu_seqlens, n_seq, max_seqlen, scale, &a);
+  if (rc != 0 || a.T == 0) return rc;
   bool sup = false;
   const hipError_t e = esep::launch_attn_fwd(a, dt, D, max_seqlen, static_cast<hipStream_t>(stream), &sup);
   if (!sup) return fail(ESEP_EINVAL, "attn_fwd: unsupported dtype / D");
@@ -606,65 +709,72 @@ int esep_attn_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, cons
                   int D, const int32_t* cu_seqlens, int n_seq, int max_seqlen, float scale,
                   void* stream) {
   g_err[0] = 0;
-  if (dt != ESEP_F16 && dt != ESEP_BF16)
-    return fail(ESEP_EINVAL, "attn_bwd: dtype %d is not fp16 / bf16", dt);
-  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "attn_bwd: D=%d not in {64, 128}", D);
-  if (T < 0 || T > 0x7fffffff || HQ < 1 || HK < 1 || HQ % HK != 0 || n_seq < 0 || max_seqlen < 0)
-    return fail(ESEP_ESHAPE, "attn_bwd: bad sizes T=%lld HQ=%d HK=%d n_seq=%d max_seqlen=%d",
-                (long long)T, HQ, HK, n_seq, max_seqlen);
-  const int64_t wq = (int64_t)HQ * D, wk = (int64_t)HK * D;
-  if (q_rs < wq || o_rs < wq || do_rs < wq || dq_rs < wq || k_rs < wk || v_rs < wk ||
-      dk_rs < wk || dv_rs < wk)
-    return fail(ESEP_ESHAPE, "attn_bwd: token stride smaller than heads * D");
-  for (int64_t rs : {q_rs, o_rs, do_rs, dq_rs, k_rs, v_rs, dk_rs, dv_rs})
-    if (rs > kAttnMaxStride)
-      return fail(ESEP_ESHAPE, "attn_bwd: token stride above %lld elements",
-                  (long long)kAttnMaxStride);
-  if (T == 0 || n_seq == 0 || max_seqlen == 0) return 0;
-  const void* ptrs[] = {q, k, v, o, dout, dq, dk, dv};
-  for (const void* p : ptrs)
-    if (p == nullptr) return fail(ESEP_EINVAL, "attn_bwd: q, k, v, o, dout, dq, dk, dv are required");
-  if (lse == nullptr || workspace == nullptr || cu_seqlens == nullptr)
-    return fail(ESEP_EINVAL, "attn_bwd: lse, the workspace and cu_seqlens are required");
-  if (!aligned16(workspace)) return fail(ESEP_EALIGN, "attn_bwd: workspace needs 16-byte alignment");
-  const int64_t rss[] = {q_rs, k_rs, v_rs, o_rs, do_rs, dq_rs, dk_rs, dv_rs};
-  for (int i = 0; i < 8; ++i)
-    if (!aligned16(ptrs[i]) || (rss[i] & 7))
-      return fail(ESEP_EALIGN, "attn_bwd: tensors need 16-byte alignment and token strides "
-                               "that are multiples of 8 elements");
-  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "attn_bwd: scale must be positive");
   esep::AttnBwdArgs b{};
-  b.f.q = q;
-  b.f.k = k;
-  b.f.v = v;
-  b.f.o = const_cast<void*>(o);
-  b.f.lse = const_cast<float*>(lse);
-  b.f.cu = cu_seqlens;
-  b.f.q_rs = q_rs;
-  b.f.k_rs = k_rs;
-  b.f.v_rs = v_rs;
-  b.f.o_rs = o_rs;
-  b.f.T = T;
-  b.f.n_seq = n_seq;
-  b.f.HQ = HQ;
-  b.f.HK = HK;
-  b.f.scale = scale;
-  b.f.scale_log2 = scale * 1.4426950408889634f;
-  b.dout = dout;
-  b.delta = workspace;
+  const int rc = attn_bwd_args("attn_bwd", q, q_rs, k, k_rs, v, v_rs, o, o_rs, dout, do_rs, lse,
+                               workspace, dq, dq_rs, dk, dk_rs, dv, dv_rs, dt, T, HQ, HK, D, cu_seqlens,
+                               n_seq, max_seqlen, scale, &b);
+  if (rc != 0 || b.f.T == 0) return rc;
   b.split = attn_split(T, HQ, HK);
-  b.part = workspace + (((int64_t)HQ * T + 3) & ~(int64_t)3);
-  b.dq = dq;
-  b.dk = dk;
-  b.dv = dv;
-  b.do_rs = do_rs;
-  b.dq_rs = dq_rs;
-  b.dk_rs = dk_rs;
-  b.dv_rs = dv_rs;
   bool sup = false;
   const hipError_t e = esep::launch_attn_bwd(b, dt, D, max_seqlen, static_cast<hipStream_t>(stream), &sup);
   if (!sup) return fail(ESEP_EINVAL, "attn_bwd: unsupported dtype / D");
   return e == hipSuccess ? 0 : hip_fail(e, "attn_bwd launch");
+}
+
+int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
+                      int64_t v_rs, void* o, int64_t o_rs, float* lse, int dt, int64_t T, int HQ,
+                      int HK, int D, const int32_t* cu_seqlens, int n_seq, float scale, int window,
+                      int sinks, int zero_rest, void* stream) {
+  g_err[0] = 0;
+  esep::AttnWinArgs p{};
+  int rc = attn_fwd_args("attn_win_fwd", q, q_rs, k, k_rs, v, v_rs, o, o_rs, lse, dt, T, HQ, HK, D,
+                         cu_seqlens, n_seq, 1, scale, &p.b.f);
+  if (rc == 0) rc = window_ok("attn_win_fwd", window, sinks);
+  if (rc != 0 || p.b.f.T == 0) return rc;
+  p.window = window;
+  p.sinks = sinks;
+  p.zero_rest = zero_rest;
+  bool sup = false;
+  const hipError_t e = esep::launch_attn_win_fwd(p, dt, D, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "attn_win_fwd: unsupported dtype / D");
+  return e == hipSuccess ? 0 : hip_fail(e, "attn_win_fwd launch");
+}
+
+int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int max_seqlen, int window,
+                                    int sinks) {
+  if (T <= 0 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || max_seqlen < 1 || window < 1 || sinks < 0)
+    return 0;
+  return win_layout(T, HQ, HK, D, max_seqlen, window, sinks).total;
+}
+
+int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
+                      int64_t v_rs, const void* o, int64_t o_rs, const void* dout, int64_t do_rs,
+                      const float* lse, float* workspace, void* dq, int64_t dq_rs, void* dk,
+                      int64_t dk_rs, void* dv, int64_t dv_rs, int dt, int64_t T, int HQ, int HK,
+                      int D, const int32_t* cu_seqlens, int n_seq, int max_seqlen, float scale,
+                      int window, int sinks, void* stream) {
+  g_err[0] = 0;
+  esep::AttnWinArgs p{};
+  int rc = attn_bwd_args("attn_win_bwd", q, q_rs, k, k_rs, v, v_rs, o, o_rs, dout, do_rs, lse, workspace,
+                         dq, dq_rs, dk, dk_rs, dv, dv_rs, dt, T, HQ, HK, D, cu_seqlens, n_seq, max_seqlen,
+                         scale, &p.b);
+  if (rc == 0) rc = window_ok("attn_win_bwd", window, sinks);
+  if (rc != 0 || p.b.f.T == 0) return rc;
+  const WinLayout w = win_layout(T, HQ, HK, D, max_seqlen, window, sinks);
+  if (w.far && esep::win_main_slots(T, window) * HK * 2 * w.sinks >= int64_t{1} << 24)
+    return fail(ESEP_ESHAPE, "attn_win_bwd: sinks=%d at a window of %d are too many for %lld tokens", sinks,
+                window, (long long)T);
+  p.window = window;
+  p.sinks = w.sinks;
+  p.far = w.far;
+  p.far_split = w.far_split;
+  p.b.split = w.split;
+  p.sink_main = workspace + w.main_at;
+  p.sink_far = workspace + w.far_at;
+  bool sup = false;
+  const hipError_t e = esep::launch_attn_win_bwd(p, dt, D, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "attn_win_bwd: unsupported dtype / D");
+  return e == hipSuccess ? 0 : hip_fail(e, "attn_win_bwd launch");
 }
 
 int esep_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, int dt,

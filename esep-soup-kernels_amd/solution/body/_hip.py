@@ -78,6 +78,12 @@ SIGNATURES = {
     "esep_attn_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
                              _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
                              _i32, _i32, _f32, _vp]),
+    "esep_attn_win_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32,
+                                 _i32, _i32, _vp, _i32, _f32, _i32, _i32, _i32, _vp]),
+    "esep_attn_win_bwd_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "esep_attn_win_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
+                                 _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
+                                 _i32, _i32, _f32, _i32, _i32, _vp]),
     "esep_rope": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64,
                          _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _f32, _vp]),
 }
@@ -183,6 +189,15 @@ except AttributeError:  # a torch without it (or without a GPU build)
 
 def _stream(dev):
     return _current_stream(dev) if _raw_stream is None else _raw_stream(dev.index)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(dev):
+    """The launch's device made current where it is not (a kernel goes to the current device's queue of
+    modules, whatever stream it is given)."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 _has_storage, _transforms = torch._C._has_storage, torch._C._are_functorch_transforms_active
@@ -419,9 +434,7 @@ def _tokens_ld(t, name):
     return t.stride(0)
 
 
-def attn_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, lse=None, name="_attn_fwd"):
-    """Varlen causal attention forward (esep_attn_fwd). q, o: [T, HQ, D]; k, v: [T, HK, D];
-    cu_seqlens int32 [n_seq + 1] on the device; lse: fp32 [HQ, T] out or None."""
+def _attn_fwd_checked(q, k, v, o, cu_seqlens, lse):
     dev = _dev(q, k, v, o, cu_seqlens, lse)
     T, HQ, D = q.shape
     HK = k.shape[1]
@@ -433,6 +446,13 @@ def attn_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, lse=None, name="_attn_fw
         raise EsepError("cu_seqlens must be a contiguous int32 tensor")
     if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != (HQ, T)):
         raise EsepError("lse must be a contiguous fp32 [HQ, T] tensor")
+    return dev, T, HQ, HK, D
+
+
+def attn_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, lse=None, name="_attn_fwd"):
+    """Varlen causal attention forward (esep_attn_fwd). q, o: [T, HQ, D]; k, v: [T, HK, D];
+    cu_seqlens int32 [n_seq + 1] on the device; lse: fp32 [HQ, T] out or None."""
+    dev, T, HQ, HK, D = _attn_fwd_checked(q, k, v, o, cu_seqlens, lse)
     rc = lib().esep_attn_fwd(
         _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
         _p(o), _tokens_ld(o, "o"), _p(lse), dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens),
@@ -441,16 +461,35 @@ def attn_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, lse=None, name="_attn_fw
     _record(name)
 
 
+def attn_win_fwd(q, k, v, o, cu_seqlens, scale, window, sinks=0, lse=None, zero_rest=False,
+                 name="_attn_win_fwd"):
+    """attn_fwd through a window (esep_attn_win_fwd): query i sees key j <= i if i - j < window or
+    j < sinks. zero_rest writes o = 0 for the tokens behind the last sequence."""
+    dev, T, HQ, HK, D = _attn_fwd_checked(q, k, v, o, cu_seqlens, lse)
+    with _on(dev):
+        rc = lib().esep_attn_win_fwd(
+            _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
+            _p(o), _tokens_ld(o, "o"), _p(lse), dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens),
+            cu_seqlens.numel() - 1, float(scale), int(window), int(sinks), int(bool(zero_rest)),
+            _stream(dev))
+    _check(rc, "esep_attn_win_fwd")
+    _record(name)
+
+
 def attn_bwd_workspace(T, HQ, HK, D):
     """Floats of fp32 workspace esep_attn_bwd needs for this shape."""
     return int(lib().esep_attn_bwd_workspace(int(T), int(HQ), int(HK), int(D)))
 
 
-def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, workspace=None,
-             name="_attn_bwd"):
-    """Backward of attn_fwd (esep_attn_bwd): dq [T, HQ, D], dk, dv [T, HK, D] out. `workspace`
-    is a contiguous fp32 tensor of >= attn_bwd_workspace(T, HQ, HK, D) elements (allocated here
-    when not given)."""
+def attn_win_bwd_workspace(T, HQ, HK, D, max_seqlen, window, sinks):
+    """Floats of fp32 workspace esep_attn_win_bwd needs for these sizes."""
+    return int(lib().esep_attn_win_bwd_workspace(int(T), int(HQ), int(HK), int(D), int(max_seqlen),
+                                                 int(window), int(sinks)))
+
+
+def _attn_bwd_checked(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace, need):
+    """Checks the operands of an attention backward; `need` gives the workspace's size for (T, HQ, HK,
+    D). Returns the device, the sizes and the workspace (allocated where it is None)."""
     dev = _dev(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace)
     T, HQ, D = q.shape
     HK = k.shape[1]
@@ -462,12 +501,22 @@ def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, w
         raise EsepError("lse must be a contiguous fp32 [HQ, T] tensor")
     if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
         raise EsepError("cu_seqlens must be a contiguous int32 tensor")
-    need = attn_bwd_workspace(T, HQ, HK, D)
+    need = need(T, HQ, HK, D)
     if workspace is None:
         workspace = torch.empty(max(need, 1), device=dev, dtype=torch.float32)
     elif (workspace.dtype != torch.float32 or not workspace.is_contiguous()
           or workspace.numel() < need or workspace.device != dev):
         raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
+    return dev, (T, HQ, HK, D), workspace
+
+
+def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, workspace=None,
+             name="_attn_bwd"):
+    """Backward of attn_fwd (esep_attn_bwd): dq [T, HQ, D], dk, dv [T, HK, D] out. `workspace`
+    is a contiguous fp32 tensor of >= attn_bwd_workspace(T, HQ, HK, D) elements (allocated here
+    when not given)."""
+    dev, (T, HQ, HK, D), workspace = _attn_bwd_checked(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens,
+                                                       workspace, attn_bwd_workspace)
     rc = lib().esep_attn_bwd(
         _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
         _p(o), _tokens_ld(o, "o"), _p(dout), _tokens_ld(dout, "dout"), _p(lse), _p(workspace),
@@ -475,6 +524,24 @@ def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, w
         dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens), cu_seqlens.numel() - 1,
         int(max_seqlen), float(scale), _stream(dev))
     _check(rc, "esep_attn_bwd")
+    _record(name)
+
+
+def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, window, sinks=0,
+                 workspace=None, name="_attn_win_bwd"):
+    """Backward of attn_win_fwd (esep_attn_win_bwd), as attn_bwd; the gradients of the tokens behind the
+    last sequence are 0. `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
+    dev, (T, HQ, HK, D), workspace = _attn_bwd_checked(
+        q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace,
+        lambda *sizes: attn_win_bwd_workspace(*sizes, max_seqlen, window, sinks))
+    with _on(dev):
+        rc = lib().esep_attn_win_bwd(
+            _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
+            _p(o), _tokens_ld(o, "o"), _p(dout), _tokens_ld(dout, "dout"), _p(lse), _p(workspace),
+            _p(dq), _tokens_ld(dq, "dq"), _p(dk), _tokens_ld(dk, "dk"), _p(dv), _tokens_ld(dv, "dv"),
+            dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens), cu_seqlens.numel() - 1,
+            int(max_seqlen), float(scale), int(window), int(sinks), _stream(dev))
+    _check(rc, "esep_attn_win_bwd")
     _record(name)
 
 

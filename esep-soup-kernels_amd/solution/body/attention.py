@@ -59,12 +59,55 @@ class VarlenAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
-def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None):
+class WindowAttention(torch.autograd.Function):
+    """VarlenAttention through a window: apply(q, k, v, cu_seqlens, max_seqlen, scale, window, sinks).
+    The output and the gradients of tokens behind the last sequence are 0."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, max_seqlen, scale, window, sinks):
+        q, k, v = _heads_packed(q), _heads_packed(k), _heads_packed(v)
+        T, HQ, D = q.shape
+        new = torch.empty if cu_seqlens.numel() > 1 else torch.zeros  # no sequence: nothing is launched
+        o = new((T, HQ, D), device=q.device, dtype=q.dtype)
+        lse = torch.empty((HQ, T), device=q.device, dtype=torch.float32)
+        _hip.attn_win_fwd(q, k, v, o, cu_seqlens, scale, window, sinks, lse=lse, zero_rest=True)
+        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        ctx.args = max_seqlen, scale, window, sinks
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, cu = ctx.saved_tensors
+        q, k, v, o, do = (_heads_packed(t) for t in (q, k, v, o, do))
+        new = torch.empty if cu.numel() > 1 else torch.zeros
+        dq, dk, dv = (new(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        _hip.attn_win_bwd(q, k, v, o, do, lse.contiguous(), dq, dk, dv, cu.contiguous(), *ctx.args)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _whole(name, value, least):
+    if isinstance(value, bool) or int(value) != value or value < least or value > 0x7FFFFFFF:
+        raise _hip.EsepError(f"{name} must be a whole number of at least {least}, got {value!r}")
+    return int(value)
+
+
+def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, sinks=0):
     """Causal attention within each sequence of the packed tokens. q [T, HQ, D] (or
     [1, T, HQ, D]), k, v [T, HK, D]; cu_seqlens int32 [n_seq + 1] on q's device; max_seqlen an
-    int >= every sequence length. Returns o [T, HQ, D] in q's dtype."""
+    int >= every sequence length. Returns o [T, HQ, D] in q's dtype.
+
+    window (None: no bound): query i of a sequence sees key j <= i only if i - j < window (the last
+    `window` tokens, its own among them, as HF's sliding_window) or j < sinks (the sequence's
+    first tokens, which stay visible; without a window they always are). Where the window bounds something
+    (window < max_seqlen), tokens behind the last sequence get an output and gradients of 0."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if q.dim() == 4:  # [1, T, H, D] views: the Function works on [T, H, D]
         q, k, v = q.squeeze(0), k.squeeze(0), v.squeeze(0)
+    sinks = _whole("sinks", sinks, 0)
+    if window is not None:
+        window = _whole("window", window, 1)
+        if window < max_seqlen:
+            return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
     return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))

@@ -9,6 +9,8 @@ as torch's scaled_dot_product_attention backward computes it:
     P = softmax(scale * Q K^T + causal mask),  O = P V
     dV = P^T dO,  dP = dO V^T,  dS = P * (dP - rowsum(dO * O)),  dQ = scale * dS K,
     dK = scale * dS^T Q     (dK, dV of a kv head summed over the query heads that read it)
+Through a window (no reference counterpart; HF's sliding_window mask with the sequence's first tokens
+left visible) the mask also hides key j of query i where i - j >= window and j >= sinks.
 Everything in float64 numpy. Pinned in tests/test_oracle_attention.py against torch's SDPA
 (math path, float64, CPU), closed forms and finite differences.
 """
@@ -21,7 +23,14 @@ def _bounds(cu):
     return [(int(cu[i]), int(cu[i + 1])) for i in range(len(cu) - 1)]
 
 
-def attn_fwd(q, k, v, cu, scale):
+def visible(n, window=None, sinks=0):
+    """[n, n] mask of the keys that each query of a sequence sees."""
+    i, j = np.arange(n)[:, None], np.arange(n)[None, :]
+    seen = j <= i
+    return seen if window is None else seen & ((i - j < window) | (j < sinks))
+
+
+def attn_fwd(q, k, v, cu, scale, window=None, sinks=0):
     """q [T, HQ, D], k, v [T, HK, D] (any float) -> (o [T, HQ, D], lse [HQ, T]) in float64.
     Tokens outside every sequence keep o = 0, lse = -inf."""
     q, k, v = (np.asarray(t, dtype=np.float64) for t in (q, k, v))
@@ -34,7 +43,7 @@ def attn_fwd(q, k, v, cu, scale):
         n = s1 - s0
         if n <= 0:
             continue
-        mask = np.tril(np.ones((n, n), dtype=bool))
+        mask = visible(n, window, sinks)
         for h in range(HQ):
             kh = h // G
             sc = scale * q[s0:s1, h] @ k[s0:s1, kh].T
@@ -47,8 +56,8 @@ def attn_fwd(q, k, v, cu, scale):
     return o, lse
 
 
-def attn_bwd(q, k, v, do, cu, scale):
-    """Gradients of sum(o * do) for o = attn_fwd(q, k, v, cu, scale)[0]: (dq, dk, dv) float64."""
+def attn_bwd(q, k, v, do, cu, scale, window=None, sinks=0):
+    """Gradients of sum(o * do) for o = attn_fwd(q, k, v, cu, scale, ...)[0]: (dq, dk, dv) float64."""
     q, k, v, do = (np.asarray(t, dtype=np.float64) for t in (q, k, v, do))
     T, HQ, D = q.shape
     HK = k.shape[1]
@@ -58,7 +67,7 @@ def attn_bwd(q, k, v, do, cu, scale):
         n = s1 - s0
         if n <= 0:
             continue
-        mask = np.tril(np.ones((n, n), dtype=bool))
+        mask = visible(n, window, sinks)
         for h in range(HQ):
             kh = h // G
             qs, ks, vs, dos = q[s0:s1, h], k[s0:s1, kh], v[s0:s1, kh], do[s0:s1, h]
