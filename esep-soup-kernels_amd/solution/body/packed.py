@@ -26,8 +26,9 @@ Per decoder layer, each piece has a guard and an HF / torch fallback (warned onc
               q/k/v on plain nn.Linear bases likewise as one GEMM against their concatenated
               weights (FUSE_QKV; the reference runs those three apart).
   RoPE        norm_rope.rope on the packed positions with the model's inv_freq.
-  attention   attention.varlen_attention over all rows in one launch per direction; else a
-              per-row SDPA loop (reference packed.py:404-436).
+  attention   attention.varlen_attention over all rows in one launch per direction, through the
+              window of a sliding-window layer (which the reference leaves to the original
+              forward); else a per-row SDPA loop (reference packed.py:404-436).
   MLP         frozen plain or NF4 projections: _RecomputeMLP (no [T, intermediate] tensor
               saved; NF4 weights dequantized on the HIP kernel, gate and up in one launch);
               otherwise the projections with the HIP SwiGLU, gate and up fed from their own
@@ -512,7 +513,8 @@ def _cu_seqlens(lens, device):
 
 def _attention(attn, q, k, v, lens):
     """Causal attention within each original row of the packed q [1, T, Hq, D] and k, v
-    [1, T, Hk, D] -> [1, T, Hq * D]; query head h reads kv head h // (Hq / Hk) (HF's repeat_kv).
+    [1, T, Hk, D] -> [1, T, Hq * D]; query head h reads kv head h // (Hq / Hk) (HF's repeat_kv). A
+    sliding-window layer's queries see the last attn.sliding_window tokens, their own among them.
     One varlen kernel launch per direction when it applies, else torch's SDPA per row
     (reference packed.py:404-436)."""
     if torch.is_autocast_enabled("cuda"):
@@ -520,21 +522,28 @@ def _attention(attn, q, k, v, lens):
         q, k, v = q.to(dt), k.to(dt), v.to(dt)
     n_tok, hq, d = q.shape[1], q.shape[2], q.shape[3]
     dropout = attn.attention_dropout if attn.training else 0.0
+    window = None
+    if "sliding_attention" in _layer_kinds(getattr(attn, "config", None)):
+        window = attn.sliding_window  # None in a full layer
     if USE_KERNELS:
         from . import attention
 
         if attention.supported(q, k, v, dropout):
             o = attention.varlen_attention(q, k, v, _cu_seqlens(tuple(lens), q.device), max(lens),
-                                           attn.scaling)
+                                           attn.scaling, window=window)
             return o.view(1, n_tok, hq * d)
         _fallback("attention kernel", f"dtype {q.dtype}, head_dim {d}, dropout {dropout}")
     rows = []
     for qs, ks, vs in zip(q[0].split(lens), k[0].split(lens), v[0].split(lens)):
         # [n, H, D] row slices as [1, H, n, D]; SDPA's grouped-query mode maps query head h to
         # kv head h // (Hq / Hk)
+        n, seen = qs.shape[0], None
+        if window is not None and window < n:
+            seen = torch.ones(n, n, dtype=torch.bool, device=q.device).tril().triu(1 - window)
         o = F.scaled_dot_product_attention(qs.transpose(0, 1)[None], ks.transpose(0, 1)[None],
-                                           vs.transpose(0, 1)[None], dropout_p=dropout,
-                                           is_causal=True, scale=attn.scaling, enable_gqa=True)
+                                           vs.transpose(0, 1)[None], attn_mask=seen,
+                                           dropout_p=dropout, is_causal=seen is None,
+                                           scale=attn.scaling, enable_gqa=True)
         rows.append(o[0].transpose(0, 1))  # [n, Hq, D]
     return torch.cat(rows).reshape(1, n_tok, hq * d)
 
@@ -738,6 +747,22 @@ def _layer(layer, residual, delta, rope_in, lens):
     return residual, _mlp(layer.mlp, xs, post, residual, eps, norm_saves_y=NORM_SAVE_OUTPUT)
 
 
+def _layer_kinds(config):
+    return set(getattr(config, "layer_types", None) or ["full_attention"])
+
+
+def _windows_ok(model):
+    """Every layer says what its queries see: the config's window in a sliding-window layer, everything
+    before them in a full one."""
+    config = model.config
+    want = {"full_attention": None, "sliding_attention": getattr(config, "sliding_window", None)}
+    if not isinstance(want["sliding_attention"], int) or want["sliding_attention"] < 1:
+        return False
+    n = config.num_hidden_layers
+    return all(getattr(layer.self_attn, "sliding_window", None) == want[kind]
+               for layer, kind in zip(model.layers[:n], config.layer_types[:n]))
+
+
 def _unsupported(model, input_ids, attention_mask, past_key_values, inputs_embeds, use_cache,
                  kwargs):
     """None when the packed path takes this call, else the reason it does not (reference
@@ -768,7 +793,9 @@ def _unsupported(model, input_ids, attention_mask, past_key_values, inputs_embed
             return key
     if getattr(config, "_attn_implementation", None) != "sdpa":
         return "attn_implementation is not sdpa"
-    if any(kind != "full_attention" for kind in getattr(config, "layer_types", ["full_attention"])):
+    if _layer_kinds(config) - {"full_attention", "sliding_attention"}:
+        return "layers of another kind than full or sliding-window attention"
+    if "sliding_attention" in _layer_kinds(config) and not _windows_ok(model):
         return "sliding window layers"
     if model.training and getattr(model, "gradient_checkpointing", False):
         return "gradient checkpointing"
@@ -785,10 +812,17 @@ class _Packing:
     arange(L) per row also under left padding, or the caller's position_ids gathered
     (reference packed.py:800-814)."""
 
-    def __init__(self, attention_mask, position_ids):
+    def __init__(self, attention_mask, position_ids, windows=False):
         real = attention_mask.bool()
         self.B, self.L = real.shape
-        self.lens = real.sum(1).tolist()
+        counts = real.sum(1)
+        if windows:  # the tokens' runs too: a window counts columns, gaps among them
+            starts = real[:, 1:] & ~real[:, :-1]
+            counts = torch.stack((counts, real[:, 0] + starts.sum(1)))
+            counts, runs = counts.tolist()
+            self.lens, self.gaps = counts, max(runs, default=0) > 1
+        else:
+            self.lens, self.gaps = counts.tolist(), False
         self.T = sum(self.lens)
         self.index = torch.nonzero_static(real.reshape(-1), size=self.T).squeeze(1)
         if position_ids is None:
@@ -811,9 +845,10 @@ class _Packing:
 
 def packed_forward(model, input_ids, attention_mask, position_ids, kwargs):
     """The packed decoder body (reference packed.py:800-840): [B, L, H] hidden states, or None
-    when a row has no token (the caller then runs the original forward)."""
-    pack = _Packing(attention_mask, position_ids)
-    if min(pack.lens) == 0:
+    when a row has no token, or under sliding-window layers a gap among its tokens (the caller then
+    runs the original forward)."""
+    pack = _Packing(attention_mask, position_ids, "sliding_attention" in _layer_kinds(model.config))
+    if min(pack.lens) == 0 or pack.gaps:
         return None
     hidden = model.embed_tokens(pack.gather(input_ids))
     _Report.training, _Report.where = bool(model.training), "embedding"
@@ -854,7 +889,7 @@ def patch():
         hidden = None
         if reason is None:
             hidden = packed_forward(self, input_ids, attention_mask, position_ids, kwargs)
-            reason = None if hidden is not None else "a row without tokens"
+            reason = None if hidden is not None else "a row without tokens, or with gaps in a window"
         training = getattr(self, "training", False)
         if hidden is None:
             if training and reason != "not a real model":
