@@ -66,6 +66,7 @@ struct AttnBwdArgs {
 
 constexpr int kAttnBM = 128;  // queries per forward / dQ block (4 wavefronts x 32)
 constexpr int kAttnThreads = 256;
+constexpr int64_t kAttnCUs = 256;
 
 hipError_t launch_attn_fwd(const AttnArgs& a, int dt, int D, int max_seqlen, hipStream_t s,
                            bool* supported);
@@ -111,6 +112,47 @@ inline int win_far_split(int64_t T, int HQ, int HK, int window, int sinks) {
 
 hipError_t launch_attn_win_fwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
 hipError_t launch_attn_win_bwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
+
+// Attention of the newest tokens over a cache (attention_cache.hip). Strides in elements.
+struct AttnCacheArgs {
+  const void* q;       // [B, n, HQ, D] by (q_bs, q_ts, q_hs)
+  const void* k;       // [B, S, HK, D] by (k_bs, k_ts, k_hs)
+  const void* v;
+  void* o;             // [B, n, HQ, D] dense
+  const int32_t* len;  // [B] tokens in each row's cache, the n new ones last
+  float* part;         // partials, cache_part_floats
+  int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
+  int B, n, S, HQ, HK;
+  int window, sinks;   // window 0x7fffffff: none
+  int units;           // wavefronts of the launch
+  float scale_log2;
+};
+
+// Query rows of a kv head: its query heads times the new tokens, in tiles of 32.
+inline int64_t cache_row_tiles(int n, int HQ, int HK) { return ((int64_t)n * (HQ / HK) + 31) / 32; }
+// 32-key tiles of a row at most.
+inline int64_t cache_key_tiles(int S, int n, int window, int sinks) {
+  const int64_t all = ((int64_t)S + 31) / 32;
+  const int64_t seen = ((int64_t)sinks + 31) / 32 + ((int64_t)window + n + 30) / 32;
+  return seen < all ? seen : all;
+}
+// Wavefronts: a ring of two 32-key K / V tiles each (32 KiB at D = 128) of a CU's 160 KiB of LDS, and two tiles or
+// more for each to walk.
+constexpr int kCacheMinTiles = 2;
+inline int64_t cache_units(int B, int n, int S, int HQ, int HK, int D, int window, int sinks) {
+  const int64_t tiles =
+      (int64_t)B * HK * cache_row_tiles(n, HQ, HK) * cache_key_tiles(S, n, window, sinks);
+  const int64_t most = kAttnCUs * (D == 128 ? 5 : 10);
+  const int64_t u = (tiles + kCacheMinTiles - 1) / kCacheMinTiles;
+  return u < 1 ? 1 : (u < most ? u : most);
+}
+// A partial per wavefront and (row, kv head, query tile) that it walks: at most units + groups of them.
+inline int64_t cache_part_floats(int64_t units, int B, int n, int HQ, int HK, int D) {
+  const int64_t rows = (int64_t)n * (HQ / HK);
+  return (units + (int64_t)B * HK * cache_row_tiles(n, HQ, HK)) * (rows < 32 ? rows : 32) * (D + 2);
+}
+
+hipError_t launch_attn_cache(const AttnCacheArgs& a, int dt, int D, hipStream_t s, bool* supported);
 
 // ---------------------------------------------------------------------------------------
 // Device helpers shared by the attention kernels
@@ -472,7 +514,6 @@ constexpr int kDkdvPerCU = 2;
 //   16384 tokens, 16 / 2 heads, backward 14.1 -> 13.4 ms; 4 x 8192, 28 / 4 heads 6.26 -> 5.99; 8 x 1024, 12 / 2
 //   heads 156 -> 155 us, forward 40 -> 41); with ragged ones it is 4 .. 10% behind.
 //   More than 64 sequences (the searches hold one per lane): the same within two rounds.
-constexpr int64_t kAttnCUs = 256;
 constexpr int kRoundsQ = 4, kRoundsKV = 16;
 inline int attn_order(int64_t blocks, int per_cu, int rounds, int D, int64_t T, int n_seq,
                       int max_seqlen) {

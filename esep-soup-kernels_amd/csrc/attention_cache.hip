@@ -1,0 +1,329 @@
+// Attention of a row's n newest tokens over its cache (decoding: n = 1), with an optional window and sinks.
+//
+// Query t of a row sits at position len - n + t and sees key j <= that position, through a window only the last
+// `window` of them and the first `sinks`. A kv head's query heads and new tokens make one tile of up to 32 query
+// rows (row r: token r / G, head r % G of the group's G), so that K and V are read once for all of them, and a
+// wavefront runs the causal kernels' 32-key step on it (attention_tiles.hpp): the matrix core is far from busy
+// (512 of about 2000 cycles that a CU's share of the memory's rate leaves for a tile), so rows that do not
+// fill the 32 cost nothing.
+//
+// Bound by the bytes of K and V, and below a few MB by the launches' latency. The 32-key tiles of all (row, kv
+// head, query tile) groups are laid end to end and cut into equal runs, one to a wavefront, whatever the rows'
+// lengths: the wavefronts end together. Each keeps a ring of two tiles in LDS for itself, filled by LDS
+// DMA, and needs no barrier. A group within one run is stored; one that is cut leaves partials (maximum, sum
+// and weighted sum in fp32, slot = wavefront + group) that k_attn_cache_join adds in their order.
+#include <cmath>
+
+#include "attention_tiles.hpp"
+
+namespace esep {
+namespace {
+
+// The walk's geometry, found by every wavefront from the lengths: tile counts of the rows, their sum.
+struct CachePlan {
+  int64_t total;  // tiles of all groups
+  int units;      // wavefronts that walk some
+};
+
+// Row b's keys for its n queries: `ns` tiles of the sinks from 0, then tiles from lo to len.
+struct CacheRow {
+  int len, lo, sink_hi, ns, tiles;
+};
+__device__ __forceinline__ CacheRow cache_row(const AttnCacheArgs& a, int b) {
+  CacheRow r;
+  const int len = a.len[b];
+  r.len = len < 0 ? 0 : (len > a.S ? a.S : len);
+  const int first = r.len > a.n ? r.len - a.n : 0;  // the first query's position
+  r.sink_hi = a.sinks < r.len ? a.sinks : r.len;
+  r.lo = first - a.window + 1;  // window >= 1
+  if (r.lo <= r.sink_hi) r.lo = 0;
+  r.ns = r.lo > 0 ? (r.sink_hi + 31) / 32 : 0;
+  r.tiles = r.ns + (r.len - r.lo + 31) / 32;
+  return r;
+}
+
+// A value that every lane holds, in scalar registers (addresses of the tile fills are made from it).
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)v);
+  const uint32_t up = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)up << 32 | lo);
+}
+__device__ __forceinline__ int64_t lane_sum(int64_t v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return uniform(v);
+}
+
+__device__ __forceinline__ CachePlan cache_plan(const AttnCacheArgs& a, int rt) {
+  const int lane = threadIdx.x & 63;
+  int64_t sum = 0;
+  for (int b = lane; b < a.B; b += 64) sum += cache_row(a, b).tiles;
+  CachePlan p;
+  p.total = lane_sum(sum) * a.HK * rt;
+  const int64_t u = (p.total + kCacheMinTiles - 1) / kCacheMinTiles;
+  p.units = u < a.units ? (int)u : a.units;
+  return p;
+}
+
+// The row whose tiles hold number x of all (x < total), and the number of its first.
+__device__ __forceinline__ int cache_find(const AttnCacheArgs& a, int per_tile, int64_t x,
+                                          int64_t* first) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int64_t mine = b < a.B ? (int64_t)cache_row(a, b).tiles * per_tile : 0;
+    int64_t run = mine;  // inclusive sums
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t o = __shfl_up(run, d);
+      if (lane >= d) run += o;
+    }
+    const uint64_t past = __ballot(before + run > x);
+    if (past != 0) {
+      const int l = (int)__builtin_ctzll(past);
+      *first = uniform(before + __shfl(run - mine, l));
+      return b0 + l;
+    }
+    before = uniform(before + __shfl(run, 63));
+  }
+  return -1;
+}
+
+// The tiles of wavefront u are [cut(u), cut(u + 1)); the wavefront whose tiles hold x.
+__device__ __forceinline__ int64_t cache_cut(const CachePlan& p, int u) {
+  return (int64_t)((uint64_t)u * (uint64_t)p.total / (uint64_t)p.units);
+}
+__device__ __forceinline__ int cache_unit_of(const CachePlan& p, int64_t x) {
+  return (int)(((uint64_t)(x + 1) * (uint64_t)p.units - 1) / (uint64_t)p.total);
+}
+
+// One wavefront's fill of a 32-row swizzled tile (attention.hpp: SwzFill, whose row groups four wavefronts
+// share).
+template <int RB>
+struct CacheFill {
+  static constexpr int GR = 1024 / RB, CH = RB / 16, N = 32 / GR, V = RB == 256 ? 4 : 2;
+  int lrow, chunk;
+  int64_t rs;  // bytes between tokens
+  uint32_t voff[V];
+  __device__ __forceinline__ CacheFill(int lane, int64_t rs_) : rs(rs_) {
+    lrow = lane / CH;
+    chunk = (lane % CH) ^ swz<RB>(lrow);
+#pragma unroll
+    for (int i = 0; i < V; ++i) voff[i] = (uint32_t)(lrow * rs) + 16u * (uint32_t)(chunk ^ i);
+  }
+  // rows r0 .. r0 + 31; those at or past rend repeat row rend - 1
+  __device__ __forceinline__ void tile(char* dst, const char* base, int r0, int rend) const {
+    if (r0 + 32 <= rend) {
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        lds_dma_x4_s(base + (int64_t)(r0 + GR * q) * rs, voff[q % V], dst + 1024 * q);
+    } else {
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int r = r0 + GR * q + lrow < rend ? r0 + GR * q + lrow : rend - 1;
+        lds_dma_x4(base + (int64_t)r * rs + 16 * (chunk ^ (q % V)), dst + 1024 * q);
+      }
+    }
+  }
+};
+
+// s_waitcnt vmcnt(N) and lgkmcnt(0) (the other counters at their maxima).
+constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+constexpr int kWaitLgkm0 = 0xC07F;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnCacheArgs a) {
+  constexpr int RB = 2 * D, TILE = 32 * RB;
+  using V8 = typename Mfma<T>::v8;
+  using Fill = CacheFill<RB>;
+  __shared__ __align__(1024) char kv[2][2][TILE];  // [buffer][K, V]
+
+  const int lane = threadIdx.x, lq = lane & 31, hi = lane >> 5;
+  const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32, per_tile = a.HK * RT;
+  const CachePlan plan = cache_plan(a, RT);
+  const int u = blockIdx.x;
+  if (u >= plan.units) return;
+  int64_t x = cache_cut(plan, u);
+  const int64_t x1 = cache_cut(plan, u + 1);
+  int64_t first;
+  int b = __builtin_amdgcn_readfirstlane(cache_find(a, per_tile, x, &first));
+  CacheRow row = cache_row(a, b);
+  const Fill fk(lane, a.k_ts * (int64_t)sizeof(T)), fv(lane, a.v_ts * (int64_t)sizeof(T));
+  const int live = rows < 32 ? rows : 32;  // rows of a partial
+
+  while (x < x1) {
+    while (x >= first + (int64_t)row.tiles * per_tile) {
+      first += (int64_t)row.tiles * per_tile;
+      row = cache_row(a, ++b);
+    }
+    const int gi = (int)((x - first) / row.tiles);  // kv head and query tile within the row
+    const int64_t g0 = first + (int64_t)gi * row.tiles;
+    const int t0 = (int)(x - g0), t1 = x1 - g0 < row.tiles ? (int)(x1 - g0) : row.tiles;
+    const int kvh = gi / RT, rt = gi % RT;
+    const char* kbase = reinterpret_cast<const char*>(
+        static_cast<const T*>(a.k) + (int64_t)b * a.k_bs + (int64_t)kvh * a.k_hs);
+    const char* vbase = reinterpret_cast<const char*>(
+        static_cast<const T*>(a.v) + (int64_t)b * a.v_bs + (int64_t)kvh * a.v_hs);
+    auto start_of = [&](int t) { return t < row.ns ? 32 * t : row.lo + 32 * (t - row.ns); };
+    auto issue = [&](int t) {
+      const int rend = t < row.ns ? row.sink_hi : row.len;
+      fk.tile(kv[t & 1][0], kbase, start_of(t), rend);
+      fv.tile(kv[t & 1][1], vbase, start_of(t), rend);
+    };
+    // every read of the ring by the group before is done
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    issue(t0);
+    if (t0 + 1 < t1) issue(t0 + 1);
+
+    const int r = 32 * rt + lq, tok = r / G, h = kvh * G + r % G;
+    const bool rok = r < rows;
+    V8 qb[D / 16];
+    {
+      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_bs + (int64_t)tok * a.q_ts +
+                      (int64_t)h * a.q_hs + 8 * hi;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) qb[c] = rok ? ld16<V8>(qrow + 16 * c) : V8{};
+    }
+    // positions: the lane's, and the tile's first and last
+    const int p0 = row.len - a.n, pos = rok ? p0 + tok : p0 + a.n - 1;
+    const int ufirst = p0 + 32 * rt / G;
+    const int ulast = 32 * rt + 31 < rows ? p0 + (32 * rt + 31) / G : p0 + a.n - 1;
+    f32x16 oacc[D / 32];
+#pragma unroll
+    for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+    // q and the first tiles are here (through the builtin: the compiler then waits for no load of its own
+    // within the loop, which would wait for the tile in flight too)
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    for (int t = t0; t < t1; ++t) {
+      const int kh = start_of(t), cap = t < row.ns ? row.sink_hi - 1 : 0x7fffffff;
+      const char* ks = kv[t & 1][0];
+      const char* vs = kv[t & 1][1];
+      fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
+                         [&](f32x16& acc) __attribute__((always_inline)) {
+                           mask_window(acc, kh, ufirst < cap ? ufirst : cap, ulast - a.window,
+                                       pos < cap ? pos : cap, pos - a.window, row.sink_hi, hi);
+                         });
+      // this tile's reads are done: its buffer takes tile t + 2; then tile t + 1 is waited for
+      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 2 < t1) {
+        issue(t + 2);
+        __builtin_amdgcn_s_waitcnt(wait_vm(2 * Fill::N));
+      } else {
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    x += t1 - t0;
+    const int64_t slot = (int64_t)u + (int64_t)b * per_tile + gi;
+    float* part = a.part + slot * live * (D + 2);
+    if (rok && t0 == 0 && t1 == row.tiles) {  // the whole group
+      store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
+                         l > 0.f ? 1.f / l : 0.f);
+    } else if (rok) {
+      if (hi == 0) {
+        part[lq] = m;
+        part[live + lq] = l;
+      }
+      float* po = part + 2 * live + lq * D + 4 * hi;
+#pragma unroll
+      for (int md = 0; md < D / 32; ++md)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+            *reinterpret_cast<float2*>(po + 32 * md + 8 * j + e) =
+                make_float2(oacc[md][4 * j + e], oacc[md][4 * j + e + 1]);
+    }
+  }
+}
+
+// The groups that were cut, and zeros for the rows without tokens: one block per query row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attn_cache_join(const AttnCacheArgs a) {
+  constexpr int PAIRS = D / 2, GROUPS = 256 / PAIRS;
+  __shared__ float2 sums[GROUPS][PAIRS];
+  __shared__ float dens[GROUPS];
+  const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32, per_tile = a.HK * RT;
+  const int rg = (int)(blockIdx.x % rows);
+  const int kvh = (int)(blockIdx.x / rows % a.HK), b = (int)(blockIdx.x / rows / a.HK);
+  const int gi = kvh * RT + rg / 32, lq = rg % 32, live = rows < 32 ? rows : 32;
+  const CachePlan plan = cache_plan(a, RT);
+  const CacheRow row = cache_row(a, b);
+  const int g = threadIdx.x / PAIRS, c = threadIdx.x % PAIRS;
+  T* out = static_cast<T*>(a.o) + (((int64_t)b * a.n + rg / G) * a.HQ + kvh * G + rg % G) * D + 2 * c;
+  if (row.tiles == 0) {
+    if (g == 0) out[0] = out[1] = (T)0.f;
+    return;
+  }
+  int64_t before = 0;  // tiles of the rows ahead of b
+  {
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < b; i += 64) before += cache_row(a, i).tiles;
+    before = lane_sum(before) * per_tile;
+  }
+  const int64_t g0 = before + (int64_t)gi * row.tiles;
+  const int u0 = cache_unit_of(plan, g0), u1 = cache_unit_of(plan, g0 + row.tiles - 1);
+  if (u0 == u1) return;  // stored by its wavefront
+  const int64_t slot = (int64_t)b * per_tile + gi, size = (int64_t)live * (D + 2);
+  const float* part = a.part + slot * size;
+  float top = -INFINITY;
+  for (int u = u0 + (int)(threadIdx.x & 63); u <= u1; u += 64) top = fmaxf(top, part[u * size + lq]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float2 acc = make_float2(0.f, 0.f);
+  float den = 0.f;
+#pragma unroll 4
+  for (int u = u0 + g; u <= u1; u += GROUPS) {
+    const float* p = part + u * size;
+    const float w = exp2_fast(p[lq] - ref);
+    den = fmaf(w, p[live + lq], den);
+    const float2 v = *reinterpret_cast<const float2*>(p + 2 * live + lq * D + 2 * c);
+    acc.x = fmaf(w, v.x, acc.x);
+    acc.y = fmaf(w, v.y, acc.y);
+  }
+  sums[g][c] = acc;
+  if (c == 0) dens[g] = den;
+  __syncthreads();
+  if (g != 0) return;
+  for (int i = 1; i < GROUPS; ++i) {
+    acc.x += sums[i][c].x;
+    acc.y += sums[i][c].y;
+    den += dens[i];
+  }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  out[0] = (T)(acc.x * inv);
+  out[1] = (T)(acc.y * inv);
+}
+
+template <typename T, int D>
+hipError_t run(const AttnCacheArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_attn_cache<T, D>), dim3((unsigned)a.units), dim3(64), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = (int64_t)a.B * a.HQ * a.n;
+  hipLaunchKernelGGL((k_attn_cache_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_d(const AttnCacheArgs& a, int D, hipStream_t s, bool* sup) {
+  *sup = D == 128 || D == 64;
+  if (D == 128) return run<T, 128>(a, s);
+  if (D == 64) return run<T, 64>(a, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_attn_cache(const AttnCacheArgs& a, int dt, int D, hipStream_t s, bool* sup) {
+  if (dt == 1) return run_d<_Float16>(a, D, s, sup);
+  if (dt == 2) return run_d<__bf16>(a, D, s, sup);
+  *sup = false;
+  return hipErrorInvalidValue;
+}
+
+}  // namespace esep

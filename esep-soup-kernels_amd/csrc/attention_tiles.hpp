@@ -23,6 +23,19 @@ __device__ __forceinline__ void mask_future(f32x16& acc, int kh, int qw0, int qi
   }
 }
 
+// Keys past `top`, or at `low` and before it but no sinks. Only where a border crosses the 32 keys: utop
+// is the least top and ulow the greatest low of the wavefront.
+__device__ __forceinline__ void mask_window(f32x16& acc, int kh, int utop, int ulow, int top, int low,
+                                            int sink_hi, int hi) {
+  if (kh + 31 > utop || kh <= ulow) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int kj = kh + 8 * (i / 4) + 4 * hi + (i % 4);
+      if (kj > top || (kj <= low && kj >= sink_hi)) acc[i] = -INFINITY;
+    }
+  }
+}
+
 // 32 keys of the online softmax for a wavefront's 32 queries: keys kh .. kh + 31, held in 32 rows of
 // the swizzled LDS tiles at ks / vs (the layout, its DMA and its readers are in attention.hpp).
 // Lane (lq, hi) gets the scores of its query qi against keys kh + 8 (i / 4) + 4 hi + i % 4, i < 16,

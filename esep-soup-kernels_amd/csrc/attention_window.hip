@@ -108,19 +108,6 @@ struct KeyWalk {
   }
 };
 
-// One step's mask: keys past `top`, or out of the window and no sinks. Only where a border crosses the 32
-// keys (uniform: `utop` is the least top of the wavefront).
-__device__ __forceinline__ void mask_window(f32x16& acc, int kh, int qw0, int utop, int top, int low,
-                                            int window, int sink_hi, int hi) {
-  if (kh + 31 > utop || kh <= qw0 + 31 - window) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int kj = kh + 8 * (i / 4) + 4 * hi + (i % 4);
-      if (kj > top || (kj <= low && kj >= sink_hi)) acc[i] = -INFINITY;
-    }
-  }
-}
-
 // Walks the tiles of a block: K and V through a ring of two LDS buffers (tile t + 1 in flight while
 // tile t is consumed), step(ks, vs, kh, utop, top) for every 32 keys that the wavefront sees.
 template <typename T, int D, int BN, class Step>
@@ -210,8 +197,8 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_win_fwd(con
                           __attribute__((always_inline)) {
                         fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
                                            [&](f32x16& acc) __attribute__((always_inline)) {
-                                             mask_window(acc, kh, qw0, utop, top, qi - p.window,
-                                                         p.window, kw.sink_hi, hi);
+                                             mask_window(acc, kh, utop, qw0 + 31 - p.window, top,
+                                                         qi - p.window, kw.sink_hi, hi);
                                            });
                       });
   if (qi >= end) return;
@@ -271,8 +258,8 @@ __global__ __launch_bounds__(kAttnThreads, kDqPerCU<D>) void k_attn_win_dq(const
                           __attribute__((always_inline)) {
                         dq_tile_swz<T, D>(ks, vs, lane, a.scale_log2, lse2, delta, qb, db, dqa,
                                           [&](f32x16& s) __attribute__((always_inline)) {
-                                            mask_window(s, kh, qw0, utop, top, qi - p.window,
-                                                        p.window, kw.sink_hi, hi);
+                                            mask_window(s, kh, utop, qw0 + 31 - p.window, top,
+                                                        qi - p.window, kw.sink_hi, hi);
                                           });
                       });
   if (!qok) return;

@@ -777,6 +777,71 @@ int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
   return e == hipSuccess ? 0 : hip_fail(e, "attn_win_bwd launch");
 }
 
+int64_t esep_attn_cache_workspace(int B, int n, int S, int HQ, int HK, int D, int window, int sinks) {
+  if (B < 1 || n < 1 || S < 1 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0)
+    return 0;
+  const int w = window == 0 || window > S ? S : window;
+  return esep::cache_part_floats(esep::cache_units(B, n, S, HQ, HK, D, w, sinks), B, n, HQ, HK, D);
+}
+
+int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                    const void* v, const int64_t* v_strides, void* o, const int32_t* lengths,
+                    float* workspace, int dt, int B, int n, int S, int HQ, int HK, int D, float scale,
+                    int window, int sinks, void* stream) {
+  g_err[0] = 0;
+  if (dt != ESEP_F16 && dt != ESEP_BF16)
+    return fail(ESEP_EINVAL, "attn_cache: dtype %d is not fp16 / bf16", dt);
+  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "attn_cache: D=%d not in {64, 128}", D);
+  if (B < 0 || n < 0 || S < 0 || HQ < 1 || HK < 1 || HQ % HK != 0 || S > (1 << 30) || n > (1 << 24) ||
+      (int64_t)B * HQ * n >= int64_t{1} << 24)
+    return fail(ESEP_ESHAPE, "attn_cache: bad sizes B=%d n=%d S=%d HQ=%d HK=%d", B, n, S, HQ, HK);
+  if (window < 0 || sinks < 0)
+    return fail(ESEP_ESHAPE, "attn_cache: window=%d sinks=%d", window, sinks);
+  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "attn_cache: scale must be positive");
+  if (B == 0 || n == 0) return 0;
+  if (q == nullptr || o == nullptr || lengths == nullptr || workspace == nullptr ||
+      q_strides == nullptr || k_strides == nullptr || v_strides == nullptr ||
+      (S > 0 && (k == nullptr || v == nullptr)))
+    return fail(ESEP_EINVAL, "attn_cache: q, k, v, o, lengths, the workspace and strides are required");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(workspace))
+    return fail(ESEP_EALIGN, "attn_cache: q, k, v, o and the workspace need 16-byte alignment");
+  for (const int64_t* st : {q_strides, k_strides, v_strides})
+    for (int i = 0; i < 3; ++i)
+      if (st[i] < 0 || (st[i] & 7))
+        return fail(ESEP_EALIGN, "attn_cache: strides need to be multiples of 8 elements");
+  if (k_strides[1] > kAttnMaxStride || v_strides[1] > kAttnMaxStride)
+    return fail(ESEP_ESHAPE, "attn_cache: token stride above %lld elements", (long long)kAttnMaxStride);
+  esep::AttnCacheArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.len = lengths;
+  a.part = workspace;
+  a.q_bs = q_strides[0];
+  a.q_ts = q_strides[1];
+  a.q_hs = q_strides[2];
+  a.k_bs = k_strides[0];
+  a.k_ts = k_strides[1];
+  a.k_hs = k_strides[2];
+  a.v_bs = v_strides[0];
+  a.v_ts = v_strides[1];
+  a.v_hs = v_strides[2];
+  a.B = B;
+  a.n = n;
+  a.S = S;
+  a.HQ = HQ;
+  a.HK = HK;
+  a.window = window == 0 || window > S ? (S > 0 ? S : 1) : window;  // none: a row's longest
+  a.sinks = sinks;
+  a.units = (int)esep::cache_units(B, n, S, HQ, HK, D, a.window, sinks);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  bool sup = false;
+  const hipError_t e = esep::launch_attn_cache(a, dt, D, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "attn_cache: unsupported dtype / D");
+  return e == hipSuccess ? 0 : hip_fail(e, "attn_cache launch");
+}
+
 int esep_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, int dt,
                     void* stream) {
   g_err[0] = 0;

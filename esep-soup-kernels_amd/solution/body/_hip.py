@@ -84,6 +84,9 @@ SIGNATURES = {
     "esep_attn_win_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
                                  _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
                                  _i32, _i32, _f32, _i32, _i32, _vp]),
+    "esep_attn_cache_workspace": (_i64, [_i32] * 8),
+    "esep_attn_cache": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i32] * 7
+                        + [_f32, _i32, _i32, _vp]),
     "esep_rope": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64,
                          _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _f32, _vp]),
 }
@@ -543,6 +546,52 @@ def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scal
             int(max_seqlen), float(scale), int(window), int(sinks), _stream(dev))
     _check(rc, "esep_attn_win_bwd")
     _record(name)
+
+
+def _bth_strides(t, name):
+    """(batch, token, head) strides of a [B, n, H, D] tensor with a dense head dim, as the kernel takes
+    them: multiples of 8 (a dimension of one element has any)."""
+    if t.stride(3) != 1:
+        raise EsepError(f"{name} needs a unit stride on the head dim")
+    return _I64x3(*(s if d > 1 else 0 for s, d in zip(t.stride()[:3], t.shape)))
+
+
+def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None, name="_attn_cache"):
+    """Attention of q [B, n, HQ, D], each row's n newest tokens, over k, v [B, S, HK, D] filled to
+    lengths (int32 [B], the new tokens among them) (esep_attn_cache). o [B, n, HQ, D] dense. `workspace` is
+    a contiguous fp32 tensor of >= attn_cache_workspace's elements (allocated here when not given)."""
+    dev = _dev(q, k, v, o, lengths, workspace)
+    if q.dim() != 4 or k.dim() != 4:
+        raise EsepError("attn_cache: q [B, n, HQ, D] and k, v [B, S, HK, D]")
+    B, n, HQ, D = q.shape
+    S, HK = k.shape[1], k.shape[2]
+    if k.shape != (B, S, HK, D) or v.shape != k.shape or o.shape != q.shape or not o.is_contiguous():
+        raise EsepError("attn_cache: q, o [B, n, HQ, D] (o dense) and k, v [B, S, HK, D]")
+    dt = q.dtype
+    if k.dtype != dt or v.dtype != dt or o.dtype != dt:
+        raise EsepError("q, k, v and o must share one dtype")
+    if lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
+        raise EsepError(f"lengths must be a contiguous int32 tensor of {B} elements")
+    code, w = dtype_code(dt), 0 if window is None else int(window)
+    need = lib().esep_attn_cache_workspace(B, n, S, HQ, HK, D, w, int(sinks))
+    if workspace is None:
+        workspace = torch.empty(max(need, 1), device=dev, dtype=torch.float32)
+    elif (workspace.dtype != torch.float32 or not workspace.is_contiguous()
+          or workspace.numel() < need):
+        raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
+    with _on(dev):
+        rc = lib().esep_attn_cache(
+            _p(q), _bth_strides(q, "q"), _p(k), _bth_strides(k, "k"), _p(v), _bth_strides(v, "v"), _p(o),
+            _p(lengths), _p(workspace), code, B, n, S, HQ, HK, D, float(scale), w, int(sinks),
+            _stream(dev))
+    _check(rc, "esep_attn_cache")
+    _record(name)
+
+
+def attn_cache_workspace(B, n, S, HQ, HK, D, window=None, sinks=0):
+    """Floats of fp32 workspace esep_attn_cache needs for these sizes."""
+    return int(lib().esep_attn_cache_workspace(B, n, S, HQ, HK, D, 0 if window is None else int(window),
+                                               int(sinks)))
 
 
 def _flat(t, name):

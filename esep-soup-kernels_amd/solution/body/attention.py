@@ -111,3 +111,40 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
         if window < max_seqlen:
             return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
     return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))
+
+
+def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks=0):
+    """Attention of each row's newest tokens over its cache: decoding (one new token a row), or a few new
+    tokens at once. q [B, n, HQ, D] (or [B, HQ, D]: n = 1), the queries of the n newest tokens; k_cache, v_cache
+    [B, S, HK, D] views of any batch, token and head strides (HF's [B, HK, S, D] cache transposed, say)
+    in which the new tokens are stored already; lengths int32 [B] on the same device: the tokens in each
+    row's cache, the new ones the last of them. Query head h reads kv head h // (HQ // HK). fp16 and bf16, D
+    in {64, 128}.
+
+    Query t of a row sits at position p = lengths - n + t and sees key j <= p, through a window only if p - j <
+    window or j < sinks, as in varlen_attention. What a cache holds past a row's length is never read; a query
+    at a position below 0 (a row shorter than n) gets 0. Lengths past S count as S.
+
+    For answering only: there is no gradient, so inputs that record one are refused in grad mode. The
+    scratch memory is of the caller's stream and, under capture, of the graph. Returns o, of q's shape and
+    dtype, dense."""
+    if any(t.requires_grad for t in (q, k_cache, v_cache)) and torch.is_grad_enabled():
+        raise _hip.EsepError("cache_attention has no gradient: call it under torch.no_grad(), or on "
+                             "detached tensors (varlen_attention is the form for training)")
+    sinks = _whole("sinks", sinks, 0)
+    if window is not None:
+        window = _whole("window", window, 1)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    q4 = q.unsqueeze(1) if q.dim() == 3 else q
+    if q4.dim() == 4 and _unaligned(q4):
+        q4 = q4.contiguous()
+    o = torch.empty(q4.shape, device=q.device, dtype=q.dtype)
+    _hip.attn_cache(q4, k_cache, v_cache, o, lengths, scale, window, sinks)
+    return o.squeeze(1) if q.dim() == 3 else o
+
+
+def _unaligned(q):
+    """The kernel reads q in 16-byte pieces."""
+    st = q.stride()
+    return st[3] != 1 or q.data_ptr() % 16 != 0 or any(s % 8 for s in st[:3])

@@ -300,6 +300,28 @@ int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
                       int window, int sinks, void* stream);
 
 /*
+ * Attention of each row's n newest tokens over its cache (decoding: n = 1), fp16 or bf16, D in {64, 128}. No
+ * reference counterpart (the reference trains; calls with a cache run the original forward,
+ * solution/body/packed.py:736-771).
+ *   q [B, n, HQ, D], k, v [B, S, HK, D]   strides of batch row, token and head (int64 [3], elements,
+ *                                         multiples of 8, token strides of k and v at most 2^22)
+ *   o [B, n, HQ, D]                       dense
+ *   lengths int32 [B]                     tokens in each row's cache, its n new ones (whose k and v are
+ *                                         stored already) the last of them; clamped into [0, S]
+ *   window (0: none), sinks               query t, at position p = lengths - n + t, sees key j <= p if p - j <
+ *                                         window or j < sinks
+ * Nothing is read past a row's length, nor between its sinks and what its first query sees. o is 0 for a query
+ * at a position below 0 (a row shorter than n). workspace: fp32, 16-byte aligned,
+ * esep_attn_cache_workspace floats (a function of the sizes). Deterministic (no atomics). B * HQ * n < 2^24,
+ * S <= 2^30.
+ */
+int64_t esep_attn_cache_workspace(int B, int n, int S, int HQ, int HK, int D, int window, int sinks);
+int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                    const void* v, const int64_t* v_strides, void* o, const int32_t* lengths,
+                    float* workspace, int dt, int B, int n, int S, int HQ, int HK, int D, float scale,
+                    int window, int sinks, void* stream);
+
+/*
  * SwiGLU of the Qwen2 MLP, element-wise over n elements of one dtype (fp32 / fp16 / bf16),
  * contiguous, 16-byte aligned. Replaces the example kernels the reference decoder calls,
  * solution/swiglu.py:15-37 (example_swiglu_fwd_kernel / example_swiglu_bwd_kernel, launched at
