@@ -1123,6 +1123,52 @@ int esep_nf4_dequant_multi(const esep_nf4_weight* weights, int n_weights, int ou
   return e == hipSuccess ? 0 : hip_fail(e, "nf4_dequant_multi launch");
 }
 
+static_assert(ESEP_NF4_MATVEC_ROWS == esep::kNf4MvRows, "row limit of the ABI and the kernel");
+
+int esep_nf4_matvec(const esep_nf4_matvec_weight* weights, int n_weights, const void* x, int64_t ldx,
+                    void* y, int64_t ldy, int64_t M, int64_t K, int dt, void* stream) {
+  g_err[0] = 0;
+  if (dt != ESEP_F16 && dt != ESEP_BF16)
+    return fail(ESEP_EINVAL, "nf4_matvec: dtype %d is not fp16 / bf16", dt);
+  if (weights == nullptr || n_weights < 1 || n_weights > ESEP_NF4_MULTI_MAX)
+    return fail(ESEP_EINVAL, "nf4_matvec: need 1..%d weights (got %d)", ESEP_NF4_MULTI_MAX, n_weights);
+  if (M < 0 || M > ESEP_NF4_MATVEC_ROWS)
+    return fail(ESEP_ESHAPE, "nf4_matvec: M=%lld outside [0, %d]", (long long)M, ESEP_NF4_MATVEC_ROWS);
+  if (K < 1 || K > (int64_t{1} << 24))
+    return fail(ESEP_ESHAPE, "nf4_matvec: K=%lld outside [1, 2^24]", (long long)K);
+  esep::Nf4MvArgs a{};
+  int64_t cols = 0;
+  for (int i = 0; i < n_weights; ++i) {
+    const esep_nf4_matvec_weight& w = weights[i];
+    if (w.N < 0 || w.N > (int64_t{1} << 24) || w.N * K % 64 != 0)
+      return fail(ESEP_ESHAPE, "nf4_matvec: weight %d: N=%lld outside [0, 2^24], or N * K no multiple of 64",
+                  i, (long long)w.N);
+    if (w.packed == nullptr || w.absmax == nullptr || w.absmax2 == nullptr || w.code2 == nullptr ||
+        w.offset == nullptr || w.nf4 == nullptr)
+      return fail(ESEP_EINVAL, "nf4_matvec: weight %d: every pointer but the bias is required", i);
+    if (w.N == 0) continue;
+    a.w[a.n++] = esep::Nf4MvWeight{w.packed, w.absmax, w.absmax2, w.code2, w.offset, w.nf4,
+                                   w.bias,   (int)w.N, (int)cols, 0};
+    cols += w.N;
+  }
+  if (cols > (int64_t{1} << 25)) return fail(ESEP_ESHAPE, "nf4_matvec: more than 2^25 outputs in all");
+  if (ldx < K || ldy < cols)
+    return fail(ESEP_ESHAPE, "nf4_matvec: row strides ldx=%lld ldy=%lld below K=%lld or the %lld outputs",
+                (long long)ldx, (long long)ldy, (long long)K, (long long)cols);
+  if (M == 0 || cols == 0) return 0;
+  if (x == nullptr || y == nullptr) return fail(ESEP_EINVAL, "nf4_matvec: x and y are required");
+  a.x = x;
+  a.y = y;
+  a.ldx = ldx;
+  a.ldy = ldy;
+  a.M = (int)M;
+  a.K = (int)K;
+  bool sup = false;
+  const hipError_t e = esep::launch_nf4_matvec(a, dt, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "nf4_matvec: unsupported dtype");
+  return e == hipSuccess ? 0 : hip_fail(e, "nf4_matvec launch");
+}
+
 namespace {
 int head_rows(void* z, int64_t ld, const int64_t* target, const float* cew, const int32_t* perm,
               float* lse, float* tlogit, float* ce, float* ent, int32_t* amax, int64_t* amax64,

@@ -30,4 +30,31 @@ struct Nf4Multi {
 
 hipError_t launch_nf4_dequant(const Nf4Multi& m, int out_dt, hipStream_t s, bool* supported);
 
+// Products of up to kNf4MvRows rows x [M, K] with NF4 weights [N, K] that follow each other in the columns
+// of y (nf4_matvec.hip).
+constexpr int kNf4MvRows = 16;
+struct Nf4MvWeight {
+  const void* packed;
+  const uint8_t* absmax;
+  const float* absmax2;
+  const float* code2;
+  const float* offset;
+  const float* nf4;
+  const void* bias;  // [N] of x's type, or null
+  int N;
+  int col0;    // its first column of y
+  int group0;  // its first group of tiles (the launcher's)
+};
+struct Nf4MvArgs {
+  Nf4MvWeight w[kNf4MultiMax];
+  int n;
+  int groups;
+  const void* x;
+  void* y;
+  int64_t ldx, ldy;
+  int M, K;
+};
+
+hipError_t launch_nf4_matvec(const Nf4MvArgs& a, int dt, hipStream_t s, bool* supported);
+
 }  // namespace esep

@@ -87,6 +87,7 @@ SIGNATURES = {
     "esep_attn_cache_workspace": (_i64, [_i32] * 8),
     "esep_attn_cache": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i32] * 7
                         + [_f32, _i32, _i32, _vp]),
+    "esep_nf4_matvec": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
     "esep_rope": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64,
                          _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _f32, _vp]),
 }
@@ -869,6 +870,53 @@ def nf4_dequant_multi(items, name="_nf4_dequant_multi"):
     rc = lib().esep_nf4_dequant_multi(ctypes.cast(arr, _vp), len(items), dtype_code(dts.pop()),
                                       _stream(dev))
     _check(rc, "esep_nf4_dequant_multi")
+    _record(name)
+
+
+class Nf4MatvecWeight(ctypes.Structure):
+    """esep_nf4_matvec_weight (include/esep_body.h)."""
+    _fields_ = [("packed", _vp), ("absmax", _vp), ("absmax2", _vp), ("code2", _vp),
+                ("offset", _vp), ("nf4", _vp), ("bias", _vp), ("N", _i64)]
+
+
+NF4_MATVEC_ROWS = 16
+
+
+def nf4_matvec(x, items, y, name="_nf4_matvec"):
+    """y [M, sum N] = x [M, K] W_i^T (+ bias_i) side by side for NF4 weights (esep_nf4_matvec), M up to
+    NF4_MATVEC_ROWS. x and y fp16 or bf16 with unit column strides; items: (packed, absmax, absmax2,
+    code2, offset, nf4, bias or None, N) tuples, the tables as for nf4_dequant, bias [N] of x's dtype."""
+    if not 1 <= len(items) <= NF4_MULTI_MAX:
+        raise EsepError(f"1..{NF4_MULTI_MAX} weights per launch")
+    dev = _dev(x, y, *[t for it in items for t in it[:7]])
+    M, K = x.shape
+    arr = (Nf4MatvecWeight * len(items))()
+    cols = 0
+    for i, (packed, absmax, absmax2, code2, offset, nf4, bias, n) in enumerate(items):
+        nb = absmax.numel()
+        if (packed.dtype != torch.uint8 or packed.numel() != nb * 32 or absmax.dtype != torch.uint8
+                or nb * 64 != n * K):
+            raise EsepError("packed must hold n_blocks * 32 uint8, absmax n_blocks uint8 and n_blocks * 64 "
+                            "be the weight's size")
+        for t in (absmax2, code2, offset, nf4):
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                raise EsepError("absmax2, code2, offset and nf4 must be contiguous fp32 tensors")
+        if (absmax2.numel() < (nb + 255) // 256 or code2.numel() < 256 or nf4.numel() < 16
+                or offset.numel() < 1):
+            raise EsepError("nf4 tables too small")
+        if not (packed.is_contiguous() and absmax.is_contiguous()):
+            raise EsepError("packed and absmax must be contiguous")
+        if bias is not None and (bias.dtype != x.dtype or bias.numel() != n or not bias.is_contiguous()):
+            raise EsepError("bias must be a contiguous [N] tensor of x's dtype")
+        arr[i] = Nf4MatvecWeight(packed.data_ptr(), absmax.data_ptr(), absmax2.data_ptr(),
+                                 code2.data_ptr(), offset.data_ptr(), nf4.data_ptr(), _p(bias), n)
+        cols += n
+    if tuple(y.shape) != (M, cols) or y.dtype != x.dtype:
+        raise EsepError(f"y must be a [{M}, {cols}] tensor of x's dtype")
+    with _on(dev):
+        rc = lib().esep_nf4_matvec(ctypes.addressof(arr), len(items), _p(x), _rows_ld(x, K), _p(y),
+                                   _rows_ld(y, cols), M, K, dtype_code(x.dtype), _stream(dev))
+    _check(rc, "esep_nf4_matvec")
     _record(name)
 
 

@@ -3,6 +3,8 @@ reference's solution/nf4 API with the Triton dequant replaced by esep_nf4_dequan
 
   supported, dequantize_nf4, dequantize_nf4_multi   the dequantization (reference dequant.py)
   NF4Linear, nf4_linear, NF4MultiLinear             the autograd linears (reference autograd.py)
+  nf4_matvec, nf4_matvec_multi                      products of a few rows (decoding) with weights that
+                                                    are decoded in registers
   linear4bit, linear4bit_multi, dequant_multi       bitsandbytes Linear4bit.forward semantics on
                                                     the kernels, for one module or 2-8 modules
                                                     reading the same input (reference
@@ -27,7 +29,8 @@ from ..body import _hip
 
 __all__ = ["patch", "linear4bit", "linear4bit_multi", "dequant_multi", "is_linear4bit",
            "supported", "dequantize_nf4", "dequantize_nf4_multi", "nf4_linear", "NF4Linear",
-           "NF4MultiLinear", "MIN_ROWS", "MULTI_MAX"]
+           "NF4MultiLinear", "nf4_matvec", "nf4_matvec_multi", "NF4Matvec", "MIN_ROWS", "MULTI_MAX",
+           "MATVEC_ROWS"]
 
 
 def supported(quant_state) -> bool:
@@ -120,7 +123,8 @@ class NF4Linear(torch.autograd.Function):
 
 
 def nf4_linear(x, packed, bias, quant_state):
-    """x (any leading dims) -> x W^T + bias for an NF4 weight (reference autograd.py:51-53)."""
+    """x (any leading dims) -> x W^T + bias for an NF4 weight (reference autograd.py:51-53). For a few rows
+    (decoding) see nf4_matvec."""
     return NF4Linear.apply(x, packed, bias, quant_state)
 
 
@@ -147,6 +151,82 @@ class NF4MultiLinear(torch.autograd.Function):
             w = dequantize_nf4_multi(weights, states)
             dx = _hip.matmul(dy if dy.dtype == w.dtype else dy.to(w.dtype), w)
         return dx, dbias, None
+
+
+# Rows that nf4_matvec takes.
+MATVEC_ROWS = _hip.NF4_MATVEC_ROWS
+
+
+def _matvec(x, weights, states, biases):
+    items = []
+    for w, qs, b in zip(weights, states, biases):
+        qs2, dt = qs.state2, x.dtype
+        if b is not None:
+            b = (b if b.dtype == dt else b.to(dt)).contiguous()
+        items.append((w.contiguous(), qs.absmax.contiguous(), _f32(qs2.absmax), _f32(qs2.code),
+                      _offset(qs), _f32(qs.code), b, qs.shape[0]))
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.shape[1] > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    n = sum(it[7] for it in items)
+    y = torch.empty((x2.shape[0], n), device=x.device, dtype=x.dtype)
+    _hip.nf4_matvec(x2, items, y)
+    return y.view(*x.shape[:-1], n)
+
+
+class NF4Matvec(torch.autograd.Function):
+    """nf4_matvec_multi where torch records it: apply(x, weights, states, *biases). The backward is
+    NF4MultiLinear's (W decoded for one dX product; each bias gets the sum of its columns of dy)."""
+
+    @staticmethod
+    def forward(ctx, x, weights, states, *biases):
+        w_dtype = x.dtype if x.dtype != torch.float32 else torch.float16
+        ctx.weights, ctx.states, ctx.x_dtype, ctx.w_dtype = weights, states, x.dtype, w_dtype
+        ctx.bias_dtypes = [None if b is None else b.dtype for b in biases]
+        return _matvec(x if x.dtype == w_dtype else x.to(w_dtype), weights, states, biases)
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx, dbias, c = None, [], 0
+        for i, qs in enumerate(ctx.states):
+            n = qs.shape[0]
+            dbias.append(dy[..., c:c + n].reshape(-1, n).sum(0, dtype=ctx.bias_dtypes[i])
+                         if ctx.needs_input_grad[3 + i] else None)
+            c += n
+        if ctx.needs_input_grad[0]:
+            w = dequantize_nf4_multi(ctx.weights, ctx.states, dtype=ctx.w_dtype)
+            dx = _hip.matmul(dy.to(ctx.w_dtype), w).to(ctx.x_dtype)
+        return dx, None, None, *dbias
+
+
+def nf4_matvec_multi(x, weights, quant_states, biases=None):
+    """cat([x W_i^T + bias_i ...], -1) for up to MATVEC_ROWS rows x (any leading dims) and up to MULTI_MAX NF4
+    weights of one K, in one launch that decodes them in registers: q / k / v, or gate / up, of tokens being
+    decoded. x and the outputs in x's 16-bit dtype (an fp32 x computes and returns fp16, as nf4_linear's);
+    biases: None, or a list of tensors or None. The codes are rounded to that dtype, products, scales and
+    sums are fp32, the output is rounded once. Differentiable (x and the biases) as nf4_linear is.
+    Caller guarantees supported(quant_state) of each."""
+    weights, states = list(weights), list(quant_states)
+    biases = [None] * len(weights) if biases is None else list(biases)
+    if not 1 <= len(weights) <= MULTI_MAX or not len(weights) == len(states) == len(biases):
+        raise _hip.EsepError(f"nf4_matvec takes 1 to {MULTI_MAX} weights, a quant state and a bias or None each")
+    K = x.shape[-1]
+    if any(len(qs.shape) != 2 or qs.shape[1] != K for qs in states):
+        raise _hip.EsepError(f"nf4_matvec: x of {K} columns against weights {[tuple(q.shape) for q in states]}")
+    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise _hip.EsepError(f"nf4_matvec: x {x.dtype}")
+    if K == 0 or x.numel() > MATVEC_ROWS * K:
+        raise _hip.EsepError(f"nf4_matvec takes up to {MATVEC_ROWS} rows, got x {tuple(x.shape)}; "
+                             "nf4_linear is the form for more")
+    if _hip.recorded(x, *biases):
+        return NF4Matvec.apply(x, weights, states, *biases)
+    return _matvec(x.to(torch.float16) if x.dtype is torch.float32 else x, weights, states, biases)
+
+
+def nf4_matvec(x, packed, bias, quant_state):
+    """nf4_linear(x, packed, bias, quant_state) for up to MATVEC_ROWS rows: W is decoded in registers, not
+    written out and read back (see nf4_matvec_multi)."""
+    return nf4_matvec_multi(x, [packed], [quant_state], [bias])
 
 
 # ----------------------------------------------------------------------------------------------

@@ -439,6 +439,32 @@ typedef struct {
 int esep_nf4_dequant_multi(const esep_nf4_weight* weights, int n_weights, int out_dt, void* stream);
 
 /*
+ * Products of a few rows with NF4 weights that are never written out: y[m, n] = sum_k x[m, k] W[n, k] (+
+ * bias[n]), fp16 or bf16 (dt), for decoding. The reference leaves fewer than 8 rows to bitsandbytes' own kernels
+ * (solution/nf4/__init__.py:80-118). `weights` is a host array of 1 .. ESEP_NF4_MULTI_MAX entries, copied into the
+ * launch; their outputs follow each other in y's columns.
+ *   x [M, K], y [M, sum N]    unit column strides, row strides ldx, ldy; M <= ESEP_NF4_MATVEC_ROWS
+ *   weights[i]                W [N, K] packed as for esep_nf4_dequant, N * K a multiple of 64; bias [N] of dt or
+ *                             NULL
+ * The codes are rounded to dt, scales, products and sums are fp32, y is rounded once. K a multiple of 64 with
+ * 16-byte aligned x, packed and x rows takes the matrix cores; anything else an element-wise kernel.
+ * Deterministic (no atomics).
+ */
+#define ESEP_NF4_MATVEC_ROWS 16
+typedef struct {
+  const void* packed;
+  const uint8_t* absmax;
+  const float* absmax2;
+  const float* code2;
+  const float* offset;
+  const float* nf4;
+  const void* bias;
+  int64_t N;
+} esep_nf4_matvec_weight;
+int esep_nf4_matvec(const esep_nf4_matvec_weight* weights, int n_weights, const void* x, int64_t ldx,
+                    void* y, int64_t ldy, int64_t M, int64_t K, int dt, void* stream);
+
+/*
  * Fused LM head: softmax statistics and dlogits of one logits chunk. Replaces the reference's
  * Triton launch at solution/head/op.py:79-84 (_run; kernel head_row_softmax_kernel,
  * solution/head/kernels.py:37-93). For each row r of z ([rows, V] of dt, row stride ld):
