@@ -43,12 +43,12 @@ struct Nf4MvWeight {
   const void* bias;  // [N] of x's type, or null
   int N;
   int col0;    // its first column of y
-  int group0;  // its first group of tiles (the launcher's)
+  int block0;  // its first block (the launcher's)
 };
 struct Nf4MvArgs {
   Nf4MvWeight w[kNf4MultiMax];
   int n;
-  int groups;
+  int per_block;  // tiles of 16 rows (the launcher's)
   const void* x;
   void* y;
   int64_t ldx, ldy;

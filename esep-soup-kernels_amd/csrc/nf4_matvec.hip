@@ -15,8 +15,9 @@
 // The codes are rounded to x's type (fp16 2^-12, bf16 2^-9 relative at most on average half of that), as
 // dequantize_nf4 rounds the whole weight to it; scales, products and sums stay in fp32.
 //
-// A wavefront takes 16 rows of W and a share of k (KS shares, added through LDS in their order); blocks of 8
-// wavefronts walk groups of 8 / KS tiles.
+// A block takes a run of tiles of 16 W rows; the tiles' 128-k steps, laid end to end, are cut into equal runs,
+// one to each of its 16 wavefronts, which streams its run four steps ahead with no barrier; parts of a tile
+// meet in LDS at the end and are added in the wavefronts' order. x lies in LDS where it fits.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -27,7 +28,8 @@
 namespace esep {
 namespace {
 
-constexpr int kMvThreads = 512, kMvWaves = 8;
+constexpr int kMvThreads = 1024, kMvWaves = 16;
+constexpr int kMvTiles = 16;  // tiles of a block at most
 
 template <typename T>
 struct Mv;
@@ -59,147 +61,166 @@ __device__ __forceinline__ uint32_t mv_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
-// What a wavefront needs of 128 k: 16 bytes of its lane's row, x, the block's scale.
-template <int MT>
+// What a wavefront needs of 128 k of W: 16 bytes of its lane's row and its block's scale.
 struct MvStage {
   uint4 w;
-  uint4 x[MT][4];
   uint8_t am;
   float a2;
 };
 
-template <typename T, int MT, int KS>
-__global__ __launch_bounds__(kMvThreads, MT == 1 ? 4 : 2) void k_nf4_matvec(const Nf4MvArgs a) {
-  constexpr int TPB = kMvWaves / KS;
+// x in LDS (XL): rows of K + 8 elements, so that the 8 rows that a read touches lie in different banks.
+constexpr int kMvXBytes = 80 * 1024;
+inline bool mv_x_fits(int M, int K) { return (int64_t)M * (K + 8) * 2 <= kMvXBytes; }
+
+template <typename T, int MT, bool XL>
+__global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a) {
   using V8 = typename Mv<T>::v8;
   __shared__ __align__(16) uint32_t tab[256 * 32];
   __shared__ float code2[256];
-  __shared__ float red[KS > 1 ? 2 : 1][KS > 1 ? kMvWaves : 1][MT * 8][16];
+  __shared__ float red[kMvWaves + kMvTiles - 1][MT * 8][16];  // a wavefront's part of a tile: [both numbers' sum]
+  __shared__ __align__(16) char xs[XL ? kMvXBytes : 16];      // [M][K + 8]
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ks = wave % KS, ti = wave / KS;
   const int lq = lane & 15, q = lane >> 4;
   const int KB = a.K / 64, steps = (KB + 1) / 2;
-  const int s0 = steps * ks / KS, s1 = steps * (ks + 1) / KS;
-  // x: this lane's row of each 8, read only against its own block's lanes
-  const bool mine = (q >> 1) == (lq >> 3);
-  const T* xp[MT];
+  int wi = 0;
+  while (wi + 1 < a.n && (int)blockIdx.x >= a.w[wi + 1].block0) ++wi;
+  const Nf4MvWeight& w = a.w[wi];
+  const int all = (w.N + 15) / 16, tile0 = ((int)blockIdx.x - w.block0) * a.per_block;
+  const int tiles = all - tile0 < a.per_block ? all - tile0 : a.per_block;
+  const int total = tiles * steps;
+  const int waves = total < kMvWaves ? total : kMvWaves;  // each has a step or more
+  const int u0 = wave < waves ? wave * total / waves : 0;
+  const int u1 = wave < waves ? (wave + 1) * total / waves : 0;
+
+  // the load cursor: step ls of tile lt, this lane's W row in it
+  const char* wp;
+  const uint8_t* ap;
+  int64_t f0;
+  auto seek = [&](int lt) {
+    const int row = (tile0 + lt) * 16 + lq, rc = row < w.N ? row : w.N - 1;
+    wp = static_cast<const char*>(w.packed) + (int64_t)rc * KB * 32 + 16 * q;
+    f0 = (int64_t)rc * KB + (lane >> 5);
+    ap = w.absmax + f0;
+  };
+  int lt = u0 / steps, ls = u0 % steps, lu = u0;
+  seek(lt);
+  auto load = [&](MvStage& st) {
+    if (lu >= u1) return;
+    const bool ok = 2 * ls + (q >> 1) < KB;
+    st.w = ok ? *reinterpret_cast<const uint4*>(wp + 64 * ls) : make_uint4(0, 0, 0, 0);
+    st.am = ok ? ap[2 * ls] : 0;
+    st.a2 = ok ? w.absmax2[(f0 + 2 * ls) >> 8] : 0.f;
+    ++lu;
+    if (++ls == steps) {
+      ls = 0;
+      seek(++lt);
+    }
+  };
+  constexpr int DEPTH = 4;
+  MvStage st[DEPTH];
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-    xp[t] = static_cast<const T*>(a.x) + (int64_t)(8 * t + (lq & 7)) * a.ldx + 32 * q;
+  for (int d = 0; d < DEPTH; ++d) load(st[d]);
+
+  // the tables and x, while the first bytes of W are on their way
+  const float off = *w.offset;
+  {
+    const float code = w.nf4[lane & 15];
+    for (int i = tid; i < 256 * 8; i += kMvThreads) {
+      const int e = i / 8;
+      const uint32_t p = mv_pair<T>(__shfl(code, e >> 4), __shfl(code, e & 15));
+      reinterpret_cast<uint4*>(tab)[i] = make_uint4(p, p, p, p);
+    }
+    if (tid < 256) code2[tid] = w.code2[tid];
+    if constexpr (XL) {
+      const int chunks = a.K / 8;
+      for (int i = tid; i < a.M * chunks; i += kMvThreads) {
+        const int m = i / chunks, c = i % chunks;
+        *reinterpret_cast<uint4*>(xs + ((int64_t)m * (a.K + 8) + 8 * c) * 2) =
+            *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 8 * c);
+      }
+    }
+  }
+  __syncthreads();
+
+  // x: this lane's row of each 8, against its own block's lanes only
+  const bool mine = (q >> 1) == (lq >> 3);
+  const char* xp[MT];
+  bool have[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int m = 8 * t + (lq & 7);
+    have[t] = mine && m < a.M;
+    xp[t] = XL ? xs + ((int64_t)m * (a.K + 8) + 32 * q) * 2
+               : reinterpret_cast<const char*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 32 * q);
+  }
   const uint32_t copy = 4 * (lane & 31);
   const char* tabb = reinterpret_cast<const char*>(tab);
-
-  int cur = -1, buf = 0;
-  float off = 0.f;
-  for (int grp = blockIdx.x; grp < a.groups; grp += gridDim.x) {
-    int wi = 0;
-    while (wi + 1 < a.n && grp >= a.w[wi + 1].group0) ++wi;
-    const Nf4MvWeight& w = a.w[wi];
-    const int row = ((grp - w.group0) * TPB + ti) * 16 + lq;
-    const int rc = row < w.N ? row : w.N - 1;
-    const char* wp = static_cast<const char*>(w.packed) + (int64_t)rc * KB * 32 + 16 * q;
-    const int64_t f0 = (int64_t)rc * KB + (lane >> 5);
-
-    auto load = [&](MvStage<MT>& st, int s) {
-      const bool ok = 2 * s + (q >> 1) < KB;
-      st.w = ok ? *reinterpret_cast<const uint4*>(wp + 64 * (int64_t)s) : make_uint4(0, 0, 0, 0);
-      st.am = ok ? w.absmax[f0 + 2 * s] : 0;
-      st.a2 = ok ? w.absmax2[(f0 + 2 * s) >> 8] : 0.f;
+  f32x4 tot[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) tot[t] = f32x4{};
+  int ct = u0 / steps, cs = u0 % steps;  // the compute cursor
+  auto comp = [&](const MvStage& st, int u) {
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{};
+    const bool ok = 2 * cs + (q >> 1) < KB;
+    const uint32_t wd[4] = {st.w.x, st.w.y, st.w.z, st.w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 b;
+      b.x = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] << 7) & 0x7f80u) | copy));
+      b.y = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 1) & 0x7f80u) | copy));
+      b.z = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 9) & 0x7f80u) | copy));
+      b.w = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 17) & 0x7f80u) | copy));
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const bool in = ok && mine && 8 * t + (lq & 7) < a.M;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          st.x[t][i] = in ? *reinterpret_cast<const uint4*>(xp[t] + 128 * s + 8 * i)
-                          : make_uint4(0, 0, 0, 0);
-      }
-    };
-    f32x4 tot[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) tot[t] = f32x4{};
-    MvStage<MT> st[2];
-    if (s0 < s1) load(st[0], s0);
-    if (s0 + 1 < s1) load(st[1], s0 + 1);
-
-    if (wi != cur) {  // the weight's tables, while its first bytes are on their way
-      if (cur >= 0) __syncthreads();
-      cur = wi;
-      off = *w.offset;
-      const float code = w.nf4[lane & 15];
-      for (int i = tid; i < 256 * 8; i += kMvThreads) {
-        const int e = i / 8;
-        const uint32_t p = mv_pair<T>(__shfl(code, e >> 4), __shfl(code, e & 15));
-        reinterpret_cast<uint4*>(tab)[i] = make_uint4(p, p, p, p);
-      }
-      if (tid < 256) code2[tid] = w.code2[tid];
-      __syncthreads();
-    }
-
-    auto comp = [&](const MvStage<MT>& st, int s) {
-      f32x4 acc[MT];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] = f32x4{};
-      const uint32_t wd[4] = {st.w.x, st.w.y, st.w.z, st.w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint4 b;
-        b.x = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] << 7) & 0x7f80u) | copy));
-        b.y = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 1) & 0x7f80u) | copy));
-        b.z = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 9) & 0x7f80u) | copy));
-        b.w = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 17) & 0x7f80u) | copy));
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          acc[t] = Mv<T>::run(__builtin_bit_cast(V8, st.x[t][i]), __builtin_bit_cast(V8, b), acc[t]);
-      }
-      const bool ok = 2 * s + (q >> 1) < KB;
-      const float sc = ok ? mv_scale(code2[st.am], st.a2, off) : 0.f;
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tot[t][r] = fmaf(sc, acc[t][r], tot[t][r]);
-    };
-    for (int s = s0; s < s1; s += 2) {
-      comp(st[0], s);
-      if (s + 2 < s1) load(st[0], s + 2);
-      if (s + 1 < s1) {
-        comp(st[1], s + 1);
-        if (s + 3 < s1) load(st[1], s + 3);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (have[t] && ok) x = *reinterpret_cast<const uint4*>(xp[t] + 256 * cs + 16 * i);
+        acc[t] = Mv<T>::run(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, b), acc[t]);
       }
     }
-    // the two blocks' sums: lanes 0 .. 31 get x rows 4 q + r of their W row
+    const float sc = ok ? mv_scale(code2[st.am], st.a2, off) : 0.f;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tot[t][r] += __shfl_xor(tot[t][r], 32);
-    auto store = [&](int m, int n, float v) {
-      if (m >= a.M || n >= w.N) return;
-      if (w.bias != nullptr) v += (float)static_cast<const T*>(w.bias)[n];
-      static_cast<T*>(a.y)[(int64_t)m * a.ldy + w.col0 + n] = (T)v;
-    };
-    if constexpr (KS == 1) {
-      if (lane < 32)
+      for (int r = 0; r < 4; ++r) tot[t][r] = fmaf(sc, acc[t][r], tot[t][r]);
+    if (++cs == steps || u + 1 == u1) {
+      // the two blocks' sums: lanes 0 .. 31 hold x rows 4 q + r of their W row
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) store(8 * t + 4 * q + r, row, tot[t][r]);
-    } else {
-      if (lane < 32)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) red[buf][wave][8 * t + 4 * q + r][lq] = tot[t][r];
-      __syncthreads();
-      for (int i = tid; i < TPB * MT * 128; i += kMvThreads) {
-        const int n = i & 15, m = i / 16 % (MT * 8), tile = i / (MT * 128);
-        float v = red[buf][tile * KS][m][n];
-#pragma unroll
-        for (int j = 1; j < KS; ++j) v += red[buf][tile * KS + j][m][n];
-        store(m, ((grp - w.group0) * TPB + tile) * 16 + n, v);
-      }
-      buf ^= 1;  // the next group's barrier comes before this buffer is written again
+        for (int r = 0; r < 4; ++r) {
+          const float v = tot[t][r] + __shfl_xor(tot[t][r], 32);
+          if (lane < 32) red[wave + ct][8 * t + 4 * q + r][lq] = v;
+          tot[t][r] = 0.f;
+        }
+      cs = 0;
+      ++ct;
     }
+  };
+  for (int u = u0; u < u1; u += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (u + d < u1) {
+        comp(st[d], u + d);
+        load(st[d]);
+      }
+    }
+  }
+  __syncthreads();
+  // a tile's parts, one of each wavefront that walked some of it, in their order
+  for (int i = tid; i < tiles * MT * 128; i += kMvThreads) {
+    const int c = i & 15, m = i / 16 % (MT * 8), t = i / (MT * 128);
+    const int n = (tile0 + t) * 16 + c;
+    if (m >= a.M || n >= w.N) continue;
+    const int first = ((t * steps + 1) * waves - 1) / total;
+    const int last = ((t + 1) * steps * waves - 1) / total;
+    float v = red[first + t][m][c];
+    for (int j = first + 1; j <= last; ++j) v += red[j + t][m][c];
+    if (w.bias != nullptr) v += (float)static_cast<const T*>(w.bias)[n];
+    static_cast<T*>(a.y)[(int64_t)m * a.ldy + w.col0 + n] = (T)v;
   }
 }
 
@@ -238,43 +259,38 @@ __global__ __launch_bounds__(256) void k_nf4_matvec_any(const Nf4MvArgs a) {
   }
 }
 
-template <typename T, int MT, int KS>
-void run(Nf4MvArgs& a, hipStream_t s) {
-  constexpr int TPB = kMvWaves / KS;
-  a.groups = 0;
-  for (int i = 0; i < a.n; ++i) {
-    a.w[i].group0 = a.groups;
-    a.groups += ((a.w[i].N + 15) / 16 + TPB - 1) / TPB;  // a group's tiles are of one weight
+template <typename T, int MT, bool XL>
+hipError_t run(Nf4MvArgs& a, hipStream_t s) {
+  // the fewest tiles to a block that one block to a CU holds, up to kMvTiles
+  int blocks = 0;
+  for (a.per_block = 1;; ++a.per_block) {
+    blocks = 0;
+    for (int i = 0; i < a.n; ++i) {
+      a.w[i].block0 = blocks;
+      blocks += ((a.w[i].N + 15) / 16 + a.per_block - 1) / a.per_block;
+    }
+    if (blocks <= 256 || a.per_block == kMvTiles) break;
   }
-  const int blocks = a.groups < 512 ? a.groups : 512;
-  hipLaunchKernelGGL((k_nf4_matvec<T, MT, KS>), dim3((unsigned)blocks), dim3(kMvThreads), 0, s, a);
+  hipLaunchKernelGGL((k_nf4_matvec<T, MT, XL>), dim3((unsigned)blocks), dim3(kMvThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 template <typename T, int MT>
-void run_ks(Nf4MvArgs& a, int64_t tiles, hipStream_t s) {
-  int ks = 1;
-  while (ks < 8 && tiles * ks < 2048) ks *= 2;
-  if (ks == 1) return run<T, MT, 1>(a, s);
-  if (ks == 2) return run<T, MT, 2>(a, s);
-  if (ks == 4) return run<T, MT, 4>(a, s);
-  run<T, MT, 8>(a, s);
+hipError_t run_x(Nf4MvArgs& a, hipStream_t s) {
+  return mv_x_fits(a.M, a.K) ? run<T, MT, true>(a, s) : run<T, MT, false>(a, s);
 }
 
 template <typename T>
-void run_t(Nf4MvArgs& a, hipStream_t s) {
-  int64_t rows = 0, tiles = 0;
+hipError_t run_t(Nf4MvArgs& a, hipStream_t s) {
+  int64_t rows = 0;
   bool whole = a.K % 64 == 0 && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   for (int i = 0; i < a.n; ++i) {
     rows += a.w[i].N;
-    tiles += (a.w[i].N + 15) / 16;
     whole = whole && (reinterpret_cast<uintptr_t>(a.w[i].packed) & 15) == 0;
   }
-  if (!whole)
-    hipLaunchKernelGGL((k_nf4_matvec_any<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-  else if (a.M <= 8)
-    run_ks<T, 1>(a, tiles, s);
-  else
-    run_ks<T, 2>(a, tiles, s);
+  if (whole) return a.M <= 8 ? run_x<T, 1>(a, s) : run_x<T, 2>(a, s);
+  hipLaunchKernelGGL((k_nf4_matvec_any<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -282,9 +298,9 @@ void run_t(Nf4MvArgs& a, hipStream_t s) {
 hipError_t launch_nf4_matvec(const Nf4MvArgs& args, int dt, hipStream_t s, bool* sup) {
   Nf4MvArgs a = args;
   *sup = dt == 1 || dt == 2;
-  if (dt == 1) run_t<_Float16>(a, s);
-  if (dt == 2) run_t<__bf16>(a, s);
-  return *sup ? hipGetLastError() : hipErrorInvalidValue;
+  if (dt == 1) return run_t<_Float16>(a, s);
+  if (dt == 2) return run_t<__bf16>(a, s);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace esep
