@@ -1140,9 +1140,9 @@ int esep_nf4_matvec(const esep_nf4_matvec_weight* weights, int n_weights, const 
   int64_t cols = 0;
   for (int i = 0; i < n_weights; ++i) {
     const esep_nf4_matvec_weight& w = weights[i];
-    if (w.N < 0 || w.N > (int64_t{1} << 24) || w.N * K % 64 != 0)
-      return fail(ESEP_ESHAPE, "nf4_matvec: weight %d: N=%lld outside [0, 2^24], or N * K no multiple of 64",
-                  i, (long long)w.N);
+    if (w.N < 0 || w.N > (int64_t{1} << 24) || w.N * K % 64 != 0 || w.N * K > (int64_t{1} << 40))
+      return fail(ESEP_ESHAPE, "nf4_matvec: weight %d: N=%lld outside [0, 2^24], or N * K no multiple of 64 "
+                  "up to 2^40", i, (long long)w.N);
     if (w.packed == nullptr || w.absmax == nullptr || w.absmax2 == nullptr || w.code2 == nullptr ||
         w.offset == nullptr || w.nf4 == nullptr)
       return fail(ESEP_EINVAL, "nf4_matvec: weight %d: every pointer but the bias is required", i);

@@ -61,24 +61,41 @@ __device__ __forceinline__ uint32_t mv_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
-// What a wavefront needs of 128 k of W: 16 bytes of its lane's row and its block's scale.
+// A wavefront's loads of one step (128 k): 16 bytes of W a lane, four lanes to the 64 bytes of a row, as memory
+// lies; the products want neighbouring lanes in neighbouring rows, which goes through 1 KiB of LDS of the
+// wavefront's own. x, where it comes from global memory, likewise: 16 lanes to a row.
+template <int XT>
 struct MvStage {
-  uint4 w;
-  uint8_t am;
-  float a2;
+  u32x4 w;
+  u32x4 x[2 * XT];
 };
 
-// x in LDS (XL): rows of K + 8 elements, so that the 8 rows that a read touches lie in different banks.
-constexpr int kMvXBytes = 80 * 1024;
-inline bool mv_x_fits(int M, int K) { return (int64_t)M * (K + 8) * 2 <= kMvXBytes; }
+// x in LDS (XL): rows of whole steps, zeros behind K, and 8 elements more, so that the 8 rows that a
+// read touches lie in different banks; before them 64 bytes of zeros that the lanes without a row read.
+// Otherwise each wavefront writes its step of x there, in the same form.
+constexpr int kMvXBytes = 64 * 1024;
+inline __host__ __device__ int mv_x_row(int K) { return 2 * ((K + 127) / 128 * 128 + 8); }
+inline bool mv_x_fits(int M, int K) { return 64 + (int64_t)M * mv_x_row(K) <= kMvXBytes; }
 
 template <typename T, int MT, bool XL>
 __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a) {
   using V8 = typename Mv<T>::v8;
-  __shared__ __align__(16) uint32_t tab[256 * 32];
-  __shared__ float code2[256];
-  __shared__ float red[kMvWaves + kMvTiles - 1][MT * 8][16];  // a wavefront's part of a tile: [both numbers' sum]
-  __shared__ __align__(16) char xs[XL ? kMvXBytes : 16];      // [M][K + 8]
+  constexpr int XT = XL ? 0 : MT, XW = 8 * MT * 272;  // a wavefront's step of x
+  constexpr int DEPTH = XT == 2 ? 2 : 4;              // steps in flight, and scales at a time
+  using Stage = MvStage<XT>;
+  struct Lds {
+    uint32_t tab[256 * 32];  // first: its entries' addresses are then what v_dot4 gives
+    float code2[256];
+    float red[kMvWaves + kMvTiles - 1][MT * 8][16];  // a wavefront's part of a tile: [both numbers' sum]
+    char ws[kMvWaves][1024];                         // a wavefront's step of W
+    char xs[XL ? kMvXBytes : 64 + kMvWaves * XW];
+  };
+  __shared__ __align__(16) Lds lds;
+  auto& tab = lds.tab;
+  auto& code2 = lds.code2;
+  auto& red = lds.red;
+  auto& ws = lds.ws;
+  auto& xs = lds.xs;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -86,7 +103,7 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
   const int KB = a.K / 64, steps = (KB + 1) / 2;
   int wi = 0;
   while (wi + 1 < a.n && (int)blockIdx.x >= a.w[wi + 1].block0) ++wi;
-  const Nf4MvWeight& w = a.w[wi];
+  const Nf4MvWeight w = a.w[wi];
   const int all = (w.N + 15) / 16, tile0 = ((int)blockIdx.x - w.block0) * a.per_block;
   const int tiles = all - tile0 < a.per_block ? all - tile0 : a.per_block;
   const int total = tiles * steps;
@@ -94,32 +111,63 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
   const int u0 = wave < waves ? wave * total / waves : 0;
   const int u1 = wave < waves ? (wave + 1) * total / waves : 0;
 
-  // the load cursor: step ls of tile lt, this lane's W row in it
-  const char* wp;
-  const uint8_t* ap;
+  // The load cursor: step ls of tile lt. A tile is read through buffer descriptors that end with the weight
+  // (and 2 GiB on, past every tile), so that rows and blocks behind its end need no branch: they read 0.
+  rsrc_t rw, ra;
+  const rsrc_t r2 = make_rsrc(w.absmax2, (uint32_t)(((int64_t)w.N * KB + 255) / 256 * 4));
+  const uint32_t vw = (uint32_t)(lane >> 2) * KB * 32 + 16 * (lane & 3);
+  const rsrc_t rx = make_rsrc(a.x, XL ? 0 : (uint32_t)(((a.M - 1) * a.ldx + a.K) * 2));
   int64_t f0;
   auto seek = [&](int lt) {
-    const int row = (tile0 + lt) * 16 + lq, rc = row < w.N ? row : w.N - 1;
-    wp = static_cast<const char*>(w.packed) + (int64_t)rc * KB * 32 + 16 * q;
-    f0 = (int64_t)rc * KB + (lane >> 5);
-    ap = w.absmax + f0;
+    const int64_t row = (int64_t)(tile0 + lt) * 16, left = (w.N - row) * KB;
+    rw = make_rsrc(static_cast<const char*>(w.packed) + row * KB * 32,
+                   left < (1 << 26) ? (uint32_t)left * 32 : 0x80000000u);
+    ra = make_rsrc(w.absmax + row * KB, left < (1 << 26) ? (uint32_t)left : 1u << 26);
+    f0 = row * KB;
   };
   int lt = u0 / steps, ls = u0 % steps, lu = u0;
   seek(lt);
-  auto load = [&](MvStage& st) {
-    if (lu >= u1) return;
-    const bool ok = 2 * ls + (q >> 1) < KB;
-    st.w = ok ? *reinterpret_cast<const uint4*>(wp + 64 * ls) : make_uint4(0, 0, 0, 0);
-    st.am = ok ? ap[2 * ls] : 0;
-    st.a2 = ok ? w.absmax2[(f0 + 2 * ls) >> 8] : 0.f;
+  // The scales of the DEPTH steps from (lt, ls) on, two steps to a register: lane l has row l / 2 % 16 of
+  // step l % 2, block l / 32 of it.
+  uint32_t am[DEPTH / 2], a2[DEPTH / 2];
+  bool in[DEPTH / 2];
+  auto load_scales = [&]() {
+#pragma unroll
+    for (int h = 0; h < DEPTH / 2; ++h) {
+      int s = ls + 2 * h + (lane & 1), row = (lane >> 1) & 15;
+      if (s >= steps) {  // in the next tile
+        const int t = steps < DEPTH ? s / steps : 1;
+        s -= t * steps;
+        row += 16 * t;
+      }
+      const int kb = 2 * s + (lane >> 5);
+      const uint32_t f = (uint32_t)row * KB + kb;
+      in[h] = kb < KB && lu < u1;
+      am[h] = __builtin_amdgcn_raw_buffer_load_b8(ra, in[h] ? f : ~0u, 0, 0);
+      a2[h] = __builtin_amdgcn_raw_buffer_load_b32(r2, (uint32_t)((f0 + f) >> 8) * 4, 0, 0);
+    }
+  };
+  // (No load stands under a condition: the compiler would wait for all of them at the next use. Past the
+  // run's end they go past the buffer's and read nothing.)
+  auto load = [&](Stage& st) {
+    st.w = __builtin_amdgcn_raw_buffer_load_b128(rw, lu < u1 ? vw : ~0u, 64 * ls, 0);
+    if constexpr (!XL) {
+#pragma unroll
+      for (int t = 0; t < 2 * MT; ++t) {
+        const int m = 4 * t + (lane >> 4), k = 128 * ls + 8 * lq;
+        // rows and columns behind x read 0
+        const bool ok = m < a.M && k < a.K && lu < u1;
+        st.x[t] = __builtin_amdgcn_raw_buffer_load_b128(rx, ok ? (uint32_t)(m * a.ldx + k) * 2 : ~0u, 0, 0);
+      }
+    }
     ++lu;
-    if (++ls == steps) {
+    if (++ls == steps && lu < u1) {
       ls = 0;
       seek(++lt);
     }
   };
-  constexpr int DEPTH = 4;
-  MvStage st[DEPTH];
+  load_scales();
+  Stage st[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) load(st[d]);
 
@@ -133,59 +181,78 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
       reinterpret_cast<uint4*>(tab)[i] = make_uint4(p, p, p, p);
     }
     if (tid < 256) code2[tid] = w.code2[tid];
+    if (tid < 4) reinterpret_cast<u32x4*>(xs)[tid] = u32x4{0, 0, 0, 0};
     if constexpr (XL) {
-      const int chunks = a.K / 8;
+      const int chunks = 16 * steps, data = a.K / 8;  // 16-byte pieces of a row
       for (int i = tid; i < a.M * chunks; i += kMvThreads) {
         const int m = i / chunks, c = i % chunks;
-        *reinterpret_cast<uint4*>(xs + ((int64_t)m * (a.K + 8) + 8 * c) * 2) =
-            *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 8 * c);
+        u32x4 v = {0, 0, 0, 0};
+        if (c < data)
+          v = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 8 * c);
+        *reinterpret_cast<u32x4*>(xs + 64 + m * mv_x_row(a.K) + 16 * c) = v;
       }
     }
   }
   __syncthreads();
 
-  // x: this lane's row of each 8, against its own block's lanes only
-  const bool mine = (q >> 1) == (lq >> 3);
-  const char* xp[MT];
-  bool have[MT];
+  // this lane's place in x: row 8 t + lq % 8, against its own block's lanes only (the others read the
+  // zeros), and whether it moves with the steps
+  uint32_t xo[MT], xm[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int m = 8 * t + (lq & 7);
-    have[t] = mine && m < a.M;
-    xp[t] = XL ? xs + ((int64_t)m * (a.K + 8) + 32 * q) * 2
-               : reinterpret_cast<const char*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 32 * q);
+    const bool have = (q >> 1) == (lq >> 3) && m < a.M;
+    xo[t] = have ? 64 + (XL ? m * mv_x_row(a.K) : wave * XW + m * 272) + 64 * q : 0;
+    xm[t] = XL && have ? ~0u : 0u;
   }
   const uint32_t copy = 4 * (lane & 31);
+  const int from_s = 128 * (q >> 1) + 8 * lq;  // 4 times the lane that has this one's scale
+  // W's 16-byte pieces in LDS: piece c of row r at 4 r + (c ^ r / 4), so that the 16 rows of a read lie in
+  // different banks
+  char* to_w = ws[wave] + 64 * (lane >> 2) + 16 * ((lane & 3) ^ (lane >> 4));
+  const char* from_w = ws[wave] + 64 * lq + 16 * (q ^ (lq >> 2));
   const char* tabb = reinterpret_cast<const char*>(tab);
   f32x4 tot[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) tot[t] = f32x4{};
   int ct = u0 / steps, cs = u0 % steps;  // the compute cursor
-  auto comp = [&](const MvStage& st, int u) {
+  float sc[DEPTH / 2];
+  auto comp = [&](const Stage& st, int u, int d) {
+    const float s = __int_as_float(
+        __builtin_amdgcn_ds_bpermute(from_s + 4 * (d & 1), __float_as_int(sc[d >> 1])));
+    *reinterpret_cast<u32x4*>(to_w) = st.w;
+    if constexpr (!XL) {
+#pragma unroll
+      for (int t = 0; t < 2 * MT; ++t)
+        *reinterpret_cast<u32x4*>(xs + 64 + wave * XW + (4 * t + (lane >> 4)) * 272 + 16 * lq) = st.x[t];
+    }
+    // the wavefront's own LDS operations run in their order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u32x4 wr = *reinterpret_cast<const u32x4*>(from_w);
     f32x4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4{};
-    const bool ok = 2 * cs + (q >> 1) < KB;
-    const uint32_t wd[4] = {st.w.x, st.w.y, st.w.z, st.w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint4 b;
-      b.x = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] << 7) & 0x7f80u) | copy));
-      b.y = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 1) & 0x7f80u) | copy));
-      b.z = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 9) & 0x7f80u) | copy));
-      b.w = *reinterpret_cast<const uint32_t*>(tabb + (((wd[i] >> 17) & 0x7f80u) | copy));
+      // byte j times 128, one v_dot4, is its entry's place in the table
+      u32x4 b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        b[j] = *reinterpret_cast<const uint32_t*>(
+            tabb + __builtin_amdgcn_udot4(wr[i], 128u << (8 * j), copy, false));
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (have[t] && ok) x = *reinterpret_cast<const uint4*>(xp[t] + 256 * cs + 16 * i);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(xs + (xo[t] + ((256u * cs) & xm[t])) + 16 * i);
         acc[t] = Mv<T>::run(__builtin_bit_cast(V8, x), __builtin_bit_cast(V8, b), acc[t]);
       }
     }
-    const float sc = ok ? mv_scale(code2[st.am], st.a2, off) : 0.f;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tot[t][r] = fmaf(sc, acc[t][r], tot[t][r]);
+      for (int r = 0; r < 4; ++r) tot[t][r] = fmaf(s, acc[t][r], tot[t][r]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next step is written
+    __builtin_amdgcn_wave_barrier();
     if (++cs == steps || u + 1 == u1) {
       // the two blocks' sums: lanes 0 .. 31 hold x rows 4 q + r of their W row
 #pragma unroll
@@ -201,12 +268,15 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
     }
   };
   for (int u = u0; u < u1; u += DEPTH) {
+    // a block behind K has a scale of 0: x is 0 there, and what W's next row has does not matter
+#pragma unroll
+    for (int h = 0; h < DEPTH / 2; ++h)
+      sc[h] = in[h] ? mv_scale(code2[am[h] & 255], __uint_as_float(a2[h]), off) : 0.f;
+    load_scales();
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      if (u + d < u1) {
-        comp(st[d], u + d);
-        load(st[d]);
-      }
+      if (u + d < u1) comp(st[d], u + d, d);
+      load(st[d]);
     }
   }
   __syncthreads();
@@ -249,11 +319,10 @@ __global__ __launch_bounds__(256) void k_nf4_matvec_any(const Nf4MvArgs a) {
   }
 #pragma unroll
   for (int m = 0; m < kNf4MvRows; ++m) {
-    if (m >= a.M) break;
     float v = sum[m];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    if (lane != 0) continue;
+    if (lane != 0 || m >= a.M) continue;
     if (w.bias != nullptr) v += (float)static_cast<const T*>(w.bias)[r];
     static_cast<T*>(a.y)[(int64_t)m * a.ldy + w.col0 + r] = (T)v;
   }
@@ -283,7 +352,7 @@ hipError_t run_x(Nf4MvArgs& a, hipStream_t s) {
 template <typename T>
 hipError_t run_t(Nf4MvArgs& a, hipStream_t s) {
   int64_t rows = 0;
-  bool whole = a.K % 64 == 0 && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  bool whole = a.K % 64 == 0 && a.ldx % 8 == 0 && a.ldx <= 1 << 26 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   for (int i = 0; i < a.n; ++i) {
     rows += a.w[i].N;
     whole = whole && (reinterpret_cast<uintptr_t>(a.w[i].packed) & 15) == 0;
