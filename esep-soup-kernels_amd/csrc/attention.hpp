@@ -120,7 +120,8 @@ struct AttnCacheArgs {
   const void* v;
   void* o;             // [B, n, HQ, D] dense
   const int32_t* len;  // [B] tokens in each row's cache, the n new ones last
-  float* part;         // partials, cache_part_floats
+  int2* ends;          // [groups] first and last wavefront of each group
+  float* part;         // partials behind them
   int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
   int B, n, S, HQ, HK;
   int window, sinks;   // window 0x7fffffff: none
@@ -146,10 +147,15 @@ inline int64_t cache_units(int B, int n, int S, int HQ, int HK, int D, int windo
   const int64_t u = (tiles + kCacheMinTiles - 1) / kCacheMinTiles;
   return u < 1 ? 1 : (u < most ? u : most);
 }
-// A partial per wavefront and (row, kv head, query tile) that it walks: at most units + groups of them.
-inline int64_t cache_part_floats(int64_t units, int B, int n, int HQ, int HK, int D) {
-  const int64_t rows = (int64_t)n * (HQ / HK);
-  return (units + (int64_t)B * HK * cache_row_tiles(n, HQ, HK)) * (rows < 32 ? rows : 32) * (D + 2);
+// The workspace in floats: the groups' ends, then a partial per wavefront and group ((row, kv head, query
+// tile)) that it walks, at most units + groups of them.
+inline int64_t cache_groups(int B, int n, int HQ, int HK) {
+  return (int64_t)B * HK * cache_row_tiles(n, HQ, HK);
+}
+inline int64_t cache_ends_floats(int64_t groups) { return (2 * groups + 3) & ~(int64_t)3; }
+inline int64_t cache_floats(int64_t units, int B, int n, int HQ, int HK, int D) {
+  const int64_t rows = (int64_t)n * (HQ / HK), groups = cache_groups(B, n, HQ, HK);
+  return cache_ends_floats(groups) + (units + groups) * (rows < 32 ? rows : 32) * (D + 2);
 }
 
 hipError_t launch_attn_cache(const AttnCacheArgs& a, int dt, int D, hipStream_t s, bool* supported);

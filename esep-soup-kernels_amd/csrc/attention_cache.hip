@@ -19,12 +19,6 @@
 namespace esep {
 namespace {
 
-// The walk's geometry, found by every wavefront from the lengths: tile counts of the rows, their sum.
-struct CachePlan {
-  int64_t total;  // tiles of all groups
-  int units;      // wavefronts that walk some
-};
-
 // Row b's keys for its n queries: `ns` tiles of the sinks from 0, then tiles from lo to len.
 struct CacheRow {
   int len, lo, sink_hi, ns, tiles;
@@ -42,60 +36,64 @@ __device__ __forceinline__ CacheRow cache_row(const AttnCacheArgs& a, int b) {
   return r;
 }
 
-// A value that every lane holds, in scalar registers (addresses of the tile fills are made from it).
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)v);
-  const uint32_t up = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
-  return (int64_t)((uint64_t)up << 32 | lo);
-}
-__device__ __forceinline__ int64_t lane_sum(int64_t v) {
+// The walk's geometry, found by every wavefront from the lengths: the tiles of all groups, dealt to `units`
+// wavefronts, the first `extra` of them one more than `each`.
+struct CachePlan {
+  int total, units, each, extra;
+  __device__ __forceinline__ int cut(int u) const { return u * each + (u < extra ? u : extra); }
+  __device__ __forceinline__ int unit_of(int x) const {
+    const int split = extra * (each + 1);
+    return x < split ? x / (each + 1) : extra + (x - split) / each;
+  }
+};
+__device__ __forceinline__ int lane_sum(int v) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  return uniform(v);
+  return __builtin_amdgcn_readfirstlane(v);
 }
-
-__device__ __forceinline__ CachePlan cache_plan(const AttnCacheArgs& a, int rt) {
-  const int lane = threadIdx.x & 63;
-  int64_t sum = 0;
-  for (int b = lane; b < a.B; b += 64) sum += cache_row(a, b).tiles;
+__device__ __forceinline__ CachePlan cache_plan(const AttnCacheArgs& a, int tiles) {
   CachePlan p;
-  p.total = lane_sum(sum) * a.HK * rt;
-  const int64_t u = (p.total + kCacheMinTiles - 1) / kCacheMinTiles;
-  p.units = u < a.units ? (int)u : a.units;
+  p.total = tiles;
+  const int u = (tiles + kCacheMinTiles - 1) / kCacheMinTiles;
+  p.units = u < a.units ? u : a.units;
+  p.each = p.units > 0 ? tiles / p.units : 0;
+  p.extra = tiles - p.each * p.units;
   return p;
 }
 
-// The row whose tiles hold number x of all (x < total), and the number of its first.
-__device__ __forceinline__ int cache_find(const AttnCacheArgs& a, int per_tile, int64_t x,
-                                          int64_t* first) {
+// The plan, and (found with the same reads where the rows are at most 64) the row whose tiles hold the first
+// of wavefront u, with the number of that row's first tile; row -1: no work. per_tile: groups of a row.
+__device__ __forceinline__ CachePlan cache_find(const AttnCacheArgs& a, int per_tile, int u, int* row,
+                                                int* first) {
   const int lane = threadIdx.x & 63;
-  int64_t before = 0;
+  auto tiles_of = [&](int b) { return b < a.B ? cache_row(a, b).tiles * per_tile : 0; };
+  const int mine0 = tiles_of(lane);
+  int sum = mine0;
+  for (int b = lane + 64; b < a.B; b += 64) sum += tiles_of(b);
+  const CachePlan p = cache_plan(a, lane_sum(sum));
+  *row = -1;
+  *first = 0;
+  if (u >= p.units) return p;
+  const int x = p.cut(u);
+  int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int64_t mine = b < a.B ? (int64_t)cache_row(a, b).tiles * per_tile : 0;
-    int64_t run = mine;  // inclusive sums
+    const int mine = b0 == 0 ? mine0 : tiles_of(b0 + lane);
+    int run = mine;  // inclusive sums
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(run, d);
+      const int o = __shfl_up(run, d);
       if (lane >= d) run += o;
     }
     const uint64_t past = __ballot(before + run > x);
     if (past != 0) {
       const int l = (int)__builtin_ctzll(past);
-      *first = uniform(before + __shfl(run - mine, l));
-      return b0 + l;
+      *row = b0 + l;
+      *first = before + __builtin_amdgcn_readlane(run - mine, l);
+      break;
     }
-    before = uniform(before + __shfl(run, 63));
+    before += __builtin_amdgcn_readlane(run, 63);
   }
-  return -1;
-}
-
-// The tiles of wavefront u are [cut(u), cut(u + 1)); the wavefront whose tiles hold x.
-__device__ __forceinline__ int64_t cache_cut(const CachePlan& p, int u) {
-  return (int64_t)((uint64_t)u * (uint64_t)p.total / (uint64_t)p.units);
-}
-__device__ __forceinline__ int cache_unit_of(const CachePlan& p, int64_t x) {
-  return (int)(((uint64_t)(x + 1) * (uint64_t)p.units - 1) / (uint64_t)p.total);
+  return p;
 }
 
 // One wavefront's fill of a 32-row swizzled tile (attention.hpp: SwzFill, whose row groups four wavefronts
@@ -141,25 +139,24 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
 
   const int lane = threadIdx.x, lq = lane & 31, hi = lane >> 5;
   const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32, per_tile = a.HK * RT;
-  const CachePlan plan = cache_plan(a, RT);
   const int u = blockIdx.x;
-  if (u >= plan.units) return;
-  int64_t x = cache_cut(plan, u);
-  const int64_t x1 = cache_cut(plan, u + 1);
-  int64_t first;
-  int b = __builtin_amdgcn_readfirstlane(cache_find(a, per_tile, x, &first));
+  int first, b;
+  const CachePlan plan = cache_find(a, per_tile, u, &b, &first);
+  if (b < 0) return;
+  int x = plan.cut(u);
+  const int x1 = plan.cut(u + 1);
   CacheRow row = cache_row(a, b);
   const Fill fk(lane, a.k_ts * (int64_t)sizeof(T)), fv(lane, a.v_ts * (int64_t)sizeof(T));
   const int live = rows < 32 ? rows : 32;  // rows of a partial
 
   while (x < x1) {
-    while (x >= first + (int64_t)row.tiles * per_tile) {
-      first += (int64_t)row.tiles * per_tile;
+    while (x >= first + row.tiles * per_tile) {
+      first += row.tiles * per_tile;
       row = cache_row(a, ++b);
     }
-    const int gi = (int)((x - first) / row.tiles);  // kv head and query tile within the row
-    const int64_t g0 = first + (int64_t)gi * row.tiles;
-    const int t0 = (int)(x - g0), t1 = x1 - g0 < row.tiles ? (int)(x1 - g0) : row.tiles;
+    const int gi = (x - first) / row.tiles;  // kv head and query tile within the row
+    const int g0 = first + gi * row.tiles;
+    const int t0 = x - g0, t1 = x1 - g0 < row.tiles ? x1 - g0 : row.tiles;
     const int kvh = gi / RT, rt = gi % RT;
     const char* kbase = reinterpret_cast<const char*>(
         static_cast<const T*>(a.k) + (int64_t)b * a.k_bs + (int64_t)kvh * a.k_hs);
@@ -217,8 +214,10 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
       __builtin_amdgcn_sched_barrier(0);
     }
     x += t1 - t0;
-    const int64_t slot = (int64_t)u + (int64_t)b * per_tile + gi;
-    float* part = a.part + slot * live * (D + 2);
+    const int group = b * per_tile + gi;
+    float* part = a.part + (int64_t)(u + group) * live * (D + 2);
+    // the wavefront with a group's first tile says for the join which others have some
+    if (t0 == 0 && lane == 0) a.ends[group] = make_int2(u, plan.unit_of(g0 + row.tiles - 1));
     if (rok && t0 == 0 && t1 == row.tiles) {  // the whole group
       store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
                          l > 0.f ? 1.f / l : 0.f);
@@ -240,59 +239,58 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
   }
 }
 
-// The groups that were cut, and zeros for the rows without tokens: one block per query row.
+// The groups that were cut, and zeros for the rows without tokens: one block per query row. A lane adds two
+// columns over every GROUPS-th part with a running maximum, so that the parts are read once.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attn_cache_join(const AttnCacheArgs a) {
   constexpr int PAIRS = D / 2, GROUPS = 256 / PAIRS;
   __shared__ float2 sums[GROUPS][PAIRS];
-  __shared__ float dens[GROUPS];
-  const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32, per_tile = a.HK * RT;
+  __shared__ float2 stat[GROUPS];  // maximum, sum
+  const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32;
   const int rg = (int)(blockIdx.x % rows);
   const int kvh = (int)(blockIdx.x / rows % a.HK), b = (int)(blockIdx.x / rows / a.HK);
-  const int gi = kvh * RT + rg / 32, lq = rg % 32, live = rows < 32 ? rows : 32;
-  const CachePlan plan = cache_plan(a, RT);
-  const CacheRow row = cache_row(a, b);
+  const int group = (b * a.HK + kvh) * RT + rg / 32, lq = rg % 32, live = rows < 32 ? rows : 32;
+  const int len = a.len[b];
+  const int2 ends = a.ends[group];  // not written where the row has no token
   const int g = threadIdx.x / PAIRS, c = threadIdx.x % PAIRS;
   T* out = static_cast<T*>(a.o) + (((int64_t)b * a.n + rg / G) * a.HQ + kvh * G + rg % G) * D + 2 * c;
-  if (row.tiles == 0) {
+  if (len <= 0 || a.S <= 0) {
     if (g == 0) out[0] = out[1] = (T)0.f;
     return;
   }
-  int64_t before = 0;  // tiles of the rows ahead of b
-  {
-    const int lane = threadIdx.x & 63;
-    for (int i = lane; i < b; i += 64) before += cache_row(a, i).tiles;
-    before = lane_sum(before) * per_tile;
-  }
-  const int64_t g0 = before + (int64_t)gi * row.tiles;
-  const int u0 = cache_unit_of(plan, g0), u1 = cache_unit_of(plan, g0 + row.tiles - 1);
-  if (u0 == u1) return;  // stored by its wavefront
-  const int64_t slot = (int64_t)b * per_tile + gi, size = (int64_t)live * (D + 2);
-  const float* part = a.part + slot * size;
-  float top = -INFINITY;
-  for (int u = u0 + (int)(threadIdx.x & 63); u <= u1; u += 64) top = fmaxf(top, part[u * size + lq]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float ref = top == -INFINITY ? 0.f : top;
+  if (ends.x == ends.y) return;  // stored by its wavefront
+  const int64_t size = (int64_t)live * (D + 2);
+  const float* part = a.part + group * size;
+  float m = -INFINITY, l = 0.f;
   float2 acc = make_float2(0.f, 0.f);
-  float den = 0.f;
 #pragma unroll 4
-  for (int u = u0 + g; u <= u1; u += GROUPS) {
+  for (int u = ends.x + g; u <= ends.y; u += GROUPS) {
     const float* p = part + u * size;
-    const float w = exp2_fast(p[lq] - ref);
-    den = fmaf(w, p[live + lq], den);
+    const float pm = p[lq], pl = p[live + lq];
     const float2 v = *reinterpret_cast<const float2*>(p + 2 * live + lq * D + 2 * c);
-    acc.x = fmaf(w, v.x, acc.x);
-    acc.y = fmaf(w, v.y, acc.y);
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float w0 = exp2_fast(m - ref), w1 = exp2_fast(pm - ref);
+    l = fmaf(w1, pl, w0 * l);
+    acc.x = fmaf(w1, v.x, w0 * acc.x);
+    acc.y = fmaf(w1, v.y, w0 * acc.y);
+    m = top;
   }
   sums[g][c] = acc;
-  if (c == 0) dens[g] = den;
+  if (c == 0) stat[g] = make_float2(m, l);
   __syncthreads();
   if (g != 0) return;
-  for (int i = 1; i < GROUPS; ++i) {
-    acc.x += sums[i][c].x;
-    acc.y += sums[i][c].y;
-    den += dens[i];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, stat[i].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float den = 0.f;
+  acc = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float w = exp2_fast(stat[i].x - ref);
+    den = fmaf(w, stat[i].y, den);
+    acc.x = fmaf(w, sums[i][c].x, acc.x);
+    acc.y = fmaf(w, sums[i][c].y, acc.y);
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
   out[0] = (T)(acc.x * inv);

@@ -781,7 +781,7 @@ int64_t esep_attn_cache_workspace(int B, int n, int S, int HQ, int HK, int D, in
   if (B < 1 || n < 1 || S < 1 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0)
     return 0;
   const int w = window == 0 || window > S ? S : window;
-  return esep::cache_part_floats(esep::cache_units(B, n, S, HQ, HK, D, w, sinks), B, n, HQ, HK, D);
+  return esep::cache_floats(esep::cache_units(B, n, S, HQ, HK, D, w, sinks), B, n, HQ, HK, D);
 }
 
 int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -797,6 +797,8 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
     return fail(ESEP_ESHAPE, "attn_cache: bad sizes B=%d n=%d S=%d HQ=%d HK=%d", B, n, S, HQ, HK);
   if (window < 0 || sinks < 0)
     return fail(ESEP_ESHAPE, "attn_cache: window=%d sinks=%d", window, sinks);
+  if (esep::cache_groups(B, n, HQ, HK) * (S / 32 + 2) > 0x7fffffff)  // tiles are numbered in 32 bits
+    return fail(ESEP_ESHAPE, "attn_cache: B=%d rows of n=%d over S=%d are too many for one launch", B, n, S);
   if (!(scale > 0.f)) return fail(ESEP_EINVAL, "attn_cache: scale must be positive");
   if (B == 0 || n == 0) return 0;
   if (q == nullptr || o == nullptr || lengths == nullptr || workspace == nullptr ||
@@ -817,7 +819,8 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
   a.v = v;
   a.o = o;
   a.len = lengths;
-  a.part = workspace;
+  a.ends = reinterpret_cast<int2*>(workspace);
+  a.part = workspace + esep::cache_ends_floats(esep::cache_groups(B, n, HQ, HK));
   a.q_bs = q_strides[0];
   a.q_ts = q_strides[1];
   a.q_hs = q_strides[2];

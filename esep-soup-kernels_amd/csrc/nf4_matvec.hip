@@ -173,6 +173,9 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
 
   // the tables and x, while the first bytes of W are on their way
   const float off = *w.offset;
+  // (the bias of the output that this thread adds up first, too)
+  const int n0 = (tile0 + tid / (MT * 128)) * 16 + (tid & 15);
+  const float bias0 = w.bias != nullptr && n0 < w.N ? (float)static_cast<const T*>(w.bias)[n0] : 0.f;
   {
     const float code = w.nf4[lane & 15];
     for (int i = tid; i < 256 * 8; i += kMvThreads) {
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
     const int last = ((t + 1) * steps * waves - 1) / total;
     float v = red[first + t][m][c];
     for (int j = first + 1; j <= last; ++j) v += red[j + t][m][c];
-    if (w.bias != nullptr) v += (float)static_cast<const T*>(w.bias)[n];
+    if (w.bias != nullptr) v += i == tid ? bias0 : (float)static_cast<const T*>(w.bias)[n];
     static_cast<T*>(a.y)[(int64_t)m * a.ldy + w.col0 + n] = (T)v;
   }
 }

@@ -24,6 +24,7 @@ def test_refusals():
     assert _call(dt=0) == -1 and _call(D=96) == -2
     assert _call(HQ=3) == -2 and _call(B=-1) == -2 and _call(S=(1 << 30) + 1) == -2
     assert _call(B=1 << 20, n=8) == -2 and b"bad sizes" in err()
+    assert _call(B=1 << 19, S=1 << 30) == -2 and b"too many" in err()
     assert _call(window=-1) == -2 and _call(sinks=-1) == -2
     assert _call(scale=0.0) == -1
     for name in ("q", "o", "len", "ws", "k", "v", "qs", "ks", "vs"):
@@ -38,11 +39,12 @@ def test_refusals():
 
 def test_workspace():
     ws = _hip.attn_cache_workspace
-    # a partial per wavefront and per group, of each query row a maximum, a sum and D values
-    assert ws(1, 1, 64, 4, 2, 64) == (2 + 2) * 2 * 66
-    assert ws(1, 1, 32768, 12, 2, 128) == (1024 + 2) * 6 * 130
-    assert ws(64, 1, 32768, 12, 2, 128) == (1280 + 128) * 6 * 130  # five wavefronts to a CU
-    assert ws(1, 16, 64, 14, 2, 64) == (8 + 8) * 32 * 66  # 112 query rows in 4 tiles
+    # two numbers per group, then a partial per wavefront and per group, of each query row a maximum, a sum
+    # and D values
+    assert ws(1, 1, 64, 4, 2, 64) == 4 + (2 + 2) * 2 * 66
+    assert ws(1, 1, 32768, 12, 2, 128) == 4 + (1024 + 2) * 6 * 130
+    assert ws(64, 1, 32768, 12, 2, 128) == 256 + (1280 + 128) * 6 * 130  # five wavefronts to a CU
+    assert ws(1, 16, 64, 14, 2, 64) == 16 + (8 + 8) * 32 * 66  # 112 query rows in 4 tiles
     assert ws(1, 1, 32768, 12, 2, 128, 64, 4) < ws(1, 1, 32768, 12, 2, 128)
     assert ws(0, 1, 1, 1, 1, 64) == 0
 
