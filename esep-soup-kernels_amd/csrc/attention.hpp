@@ -125,27 +125,29 @@ struct AttnCacheArgs {
   int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
   int B, n, S, HQ, HK;
   int window, sinks;   // window 0x7fffffff: none
-  int units;           // wavefronts of the launch
   float scale_log2;
 };
 
 // Query rows of a kv head: its query heads times the new tokens, in tiles of 32.
 inline int64_t cache_row_tiles(int n, int HQ, int HK) { return ((int64_t)n * (HQ / HK) + 31) / 32; }
-// 32-key tiles of a row at most.
+// 32-key tiles of a row at most (the sinks' and the window's end in a tile of their own each).
 inline int64_t cache_key_tiles(int S, int n, int window, int sinks) {
-  const int64_t all = ((int64_t)S + 31) / 32;
+  const int64_t all = ((int64_t)S + 31) / 32 + 1;
   const int64_t seen = ((int64_t)sinks + 31) / 32 + ((int64_t)window + n + 30) / 32;
   return seen < all ? seen : all;
 }
-// Wavefronts: a ring of two 32-key K / V tiles each (32 KiB at D = 128) of a CU's 160 KiB of LDS, and two tiles or
-// more for each to walk.
-constexpr int kCacheMinTiles = 2;
-inline int64_t cache_units(int B, int n, int S, int HQ, int HK, int D, int window, int sinks) {
-  const int64_t tiles =
-      (int64_t)B * HK * cache_row_tiles(n, HQ, HK) * cache_key_tiles(S, n, window, sinks);
-  const int64_t most = kAttnCUs * (D == 128 ? 5 : 10);
-  const int64_t u = (tiles + kCacheMinTiles - 1) / kCacheMinTiles;
-  return u < 1 ? 1 : (u < most ? u : most);
+// Wavefronts for a number of tiles: one to a tile up to 256, from 1024 tiles on four tiles to each, up to four
+// (D = 64: eight) to a CU. Each keeps a ring of two K / V tiles in LDS (32 KiB at D = 128, of a CU's 160); a
+// fifth made the four SIMDs uneven (32 rows of up to 8192 tokens, 28 / 4 heads, D = 128: 79 us, with four 69),
+// two tiles to each more partials to join than it saved (one row of 32768 tokens 29 us, four 20.6; 700 tokens 9.8,
+// one 8.8). Device and host use the same rule: the host's tiles are a bound of the device's.
+__host__ __device__ inline int64_t cache_units(int64_t tiles, int D) {
+  const int64_t most = kAttnCUs * (D == 128 ? 4 : 8);
+  const int64_t u = tiles <= kAttnCUs ? tiles : (tiles / 4 > kAttnCUs ? tiles / 4 : kAttnCUs);
+  return u < most ? u : most;
+}
+inline int64_t cache_tiles(int B, int n, int S, int HQ, int HK, int window, int sinks) {
+  return (int64_t)B * HK * cache_row_tiles(n, HQ, HK) * cache_key_tiles(S, n, window, sinks);
 }
 // The workspace in floats: the groups' ends, then a partial per wavefront and group ((row, kv head, query
 // tile)) that it walks, at most units + groups of them.
@@ -249,10 +251,17 @@ constexpr int kWaitVm0 = 0x0F70;
 // on the device), so one instruction fills 1024 / RB whole rows: each lane loads the global chunk
 // that belongs at its position.
 // ---------------------------------------------------------------------------------------
+#define ESEP_LDS_DMA_X4_S "s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
 __device__ __forceinline__ void lds_dma_x4_s(const void* base, uint32_t voff, const void* lds) {
   const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "{m0}"(m) : "memory");
+  asm volatile(ESEP_LDS_DMA_X4_S ::"v"(voff), "s"(base), "{m0}"(m) : "memory");
 }
+// The same past the caches (non-temporal), for what is read once.
+__device__ __forceinline__ void lds_dma_x4_s_nt(const void* base, uint32_t voff, const void* lds) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  asm volatile(ESEP_LDS_DMA_X4_S " nt" ::"v"(voff), "s"(base), "{m0}"(m) : "memory");
+}
+#undef ESEP_LDS_DMA_X4_S
 __device__ __forceinline__ void lds_dma_x4(const void* g, const void* lds) {
   const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(m) : "memory");

@@ -51,11 +51,10 @@ __device__ __forceinline__ int lane_sum(int v) {
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   return __builtin_amdgcn_readfirstlane(v);
 }
-__device__ __forceinline__ CachePlan cache_plan(const AttnCacheArgs& a, int tiles) {
+__device__ __forceinline__ CachePlan cache_plan(int tiles, int D) {
   CachePlan p;
   p.total = tiles;
-  const int u = (tiles + kCacheMinTiles - 1) / kCacheMinTiles;
-  p.units = u < a.units ? u : a.units;
+  p.units = (int)cache_units(tiles, D);
   p.each = p.units > 0 ? tiles / p.units : 0;
   p.extra = tiles - p.each * p.units;
   return p;
@@ -63,6 +62,7 @@ __device__ __forceinline__ CachePlan cache_plan(const AttnCacheArgs& a, int tile
 
 // The plan, and (found with the same reads where the rows are at most 64) the row whose tiles hold the first
 // of wavefront u, with the number of that row's first tile; row -1: no work. per_tile: groups of a row.
+template <int D>
 __device__ __forceinline__ CachePlan cache_find(const AttnCacheArgs& a, int per_tile, int u, int* row,
                                                 int* first) {
   const int lane = threadIdx.x & 63;
@@ -70,7 +70,7 @@ __device__ __forceinline__ CachePlan cache_find(const AttnCacheArgs& a, int per_
   const int mine0 = tiles_of(lane);
   int sum = mine0;
   for (int b = lane + 64; b < a.B; b += 64) sum += tiles_of(b);
-  const CachePlan p = cache_plan(a, lane_sum(sum));
+  const CachePlan p = cache_plan(lane_sum(sum), D);
   *row = -1;
   *first = 0;
   if (u >= p.units) return p;
@@ -98,7 +98,7 @@ __device__ __forceinline__ CachePlan cache_find(const AttnCacheArgs& a, int per_
 
 // One wavefront's fill of a 32-row swizzled tile (attention.hpp: SwzFill, whose row groups four wavefronts
 // share).
-template <int RB>
+template <int RB, bool NT>
 struct CacheFill {
   static constexpr int GR = 1024 / RB, CH = RB / 16, N = 32 / GR, V = RB == 256 ? 4 : 2;
   int lrow, chunk;
@@ -115,7 +115,10 @@ struct CacheFill {
     if (r0 + 32 <= rend) {
 #pragma unroll
       for (int q = 0; q < N; ++q)
-        lds_dma_x4_s(base + (int64_t)(r0 + GR * q) * rs, voff[q % V], dst + 1024 * q);
+        if constexpr (NT)
+          lds_dma_x4_s_nt(base + (int64_t)(r0 + GR * q) * rs, voff[q % V], dst + 1024 * q);
+        else
+          lds_dma_x4_s(base + (int64_t)(r0 + GR * q) * rs, voff[q % V], dst + 1024 * q);
     } else {
 #pragma unroll
       for (int q = 0; q < N; ++q) {
@@ -130,18 +133,20 @@ struct CacheFill {
 constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 constexpr int kWaitLgkm0 = 0xC07F;
 
-template <typename T, int D>
+// NT: K and V past the caches, where one query tile alone reads them, in rows of 256 bytes (32 rows of up to
+// 8192 tokens, 28 / 4 heads: 69 -> 63 us; at D = 64 24 -> 25 for 64 rows of up to 4096, 14 / 2 heads).
+template <typename T, int D, bool NT>
 __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnCacheArgs a) {
   constexpr int RB = 2 * D, TILE = 32 * RB;
   using V8 = typename Mfma<T>::v8;
-  using Fill = CacheFill<RB>;
+  using Fill = CacheFill<RB, NT>;
   __shared__ __align__(1024) char kv[2][2][TILE];  // [buffer][K, V]
 
   const int lane = threadIdx.x, lq = lane & 31, hi = lane >> 5;
   const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32, per_tile = a.HK * RT;
   const int u = blockIdx.x;
   int first, b;
-  const CachePlan plan = cache_find(a, per_tile, u, &b, &first);
+  const CachePlan plan = cache_find<D>(a, per_tile, u, &b, &first);
   if (b < 0) return;
   int x = plan.cut(u);
   const int x1 = plan.cut(u + 1);
@@ -239,11 +244,15 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
   }
 }
 
+// Parts of a group from which its rows, where there are no more than CUs, are joined by blocks of 1024 threads
+// instead of 256 (12 rows of 512 parts each 17 -> 5.5 us; 896 rows of 27 4.9 -> 8.7).
+constexpr int64_t kCacheManyParts = 24;
+
 // The groups that were cut, and zeros for the rows without tokens: one block per query row. A lane adds two
 // columns over every GROUPS-th part with a running maximum, so that the parts are read once.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_attn_cache_join(const AttnCacheArgs a) {
-  constexpr int PAIRS = D / 2, GROUPS = 256 / PAIRS;
+template <typename T, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_attn_cache_join(const AttnCacheArgs a) {
+  constexpr int PAIRS = D / 2, GROUPS = THREADS / PAIRS;
   __shared__ float2 sums[GROUPS][PAIRS];
   __shared__ float2 stat[GROUPS];  // maximum, sum
   const int G = a.HQ / a.HK, rows = G * a.n, RT = (rows + 31) / 32;
@@ -299,11 +308,19 @@ __global__ __launch_bounds__(256) void k_attn_cache_join(const AttnCacheArgs a) 
 
 template <typename T, int D>
 hipError_t run(const AttnCacheArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_attn_cache<T, D>), dim3((unsigned)a.units), dim3(64), 0, s, a);
+  const int64_t units = cache_units(cache_tiles(a.B, a.n, a.S, a.HQ, a.HK, a.window, a.sinks), D);
+  const dim3 grid((unsigned)(units > 0 ? units : 1)), rows((unsigned)(a.B * a.HQ * a.n));
+  const bool once = D == 128 && cache_row_tiles(a.n, a.HQ, a.HK) == 1;
+  if (once)
+    hipLaunchKernelGGL((k_attn_cache<T, D, D == 128>), grid, dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attn_cache<T, D, false>), grid, dim3(64), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t rows = (int64_t)a.B * a.HQ * a.n;
-  hipLaunchKernelGGL((k_attn_cache_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  if (units > kCacheManyParts * cache_groups(a.B, a.n, a.HQ, a.HK) && rows.x <= 256)
+    hipLaunchKernelGGL((k_attn_cache_join<T, D, 1024>), rows, dim3(1024), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attn_cache_join<T, D, 256>), rows, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -781,7 +781,8 @@ int64_t esep_attn_cache_workspace(int B, int n, int S, int HQ, int HK, int D, in
   if (B < 1 || n < 1 || S < 1 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0)
     return 0;
   const int w = window == 0 || window > S ? S : window;
-  return esep::cache_floats(esep::cache_units(B, n, S, HQ, HK, D, w, sinks), B, n, HQ, HK, D);
+  const int64_t units = esep::cache_units(esep::cache_tiles(B, n, S, HQ, HK, w, sinks), D);
+  return esep::cache_floats(units, B, n, HQ, HK, D);
 }
 
 int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -837,7 +838,6 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
   a.HK = HK;
   a.window = window == 0 || window > S ? (S > 0 ? S : 1) : window;  // none: a row's longest
   a.sinks = sinks;
-  a.units = (int)esep::cache_units(B, n, S, HQ, HK, D, a.window, sinks);
   a.scale_log2 = scale * 1.4426950408889634f;
   bool sup = false;
   const hipError_t e = esep::launch_attn_cache(a, dt, D, static_cast<hipStream_t>(stream), &sup);

@@ -41,10 +41,10 @@ def test_workspace():
     ws = _hip.attn_cache_workspace
     # two numbers per group, then a partial per wavefront and per group, of each query row a maximum, a sum
     # and D values
-    assert ws(1, 1, 64, 4, 2, 64) == 4 + (2 + 2) * 2 * 66
-    assert ws(1, 1, 32768, 12, 2, 128) == 4 + (1024 + 2) * 6 * 130
-    assert ws(64, 1, 32768, 12, 2, 128) == 256 + (1280 + 128) * 6 * 130  # five wavefronts to a CU
-    assert ws(1, 16, 64, 14, 2, 64) == 16 + (8 + 8) * 32 * 66  # 112 query rows in 4 tiles
+    assert ws(1, 1, 64, 4, 2, 64) == 4 + (4 + 2) * 2 * 66  # a wavefront to a tile
+    assert ws(1, 1, 32768, 12, 2, 128) == 4 + (512 + 2) * 6 * 130  # four tiles to each
+    assert ws(64, 1, 32768, 12, 2, 128) == 256 + (1024 + 128) * 6 * 130  # four wavefronts to a CU
+    assert ws(1, 16, 64, 14, 2, 64) == 16 + (24 + 8) * 32 * 66  # 112 query rows in 4 tiles
     assert ws(1, 1, 32768, 12, 2, 128, 64, 4) < ws(1, 1, 32768, 12, 2, 128)
     assert ws(0, 1, 1, 1, 1, 64) == 0
 
