@@ -53,13 +53,20 @@ __device__ __forceinline__ int win_search(int n_seq, int p, Base&& base) {
 // A block's (sequence, 128-row tile, head) among H heads, or a number among the spare blocks.
 struct WinPlace {
   int seq, tile, head;   // seq < 0: no work
+  int start, end;        // the sequence's tokens
+  int rest;              // the first token behind the last sequence
   int spare, n_spare;    // spare >= 0: one of n_spare blocks without a tile (8 or more of them)
 };
 __device__ __forceinline__ WinPlace win_place(int b, int nblk, int H, const int32_t* cu, int n_seq,
                                               int64_t T) {
-  const int live = (cu_at(cu, n_seq, T) / kAttnBM + n_seq) * H;
+  // the offsets of up to 63 sequences in one read, a lane each: a block's place then costs one trip to memory
+  const int lane = (int)(threadIdx.x & 63);
+  const bool few = n_seq < 64;
+  const int mine = few ? cu_at(cu, lane < n_seq ? lane : n_seq, T) : 0;
+  const int rest = few ? __builtin_amdgcn_readlane(mine, n_seq) : cu_at(cu, n_seq, T);
+  const int live = (rest / kAttnBM + n_seq) * H;
   const int per = (live + 7) / 8, xcd = b & 7, slot = b >> 3;
-  WinPlace w{-1, 0, 0, -1, nblk - 8 * per};
+  WinPlace w{-1, 0, 0, 0, 0, rest, -1, nblk - 8 * per};
   if (slot >= per) {
     w.spare = 8 * (slot - per) + xcd;
     return w;
@@ -67,11 +74,22 @@ __device__ __forceinline__ WinPlace win_place(int b, int nblk, int H, const int3
   const int i = xcd * per + slot;
   if (i >= live) return w;
   const int p = i / H;
-  const int s = win_search(n_seq, p, [&](int j) { return cu_at(cu, j, T) / kAttnBM + j; });
-  if (s < 0) return w;
+  int s;
+  if (few) {
+    s = __popcll(__ballot(lane < n_seq && mine / kAttnBM + lane <= p)) - 1;
+    if (s < 0) return w;
+    w.start = __builtin_amdgcn_readlane(mine, s);
+    w.end = __builtin_amdgcn_readlane(mine, s + 1);
+  } else {
+    s = win_search(n_seq, p, [&](int j) { return cu_at(cu, j, T) / kAttnBM + j; });
+    if (s < 0) return w;
+    w.start = cu_at(cu, s, T);
+    w.end = cu_at(cu, s + 1, T);
+  }
+  if (w.end < w.start) w.end = w.start;
   w.seq = s;
-  w.tile = p - (cu_at(cu, s, T) / kAttnBM + s);
-  w.head = i % H;
+  w.tile = p - (w.start / kAttnBM + s);
+  w.head = i - p * H;
   return w;
 }
 inline int64_t win_blocks(int64_t T, int n_seq, int64_t H) {
@@ -168,10 +186,9 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_win_fwd(con
 
   const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HQ, a.cu, a.n_seq, a.T);
   if (pl.spare >= 0 && p.zero_rest)
-    zero_rest<T>(static_cast<T*>(a.o), a.o_rs, a.HQ * D, cu_at(a.cu, a.n_seq, a.T), a.T, pl);
+    zero_rest<T>(static_cast<T*>(a.o), a.o_rs, a.HQ * D, pl.rest, a.T, pl);
   if (pl.seq < 0) return;
-  int start, end;
-  seq_bounds(a.cu, pl.seq, a.T, &start, &end);
+  const int start = pl.start, end = pl.end;
   const int q0 = start + pl.tile * kAttnBM, h = pl.head;
   if (q0 >= end) return;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -217,10 +234,9 @@ __global__ __launch_bounds__(kAttnThreads, kDqPerCU<D>) void k_attn_win_dq(const
 
   const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HQ, a.cu, a.n_seq, a.T);
   if (pl.spare >= 0)
-    zero_rest<T>(static_cast<T*>(b.dq), b.dq_rs, a.HQ * D, cu_at(a.cu, a.n_seq, a.T), a.T, pl);
+    zero_rest<T>(static_cast<T*>(b.dq), b.dq_rs, a.HQ * D, pl.rest, a.T, pl);
   if (pl.seq < 0) return;
-  int start, end;
-  seq_bounds(a.cu, pl.seq, a.T, &start, &end);
+  const int start = pl.start, end = pl.end;
   const int q0 = start + pl.tile * kAttnBM, h = pl.head;
   if (q0 >= end) return;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -390,15 +406,16 @@ __global__ __launch_bounds__(kAttnThreads, kDkdvPerCU) void k_attn_win_dkdv(cons
   const int G = a.HQ / a.HK, bid = attn_block();
   const bool far = bid >= p.n_main;
   if (far && !p.far) return;
-  int seq, kh, part, tile, chunk = 0, gs;
+  int seq, kh, part, tile, chunk = 0, gs, start = 0, end = 0;
   if (!far) {
     const WinPlace pl = win_place(bid, p.n_main, a.HK * b.split, a.cu, a.n_seq, a.T);
     if (pl.spare >= 0) {
-      const int from = cu_at(a.cu, a.n_seq, a.T);
-      zero_rest<T>(static_cast<T*>(b.dk), b.dk_rs, a.HK * D, from, a.T, pl);
-      zero_rest<T>(static_cast<T*>(b.dv), b.dv_rs, a.HK * D, from, a.T, pl);
+      zero_rest<T>(static_cast<T*>(b.dk), b.dk_rs, a.HK * D, pl.rest, a.T, pl);
+      zero_rest<T>(static_cast<T*>(b.dv), b.dv_rs, a.HK * D, pl.rest, a.T, pl);
     }
     seq = pl.seq;
+    start = pl.start;
+    end = pl.end;
     kh = pl.head / b.split;
     part = pl.head % b.split;
     tile = pl.tile;
@@ -408,15 +425,16 @@ __global__ __launch_bounds__(kAttnThreads, kDkdvPerCU) void k_attn_win_dkdv(cons
     const int slot = (bid - p.n_main) / per, r = (bid - p.n_main) % per;
     seq = win_search(a.n_seq, slot,
                      [&](int j) { return win_far_base(cu_at(a.cu, j, a.T), p.window); });
-    if (seq >= 0) chunk = slot - win_far_base(cu_at(a.cu, seq, a.T), p.window);
+    if (seq >= 0) {
+      seq_bounds(a.cu, seq, a.T, &start, &end);
+      chunk = slot - win_far_base(start, p.window);
+    }
     tile = r % kts;
     kh = r / kts % a.HK;
     part = r / kts / a.HK;
     gs = G / p.far_split;
   }
   if (seq < 0) return;
-  int start, end;
-  seq_bounds(a.cu, seq, a.T, &start, &end);
   const int len = end - start;
   const bool lng = p.far && len - kWinFar > p.window;  // its sink keys have far blocks
   const int sink_hi = start + (p.sinks < len ? p.sinks : len);
