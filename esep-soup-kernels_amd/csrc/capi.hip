@@ -122,9 +122,35 @@ struct WinLayout {
   int split, sinks, far, far_split;
   int64_t main_at, far_at, total;
 };
+// Blocks per (kv head, key tile) of the windowed dK / dV kernel: the divisor of HQ / HK with the least
+// estimated time. Its blocks do near-equal work, so what counts beside the partials' bytes is how the blocks
+// fill the 512 that are resident: half of them or fewer run a third faster each, and a round that is begun costs
+// about half of one more. A 32-query item of two blocks to a CU takes 2.6 us (D = 64: 1.3), the partials are
+// written and read at 5 TB/s. Backward in us with 1 / 2 / 3 / 6 blocks, 12 / 2 heads, D = 128 (* what it picks):
+// 5933 tokens in 8 sequences, window 256, 143 / 109 / 108* / 117; 8192, 512: 234 / 193 / 171* / 190; 32768, 4096:
+// 3448 / 2992 / 2874 / 2794*; with 1 / 7, 28 / 4 heads, window 512: 4096 tokens 256 / 216*, 8192 365* / 403.
+int win_split(int64_t T, int HQ, int HK, int D, int max_seqlen, int window) {
+  const int G = HQ / HK;
+  const double head = ((window < max_seqlen ? window : max_seqlen) + 160) / 32 * (D == 128 ? 2.6 : 1.3);
+  const double part = 16.0 * (double)T * HK * D / 5e6;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= G; ++s) {
+    if (G % s) continue;
+    const double r = (double)(T / 128 + 1) * HK * s / 512;
+    const double fill = r < 0.5 ? 0.75 : (r <= 1 ? 0.5 + 0.5 * r : 0.5 * (r + (double)(int64_t)(r + 0.999999)));
+    const double cost = G / s * fill * head + (s > 1 ? s * part : 0);
+    if (s == 1 || cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 WinLayout win_layout(int64_t T, int HQ, int HK, int D, int max_seqlen, int window, int sinks) {
   WinLayout w{};
-  w.split = attn_split(T, HQ, HK);
+  w.split = win_split(T, HQ, HK, D, max_seqlen, window);
   w.sinks = sinks < max_seqlen ? sinks : max_seqlen;
   w.far = esep::win_has_far(window, w.sinks, max_seqlen);
   w.far_split = w.far ? esep::win_far_split(T, HQ, HK, window, w.sinks) : 1;

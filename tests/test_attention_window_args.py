@@ -50,8 +50,9 @@ def test_backward_refusals():
 
 def test_workspace():
     ws = _hip.attn_win_bwd_workspace
-    base = _hip.attn_bwd_workspace(5000, 4, 2, 64)
-    assert ws(5000, 4, 2, 64, 5000, 100, 0) == base  # no sinks
+    base = ws(5000, 4, 2, 64, 5000, 100, 0)  # no sinks
+    # delta, and dK / dV partials of two blocks per kv head or none
+    assert base in (5000 * 4, 5000 * 4 + 2 * 2 * 5000 * 2 * 64)
     assert ws(5000, 4, 2, 64, 612, 100, 4) == base  # no sequence long enough for far queries
     assert ws(5000, 4, 2, 64, 613, 100, 4) > base
     # no more sink rows than a sequence has
