@@ -393,7 +393,7 @@ __device__ __forceinline__ void store_sink(float* buf, int64_t idx, int HK, int 
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads, kDkdvPerCU) void k_attn_win_dkdv(const AttnWinArgs p) {
+__global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_attn_win_dkdv(const AttnWinArgs p) {
   constexpr int NW = 4, BQ = 32, BK = kAttnBM, ROWB = 2 * D;
   using V8 = typename Mfma<T>::v8;
   const AttnBwdArgs& b = p.b;
