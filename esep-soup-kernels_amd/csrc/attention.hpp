@@ -39,6 +39,7 @@ struct AttnArgs {
   const void* k;
   const void* v;
   void* o;
+  void* o_low;             // [T, HQ, D] what o's rounding dropped, or null (the forward writes, dQ reads)
   float* lse;              // [HQ, T]
   const int32_t* cu;       // [n_seq + 1]
   int64_t q_rs, k_rs, v_rs, o_rs;  // token strides (elements)
@@ -109,6 +110,17 @@ inline int win_far_split(int64_t T, int HQ, int HK, int window, int sinks) {
   }
   return s;
 }
+
+// 0 to the tokens behind the last sequence of up to three tensors (null: none) of rows of w elements.
+struct AttnRestArgs {
+  void* t[3];
+  int64_t rs[3];
+  int w[3];
+  const int32_t* cu;
+  int n_seq;
+  int64_t T;
+};
+hipError_t launch_attn_rest(const AttnRestArgs& a, hipStream_t s);
 
 hipError_t launch_attn_win_fwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
 hipError_t launch_attn_win_bwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
@@ -591,6 +603,19 @@ __device__ __forceinline__ void store_rows_t(T* row, const f32x16 (&acc)[D / 32]
       w = make_uint4(a[0], b[0], a[1], b[1]);
       *reinterpret_cast<uint4*>(row + 32 * md + 8 * (j + hi)) = w;
     }
+}
+
+// What the rounding of o = acc * mul to T drops, stored in T as o is: its own rounding is 2^-8 (bf16) of a half step.
+template <typename T, int D>
+__device__ __forceinline__ void store_low_t(T* row, f32x16 (&acc)[D / 32], int hi, float mul) {
+#pragma unroll
+  for (int md = 0; md < D / 32; ++md)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float o = acc[md][i] * mul;
+      acc[md][i] = o - (float)(T)o;
+    }
+  store_rows_t<T, D>(row, acc, hi, 1.f);
 }
 
 }  // namespace esep

@@ -33,8 +33,9 @@ namespace {
 // dQ with the K / V tiles moved as the forward moves them: swizzled BN-key tiles filled by dwordx4
 // LDS DMA through a ring of two buffers (tile t + 1 in flight while tile t is consumed, one
 // barrier per tile). At D = 64 (the dK / dV kernel's sizes below) 78 us, against 133 staged through
-// registers into padded tiles in the hardware's block order (65 in level_order).
-template <typename T, int D, int BN, int NW>
+// registers into padded tiles in the hardware's block order (65 in level_order). LOW: delta from o
+// and what its rounding dropped.
+template <typename T, int D, int BN, int NW, bool LOW>
 __global__ __launch_bounds__(64 * NW, kDqPerCU<D>) void k_attn_bwd_dq_dma(const AttnBwdArgs b,
                                                                           int qtiles, int order) {
   constexpr int RB = 2 * D;
@@ -70,13 +71,17 @@ __global__ __launch_bounds__(64 * NW, kDqPerCU<D>) void k_attn_bwd_dq_dma(const 
     const T* qrow = static_cast<const T*>(a.q) + (int64_t)qi * a.q_rs + col;
     const T* drow = static_cast<const T*>(b.dout) + (int64_t)qi * b.do_rs + col;
     const T* orow = static_cast<const T*>(a.o) + (int64_t)qi * a.o_rs + col;
+    const T* lrow = static_cast<const T*>(a.o_low) + (int64_t)qi * a.HQ * D + col;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       qb[c] = qok ? ld16<V8>(qrow + 16 * c) : V8{};
       db[c] = qok ? ld16<V8>(drow + 16 * c) : V8{};
       const V8 o8 = qok ? ld16<V8>(orow + 16 * c) : V8{};
+      V8 l8{};
+      if constexpr (LOW) l8 = qok ? ld16<V8>(lrow + 16 * c) : V8{};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf((float)db[c][e], (float)o8[e], delta);
+      for (int e = 0; e < 8; ++e)
+        delta = fmaf((float)db[c][e], LOW ? (float)o8[e] + (float)l8[e] : (float)o8[e], delta);
     }
     delta = pair_sum(delta);
     if (qok && hi == 0) b.delta[(int64_t)h * a.T + qi] = delta;
@@ -398,9 +403,14 @@ hipError_t bwd_run(const AttnBwdArgs& b, int max_seqlen, hipStream_t s) {
   const int64_t C = (max_seqlen + 32 * QW - 1) / (32 * QW);
   const int64_t nq = xcd_grid(C, (int64_t)f.HQ * f.n_seq);
   if (!attn_grid_ok(nq)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_attn_bwd_dq_dma<T, D, D == 128 ? 32 : 64, QW>), attn_grid(nq), dim3(64 * QW),
-                     0, s, b, (int)C,
-                     attn_order(nq, kDqPerCU<D>, kRoundsQ, D, f.T, f.n_seq, max_seqlen));
+  constexpr int BN = D == 128 ? 32 : 64;
+  const int order = attn_order(nq, kDqPerCU<D>, kRoundsQ, D, f.T, f.n_seq, max_seqlen);
+  if (f.o_low != nullptr)
+    hipLaunchKernelGGL((k_attn_bwd_dq_dma<T, D, BN, QW, true>), attn_grid(nq), dim3(64 * QW), 0, s, b, (int)C,
+                       order);
+  else
+    hipLaunchKernelGGL((k_attn_bwd_dq_dma<T, D, BN, QW, false>), attn_grid(nq), dim3(64 * QW), 0, s, b, (int)C,
+                       order);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int NW = 4, BQ = 32;

@@ -13,8 +13,8 @@ namespace {
 // publishing it and freeing the buffer consumed before). At D = 64 (rows of 128 bytes, 64-key tiles:
 // half the barriers) 12011 tokens in 9 sequences, 14 / 2 heads, bf16, take 64 us, against 121 with K
 // and V staged through registers into padded tiles in the hardware's block order (48 in
-// level_order).
-template <typename T, int D, int BN, int NBUF>
+// level_order). LOW: what o's rounding drops is stored too.
+template <typename T, int D, int BN, int NBUF, bool LOW>
 __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_fwd_swz(const AttnArgs a,
                                                                              int qtiles,
                                                                              int order) {
@@ -103,8 +103,10 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_fwd_swz(con
   if (t < ntiles) tile(t, std::integral_constant<int, 0>{});
 
   if (!wave_live || qi >= end) return;
-  store_rows_t<T, D>(static_cast<T*>(a.o) + (int64_t)qi * a.o_rs + (int64_t)h * D, oacc, hi,
-                     l > 0.f ? 1.f / l : 0.f);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  store_rows_t<T, D>(static_cast<T*>(a.o) + (int64_t)qi * a.o_rs + (int64_t)h * D, oacc, hi, inv);
+  if constexpr (LOW)
+    store_low_t<T, D>(static_cast<T*>(a.o_low) + ((int64_t)qi * a.HQ + h) * D, oacc, hi, inv);
   if (hi == 0 && a.lse != nullptr)
     a.lse[(int64_t)h * a.T + qi] = (m + log2f(l)) * 0.69314718055994531f;
 }
@@ -114,8 +116,13 @@ hipError_t fwd_run(const AttnArgs& a, int max_seqlen, hipStream_t s) {
   const int64_t C = (max_seqlen + kAttnBM - 1) / kAttnBM;
   const int64_t n = xcd_grid(C, (int64_t)a.HQ * a.n_seq);
   if (!attn_grid_ok(n)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_attn_fwd_swz<T, D, BN, 2>), attn_grid(n), dim3(kAttnThreads), 0, s, a,
-                     (int)C, attn_order(n, kFwdPerCU<D>, kRoundsQ, D, a.T, a.n_seq, max_seqlen));
+  const int order = attn_order(n, kFwdPerCU<D>, kRoundsQ, D, a.T, a.n_seq, max_seqlen);
+  if (a.o_low != nullptr)
+    hipLaunchKernelGGL((k_attn_fwd_swz<T, D, BN, 2, true>), attn_grid(n), dim3(kAttnThreads), 0, s, a, (int)C,
+                       order);
+  else
+    hipLaunchKernelGGL((k_attn_fwd_swz<T, D, BN, 2, false>), attn_grid(n), dim3(kAttnThreads), 0, s, a, (int)C,
+                       order);
   return hipGetLastError();
 }
 

@@ -78,10 +78,10 @@ SIGNATURES = {
     "esep_attn_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
                              _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
                              _i32, _i32, _f32, _vp]),
-    "esep_attn_win_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32,
-                                 _i32, _i32, _vp, _i32, _f32, _i32, _i32, _i32, _vp]),
+    "esep_attn_win_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32,
+                                 _i32, _i32, _vp, _i32, _i32, _f32, _i32, _i32, _i32, _vp]),
     "esep_attn_win_bwd_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
-    "esep_attn_win_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
+    "esep_attn_win_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
                                  _i32, _i32, _f32, _i32, _i32, _vp]),
     "esep_attn_cache_workspace": (_i64, [_i32] * 8),
@@ -465,16 +465,24 @@ def attn_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, lse=None, name="_attn_fw
     _record(name)
 
 
-def attn_win_fwd(q, k, v, o, cu_seqlens, scale, window, sinks=0, lse=None, zero_rest=False,
+def _low(o_low, q):
+    if o_low is not None and (o_low.shape != q.shape or o_low.dtype != q.dtype
+                              or o_low.device != q.device or not o_low.is_contiguous()):
+        raise EsepError("o_low must be a contiguous tensor like q")
+    return _p(o_low)
+
+
+def attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks=0, lse=None, o_low=None, zero_rest=False,
                  name="_attn_win_fwd"):
     """attn_fwd through a window (esep_attn_win_fwd): query i sees key j <= i if i - j < window or
-    j < sinks. zero_rest writes o = 0 for the tokens behind the last sequence."""
+    j < sinks. o_low (like q, dense) gets what the rounding of o dropped, for attn_win_bwd; zero_rest
+    writes o = 0 for the tokens behind the last sequence."""
     dev, T, HQ, HK, D = _attn_fwd_checked(q, k, v, o, cu_seqlens, lse)
     with _on(dev):
         rc = lib().esep_attn_win_fwd(
             _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
-            _p(o), _tokens_ld(o, "o"), _p(lse), dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens),
-            cu_seqlens.numel() - 1, float(scale), int(window), int(sinks), int(bool(zero_rest)),
+            _p(o), _tokens_ld(o, "o"), _low(o_low, q), _p(lse), dtype_code(q.dtype), T, HQ, HK, D,
+            _p(cu_seqlens), cu_seqlens.numel() - 1, int(max_seqlen), float(scale), int(window), int(sinks), int(bool(zero_rest)),
             _stream(dev))
     _check(rc, "esep_attn_win_fwd")
     _record(name)
@@ -532,16 +540,17 @@ def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, w
 
 
 def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, window, sinks=0,
-                 workspace=None, name="_attn_win_bwd"):
-    """Backward of attn_win_fwd (esep_attn_win_bwd), as attn_bwd; the gradients of the tokens behind the
-    last sequence are 0. `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
+                 o_low=None, workspace=None, name="_attn_win_bwd"):
+    """Backward of attn_win_fwd (esep_attn_win_bwd), as attn_bwd; o_low as attn_win_fwd wrote it, or None
+    (dq and dk then carry the rounding of o too). The gradients of the tokens behind the last sequence are 0. `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
     dev, (T, HQ, HK, D), workspace = _attn_bwd_checked(
         q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace,
         lambda *sizes: attn_win_bwd_workspace(*sizes, max_seqlen, window, sinks))
     with _on(dev):
         rc = lib().esep_attn_win_bwd(
             _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
-            _p(o), _tokens_ld(o, "o"), _p(dout), _tokens_ld(dout, "dout"), _p(lse), _p(workspace),
+            _p(o), _tokens_ld(o, "o"), _low(o_low, q), _p(dout), _tokens_ld(dout, "dout"), _p(lse),
+            _p(workspace),
             _p(dq), _tokens_ld(dq, "dq"), _p(dk), _tokens_ld(dk, "dk"), _p(dv), _tokens_ld(dv, "dv"),
             dtype_code(q.dtype), T, HQ, HK, D, _p(cu_seqlens), cu_seqlens.numel() - 1,
             int(max_seqlen), float(scale), int(window), int(sinks), _stream(dev))

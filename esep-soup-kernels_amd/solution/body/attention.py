@@ -61,28 +61,36 @@ class VarlenAttention(torch.autograd.Function):
 
 class WindowAttention(torch.autograd.Function):
     """VarlenAttention through a window: apply(q, k, v, cu_seqlens, max_seqlen, scale, window, sinks).
-    The output and the gradients of tokens behind the last sequence are 0."""
+    Saved beside VarlenAttention's: what the rounding of o dropped, so that dq and dk do not carry it. The
+    output and the gradients of tokens behind the last sequence are 0."""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, max_seqlen, scale, window, sinks):
         q, k, v = _heads_packed(q), _heads_packed(k), _heads_packed(v)
         T, HQ, D = q.shape
-        new = torch.empty if cu_seqlens.numel() > 1 else torch.zeros  # no sequence: nothing is launched
+        some = cu_seqlens.numel() > 1 and max_seqlen > 0  # else nothing is launched
+        new = torch.empty if some else torch.zeros
         o = new((T, HQ, D), device=q.device, dtype=q.dtype)
-        lse = torch.empty((HQ, T), device=q.device, dtype=torch.float32)
-        _hip.attn_win_fwd(q, k, v, o, cu_seqlens, scale, window, sinks, lse=lse, zero_rest=True)
-        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        low = lse = None
+        if any(ctx.needs_input_grad):
+            low = torch.empty_like(o)
+            lse = torch.empty((HQ, T), device=q.device, dtype=torch.float32)
+        _hip.attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks, lse=lse, o_low=low,
+                          zero_rest=True)
+        ctx.save_for_backward(q, k, v, o, low, lse, cu_seqlens)
         ctx.args = max_seqlen, scale, window, sinks
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, cu = ctx.saved_tensors
+        q, k, v, o, low, lse, cu = ctx.saved_tensors
         q, k, v, o, do = (_heads_packed(t) for t in (q, k, v, o, do))
-        new = torch.empty if cu.numel() > 1 else torch.zeros
+        new = torch.empty if cu.numel() > 1 and ctx.args[0] > 0 else torch.zeros
         dq, dk, dv = (new(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-        _hip.attn_win_bwd(q, k, v, o, do, lse.contiguous(), dq, dk, dv, cu.contiguous(), *ctx.args)
+        low = low if _hip.dense16(low) else low.contiguous().clone()
+        _hip.attn_win_bwd(q, k, v, o, do, lse.contiguous(), dq, dk, dv, cu.contiguous(), *ctx.args,
+                          o_low=low)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -99,8 +107,9 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
 
     window (None: no bound): query i of a sequence sees key j <= i only if i - j < window (the last
     `window` tokens, its own among them, as HF's sliding_window) or j < sinks (the sequence's
-    first tokens, which stay visible; without a window they always are). Where the window bounds something
-    (window < max_seqlen), tokens behind the last sequence get an output and gradients of 0."""
+    first tokens, which stay visible; without a window they always are). With a window, tokens behind the
+    last sequence get an output and gradients of 0, and dq and dk do not carry the rounding of o. Where
+    window + sinks reach max_seqlen it is the causal kernels that run."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if q.dim() == 4:  # [1, T, H, D] views: the Function works on [T, H, D]
@@ -108,8 +117,7 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
     sinks = _whole("sinks", sinks, 0)
     if window is not None:
         window = _whole("window", window, 1)
-        if window < max_seqlen:
-            return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
+        return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
     return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))
 
 

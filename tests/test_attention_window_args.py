@@ -10,14 +10,14 @@ from solution.body.attention import varlen_attention
 
 
 def _fwd(**kw):
-    a = dict(q=16, q_rs=256, k=16, k_rs=128, v=16, v_rs=128, o=16, o_rs=256, lse=None, dt=1, T=10, HQ=4,
-             HK=2, D=64, cu=16, n_seq=1, scale=0.1, window=4, sinks=1, zero_rest=0, stream=None)
+    a = dict(q=16, q_rs=256, k=16, k_rs=128, v=16, v_rs=128, o=16, o_rs=256, low=None, lse=None, dt=1, T=10, HQ=4,
+             HK=2, D=64, cu=16, n_seq=1, max_seqlen=10, scale=0.1, window=4, sinks=1, zero_rest=0, stream=None)
     a.update(kw)
     return _hip.lib().esep_attn_win_fwd(*a.values())
 
 
 def _bwd(**kw):
-    a = dict(q=16, q_rs=256, k=16, k_rs=128, v=16, v_rs=128, o=16, o_rs=256, dout=16, do_rs=256, lse=16,
+    a = dict(q=16, q_rs=256, k=16, k_rs=128, v=16, v_rs=128, o=16, o_rs=256, low=16, dout=16, do_rs=256, lse=16,
              ws=16, dq=16, dq_rs=256, dk=16, dk_rs=128, dv=16, dv_rs=128, dt=1, T=10, HQ=4, HK=2, D=64,
              cu=16, n_seq=1, max_seqlen=10, scale=0.1, window=4, sinks=1, stream=None)
     a.update(kw)
@@ -37,6 +37,7 @@ def test_refusals(call):
     assert call(k_rs=(1 << 22) + 8) == -2
     assert call(q=None) == -1 and call(cu=None) == -1
     assert call(v=8) == -3 and call(k_rs=129) == -3
+    assert call(low=8) == -3 and b"o_low" in err()
     assert call(scale=0.0) == -1
     assert call(T=0) == 0 and call(n_seq=0) == 0
 
@@ -55,9 +56,11 @@ def test_workspace():
     assert base in (5000 * 4, 5000 * 4 + 2 * 2 * 5000 * 2 * 64)
     assert ws(5000, 4, 2, 64, 612, 100, 4) == base  # no sequence long enough for far queries
     assert ws(5000, 4, 2, 64, 613, 100, 4) > base
-    # no more sink rows than a sequence has
-    assert ws(5000, 4, 2, 64, 700, 100, 700) == ws(5000, 4, 2, 64, 700, 100, 1 << 30)
+    assert ws(5000, 4, 2, 64, 700, 100, 599) > ws(5000, 4, 2, 64, 700, 100, 4)
     assert ws(0, 4, 2, 64, 1, 1, 0) == 0
+    # a window and sinks that leave nothing out: the causal backward's
+    for window, sinks in ((700, 0), (1 << 30, 5), (100, 600)):
+        assert ws(5000, 4, 2, 64, 700, window, sinks) == _hip.attn_bwd_workspace(5000, 4, 2, 64)
 
 
 @pytest.mark.parametrize("kw", [dict(window=0), dict(window=-3), dict(window=2.5), dict(window=True),

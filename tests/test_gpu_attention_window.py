@@ -7,7 +7,8 @@ sums taken over the keys (or queries) that the definition lets through:
       u (sum p |v| + |o|)
   dv  the same with dO: u (sum p |do| + |dv|)
   dq  dS is rounded (u), and delta = rowsum(dO o) sees the o above, so each dS is off by p sum |do| |o's error|:
-      scale (u sum |ds| |k| + sum p |k| E) + u |dq|, E = u sum_d |do| (sum p |v| + |o|)
+      scale (u sum |ds| |k| + sum p |k| E) + u |dq|, E = u sum_d |do| (sum p |v| + |o|); with o_low, o's own
+      rounding is not in it: E = u sum_d |do| (sum p |v|) + u^2 |do| |o|
   dk  the same over queries.
 fp16 holds small probabilities and dS as subnormals, 2^-25 off at most: 2^-25 times the sum of |v| (|do|, |k|,
 |q|). The 32-bit arithmetic (scores of up to about 30, their exponentials, sums) adds less than 4e-5 of the same
@@ -39,8 +40,8 @@ CASES = [
 ]
 
 
-def _reference(q, k, v, do, lengths, scale, window, sinks, u, sub):
-    """(o, dq, dk, dv) in float64 and their bounds."""
+def _reference(q, k, v, do, lengths, scale, window, sinks, u, sub, low=True):
+    """(o, dq, dk, dv) in float64 and their bounds (low: the backward has o_low)."""
     q, k, v, do = (t.double() for t in (q, k, v, do))
     res = [torch.zeros_like(t) for t in (q, q, k, v)]
     tol = [torch.zeros_like(t) for t in (q, q, k, v)]
@@ -66,7 +67,7 @@ def _reference(q, k, v, do, lengths, scale, window, sinks, u, sub):
             res[2][s, kh] += scale * ds.t() @ Q
             res[3][s, kh] += p.t() @ DO
             eo = f * (p @ V.abs() + o.abs()) + sub * (w @ V.abs())
-            E = (DO.abs() * eo).sum(1, keepdim=True)
+            E = (DO.abs() * (eo - (u - u * u) * o.abs() if low else eo)).sum(1, keepdim=True)
             tol[0][s, h] = eo
             tol[1][s, h] = (scale * (f * ds.abs() + p * E + sub * w) @ K.abs()
                             + f * res[1][s, h].abs())
@@ -115,19 +116,24 @@ def test_window_vs_float64(case, dtype):
     q, k, v, do, cu = _inputs(lengths, HQ, HK, D, dtype, 300 + case)
     scale = D ** -0.5
     ref, tol = _reference(q, k, v, do, lengths, scale, window, sinks, *_limits(dtype))
-    # the entries themselves, also where varlen_attention would leave the window out
     o = torch.full_like(q, float("nan"))
     lse = torch.full((HQ, q.shape[0]), float("nan"), device=DEV)
-    _hip.attn_win_fwd(q, k, v, o, cu, scale, window, sinks, lse=lse)
+    low = torch.full_like(q, float("nan"))
+    _hip.attn_win_fwd(q, k, v, o, cu, max(lengths), scale, window, sinks, lse=lse, o_low=low)
     grads = [torch.full_like(t, float("nan")) for t in (q, k, v)]
-    _hip.attn_win_bwd(q, k, v, o, do, lse, *grads, cu, max(lengths), scale, window, sinks)
+    back = (q, k, v, o, do, lse, *grads, cu, max(lengths), scale, window, sinks)
+    _hip.attn_win_bwd(*back)
+    _check([o, *grads], ref, _reference(q, k, v, do, lengths, scale, window, sinks, *_limits(dtype),
+                                        low=False)[1], CASES[case])
+    _hip.attn_win_bwd(*back, o_low=low)
     _check([o, *grads], ref, tol, CASES[case])
+    assert ((o.double() + low.double() - ref[0]).abs() <= tol[0]).all()
     again = _run(q, k, v, do, cu, max(lengths), window=window, sinks=sinks)
-    if window < max(lengths):
-        for a, b in zip([o, *grads], again):
-            assert torch.equal(a, b)  # the public entry, and the same bits twice
-    else:
-        _check(again, ref, tol, CASES[case])
+    for a, b in zip([o, *grads], again):
+        assert torch.equal(a, b)  # the public entry, and the same bits twice
+    # a looser bound on the lengths: the windowed kernels also where nothing is left out
+    _check(_run(q, k, v, do, cu, max(lengths) + window + sinks, window=window, sinks=sinks), ref, tol,
+           CASES[case])
 
 
 @pytest.mark.parametrize("n_seq", [65, 200, 700])
@@ -149,8 +155,9 @@ def test_longer_bound_and_scale():
     _check(_run(q, k, v, do, cu, 30000, scale=0.2, window=90, sinks=6), ref, tol, "bound")
 
 
+@pytest.mark.parametrize("window", [60, 200])
 @pytest.mark.parametrize("tail", [1, 127, 128, 3000])
-def test_tokens_behind_the_last_sequence(tail):
+def test_tokens_behind_the_last_sequence(tail, window):
     """They get an output and gradients of 0 from varlen_attention, whatever they hold; the entry itself
     leaves their output as it was."""
     from solution.body import _hip
@@ -160,12 +167,12 @@ def test_tokens_behind_the_last_sequence(tail):
     n = 190
     for t in (q, k, v, do):
         t[n:] = float("nan")
-    got = _run(q, k, v, do, cu, 150, window=60, sinks=3)
-    alone = _run(*(t[:n] for t in (q, k, v, do)), cu, 150, window=60, sinks=3)
+    got = _run(q, k, v, do, cu, 150, window=window, sinks=3)
+    alone = _run(*(t[:n] for t in (q, k, v, do)), cu, 150, window=window, sinks=3)
     for a, b in zip(got, alone):
         assert torch.equal(a[:n], b) and not a[n:].any()
     o = torch.full_like(q, 7.0)
-    _hip.attn_win_fwd(q, k, v, o, cu, 128 ** -0.5, 60, 3)
+    _hip.attn_win_fwd(q, k, v, o, cu, 150, 128 ** -0.5, window, 3)
     assert torch.equal(o[:n], alone[0]) and (o[n:] == 7.0).all()
 
 
@@ -270,8 +277,10 @@ def test_window_of_everything_is_causal():
     lengths = [200, 90]
     q, k, v, do, cu = _inputs(lengths, 4, 2, 128, torch.bfloat16, 15)
     want = _run(q, k, v, do, cu, 200)
-    for a, b in zip(_run(q, k, v, do, cu, 200, window=200, sinks=9), want):
-        assert torch.equal(a, b)
+    got = _run(q, k, v, do, cu, 200, window=200, sinks=9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])  # o and dv
+    ref, tol = _reference(q, k, v, do, lengths, 128 ** -0.5, None, 0, 2.0 ** -8, 0.0)
+    _check(got, ref, tol, "causal")  # dq and dk without o's rounding
 
 
 def test_empty_inputs():

@@ -5,7 +5,7 @@ through torch's operations; what still goes to the original forward."""
 import pytest
 import torch
 
-from test_gpu_packed import (L, LENS, VOCAB, _batch, _compare, _config, _counts, _original_forward,
+from test_gpu_packed import (LENS, VOCAB, _batch, _compare, _config, _counts, _original_forward,
                              _run)
 
 pytestmark = pytest.mark.gpu
@@ -90,7 +90,7 @@ def test_a_layer_that_differs_from_the_config_takes_the_original_forward():
     assert not names
 
 
-def test_window_past_the_rows_is_the_causal_kernel():
+def test_window_past_the_rows_is_full_attention():
     from solution.body import _hip, patch
 
     patch()
@@ -98,5 +98,11 @@ def test_window_past_the_rows_is_the_causal_kernel():
     ids, mask, _ = _batch()
     with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16), _hip.count_launches() as names:
         base(input_ids=ids, attention_mask=mask, use_cache=False)
-    assert names.count("_attn_fwd") == 3 and "_attn_win_fwd" not in names
-    assert L > max(LENS)
+    assert names.count("_attn_fwd") == 1 and names.count("_attn_win_fwd") == 2
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+        got = base(input_ids=ids, attention_mask=mask, use_cache=False).last_hidden_state
+        for layer in base.layers:
+            layer.self_attn.sliding_window = None
+        base.config.layer_types = ["full_attention"] * 3
+        want = base(input_ids=ids, attention_mask=mask, use_cache=False).last_hidden_state
+    assert torch.equal(got, want)
