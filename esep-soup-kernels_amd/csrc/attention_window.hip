@@ -3,9 +3,9 @@
 // kernels (attention.hpp, attention_tiles.hpp); what differs is which tiles a block walks, what a
 // query sees, and where the blocks run.
 //
-// Forward and dQ: a block of 128 queries q0 .. q0 + 127 walks the tiles of the sinks, then those of keys
-// q0 - window + 1 .. q0 + 127 (one run of tiles where the two meet). A wavefront skips the 32-key
-// steps that none of its queries sees, and masks only where a border crosses.
+// Forward and dQ: a block (4 x 32 queries of one kv head, WinItem) of queries q0 .. q1 - 1 walks the tiles of the
+// sinks, then those of keys q0 - window + 1 .. q1 - 1 (one run of tiles where the two meet). A wavefront skips
+// the 32-key steps that none of its queries sees, and masks only where a border crosses.
 //
 // dK / dV: a block of 128 keys walks the queries k0 .. k0 + 127 + window - 1. A sink key is also seen by every
 // query after that: in a long sequence 32 times as many as another key, which one block would walk
@@ -22,9 +22,9 @@
 //
 // All blocks of a launch do near-equal work, so no order by length is needed: the (sequence, tile,
 // head) triples are numbered with the heads innermost and cut into 8 contiguous runs, one to an XCD,
-// where neighbouring tiles and the heads of a kv head share K and V in the L2. A sequence's tiles
-// start at number cu[s] / 128 + s, which never overlap and need no sums over the other sequences; the
-// grid is T / 128 + n_seq tiles whatever max_seqlen is.
+// where neighbouring tiles and the heads of a kv head share K and V in the L2. A sequence's tiles start at a
+// number that its offset gives (WinBase), which never overlap and need no sums over the other sequences; the grid
+// is sized by T and n_seq whatever max_seqlen is.
 #include <cmath>
 #include <type_traits>
 
@@ -56,7 +56,21 @@ __device__ __forceinline__ int win_search(int n_seq, int p, Base&& base) {
   return lo;
 }
 
-// A block's (sequence, 128-row tile, head) among H heads, or a number among the spare blocks.
+// The blocks of a sequence that starts at token c are numbered from c * per / 128 + s * pad: per (blocks per
+// 128 tokens) and pad such that no sequence has more blocks than numbers.
+struct WinBase {
+  int per, pad;
+  __host__ __device__ __forceinline__ int64_t at(int64_t c, int64_t s) const {
+    return ((c * per) >> 7) + s * pad;
+  }
+};
+// 128 keys a block.
+constexpr WinBase kWinKeys{1, 1};
+// 4 of a sequence's ceil(len / 32) * G items a block: at most G len / 128 + 31 G / 128 + 127 / 128 blocks, and
+// two floors are up to 127 / 128 less than G len / 128 apart.
+__host__ __device__ __forceinline__ WinBase win_queries(int G) { return {G, (31 * G + 254) / 128}; }
+
+// A block's (sequence, tile, head) among H heads, or a number among the spare blocks.
 struct WinPlace {
   int seq, tile, head;   // seq < 0: no work
   int start, end;        // the sequence's tokens
@@ -64,13 +78,13 @@ struct WinPlace {
   int spare, n_spare;    // spare >= 0: one of n_spare blocks without a tile (8 or more of them)
 };
 __device__ __forceinline__ WinPlace win_place(int b, int nblk, int H, const int32_t* cu, int n_seq,
-                                              int64_t T) {
+                                              int64_t T, WinBase base) {
   // the offsets of up to 63 sequences in one read, a lane each: a block's place then costs one trip to memory
   const int lane = (int)(threadIdx.x & 63);
   const bool few = n_seq < 64;
   const int mine = few ? cu_at(cu, lane < n_seq ? lane : n_seq, T) : 0;
   const int rest = few ? __builtin_amdgcn_readlane(mine, n_seq) : cu_at(cu, n_seq, T);
-  const int live = (rest / kAttnBM + n_seq) * H;
+  const int live = (int)base.at(rest, n_seq) * H;
   const int per = (live + 7) / 8, xcd = b & 7, slot = b >> 3;
   WinPlace w{-1, 0, 0, 0, 0, rest, -1, nblk - 8 * per};
   if (slot >= per) {
@@ -82,24 +96,24 @@ __device__ __forceinline__ WinPlace win_place(int b, int nblk, int H, const int3
   const int p = i / H;
   int s;
   if (few) {
-    s = __popcll(__ballot(lane < n_seq && mine / kAttnBM + lane <= p)) - 1;
+    s = __popcll(__ballot(lane < n_seq && base.at(mine, lane) <= p)) - 1;
     if (s < 0) return w;
     w.start = __builtin_amdgcn_readlane(mine, s);
     w.end = __builtin_amdgcn_readlane(mine, s + 1);
   } else {
-    s = win_search(n_seq, p, [&](int j) { return cu_at(cu, j, T) / kAttnBM + j; });
+    s = win_search(n_seq, p, [&](int j) { return base.at(cu_at(cu, j, T), j); });
     if (s < 0) return w;
     w.start = cu_at(cu, s, T);
     w.end = cu_at(cu, s + 1, T);
   }
   if (w.end < w.start) w.end = w.start;
   w.seq = s;
-  w.tile = p - (w.start / kAttnBM + s);
+  w.tile = p - (int)base.at(w.start, s);
   w.head = i - p * H;
   return w;
 }
-inline int64_t win_blocks(int64_t T, int n_seq, int64_t H) {
-  return ((T / kAttnBM + n_seq) * H + 7) / 8 * 8 + 8;
+inline int64_t win_blocks(int64_t T, int n_seq, int64_t H, WinBase base) {
+  return (base.at(T, n_seq) * H + 7) / 8 * 8 + 8;
 }
 
 // out = 0 for the tokens behind the last sequence (W elements each, W a multiple of 8), dealt to the
@@ -116,15 +130,33 @@ __device__ __forceinline__ void zero_rest(T* out, int64_t rs, int W, int from, i
   }
 }
 
-// The key tiles of a block of queries q0 ..: `ns` tiles of the sinks from `start`, then tiles from `lo` to
+// A wavefront's 32 queries of one head. A block's 4 wavefronts take 4 of a kv head's (32 queries, head) items,
+// the heads innermost: with 3 and more query heads to a kv head a block spans at most 64 queries, and walks
+// window + 64 keys where 128 queries of one head walk window + 128 (of which a wavefront sees window + 32). 32768
+// tokens in 4 sequences, 28 / 4 heads, window 128, bf16: forward 171 us against 200, backward 614 against 708;
+// 65536 tokens at window 1024 869 against 912 and 3047 against 3104.
+struct WinItem {
+  int q0, q1;   // the block's queries
+  int qw0, h;   // the wavefront's first query (past the end: none) and head
+  __device__ __forceinline__ WinItem(const WinPlace& pl, int G, int w) {
+    const int n = (pl.end - pl.start + 31) / 32;
+    const int s0 = 4 * pl.tile / G, s1 = (4 * pl.tile + 3) / G, i = 4 * pl.tile + w, s = i / G;
+    q0 = s0 < n ? pl.start + 32 * s0 : pl.end;
+    q1 = s1 + 1 < n ? pl.start + 32 * (s1 + 1) : pl.end;
+    qw0 = s < n ? pl.start + 32 * s : pl.end;
+    h = pl.head * G + i - s * G;
+  }
+};
+
+// The key tiles of a block of queries q0 .. q1 - 1: `ns` tiles of the sinks from `start`, then tiles from `lo` to
 // kend. Where the sinks reach the window they are one run.
 struct KeyWalk {
   int start, lo, kend, sink_hi, ns, n;
   template <int BN>
-  __device__ __forceinline__ void init(int start_, int end, int q0, int window, int sinks) {
+  __device__ __forceinline__ void init(int start_, int end, int q0, int q1, int window, int sinks) {
     start = start_;
     sink_hi = start + (sinks < end - start ? sinks : end - start);
-    kend = end < q0 + kAttnBM ? end : q0 + kAttnBM;
+    kend = q1;
     lo = q0 - window + 1;
     if (lo <= sink_hi) lo = start;
     ns = lo > start ? (sink_hi - start + BN - 1) / BN : 0;
@@ -190,17 +222,18 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_win_fwd(con
   const AttnArgs& a = p.b.f;
   __shared__ __align__(1024) char kv[2][2][BN * 2 * D];  // [buffer][K, V][swizzled rows]
 
-  const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HQ, a.cu, a.n_seq, a.T);
+  const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HK, a.cu, a.n_seq, a.T,
+                                win_queries(a.HQ / a.HK));
   if (pl.spare >= 0 && p.zero_rest)
     zero_rest<T>(static_cast<T*>(a.o), a.o_rs, a.HQ * D, pl.rest, a.T, pl);
   if (pl.seq < 0) return;
   const int start = pl.start, end = pl.end;
-  const int q0 = start + pl.tile * kAttnBM, h = pl.head;
-  if (q0 >= end) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const WinItem it(pl, a.HQ / a.HK, w);
+  if (it.q0 >= end) return;
   const int lq = lane & 31, hi = lane >> 5;
-  const int qw0 = q0 + 32 * w, qi = qw0 + lq;
+  const int h = it.h, qw0 = it.qw0, qi = qw0 + lq;
 
   V8 qb[D / 16];
   {
@@ -214,8 +247,8 @@ __global__ __launch_bounds__(kAttnThreads, kFwdPerCU<D>) void k_attn_win_fwd(con
   for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
   float m = -INFINITY, l = 0.f;
   KeyWalk kw;
-  kw.init<BN>(start, end, q0, p.window, p.sinks);
-  walk_keys<T, D, BN>(a, kw, h / (a.HQ / a.HK), p.window, kv, lane, w, qw0, qi, end,
+  kw.init<BN>(start, end, it.q0, it.q1, p.window, p.sinks);
+  walk_keys<T, D, BN>(a, kw, pl.head, p.window, kv, lane, w, qw0, qi, end,
                       [&](const char* ks, const char* vs, int kh, int utop, int top)
                           __attribute__((always_inline)) {
                         fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
@@ -240,17 +273,18 @@ __global__ __launch_bounds__(kAttnThreads, kDqPerCU<D>) void k_attn_win_dq(const
   const AttnArgs& a = b.f;
   __shared__ __align__(1024) char kv[2][2][BN * 2 * D];
 
-  const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HQ, a.cu, a.n_seq, a.T);
+  const WinPlace pl = win_place(attn_block(), (int)(gridDim.x * gridDim.y), a.HK, a.cu, a.n_seq, a.T,
+                                win_queries(a.HQ / a.HK));
   if (pl.spare >= 0)
     zero_rest<T>(static_cast<T*>(b.dq), b.dq_rs, a.HQ * D, pl.rest, a.T, pl);
   if (pl.seq < 0) return;
   const int start = pl.start, end = pl.end;
-  const int q0 = start + pl.tile * kAttnBM, h = pl.head;
-  if (q0 >= end) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const WinItem it(pl, a.HQ / a.HK, w);
+  if (it.q0 >= end) return;
   const int lq = lane & 31, hi = lane >> 5;
-  const int qw0 = q0 + 32 * w, qi = qw0 + lq;
+  const int h = it.h, qw0 = it.qw0, qi = qw0 + lq;
   const bool qok = qi < end;
 
   V8 qb[D / 16], db[D / 16];
@@ -280,8 +314,8 @@ __global__ __launch_bounds__(kAttnThreads, kDqPerCU<D>) void k_attn_win_dq(const
 #pragma unroll
   for (int md = 0; md < D / 32; ++md) dqa[md] = f32x16{};
   KeyWalk kw;
-  kw.init<BN>(start, end, q0, p.window, p.sinks);
-  walk_keys<T, D, BN>(a, kw, h / (a.HQ / a.HK), p.window, kv, lane, w, qw0, qi, end,
+  kw.init<BN>(start, end, it.q0, it.q1, p.window, p.sinks);
+  walk_keys<T, D, BN>(a, kw, pl.head, p.window, kv, lane, w, qw0, qi, end,
                       [&](const char* ks, const char* vs, int kh, int utop, int top)
                           __attribute__((always_inline)) {
                         dq_tile_swz<T, D>(ks, vs, lane, a.scale_log2, lse2, delta, qb, db, dqa,
@@ -420,7 +454,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
   if (far && !p.far) return;
   int seq, kh, part, tile, chunk = 0, gs, start = 0, end = 0;
   if (!far) {
-    const WinPlace pl = win_place(bid, p.n_main, a.HK * b.split, a.cu, a.n_seq, a.T);
+    const WinPlace pl = win_place(bid, p.n_main, a.HK * b.split, a.cu, a.n_seq, a.T, kWinKeys);
     if (pl.spare >= 0) {
       zero_rest<T>(static_cast<T*>(b.dk), b.dk_rs, a.HK * D, pl.rest, a.T, pl);
       zero_rest<T>(static_cast<T*>(b.dv), b.dv_rs, a.HK * D, pl.rest, a.T, pl);
@@ -675,7 +709,7 @@ constexpr int64_t kWinMaxSums = (int64_t{1} << 24) - 1;
 template <typename T, int D>
 hipError_t fwd_run(const AttnWinArgs& p, hipStream_t s) {
   const AttnArgs& f = p.b.f;
-  const int64_t n = win_blocks(f.T, f.n_seq, f.HQ);
+  const int64_t n = win_blocks(f.T, f.n_seq, f.HK, win_queries(f.HQ / f.HK));
   if (!attn_grid_ok(n)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((k_attn_win_fwd<T, D, D == 128 ? 32 : 64>), attn_grid(n), dim3(kAttnThreads), 0, s,
                      p);
@@ -686,8 +720,8 @@ template <typename T, int D>
 hipError_t bwd_run(const AttnWinArgs& a, hipStream_t s) {
   AttnWinArgs p = a;
   const AttnArgs& f = p.b.f;
-  const int64_t nq = win_blocks(f.T, f.n_seq, f.HQ);
-  const int64_t nk = win_blocks(f.T, f.n_seq, (int64_t)f.HK * p.b.split);
+  const int64_t nq = win_blocks(f.T, f.n_seq, f.HK, win_queries(f.HQ / f.HK));
+  const int64_t nk = win_blocks(f.T, f.n_seq, (int64_t)f.HK * p.b.split, kWinKeys);
   const int64_t per = (int64_t)((p.sinks + kAttnBM - 1) / kAttnBM) * f.HK * p.far_split;
   const int64_t nfar = p.far ? win_far_slots(f.T, p.window) * per : 0;
   const int64_t nsum = p.far ? win_main_slots(f.T, p.window) * f.HK * 2 * p.sinks : 0;

@@ -37,6 +37,10 @@ CASES = [
     ([700], 2, 1, 64, 100, 650),                # a tile of sinks that no far query sees
     ([1300], 2, 1, 128, 40, 1300),              # all sinks: causal
     ([2100], 3, 1, 64, 1, 1),
+    ([95, 33, 0, 1, 250, 32], 10, 2, 128, 20, 2),  # items of several heads to a block
+    ([70, 129, 31, 160], 16, 1, 64, 50, 0),
+    ([257, 64, 31, 97], 9, 3, 128, 32, 5),
+    ([40] * 70 + [0] * 3 + [33], 5, 1, 64, 17, 1),
 ]
 
 
