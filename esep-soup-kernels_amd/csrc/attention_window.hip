@@ -25,6 +25,11 @@
 // where neighbouring tiles and the heads of a kv head share K and V in the L2. A sequence's tiles start at a
 // number that its offset gives (WinBase), which never overlap and need no sums over the other sequences; the grid
 // is sized by T and n_seq whatever max_seqlen is.
+//
+// Bound by SIMD issue (MFMAs and softmax arithmetic of a wavefront overlap little), and by a block's start where
+// its walk is short. In bf16, 12 / 2 heads of 128: 32768 tokens, window 4096, 4 sinks forward 797 us (0.97
+// PFLOP/s), backward 2766 (0.70, counting 10 D per pair; S and dP are computed twice, 14 D run); 5933 tokens in 8
+// sequences, window 256 25 (0.31) and 104 (0.19).
 #include <cmath>
 #include <type_traits>
 

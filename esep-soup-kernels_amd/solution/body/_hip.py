@@ -472,8 +472,8 @@ def _low(o_low, q):
     return _p(o_low)
 
 
-def attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks=0, lse=None, o_low=None, zero_rest=False,
-                 name="_attn_win_fwd"):
+def attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks=0, lse=None, o_low=None,
+                 zero_rest=False, name="_attn_win_fwd"):
     """attn_fwd through a window (esep_attn_win_fwd): query i sees key j <= i if i - j < window or
     j < sinks. o_low (like q, dense) gets what the rounding of o dropped, for attn_win_bwd; zero_rest
     writes o = 0 for the tokens behind the last sequence."""
@@ -482,8 +482,8 @@ def attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks=0, lse
         rc = lib().esep_attn_win_fwd(
             _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),
             _p(o), _tokens_ld(o, "o"), _low(o_low, q), _p(lse), dtype_code(q.dtype), T, HQ, HK, D,
-            _p(cu_seqlens), cu_seqlens.numel() - 1, int(max_seqlen), float(scale), int(window), int(sinks), int(bool(zero_rest)),
-            _stream(dev))
+            _p(cu_seqlens), cu_seqlens.numel() - 1, int(max_seqlen), float(scale), int(window), int(sinks),
+            int(bool(zero_rest)), _stream(dev))
     _check(rc, "esep_attn_win_fwd")
     _record(name)
 
@@ -542,7 +542,8 @@ def attn_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, w
 def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scale, window, sinks=0,
                  o_low=None, workspace=None, name="_attn_win_bwd"):
     """Backward of attn_win_fwd (esep_attn_win_bwd), as attn_bwd; o_low as attn_win_fwd wrote it, or None
-    (dq and dk then carry the rounding of o too). The gradients of the tokens behind the last sequence are 0. `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
+    (dq and dk then carry the rounding of o too). The gradients of the tokens behind the last sequence are 0.
+    `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
     dev, (T, HQ, HK, D), workspace = _attn_bwd_checked(
         q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace,
         lambda *sizes: attn_win_bwd_workspace(*sizes, max_seqlen, window, sinks))

@@ -275,11 +275,11 @@ int esep_attn_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, cons
  * sequence sees key j <= i of it if i - j < window or j < sinks, positions counted within the sequence. The
  * reference has no counterpart: it hands models with sliding-window layers to their original forward
  * (solution/body/packed.py:736-771).
- *   window >= 1, sinks >= 0   where window + sinks >= max_seqlen, esep_attn_fwd's kernels run, and its bits come
- *   o_low [T, HQ, D] or NULL  dense, dt: what the rounding of o dropped, for the backward (its delta = rowsum(dout * o)
- *                             is otherwise off by o's rounding, as esep_attn_bwd's is)
+ *   window >= 1, sinks >= 0   where window + sinks >= max_seqlen nothing is left out: esep_attn_fwd's kernels run
+ *   max_seqlen                >= every sequence length
+ *   o_low [T, HQ, D] or NULL  dense, dt: what the rounding of o dropped, for the backward (whose delta =
+ *                             rowsum(dout * o) is otherwise off by o's rounding, as esep_attn_bwd's is)
  *   zero_rest                 nonzero: o = 0 for the tokens behind the last sequence; 0: left as they are
- * Otherwise the launch is sized by T and n_seq alone.
  */
 int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
                       int64_t v_rs, void* o, int64_t o_rs, void* o_low, float* lse, int dt, int64_t T, int HQ,
@@ -287,10 +287,10 @@ int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
                       int window, int sinks, int zero_rest, void* stream);
 
 /*
- * Its backward, deterministic (esep_attn_bwd's arguments; o_low as the forward wrote it, or NULL). workspace: fp32, 16-byte aligned,
- * esep_attn_win_bwd_workspace floats, a function of the sizes only; max_seqlen >= every sequence length
- * (a sequence past it gets wrong gradients of its sink keys). dq, dk and dv are 0 for the tokens behind the
- * last sequence. ESEP_ESHAPE where the sink rows are more than one launch takes.
+ * Its backward, deterministic (esep_attn_bwd's arguments; o_low as the forward wrote it, or NULL). workspace:
+ * fp32, 16-byte aligned, esep_attn_win_bwd_workspace floats, a function of the sizes only; max_seqlen >= every
+ * sequence length, as the forward's. dq, dk and dv are 0 for the tokens behind the last sequence. ESEP_ESHAPE
+ * where the sink rows are more than one launch takes.
  */
 int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int max_seqlen, int window,
                                     int sinks);
