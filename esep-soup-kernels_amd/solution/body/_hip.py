@@ -16,6 +16,7 @@ reference's tests wrap JITFunction.run (reference solution/test_body_norm_rope.p
 import contextlib
 import ctypes
 import threading
+from array import array
 from pathlib import Path
 
 import torch
@@ -562,9 +563,11 @@ def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scal
 def _bth_strides(t, name):
     """(batch, token, head) strides of a [B, n, H, D] tensor with a dense head dim, as the kernel takes
     them: multiples of 8 (a dimension of one element has any)."""
-    if t.stride(3) != 1:
+    b, n, h, d = t.stride()
+    if d != 1:
         raise EsepError(f"{name} needs a unit stride on the head dim")
-    return _I64x3(*(s if d > 1 else 0 for s, d in zip(t.stride()[:3], t.shape)))
+    B, N, H, _ = t.shape
+    return b if B > 1 else 0, n if N > 1 else 0, h if H > 1 else 0
 
 
 def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None, name="_attn_cache"):
@@ -574,9 +577,10 @@ def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None,
     dev = _dev(q, k, v, o, lengths, workspace)
     if q.dim() != 4 or k.dim() != 4:
         raise EsepError("attn_cache: q [B, n, HQ, D] and k, v [B, S, HK, D]")
-    B, n, HQ, D = q.shape
-    S, HK = k.shape[1], k.shape[2]
-    if k.shape != (B, S, HK, D) or v.shape != k.shape or o.shape != q.shape or not o.is_contiguous():
+    shape, kshape = q.shape, k.shape
+    B, n, HQ, D = shape
+    S, HK = kshape[1], kshape[2]
+    if kshape != (B, S, HK, D) or v.shape != kshape or o.shape != shape or not o.is_contiguous():
         raise EsepError("attn_cache: q, o [B, n, HQ, D] (o dense) and k, v [B, S, HK, D]")
     dt = q.dtype
     if k.dtype != dt or v.dtype != dt or o.dtype != dt:
@@ -590,11 +594,12 @@ def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None,
     elif (workspace.dtype != torch.float32 or not workspace.is_contiguous()
           or workspace.numel() < need):
         raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
+    strides = array("q", (*_bth_strides(q, "q"), *_bth_strides(k, "k"), *_bth_strides(v, "v")))
+    at = strides.buffer_info()[0]
     with _on(dev):
         rc = lib().esep_attn_cache(
-            _p(q), _bth_strides(q, "q"), _p(k), _bth_strides(k, "k"), _p(v), _bth_strides(v, "v"), _p(o),
-            _p(lengths), _p(workspace), code, B, n, S, HQ, HK, D, float(scale), w, int(sinks),
-            _stream(dev))
+            q.data_ptr(), at, k.data_ptr(), at + 24, v.data_ptr(), at + 48, o.data_ptr(), lengths.data_ptr(),
+            workspace.data_ptr(), code, B, n, S, HQ, HK, D, float(scale), w, int(sinks), _stream(dev))
     _check(rc, "esep_attn_cache")
     _record(name)
 
@@ -883,12 +888,6 @@ def nf4_dequant_multi(items, name="_nf4_dequant_multi"):
     _record(name)
 
 
-class Nf4MatvecWeight(ctypes.Structure):
-    """esep_nf4_matvec_weight (include/esep_body.h)."""
-    _fields_ = [("packed", _vp), ("absmax", _vp), ("absmax2", _vp), ("code2", _vp),
-                ("offset", _vp), ("nf4", _vp), ("bias", _vp), ("N", _i64)]
-
-
 NF4_MATVEC_ROWS = 16
 
 
@@ -900,32 +899,33 @@ def nf4_matvec(x, items, y, name="_nf4_matvec"):
         raise EsepError(f"1..{NF4_MULTI_MAX} weights per launch")
     dev = _dev(x, y, *[t for it in items for t in it[:7]])
     M, K = x.shape
-    arr = (Nf4MatvecWeight * len(items))()
-    cols = 0
-    for i, (packed, absmax, absmax2, code2, offset, nf4, bias, n) in enumerate(items):
+    dt, f32 = x.dtype, torch.float32
+    words, cols = [], 0  # esep_nf4_matvec_weight's: seven addresses and N
+    for packed, absmax, absmax2, code2, offset, nf4, bias, n in items:
         nb = absmax.numel()
-        if (packed.dtype != torch.uint8 or packed.numel() != nb * 32 or absmax.dtype != torch.uint8
+        if (packed.dtype is not torch.uint8 or packed.numel() != nb * 32 or absmax.dtype is not torch.uint8
                 or nb * 64 != n * K):
             raise EsepError("packed must hold n_blocks * 32 uint8, absmax n_blocks uint8 and n_blocks * 64 "
                             "be the weight's size")
         for t in (absmax2, code2, offset, nf4):
-            if t.dtype != torch.float32 or not t.is_contiguous():
+            if t.dtype is not f32 or not t.is_contiguous():
                 raise EsepError("absmax2, code2, offset and nf4 must be contiguous fp32 tensors")
         if (absmax2.numel() < (nb + 255) // 256 or code2.numel() < 256 or nf4.numel() < 16
                 or offset.numel() < 1):
             raise EsepError("nf4 tables too small")
         if not (packed.is_contiguous() and absmax.is_contiguous()):
             raise EsepError("packed and absmax must be contiguous")
-        if bias is not None and (bias.dtype != x.dtype or bias.numel() != n or not bias.is_contiguous()):
+        if bias is not None and (bias.dtype is not dt or bias.numel() != n or not bias.is_contiguous()):
             raise EsepError("bias must be a contiguous [N] tensor of x's dtype")
-        arr[i] = Nf4MatvecWeight(packed.data_ptr(), absmax.data_ptr(), absmax2.data_ptr(),
-                                 code2.data_ptr(), offset.data_ptr(), nf4.data_ptr(), _p(bias), n)
+        words += (packed.data_ptr(), absmax.data_ptr(), absmax2.data_ptr(), code2.data_ptr(), offset.data_ptr(),
+                  nf4.data_ptr(), 0 if bias is None else bias.data_ptr(), n)
         cols += n
-    if tuple(y.shape) != (M, cols) or y.dtype != x.dtype:
+    if y.shape != (M, cols) or y.dtype is not dt:
         raise EsepError(f"y must be a [{M}, {cols}] tensor of x's dtype")
+    table = array("q", words)
     with _on(dev):
-        rc = lib().esep_nf4_matvec(ctypes.addressof(arr), len(items), _p(x), _rows_ld(x, K), _p(y),
-                                   _rows_ld(y, cols), M, K, dtype_code(x.dtype), _stream(dev))
+        rc = lib().esep_nf4_matvec(table.buffer_info()[0], len(items), x.data_ptr(), _rows_ld(x, K), y.data_ptr(),
+                                   _rows_ld(y, cols), M, K, dtype_code(dt), _stream(dev))
     _check(rc, "esep_nf4_matvec")
     _record(name)
 

@@ -136,7 +136,7 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
     For answering only: there is no gradient, so inputs that record one are refused in grad mode. The
     scratch memory is of the caller's stream and, under capture, of the graph. Returns o, of q's shape and
     dtype, dense."""
-    if any(t.requires_grad for t in (q, k_cache, v_cache)) and torch.is_grad_enabled():
+    if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
         raise _hip.EsepError("cache_attention has no gradient: call it under torch.no_grad(), or on "
                              "detached tensors (varlen_attention is the form for training)")
     sinks = _whole("sinks", sinks, 0)
@@ -154,5 +154,5 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
 
 def _unaligned(q):
     """The kernel reads q in 16-byte pieces."""
-    st = q.stride()
-    return st[3] != 1 or q.data_ptr() % 16 != 0 or any(s % 8 for s in st[:3])
+    b, n, h, d = q.stride()
+    return d != 1 or q.data_ptr() % 16 != 0 or b % 8 != 0 or n % 8 != 0 or h % 8 != 0

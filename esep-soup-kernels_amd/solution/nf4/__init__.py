@@ -158,20 +158,20 @@ MATVEC_ROWS = _hip.NF4_MATVEC_ROWS
 
 
 def _matvec(x, weights, states, biases):
-    items = []
+    items, dt, n = [], x.dtype, 0
     for w, qs, b in zip(weights, states, biases):
-        qs2, dt = qs.state2, x.dtype
-        if b is not None:
-            b = (b if b.dtype == dt else b.to(dt)).contiguous()
-        items.append((w.contiguous(), qs.absmax.contiguous(), _f32(qs2.absmax), _f32(qs2.code),
-                      _offset(qs), _f32(qs.code), b, qs.shape[0]))
-    x2 = x.reshape(-1, x.shape[-1])
+        qs2, rows = qs.state2, qs.shape[0]
+        if b is not None and (b.dtype is not dt or not b.is_contiguous()):
+            b = b.to(dt).contiguous()
+        items.append((w.contiguous(), qs.absmax.contiguous(), _f32(qs2.absmax), _f32(qs2.code), _offset(qs),
+                      _f32(qs.code), b, rows))
+        n += rows
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.shape[1] > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()
-    n = sum(it[7] for it in items)
-    y = torch.empty((x2.shape[0], n), device=x.device, dtype=x.dtype)
+    y = torch.empty((x2.shape[0], n), device=x.device, dtype=dt)
     _hip.nf4_matvec(x2, items, y)
-    return y.view(*x.shape[:-1], n)
+    return y if x2 is x else y.view(*x.shape[:-1], n)
 
 
 class NF4Matvec(torch.autograd.Function):

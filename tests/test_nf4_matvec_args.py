@@ -12,13 +12,19 @@ from solution import nf4
 from solution.body import _hip
 
 
+class _Weight(ctypes.Structure):
+    """esep_nf4_matvec_weight (include/esep_body.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("packed", "absmax", "absmax2", "code2", "offset", "nf4", "bias")]
+    _fields_ += [("N", ctypes.c_int64)]
+
+
 def _call(n=1, K=64, dt=1, M=1, ldx=64, ldy=64, x=16, y=16, weights=True, **kw):
-    arr = (_hip.Nf4MatvecWeight * 9)()
+    arr = (_Weight * 9)()
     for i in range(9):
         f = dict(packed=16, absmax=16, absmax2=16, code2=16, offset=16, nf4=16, bias=None, N=16)
         if i == 0:
             f.update(kw)
-        arr[i] = _hip.Nf4MatvecWeight(*f.values())
+        arr[i] = _Weight(*f.values())
     p = ctypes.addressof(arr) if weights else None
     return _hip.lib().esep_nf4_matvec(p, n, x, ldx, y, ldy, M, K, dt, None)
 
