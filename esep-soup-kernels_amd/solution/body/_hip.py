@@ -434,9 +434,10 @@ def rope(q, k, qo, ko, inv_freq, sign, q_delta=None, positions=None, cu_seqlens=
 
 def _tokens_ld(t, name):
     """Token stride of a [T, H, D] tensor whose heads and head dim are packed (stride D, 1)."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (shape[2] > 1 and stride[2] != 1) or (shape[1] > 1 and stride[1] != shape[2]):
         raise EsepError(f"{name} must be a [T, H, D] tensor with contiguous heads")
-    return t.stride(0)
+    return stride[0]
 
 
 def _attn_fwd_checked(q, k, v, o, cu_seqlens, lse):
@@ -504,11 +505,13 @@ def _attn_bwd_checked(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace, 
     """Checks the operands of an attention backward; `need` gives the workspace's size for (T, HQ, HK,
     D). Returns the device, the sizes and the workspace (allocated where it is None)."""
     dev = _dev(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace)
-    T, HQ, D = q.shape
-    HK = k.shape[1]
-    for t, shp in ((o, (T, HQ, D)), (dout, (T, HQ, D)), (dq, (T, HQ, D)), (k, (T, HK, D)),
-                   (v, (T, HK, D)), (dk, (T, HK, D)), (dv, (T, HK, D))):
-        if tuple(t.shape) != shp or t.dtype != q.dtype:
+    shape, kshape, dt = q.shape, k.shape, q.dtype
+    T, HQ, D = shape
+    HK = kshape[1]
+    if kshape != (T, HK, D):
+        raise EsepError("attention backward shapes do not match q [T, HQ, D], k [T, HK, D]")
+    for t, shp in ((o, shape), (dout, shape), (dq, shape), (k, kshape), (v, kshape), (dk, kshape), (dv, kshape)):
+        if t.shape != shp or t.dtype is not dt:
             raise EsepError("attention backward shapes / dtypes do not match q [T, HQ, D], k [T, HK, D]")
     if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (HQ, T):
         raise EsepError("lse must be a contiguous fp32 [HQ, T] tensor")

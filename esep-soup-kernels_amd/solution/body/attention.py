@@ -33,7 +33,8 @@ def supported(q, k, v, dropout=0.0):
 
 
 def _heads_packed(t):
-    if t.stride(2) != 1 or t.stride(1) != t.shape[2] or t.stride(0) % 8 or t.data_ptr() % 16:
+    rs, hs, ds = t.stride()
+    if ds != 1 or hs != t.shape[2] or rs % 8 or t.data_ptr() % 16:
         t = t.contiguous()
     return t
 
