@@ -62,7 +62,7 @@ struct AttnBwdArgs {
   void* dk;
   void* dv;
   int64_t do_rs, dq_rs, dk_rs, dv_rs;
-  int split;  // blocks per kv head and key tile (a divisor of HQ / HK)
+  int split;  // blocks per kv head and key tile (a divisor of HQ / HK; windowed: up to HQ / HK)
 };
 
 constexpr int kAttnBM = 128;  // queries per forward / dQ block (4 wavefronts x 32)

@@ -457,7 +457,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
   const int G = a.HQ / a.HK, bid = attn_block();
   const bool far = bid >= p.n_main;
   if (far && !p.far) return;
-  int seq, kh, part, tile, chunk = 0, gs, start = 0, end = 0;
+  int seq, kh, part, parts, tile, chunk = 0, start = 0, end = 0;
   if (!far) {
     const WinPlace pl = win_place(bid, p.n_main, a.HK * b.split, a.cu, a.n_seq, a.T, kWinKeys);
     if (pl.spare >= 0) {
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
     kh = pl.head / b.split;
     part = pl.head % b.split;
     tile = pl.tile;
-    gs = G / b.split;
+    parts = b.split;
   } else {
     const int kts = (p.sinks + BK - 1) / BK, per = kts * a.HK * p.far_split;
     const int slot = (bid - p.n_main) / per, r = (bid - p.n_main) % per;
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
     tile = r % kts;
     kh = r / kts % a.HK;
     part = r / kts / a.HK;
-    gs = G / p.far_split;
+    parts = p.far_split;
   }
   if (seq < 0) return;
   const int len = end - start;
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
   const int lq = lane & 31, hi = lane >> 5;
   const int kw0 = k0 + 32 * w, kj = kw0 + lq;
   const bool kok = kj < kend, wave_live = kw0 < kend;
-  const int h0 = kh * G + part * gs;
+  const int g0 = part * G / parts, gs = (part + 1) * G / parts - g0, h0 = kh * G + g0;
   // the queries that see this lane's key in this block: tlo <= t < thi; wlo, wmin and wmax are the
   // wavefront's greatest tlo and least and greatest thi
   const bool open = !lng || far;  // a sink key is seen to the end

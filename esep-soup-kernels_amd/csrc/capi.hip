@@ -128,13 +128,15 @@ struct WinLayout {
   int split, sinks, far, far_split;
   int64_t main_at, far_at, total;
 };
-// Blocks per (kv head, key tile) of the windowed dK / dV kernel: the divisor of HQ / HK with the least
-// estimated time. Its blocks do near-equal work, so what counts beside the partials' bytes is how the blocks
-// fill the 512 that are resident: half of them or fewer run a third faster each, and a round that is begun costs
-// about half of one more. A 32-query item of two blocks to a CU takes 2.6 us (D = 64: 1.3), the partials are
-// written and read at 5 TB/s. Backward in us with 1 / 2 / 3 / 6 blocks, 12 / 2 heads, D = 128 (* what it picks):
-// 5933 tokens in 8 sequences, window 256, 143 / 109 / 108* / 117; 8192, 512: 234 / 193 / 171* / 190; 32768, 4096:
-// 3448 / 2992 / 2874 / 2794*; with 1 / 7, 28 / 4 heads, window 512: 4096 tokens 256 / 216*, 8192 365* / 403.
+// Blocks per (kv head, key tile) of the windowed dK / dV kernel: of 1 .. HQ / HK the number with the least
+// estimated time; its blocks take G / s of the G query heads, rounded down or up. They do near-equal work, so
+// what counts beside the partials' bytes is how they fill the 512 that are resident: half of them or fewer run a
+// quarter faster each, and a round that is begun costs about a third of one more. A 32-query item of two blocks
+// to a CU takes 2.6 us (D = 64: 1.3), the partials are written and read at 5 TB/s. Backward in us with 1 / 2 / 3 /
+// 4 / 5 / 6 (/ 7) blocks, bf16 (* what it picks): 12 / 2 heads, D = 128, 5933 tokens in 8 sequences, window 256,
+// 136 / 104 / 102* / 102 / 113 / 110; 8192, 512: 220 / 180 / 159* / 204 / 188 / 177; 32768, 4096: 3396 / 2981 / 2849 /
+// 3004 / 2788 / 2780*; 28 / 4 heads, 8192, 512: 344 / 383 / 335* / 357 / 352 / 371 / 380; 14 / 2 heads, D = 64, 12011
+// tokens in 9 sequences, 512: 276 / 197 / 172 / 146* / 152 / 160 / 157.
 int win_split(int64_t T, int HQ, int HK, int D, int max_seqlen, int window) {
   const int G = HQ / HK;
   const double head = ((window < max_seqlen ? window : max_seqlen) + 160) / 32 * (D == 128 ? 2.6 : 1.3);
@@ -142,10 +144,10 @@ int win_split(int64_t T, int HQ, int HK, int D, int max_seqlen, int window) {
   int best = 1;
   double least = 0;
   for (int s = 1; s <= G; ++s) {
-    if (G % s) continue;
-    const double r = (double)(T / 128 + 1) * HK * s / 512;
-    const double fill = r < 0.5 ? 0.75 : (r <= 1 ? 0.5 + 0.5 * r : 0.5 * (r + (double)(int64_t)(r + 0.999999)));
-    const double cost = G / s * fill * head + (s > 1 ? s * part : 0);
+    const double r = (double)(T / 128 + 1) * HK * s / 512, mean = (double)G / s, most = (G + s - 1) / s;
+    const double heads = r <= 1 ? most * (0.5 + 0.5 * (r > 0.5 ? r : 0.5))
+                                : 0.7 * r * mean + 0.3 * (((double)(int64_t)(r + 0.999999) - 1) * mean + most);
+    const double cost = heads * head + (s > 1 ? s * part : 0);
     if (s == 1 || cost < least) {
       best = s;
       least = cost;

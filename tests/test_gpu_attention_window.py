@@ -41,6 +41,8 @@ CASES = [
     ([70, 129, 31, 160], 16, 1, 64, 50, 0),
     ([257, 64, 31, 97], 9, 3, 128, 32, 5),
     ([40] * 70 + [0] * 3 + [33], 5, 1, 64, 17, 1),
+    ([3001, 1400, 1607], 14, 2, 64, 300, 5),       # heads dealt unevenly to the dK / dV blocks
+    ([1501, 900, 1607], 28, 4, 128, 300, 0),
 ]
 
 
