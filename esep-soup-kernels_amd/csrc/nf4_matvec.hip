@@ -172,34 +172,31 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
       seek(++lt);
     }
   };
+  // What the tables are made of is asked for first: its wait then leaves W's first bytes on their way.
+  const float code = w.nf4[lane & 15], code_2 = w.code2[tid & 255];
   load_scales();
   Stage st[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) load(st[d]);
-
-  // the tables and x, while the first bytes of W are on their way
   const float off = *w.offset;
   // (the bias of the output that this thread adds up first, too)
   const int n0 = (tile0 + tid / (MT * 128)) * 16 + (tid & 15);
   const float bias0 = w.bias != nullptr && n0 < w.N ? (float)static_cast<const T*>(w.bias)[n0] : 0.f;
-  {
-    const float code = w.nf4[lane & 15];
-    for (int i = tid; i < 256 * 8; i += kMvThreads) {
-      const int e = i / 8;
-      const uint32_t p = mv_pair<T>(__shfl(code, e >> 4), __shfl(code, e & 15));
-      reinterpret_cast<uint4*>(tab)[i] = make_uint4(p, p, p, p);
-    }
-    if (tid < 256) code2[tid] = w.code2[tid];
-    if (tid < 4) reinterpret_cast<u32x4*>(xs)[tid] = u32x4{0, 0, 0, 0};
-    if constexpr (XL) {
-      const int chunks = 16 * steps, data = a.K / 8;  // 16-byte pieces of a row
-      for (int i = tid; i < a.M * chunks; i += kMvThreads) {
-        const int m = i / chunks, c = i % chunks;
-        u32x4 v = {0, 0, 0, 0};
-        if (c < data)
-          v = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 8 * c);
-        *reinterpret_cast<u32x4*>(xs + 64 + m * mv_x_row(a.K) + 16 * c) = v;
-      }
+  for (int i = tid; i < 256 * 8; i += kMvThreads) {
+    const int e = i / 8;
+    const uint32_t p = mv_pair<T>(__shfl(code, e >> 4), __shfl(code, e & 15));
+    reinterpret_cast<uint4*>(tab)[i] = make_uint4(p, p, p, p);
+  }
+  if (tid < 256) code2[tid] = code_2;
+  if (tid < 4) reinterpret_cast<u32x4*>(xs)[tid] = u32x4{0, 0, 0, 0};
+  if constexpr (XL) {
+    const int chunks = 16 * steps, data = a.K / 8;  // 16-byte pieces of a row
+    for (int i = tid; i < a.M * chunks; i += kMvThreads) {
+      const int m = i / chunks, c = i % chunks;
+      u32x4 v = {0, 0, 0, 0};
+      if (c < data)
+        v = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.x) + (int64_t)m * a.ldx + 8 * c);
+      *reinterpret_cast<u32x4*>(xs + 64 + m * mv_x_row(a.K) + 16 * c) = v;
     }
   }
   __syncthreads();
