@@ -15,7 +15,7 @@
 //
 // Kernel trace, walk + join: 32 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16 56.9 + 4.6 us (334 MB, 5.4
 // TB/s; a copy reaches 5.0, half of it writes); 8 rows of up to 32768 through a window of 4096, 12 / 2 heads 12.7
-// + 3.9; one row of 700 tokens 6.0 + 3.8; 16 new tokens over 4 rows of up to 4001, 14 / 2 heads of 64 14.4 + 4.2.
+// + 3.9; one row of 700 tokens 6.0 + 3.8; 16 new tokens over 4 rows of up to 4001, 14 / 2 heads of 64 14.2 + 4.2.
 #include <cmath>
 
 #include "attention_tiles.hpp"

@@ -19,11 +19,12 @@
 // one to each of its 16 wavefronts, which streams its run four steps ahead with no barrier; parts of a tile
 // meet in LDS at the end and are added in the wavefronts' order. x lies in LDS where it fits.
 //
-// Kernel trace, one row of x in fp16: 2 x 18944 rows of W of 3584 in 21.1 us (70 MB, 3.3 TB/s; 14.0 is the copy
-// rate's time), q / k / v of 1536 in 7.1; 7 rows in bf16, 1536 of 8960 in 11.6 (96 blocks for 256 CUs: a finer
-// cut would add parts of a tile across blocks in a second launch). A copy without the table reads takes 19.2 of
-// 20.3 us, one without the loads of W 16.9: loads and decode overlap. Slower: six or eight steps ahead (21.0,
-// 22.8), x in registers (20.8), loads of 128 bytes of a row (21.0), W past the caches (22.4).
+// Kernel trace, one row of x in fp16: 2 x 18944 rows of W of 3584 in 20.6 us (70 MB, 3.4 TB/s; 14.0 is the copy
+// rate's time), q / k / v of 1536 in 7.0; 7 rows in bf16, 1536 of 8960 in 11.4 (96 blocks for 256 CUs: a finer
+// cut would add parts of a tile across blocks in a second launch). Parts left out in a copy for timing, 20.3 us
+// with all: without the table reads 19.2, without the loads of W 16.9, so loads and decode overlap. Slower: six or
+// eight steps ahead (21.0, 22.8), x in registers (20.8), loads of 128 bytes of a row (21.0), W past the caches
+// (22.4).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
