@@ -80,9 +80,13 @@ struct MvStage {
 // x in LDS (XL): rows of whole steps, zeros behind K, and 8 elements more, so that the 8 rows that a
 // read touches lie in different banks; before them 64 bytes of zeros that the lanes without a row read.
 // Otherwise each wavefront writes its step of x there, in the same form.
-constexpr int kMvXBytes = 64 * 1024;
+constexpr int mv_x_bytes(int MT) { return (MT == 1 ? 95 : 80) * 1024; }  // what a CU's 160 KiB leave
 inline __host__ __device__ int mv_x_row(int K) { return 2 * ((K + 127) / 128 * 128 + 8); }
-inline bool mv_x_fits(int M, int K) { return 64 + (int64_t)M * mv_x_row(K) <= kMvXBytes; }
+// A block with one tile reads x once, and gains from its copy up to 64 KiB only (8 rows of 5632, 2048 outputs:
+// 9.0 us with it, 8.7 without; 10 rows of 3584, 2 x 18944 outputs, ten tiles to a block: 24.9 and 31.4).
+inline bool mv_x_fits(int M, int K, int MT, int per_block) {
+  return 64 + (int64_t)M * mv_x_row(K) <= (per_block > 1 ? mv_x_bytes(MT) : 64 * 1024);
+}
 
 template <typename T, int MT, bool XL>
 __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a) {
@@ -95,7 +99,7 @@ __global__ __launch_bounds__(kMvThreads, 4) void k_nf4_matvec(const Nf4MvArgs a)
     float code2[256];
     float red[kMvWaves + kMvTiles - 1][MT * 8][16];  // a wavefront's part of a tile: [both numbers' sum]
     char ws[kMvWaves][1024];                         // a wavefront's step of W
-    char xs[XL ? kMvXBytes : 64 + kMvWaves * XW];
+    char xs[XL ? mv_x_bytes(MT) : 64 + kMvWaves * XW];
   };
   __shared__ __align__(16) Lds lds;
   auto& tab = lds.tab;
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(256) void k_nf4_matvec_any(const Nf4MvArgs a) {
   }
 }
 
-template <typename T, int MT, bool XL>
+template <typename T, int MT>
 hipError_t run(Nf4MvArgs& a, hipStream_t s) {
   // the fewest tiles to a block that one block to a CU holds, up to kMvTiles
   int blocks = 0;
@@ -347,13 +351,11 @@ hipError_t run(Nf4MvArgs& a, hipStream_t s) {
     }
     if (blocks <= 256 || a.per_block == kMvTiles) break;
   }
-  hipLaunchKernelGGL((k_nf4_matvec<T, MT, XL>), dim3((unsigned)blocks), dim3(kMvThreads), 0, s, a);
+  if (mv_x_fits(a.M, a.K, MT, a.per_block))
+    hipLaunchKernelGGL((k_nf4_matvec<T, MT, true>), dim3((unsigned)blocks), dim3(kMvThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_nf4_matvec<T, MT, false>), dim3((unsigned)blocks), dim3(kMvThreads), 0, s, a);
   return hipGetLastError();
-}
-
-template <typename T, int MT>
-hipError_t run_x(Nf4MvArgs& a, hipStream_t s) {
-  return mv_x_fits(a.M, a.K) ? run<T, MT, true>(a, s) : run<T, MT, false>(a, s);
 }
 
 template <typename T>
@@ -364,7 +366,7 @@ hipError_t run_t(Nf4MvArgs& a, hipStream_t s) {
     rows += a.w[i].N;
     whole = whole && (reinterpret_cast<uintptr_t>(a.w[i].packed) & 15) == 0;
   }
-  if (whole) return a.M <= 8 ? run_x<T, 1>(a, s) : run_x<T, 2>(a, s);
+  if (whole) return a.M <= 8 ? run<T, 1>(a, s) : run<T, 2>(a, s);
   hipLaunchKernelGGL((k_nf4_matvec_any<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
   return hipGetLastError();
 }

@@ -47,7 +47,8 @@ def _check(y, x, w, bias, what):
 
 
 SIZES = [(1, 64), (16, 64), (17, 128), (40, 192), (256, 1536), (1536, 896), (1000, 960), (4864, 896),
-         (33, 8960), (2112, 64), (64, 18944)]
+         (33, 8960), (2112, 64), (64, 18944),
+         (4112, 4160)]  # two tiles to a block, 8 and 9 rows of x in LDS
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
