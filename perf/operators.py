@@ -195,7 +195,7 @@ def prepare(case, seed):
                  weights=[_quant_state(d, n, case["n_in"]) for n in outs],
                  biases=[d.normal(n, dtype=dt) if case["bias"] else None for n in outs])
     if own:
-        s["attention"], s["nf4"] = _entries()  # imported before the first pass, as a program does
+        _entries()  # the framework is imported before the first pass
     return s
 
 
@@ -213,20 +213,22 @@ def _entries():
 
 
 def _own_window(s):
+    attention, _ = _entries()
     c = s["case"]
-    o = s["attention"].varlen_attention(s["q"], s["k"], s["v"], s["cu"], max(s["lens"]),
-                                        window=c["window"], sinks=c["sinks"])
+    o = attention.varlen_attention(s["q"], s["k"], s["v"], s["cu"], max(s["lens"]), window=c["window"],
+                                   sinks=c["sinks"])
     return o.detach(), *torch.autograd.grad(o, (s["q"], s["k"], s["v"]), s["do"])
 
 
 def _own_cache(s):
+    attention, _ = _entries()
     c = s["case"]
-    return s["attention"].cache_attention(s["q"], s["k"], s["v"], s["lengths"],
-                                          window=c["window"] or None, sinks=c["sinks"])
+    return attention.cache_attention(s["q"], s["k"], s["v"], s["lengths"], window=c["window"] or None,
+                                     sinks=c["sinks"])
 
 
 def _own_nf4(s):
-    nf4 = s["nf4"]
+    _, nf4 = _entries()
     if len(s["weights"]) == 1:
         packed, state = s["weights"][0]
         return nf4.nf4_matvec(s["x"], packed, s["biases"][0], state)
