@@ -122,6 +122,27 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
     return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))
 
 
+_NO_GRADIENT = ("cache_attention has no gradient: call it under torch.no_grad(), or on detached tensors "
+                "(varlen_attention is the form for training)")
+
+
+class CacheAttention(torch.autograd.Function):
+    """cache_attention where torch looks on: one node of a trace, which runs it again, and tangents are refused
+    (the kernel fills its buffer behind torch's back)."""
+
+    @staticmethod
+    def forward(ctx, q, k_cache, v_cache, lengths, scale, window, sinks):
+        return _cache(q, k_cache, v_cache, lengths, scale, window, sinks)
+
+    @staticmethod
+    def backward(ctx, do):
+        raise _hip.EsepError(_NO_GRADIENT)
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise _hip.EsepError(_NO_GRADIENT)
+
+
 def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks=0):
     """Attention of each row's newest tokens over its cache: decoding (one new token a row), or a few new
     tokens at once. q [B, n, HQ, D] (or [B, HQ, D]: n = 1), the queries of the n newest tokens; k_cache, v_cache
@@ -134,17 +155,22 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
     window or j < sinks, as in varlen_attention. What a cache holds past a row's length is never read; a query
     at a position below 0 (a row shorter than n) gets 0. Lengths past S count as S.
 
-    For answering only: there is no gradient, so inputs that record one are refused in grad mode. The
-    scratch memory is of the caller's stream and, under capture, of the graph. Returns o, of q's shape and
-    dtype, dense."""
+    For answering only: there is no gradient, so inputs that record one in grad mode, or carry a forward-mode
+    tangent, are refused. The scratch memory is of the caller's stream and, under capture, of the graph. A
+    traced module (torch.jit.trace) calls it again. Returns o, of q's shape and dtype, dense."""
     if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
-        raise _hip.EsepError("cache_attention has no gradient: call it under torch.no_grad(), or on "
-                             "detached tensors (varlen_attention is the form for training)")
+        raise _hip.EsepError(_NO_GRADIENT)
     sinks = _whole("sinks", sinks, 0)
     if window is not None:
         window = _whole("window", window, 1)
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    if _hip.recorded(q, k_cache, v_cache, lengths):
+        return CacheAttention.apply(q, k_cache, v_cache, lengths, scale, window, sinks)
+    return _cache(q, k_cache, v_cache, lengths, scale, window, sinks)
+
+
+def _cache(q, k_cache, v_cache, lengths, scale, window, sinks):
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
     if q4.dim() == 4 and _unaligned(q4):
         q4 = q4.contiguous()
