@@ -228,6 +228,16 @@ def recorded(*tensors):
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def refuse_proxies(what):
+    """A graph made by torch's proxy tensors (make_fx) holds only the torch operations of a call: of a
+    kernel's output it would keep the empty buffer."""
+    if _dispatch_modes():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise EsepError(f"{what} runs a kernel that proxy tensors cannot put into a graph")
+
+
 def dense16(*tensors):
     """Contiguous, at 16-byte addresses: asked of saved tensors, whose hooks may give back other
     strides and addresses than the forward pass saw."""

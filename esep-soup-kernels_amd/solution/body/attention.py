@@ -118,6 +118,7 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
     sinks = _whole("sinks", sinks, 0)
     if window is not None:
         window = _whole("window", window, 1)
+        _hip.refuse_proxies("varlen_attention")
         return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
     return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))
 
@@ -166,6 +167,7 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if _hip.recorded(q, k_cache, v_cache, lengths):
+        _hip.refuse_proxies("cache_attention")
         return CacheAttention.apply(q, k_cache, v_cache, lengths, scale, window, sinks)
     return _cache(q, k_cache, v_cache, lengths, scale, window, sinks)
 

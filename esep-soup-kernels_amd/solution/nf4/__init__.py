@@ -219,6 +219,7 @@ def nf4_matvec_multi(x, weights, quant_states, biases=None):
         raise _hip.EsepError(f"nf4_matvec takes up to {MATVEC_ROWS} rows, got x {tuple(x.shape)}; "
                              "nf4_linear is the form for more")
     if _hip.recorded(x, *biases):
+        _hip.refuse_proxies("nf4_matvec")
         return NF4Matvec.apply(x, weights, states, *biases)
     return _matvec(x.to(torch.float16) if x.dtype is torch.float32 else x, weights, states, biases)
 

@@ -1,6 +1,6 @@
 """The windowed, cache and few-row operators where torch records them, without a GPU: a stand-in takes the
 kernel's place and fills the output by its address, as the kernel does. A trace runs the operator again on its
-inputs, tangents are refused, modes that only look on change nothing."""
+inputs, tangents and proxy graphs are refused, modes that only look on change nothing."""
 
 import ctypes
 import types
@@ -8,6 +8,7 @@ import types
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from solution import nf4
@@ -72,6 +73,13 @@ def test_a_tangent_of_the_cache_is_refused(stand_ins):
         for k, v in ((dual, K), (K, dual)):
             with pytest.raises(_hip.EsepError, match="no gradient"):
                 cache_attention(q, k, v, LENGTHS)
+
+
+@call
+def test_proxy_graphs_are_refused(stand_ins, name):
+    f, shape = CALLS[name]
+    with pytest.raises(_hip.EsepError, match="proxy"):
+        make_fx(f)(torch.randn(shape).half())
 
 
 @call
