@@ -83,26 +83,48 @@ struct AttnWinArgs {
   int zero_rest;     // the forward writes o = 0 behind the last sequence
   int far;           // some sequence may be long enough for the separate pass over sink keys
   int far_split;     // blocks per kv head in that pass (a divisor of HQ / HK)
-  float* sink_main;  // [T / (window + kWinFar) + 1][split][HK][2][sinks][D]
-  float* sink_far;   // [win_far_slots][far_split][HK][2][sinks][D]
+  int far_len;       // queries of a block in it
+  int by_seq;        // a sequence's place in sink_main is its number
+  float* sink_main;  // [WinSlots::main][split][HK][2][sinks][D]
+  float* sink_far;   // [WinSlots::far][far_split][HK][2][sinks][D]
   int n_main;        // dK / dV blocks before the far ones
 };
 
-// Queries of a far block, and the length past the window from which a sequence has them.
+// Queries of a far block where there are few, and the length past the window from which a sequence has them.
 constexpr int kWinFar = 512;
-inline int64_t win_main_slots(int64_t T, int window) { return T / ((int64_t)window + kWinFar) + 1; }
-inline int64_t win_far_slots(int64_t T, int window) {
-  return T / kWinFar + win_main_slots(T, window);
-}
 // The separate pass over sink keys runs only where the bound on the lengths admits a long sequence.
 inline bool win_has_far(int window, int sinks, int max_seqlen) {
   return sinks > 0 && (int64_t)max_seqlen > (int64_t)window + kWinFar;
+}
+
+// Where the long sequences' sink partials lie: `main` places for the near ones, one to a sequence, numbered by
+// the sequences or, where that is less, by the offset's multiple of window + kWinFar (two long sequences
+// never share one); `far` for the far ones, place offset / far_len + near place + chunk. From kWinFarBlocks
+// blocks on (eight rounds of two to a CU) the far blocks take more queries each, up to kWinFarMost, so that
+// their partials, of 128 sink rows a block, stay within about half a GB, or T / 32768 times the sink rows.
+constexpr int64_t kWinFarBlocks = 4096;
+constexpr int kWinFarMost = 32768;
+struct WinSlots {
+  int by_seq, far_len;
+  int64_t main, far;
+};
+inline WinSlots win_slots(int64_t T, int n_seq, int HK, int window, int sinks) {
+  WinSlots w{};
+  const int64_t most = T / ((int64_t)window + kWinFar) + 1;
+  w.by_seq = n_seq < most;
+  w.main = w.by_seq ? n_seq : most;
+  const int64_t tiles = (int64_t)HK * (((int64_t)sinks + kAttnBM - 1) / kAttnBM);
+  w.far_len = kWinFar;
+  while (T / w.far_len * tiles > kWinFarBlocks && w.far_len < kWinFarMost) w.far_len *= 2;
+  w.far = T / w.far_len + w.main;
+  return w;
 }
 // Blocks per kv head of that pass: enough of them for two rounds of its two blocks per CU, short of one
 // head per block.
 inline int win_far_split(int64_t T, int HQ, int HK, int window, int sinks) {
   const int G = HQ / HK;
-  const int64_t blocks = win_far_slots(T, window) * HK * ((sinks + 127) / 128);
+  const int64_t most = T / kWinFar + T / ((int64_t)window + kWinFar) + 1;
+  const int64_t blocks = most * HK * (((int64_t)sinks + kAttnBM - 1) / kAttnBM);
   int s = 1;
   while (blocks * s < 1024 && s < G) {
     ++s;
@@ -124,6 +146,9 @@ hipError_t launch_attn_rest(const AttnRestArgs& a, hipStream_t s);
 
 hipError_t launch_attn_win_fwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
 hipError_t launch_attn_win_bwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* supported);
+// Whether the backward's launches hold a call of these sizes (of p: b.f's sizes, b.split, window, sinks, far,
+// far_split, far_len).
+bool attn_win_bwd_fits(const AttnWinArgs& p);
 
 // Attention of the newest tokens over a cache (attention_cache.hip). Strides in elements.
 struct AttnCacheArgs {

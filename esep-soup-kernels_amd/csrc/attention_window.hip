@@ -10,7 +10,7 @@
 // dK / dV: a block of 128 keys walks the queries k0 .. k0 + 127 + window - 1. A sink key is also seen by every
 // query after that: in a long sequence 32 times as many as another key, which one block would walk
 // alone long after the launch's others had ended. Those far queries (i - j >= window) go to blocks of
-// their own, kWinFar queries each, in the same launch; they and the sink keys' near part write fp32
+// their own, kWinFar queries each or more, in the same launch; they and the sink keys' near part write fp32
 // partials that k_attn_win_sinks adds in a fixed order. A sequence of up to window + kWinFar tokens has its sink
 // keys' blocks walk on to its end instead.
 //
@@ -418,11 +418,12 @@ __device__ __forceinline__ void dkdv_tile_swz(const char* qrow, const char* drow
   __builtin_amdgcn_s_setprio(0);
 }
 
-__device__ __forceinline__ int win_main_base(int c, int window) {
-  return (int)(c / ((int64_t)window + kWinFar));
+// The places of a sequence's sink partials (attention.hpp: WinSlots); it starts at token c.
+__device__ __forceinline__ int win_main_base(const AttnWinArgs& p, int seq, int c) {
+  return p.by_seq ? seq : (int)(c / ((int64_t)p.window + kWinFar));
 }
-__device__ __forceinline__ int win_far_base(int c, int window) {
-  return c / kWinFar + win_main_base(c, window);
+__device__ __forceinline__ int win_far_base(const AttnWinArgs& p, int seq, int c) {
+  return c / p.far_len + win_main_base(p, seq, c);
 }
 
 // fp32 dK^T / scale and dV^T of a lane's key into partial `idx` of a sink buffer, [idx][HK][2][sinks][D].
@@ -475,10 +476,10 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
     const int kts = (p.sinks + BK - 1) / BK, per = kts * a.HK * p.far_split;
     const int slot = (bid - p.n_main) / per, r = (bid - p.n_main) % per;
     seq = win_search(a.n_seq, slot,
-                     [&](int j) { return win_far_base(cu_at(a.cu, j, a.T), p.window); });
+                     [&](int j) { return win_far_base(p, j, cu_at(a.cu, j, a.T)); });
     if (seq >= 0) {
       seq_bounds(a.cu, seq, a.T, &start, &end);
-      chunk = slot - win_far_base(start, p.window);
+      chunk = slot - win_far_base(p, seq, start);
     }
     tile = r % kts;
     kh = r / kts % a.HK;
@@ -495,9 +496,9 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
   // the block's queries [qa, qe)
   int qa = k0, qe = end;
   if (far) {
-    if (!lng || (int64_t)chunk * kWinFar >= len - p.window) return;
-    qa = start + p.window + chunk * kWinFar;
-    qe = end - qa < kWinFar ? end : qa + kWinFar;
+    if (!lng || (int64_t)chunk * p.far_len >= len - p.window) return;
+    qa = start + p.window + chunk * p.far_len;
+    qe = end - qa < p.far_len ? end : qa + p.far_len;
     if (qe <= k0 + p.window) return;
   } else if ((lng || k0 >= sink_hi) && end - k0 - (BK - 1) > p.window) {
     qe = k0 + BK - 1 + p.window;
@@ -581,12 +582,12 @@ __global__ __launch_bounds__(kAttnThreads, D == 128 ? kDkdvPerCU : 3) void k_att
   }
   if (!kok) return;
   if (far) {
-    const int64_t idx = (int64_t)(win_far_base(start, p.window) + chunk) * p.far_split + part;
+    const int64_t idx = (int64_t)(win_far_base(p, seq, start) + chunk) * p.far_split + part;
     store_sink<D>(p.sink_far, idx, a.HK, kh, p.sinks, kj - start, hi, dka, dva);
     return;
   }
   if (lng && kj < sink_hi) {
-    const int64_t idx = (int64_t)win_main_base(start, p.window) * b.split + part;
+    const int64_t idx = (int64_t)win_main_base(p, seq, start) * b.split + part;
     store_sink<D>(p.sink_main, idx, a.HK, kh, p.sinks, kj - start, hi, dka, dva);
     return;
   }
@@ -654,22 +655,22 @@ __global__ __launch_bounds__(256) void k_attn_win_sinks(const AttnWinArgs p) {
   const int r = (int)(blockIdx.x % p.sinks), which = (int)(blockIdx.x / p.sinks % 2);
   const int kh = (int)(blockIdx.x / p.sinks / 2 % a.HK), slot = (int)(blockIdx.x / p.sinks / 2 / a.HK);
   const int seq = win_search(a.n_seq, slot,
-                             [&](int j) { return win_main_base(cu_at(a.cu, j, a.T), p.window); });
+                             [&](int j) { return win_main_base(p, j, cu_at(a.cu, j, a.T)); });
   if (seq < 0) return;
   int start, end;
   seq_bounds(a.cu, seq, a.T, &start, &end);
   const int len = end - start;
-  if (len - kWinFar <= p.window || r >= len || win_main_base(start, p.window) != slot) return;
+  if (len - kWinFar <= p.window || r >= len || win_main_base(p, seq, start) != slot) return;
   // chunks whose far block wrote this row: those with a query that sees a key of its tile from afar
   const int off = r / kAttnBM * kAttnBM;
-  const int first = off / kWinFar, chunks = (len - p.window + kWinFar - 1) / kWinFar;
+  const int first = off / p.far_len, chunks = (int)(((int64_t)len - p.window + p.far_len - 1) / p.far_len);
   const int n = b.split + (len - p.window > off ? (chunks - first) * p.far_split : 0);
   const int64_t stride = (int64_t)a.HK * 2 * p.sinks * D;
   const int g = threadIdx.x / QUADS, x = threadIdx.x % QUADS;
   const int64_t at = ((int64_t)(kh * 2 + which) * p.sinks + r) * D + 4 * x;
   const float* near = p.sink_main + (int64_t)slot * b.split * stride + at;
   const float* away = p.sink_far +
-                      (int64_t)(win_far_base(start, p.window) + first) * p.far_split * stride + at;
+                      (int64_t)(win_far_base(p, seq, start) + first) * p.far_split * stride + at;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = g; i < n; i += GROUPS) {
@@ -721,16 +722,27 @@ hipError_t fwd_run(const AttnWinArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
+struct WinGrids {
+  int64_t nq, nk, nfar, nsum;
+  explicit WinGrids(const AttnWinArgs& p) {
+    const AttnArgs& f = p.b.f;
+    const int64_t tiles = ((int64_t)p.sinks + kAttnBM - 1) / kAttnBM;
+    const WinSlots w = win_slots(f.T, f.n_seq, f.HK, p.window, p.sinks);
+    nq = win_blocks(f.T, f.n_seq, f.HK, win_queries(f.HQ / f.HK));
+    nk = win_blocks(f.T, f.n_seq, (int64_t)f.HK * p.b.split, kWinKeys);
+    nfar = p.far ? w.far * tiles * f.HK * p.far_split : 0;
+    nsum = p.far ? w.main * f.HK * 2 * p.sinks : 0;
+  }
+  bool ok() const { return attn_grid_ok(nq) && attn_grid_ok(nk + nfar) && nsum <= kWinMaxSums; }
+};
+
 template <typename T, int D>
 hipError_t bwd_run(const AttnWinArgs& a, hipStream_t s) {
   AttnWinArgs p = a;
   const AttnArgs& f = p.b.f;
-  const int64_t nq = win_blocks(f.T, f.n_seq, f.HK, win_queries(f.HQ / f.HK));
-  const int64_t nk = win_blocks(f.T, f.n_seq, (int64_t)f.HK * p.b.split, kWinKeys);
-  const int64_t per = (int64_t)((p.sinks + kAttnBM - 1) / kAttnBM) * f.HK * p.far_split;
-  const int64_t nfar = p.far ? win_far_slots(f.T, p.window) * per : 0;
-  const int64_t nsum = p.far ? win_main_slots(f.T, p.window) * f.HK * 2 * p.sinks : 0;
-  if (!attn_grid_ok(nq) || !attn_grid_ok(nk + nfar) || nsum > kWinMaxSums) return hipErrorInvalidValue;
+  const WinGrids g(p);
+  if (!g.ok()) return hipErrorInvalidValue;
+  const int64_t nq = g.nq, nk = g.nk, nfar = g.nfar, nsum = g.nsum;
   p.n_main = (int)nk;
   hipLaunchKernelGGL((k_attn_win_dq<T, D, D == 128 ? 32 : 64>), attn_grid(nq), dim3(kAttnThreads), 0, s,
                      p);
@@ -774,6 +786,8 @@ hipError_t launch_attn_rest(const AttnRestArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k_attn_rest, dim3(64, 3), dim3(256), 0, s, a);
   return hipGetLastError();
 }
+
+bool attn_win_bwd_fits(const AttnWinArgs& p) { return WinGrids(p).ok(); }
 
 hipError_t launch_attn_win_fwd(const AttnWinArgs& a, int dt, int D, hipStream_t s, bool* sup) {
   if (dt == 1) return fwd_d<_Float16>(a, D, s, sup);

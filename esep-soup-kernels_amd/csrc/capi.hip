@@ -126,6 +126,7 @@ bool sees_all(int max_seqlen, int window, int sinks) {
 // near and far ones. (Where the window leaves something out: sinks < max_seqlen.)
 struct WinLayout {
   int split, sinks, far, far_split;
+  esep::WinSlots at;
   int64_t main_at, far_at, total;
 };
 // Blocks per (kv head, key tile) of the windowed dK / dV kernel: of 1 .. HQ / HK the number with the least
@@ -156,17 +157,34 @@ int win_split(int64_t T, int HQ, int HK, int D, int max_seqlen, int window) {
   return best;
 }
 
-WinLayout win_layout(int64_t T, int HQ, int HK, int D, int max_seqlen, int window, int sinks) {
+WinLayout win_layout(int64_t T, int HQ, int HK, int D, int n_seq, int max_seqlen, int window, int sinks) {
   WinLayout w{};
   w.split = win_split(T, HQ, HK, D, max_seqlen, window);
   w.sinks = sinks;
   w.far = esep::win_has_far(window, w.sinks, max_seqlen);
   w.far_split = w.far ? esep::win_far_split(T, HQ, HK, window, w.sinks) : 1;
+  w.at = esep::win_slots(T, n_seq, HK, window, w.sinks);
   const int64_t row = (int64_t)HK * 2 * w.sinks * D;
   w.main_at = (((int64_t)HQ * T + 3) & ~(int64_t)3) + (w.split > 1 ? 2 * w.split * T * HK * D : 0);
-  w.far_at = w.main_at + (w.far ? esep::win_main_slots(T, window) * w.split * row : 0);
-  w.total = w.far_at + (w.far ? esep::win_far_slots(T, window) * w.far_split * row : 0);
+  w.far_at = w.main_at + (w.far ? w.at.main * w.split * row : 0);
+  w.total = w.far_at + (w.far ? w.at.far * w.far_split * row : 0);
   return w;
+}
+
+// Fills what the windowed backward takes from its layout; refuses what its launches cannot hold, and sink
+// partials of 256 GiB.
+int win_bwd_plan(const char* what, const WinLayout& w, int window, esep::AttnWinArgs* p) {
+  p->window = window;
+  p->sinks = w.sinks;
+  p->far = w.far;
+  p->far_split = w.far_split;
+  p->far_len = w.at.far_len;
+  p->by_seq = w.at.by_seq;
+  p->b.split = w.split;
+  if (!esep::attn_win_bwd_fits(*p) || w.total - w.main_at >= int64_t{1} << 36)
+    return fail(ESEP_ESHAPE, "%s: sinks=%d at a window of %d are too many for %lld tokens in %d sequences", what,
+                w.sinks, window, (long long)p->b.f.T, p->b.f.n_seq);
+  return 0;
 }
 
 // Token strides of the attention tensors, in elements, at most 2^22 (8 MiB of 16-bit
@@ -786,12 +804,21 @@ int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
   return e == hipSuccess ? 0 : hip_fail(e, "attn_win_fwd launch");
 }
 
-int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int max_seqlen, int window,
+int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int n_seq, int max_seqlen, int window,
                                     int sinks) {
-  if (T <= 0 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || max_seqlen < 1 || window < 1 || sinks < 0)
+  g_err[0] = 0;
+  if (T <= 0 || T > 0x7fffffff || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || n_seq < 1 || max_seqlen < 1 ||
+      window < 1 || sinks < 0)
     return 0;
   if (sees_all(max_seqlen, window, sinks)) return esep_attn_bwd_workspace(T, HQ, HK, D);
-  return win_layout(T, HQ, HK, D, max_seqlen, window, sinks).total;
+  const WinLayout w = win_layout(T, HQ, HK, D, n_seq, max_seqlen, window, sinks);
+  esep::AttnWinArgs p{};
+  p.b.f.T = T;
+  p.b.f.n_seq = n_seq;
+  p.b.f.HQ = HQ;
+  p.b.f.HK = HK;
+  const int rc = win_bwd_plan("attn_win_bwd_workspace", w, window, &p);
+  return rc != 0 ? rc : w.total;
 }
 
 int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
@@ -819,15 +846,9 @@ int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
     if (e == hipSuccess) e = esep::launch_attn_rest(r, s);
     return e == hipSuccess ? 0 : hip_fail(e, "attn_win_bwd launch");
   }
-  const WinLayout w = win_layout(T, HQ, HK, D, max_seqlen, window, sinks);
-  if (w.far && esep::win_main_slots(T, window) * HK * 2 * w.sinks >= int64_t{1} << 24)
-    return fail(ESEP_ESHAPE, "attn_win_bwd: sinks=%d at a window of %d are too many for %lld tokens", sinks,
-                window, (long long)T);
-  p.window = window;
-  p.sinks = w.sinks;
-  p.far = w.far;
-  p.far_split = w.far_split;
-  p.b.split = w.split;
+  const WinLayout w = win_layout(T, HQ, HK, D, n_seq, max_seqlen, window, sinks);
+  rc = win_bwd_plan("attn_win_bwd", w, window, &p);
+  if (rc != 0) return rc;
   p.sink_main = workspace + w.main_at;
   p.sink_far = workspace + w.far_at;
   const hipError_t e = esep::launch_attn_win_bwd(p, dt, D, s, &sup);

@@ -81,7 +81,7 @@ SIGNATURES = {
                              _i32, _i32, _f32, _vp]),
     "esep_attn_win_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32,
                                  _i32, _i32, _vp, _i32, _i32, _f32, _i32, _i32, _i32, _vp]),
-    "esep_attn_win_bwd_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "esep_attn_win_bwd_workspace": (_i64, [_i64] + [_i32] * 7),
     "esep_attn_win_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp,
                                  _i32, _i32, _f32, _i32, _i32, _vp]),
@@ -505,10 +505,16 @@ def attn_bwd_workspace(T, HQ, HK, D):
     return int(lib().esep_attn_bwd_workspace(int(T), int(HQ), int(HK), int(D)))
 
 
-def attn_win_bwd_workspace(T, HQ, HK, D, max_seqlen, window, sinks):
-    """Floats of fp32 workspace esep_attn_win_bwd needs for these sizes."""
-    return int(lib().esep_attn_win_bwd_workspace(int(T), int(HQ), int(HK), int(D), int(max_seqlen),
-                                                 int(window), int(sinks)))
+def attn_win_bwd_workspace(T, HQ, HK, D, max_seqlen, window, sinks, n_seq=None):
+    """Floats of fp32 workspace esep_attn_win_bwd needs for these sizes (n_seq None: a sequence to every
+    token).
+    Raises where the backward refuses them."""
+    n = int(lib().esep_attn_win_bwd_workspace(int(T), int(HQ), int(HK), int(D),
+                                              int(T if n_seq is None else n_seq), int(max_seqlen), int(window),
+                                              int(sinks)))
+    if n < 0:
+        _check(n, "esep_attn_win_bwd_workspace")
+    return n
 
 
 def _attn_bwd_checked(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace, need):
@@ -560,7 +566,7 @@ def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scal
     `workspace` as attn_bwd's, of attn_win_bwd_workspace's size."""
     dev, (T, HQ, HK, D), workspace = _attn_bwd_checked(
         q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, workspace,
-        lambda *sizes: attn_win_bwd_workspace(*sizes, max_seqlen, window, sinks))
+        lambda *sizes: attn_win_bwd_workspace(*sizes, max_seqlen, window, sinks, cu_seqlens.numel() - 1))
     with _on(dev):
         rc = lib().esep_attn_win_bwd(
             _p(q), _tokens_ld(q, "q"), _p(k), _tokens_ld(k, "k"), _p(v), _tokens_ld(v, "v"),

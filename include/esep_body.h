@@ -289,10 +289,14 @@ int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
 /*
  * Its backward, deterministic (esep_attn_bwd's arguments; o_low as the forward wrote it, or NULL). workspace:
  * fp32, 16-byte aligned, esep_attn_win_bwd_workspace floats, a function of the sizes only; max_seqlen >= every
- * sequence length, as the forward's. dq, dk and dv are 0 for the tokens behind the last sequence. ESEP_ESHAPE
- * where the sink rows are more than one launch takes.
+ * sequence length, as the forward's. dq, dk and dv are 0 for the tokens behind the last sequence.
+ * The workspace holds delta (HQ T floats), up to HQ / HK partials of dK and dV (2 HK T D each) and, where max_seqlen
+ * passes window + 512, the sink rows': up to HQ / HK times 2 HK sinks D for each of min(n_seq, T / (window + 512) + 1)
+ * sequences, and as much again for each of them and for every 512 tokens (where that makes more than 4096 blocks
+ * of 128 sink rows, for every 1024, 2048 .. 32768). Both return ESEP_ESHAPE where the sink rows of those
+ * sequences, 2 HK sinks each, reach 2^24, or their partials 2^36 floats.
  */
-int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int max_seqlen, int window,
+int64_t esep_attn_win_bwd_workspace(int64_t T, int HQ, int HK, int D, int n_seq, int max_seqlen, int window,
                                     int sinks);
 int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, const void* v,
                       int64_t v_rs, const void* o, int64_t o_rs, const void* o_low, const void* dout, int64_t do_rs,
