@@ -74,6 +74,9 @@ class WindowAttention(torch.autograd.Function):
         o = new((T, HQ, D), device=q.device, dtype=q.dtype)
         low = lse = None
         if any(ctx.needs_input_grad):
+            if sinks:  # more sink rows than the backward takes are refused here already
+                _hip.attn_win_bwd_workspace(T, HQ, k.shape[1], D, max_seqlen, window, sinks,
+                                            cu_seqlens.numel() - 1)
             low = torch.empty_like(o)
             lse = torch.empty((HQ, T), device=q.device, dtype=torch.float32)
         _hip.attn_win_fwd(q, k, v, o, cu_seqlens, max_seqlen, scale, window, sinks, lse=lse, o_low=low,

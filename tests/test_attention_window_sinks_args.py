@@ -1,8 +1,10 @@
-"""The windowed backward's sink partials without a GPU: their size follows the sequences there are."""
+"""The windowed backward's sink partials without a GPU: their size follows the sequences there are, and what the
+backward refuses is refused before the forward runs."""
 
 import pytest
+import torch
 
-from solution.body import _hip
+from solution.body import _hip, attention
 
 # (T, query heads, kv heads, D, max_seqlen, window, sinks)
 LONG = (131072, 32, 8, 128, 131072, 16, 4096)
@@ -38,3 +40,18 @@ def test_partials_no_card_holds_are_refused():
     with pytest.raises(_hip.EsepError, match="sinks"):
         w(1 << 30, 4, 2, 64, 1 << 30, 1, 1 << 20, 1)
 
+
+def test_the_forward_refuses_what_the_backward_would(monkeypatch):
+    ran = []
+    monkeypatch.setattr(_hip, "attn_win_fwd", lambda *a, **kw: ran.append(1))
+    T, n_seq, sinks = 32768, 64, 16384
+    q = torch.zeros(T, 8, 64, dtype=torch.float16)
+    cu = torch.arange(n_seq + 1, dtype=torch.int32) * (T // n_seq)
+    args = (cu, T)
+    with pytest.raises(_hip.EsepError, match="sinks"):
+        attention.varlen_attention(q.requires_grad_(), q, q, *args, window=1, sinks=sinks)
+    assert not ran
+    attention.varlen_attention(q, q, q, *args, window=1, sinks=sinks // 2)  # half the rows
+    q = q.detach()
+    attention.varlen_attention(q, q, q, *args, window=1, sinks=sinks)  # no gradient is asked for
+    assert len(ran) == 2
