@@ -157,6 +157,15 @@ class NF4MultiLinear(torch.autograd.Function):
 MATVEC_ROWS = _hip.NF4_MATVEC_ROWS
 
 
+def _unread(x):
+    """Rows that the kernel does not read (columns apart, rows that overlap), or, at a K of whole scale blocks,
+    only an element at a time (not 16 bytes at a time): up to 16 of them are copied first."""
+    (m, k), (row, col) = x.shape, x.stride()
+    if (k > 1 and col != 1) or (m > 1 and row < k):
+        return True
+    return k % 64 == 0 and (x.data_ptr() % 16 != 0 or (m > 1 and (row % 8 != 0 or row > 1 << 26)))
+
+
 def _matvec(x, weights, states, biases):
     items, dt, n = [], x.dtype, 0
     for w, qs, b in zip(weights, states, biases):
@@ -167,8 +176,8 @@ def _matvec(x, weights, states, biases):
                       _f32(qs.code), b, rows))
         n += rows
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.shape[1] > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    if _unread(x2):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
     y = torch.empty((x2.shape[0], n), device=x.device, dtype=dt)
     _hip.nf4_matvec(x2, items, y)
     return y if x2 is x else y.view(*x.shape[:-1], n)
