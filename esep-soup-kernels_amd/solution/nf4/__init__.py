@@ -191,7 +191,7 @@ class NF4Matvec(torch.autograd.Function):
     def forward(ctx, x, weights, states, *biases):
         w_dtype = x.dtype if x.dtype != torch.float32 else torch.float16
         ctx.weights, ctx.states, ctx.x_dtype, ctx.w_dtype = weights, states, x.dtype, w_dtype
-        ctx.bias_dtypes = [None if b is None else b.dtype for b in biases]
+        ctx.bias_like = [None if b is None else (b.dtype, b.shape) for b in biases]
         return _matvec(x if x.dtype == w_dtype else x.to(w_dtype), weights, states, biases)
 
     @staticmethod
@@ -199,8 +199,11 @@ class NF4Matvec(torch.autograd.Function):
         dx, dbias, c = None, [], 0
         for i, qs in enumerate(ctx.states):
             n = qs.shape[0]
-            dbias.append(dy[..., c:c + n].reshape(-1, n).sum(0, dtype=ctx.bias_dtypes[i])
-                         if ctx.needs_input_grad[3 + i] else None)
+            if ctx.needs_input_grad[3 + i]:
+                dt, shape = ctx.bias_like[i]
+                dbias.append(dy[..., c:c + n].reshape(-1, n).sum(0, dtype=dt).reshape(shape))
+            else:
+                dbias.append(None)
             c += n
         if ctx.needs_input_grad[0]:
             w = dequantize_nf4_multi(ctx.weights, ctx.states, dtype=ctx.w_dtype)

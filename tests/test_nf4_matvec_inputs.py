@@ -51,3 +51,13 @@ def test_expanded_leading_dimensions(handed):
     x = torch.randn(K).half().expand(2, 3, K)
     assert _call(x).shape == (2, 3, N)
     assert torch.equal(handed[0], x.reshape(6, K)) and _hip._rows_ld(handed[0], K) == K
+
+
+@pytest.mark.parametrize("shape", [(N,), (1, N), (N, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_a_bias_gets_a_gradient_of_its_shape(handed, shape, dtype):
+    x = torch.randn(3, K).half()
+    bias = torch.zeros(shape, dtype=dtype).requires_grad_()
+    dy = torch.arange(3 * N).view(3, N).half()
+    (g,) = torch.autograd.grad(_call(x, bias), bias, dy)
+    assert g.shape == shape and g.dtype == dtype and torch.equal(g.reshape(-1), dy.sum(0).to(dtype))
