@@ -35,8 +35,13 @@ def supported(q, k, v, dropout=0.0):
 def _heads_packed(t):
     rs, hs, ds = t.stride()
     if ds != 1 or hs != t.shape[2] or rs % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
+        t = _copy(t)
     return t
+
+
+def _copy(t):
+    """A dense copy at an address of its own (contiguous() gives a dense tensor back at its odd address)."""
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 class VarlenAttention(torch.autograd.Function):
@@ -178,7 +183,7 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
 def _cache(q, k_cache, v_cache, lengths, scale, window, sinks):
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
     if q4.dim() == 4 and _unaligned(q4):
-        q4 = q4.contiguous()
+        q4 = _copy(q4)
     o = torch.empty(q4.shape, device=q.device, dtype=q.dtype)
     _hip.attn_cache(q4, k_cache, v_cache, o, lengths, scale, window, sinks)
     return o.squeeze(1) if q.dim() == 3 else o
