@@ -601,6 +601,8 @@ def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None,
     S, HK = kshape[1], kshape[2]
     if kshape != (B, S, HK, D) or v.shape != kshape or o.shape != shape or not o.is_contiguous():
         raise EsepError("attn_cache: q, o [B, n, HQ, D] (o dense) and k, v [B, S, HK, D]")
+    if B > 0x7FFFFFFF or n > 0x7FFFFFFF or S > 0x7FFFFFFF:  # the library counts in 32 bits
+        raise EsepError(f"attn_cache: bad sizes B={B} n={n} S={S}")
     dt = q.dtype
     if k.dtype != dt or v.dtype != dt or o.dtype != dt:
         raise EsepError("q, k, v and o must share one dtype")

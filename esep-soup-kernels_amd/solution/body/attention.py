@@ -109,6 +109,17 @@ def _whole(name, value, least):
     return int(value)
 
 
+def _bound(max_seqlen, T):
+    """A bound on the lengths that fits 32 bits: past those, the number of tokens says as much."""
+    n = int(max_seqlen)
+    if n < 0:
+        raise _hip.EsepError(f"max_seqlen must be 0 or more, got {max_seqlen!r}")
+    return n if n <= 0x7FFFFFFF - _ROUND else T
+
+
+_ROUND = 1024  # the launches round it up to a block's tokens
+
+
 def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, sinks=0):
     """Causal attention within each sequence of the packed tokens. q [T, HQ, D] (or
     [1, T, HQ, D]), k, v [T, HK, D]; cu_seqlens int32 [n_seq + 1] on q's device; max_seqlen an
@@ -123,12 +134,12 @@ def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, s
         scale = q.shape[-1] ** -0.5
     if q.dim() == 4:  # [1, T, H, D] views: the Function works on [T, H, D]
         q, k, v = q.squeeze(0), k.squeeze(0), v.squeeze(0)
-    sinks = _whole("sinks", sinks, 0)
+    max_seqlen, sinks = _bound(max_seqlen, q.shape[0]), _whole("sinks", sinks, 0)
     if window is not None:
         window = _whole("window", window, 1)
         _hip.refuse_proxies("varlen_attention")
-        return WindowAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale), window, sinks)
-    return VarlenAttention.apply(q, k, v, cu_seqlens, int(max_seqlen), float(scale))
+        return WindowAttention.apply(q, k, v, cu_seqlens, max_seqlen, float(scale), window, sinks)
+    return VarlenAttention.apply(q, k, v, cu_seqlens, max_seqlen, float(scale))
 
 
 _NO_GRADIENT = ("cache_attention has no gradient: call it under torch.no_grad(), or on detached tensors "
