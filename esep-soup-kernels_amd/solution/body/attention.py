@@ -104,9 +104,14 @@ class WindowAttention(torch.autograd.Function):
 
 
 def _whole(name, value, least):
-    if isinstance(value, bool) or int(value) != value or value < least or value > 0x7FFFFFFF:
+    try:
+        n = int(value)
+        whole = not isinstance(value, bool) and bool(n == value) and least <= n <= 0x7FFFFFFF
+    except (TypeError, ValueError, OverflowError, RuntimeError):  # no number, NaN, an infinity, a tensor of many
+        whole = False
+    if not whole:
         raise _hip.EsepError(f"{name} must be a whole number of at least {least}, got {value!r}")
-    return int(value)
+    return n
 
 
 def _bound(max_seqlen, T):
