@@ -818,7 +818,7 @@ class _Packing:
         counts = real.sum(1)
         if windows:  # the tokens' runs too: a window counts columns, gaps among them
             starts = real[:, 1:] & ~real[:, :-1]
-            counts = torch.stack((counts, real[:, 0] + starts.sum(1)))
+            counts = torch.stack((counts, real[:, :1].sum(1) + starts.sum(1)))
             counts, runs = counts.tolist()
             self.lens, self.gaps = counts, max(runs, default=0) > 1
         else:
