@@ -857,7 +857,7 @@ int esep_attn_win_bwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
 }
 
 int64_t esep_attn_cache_workspace(int B, int n, int S, int HQ, int HK, int D, int window, int sinks) {
-  if (B < 1 || n < 1 || S < 1 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0)
+  if (B < 1 || n < 1 || S < 0 || HQ < 1 || HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0)
     return 0;
   const int w = window == 0 || window > S ? S : window;
   const int64_t units = esep::cache_units(esep::cache_tiles(B, n, S, HQ, HK, w, sinks), D);
