@@ -183,14 +183,14 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
     For answering only: there is no gradient, so inputs that record one in grad mode, or carry a forward-mode
     tangent, are refused. The scratch memory is of the caller's stream and, under capture, of the graph. A
     traced module (torch.jit.trace) calls it again. Returns o, of q's shape and dtype, dense."""
-    if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
-        raise _hip.EsepError(_NO_GRADIENT)
     sinks = _whole("sinks", sinks, 0)
     if window is not None:
         window = _whole("window", window, 1)
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if _hip.recorded(q, k_cache, v_cache, lengths):
+        if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
+            raise _hip.EsepError(_NO_GRADIENT)
         _hip.refuse_proxies("cache_attention")
         return CacheAttention.apply(q, k_cache, v_cache, lengths, scale, window, sinks)
     return _cache(q, k_cache, v_cache, lengths, scale, window, sinks)
