@@ -161,7 +161,7 @@ struct AttnCacheArgs {
   float* part;         // partials behind them
   int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
   int B, n, S, HQ, HK;
-  int window, sinks;   // window 0x7fffffff: none
+  int window, sinks;   // window at least 1; none: S, a row's longest
   float scale_log2;
 };
 
@@ -175,9 +175,13 @@ inline int64_t cache_key_tiles(int S, int n, int window, int sinks) {
 }
 // Wavefronts for a number of tiles: one to a tile up to 256, from 1024 tiles on four tiles to each, up to four
 // (D = 64: eight) to a CU. Each keeps a ring of two K / V tiles in LDS (32 KiB at D = 128, of a CU's 160); a
-// fifth made the four SIMDs uneven (32 rows of up to 8192 tokens, 28 / 4 heads, D = 128: 79 us, with four 69),
-// two tiles to each more partials to join than it saved (one row of 32768 tokens 29 us, four 20.6; 700 tokens 9.8,
-// one 8.8). Device and host use the same rule: the host's tiles are a bound of the device's.
+// fifth made the four SIMDs uneven (32 rows of up to 8192 tokens, 28 / 4 heads, D = 128: 79 us, with four 69).
+// Fewer tiles to each make more partials, which a few long rows pay in the join. Walk and join in us with 1 / 2 / 3 /
+// 4 tiles to a wavefront, bf16, 12 / 2 heads of 128: one row of 32768 tokens 21.1 / 21.1 / 18.3 / 16.7, of 8192
+// 12.3 / 11.1 / 11.1 / 11.1; 8 rows of 2048 12.4 / 11.6 / 13.0 / 11.7; 32 of 1024 14.9 / 14.9 / 15.5 / 13.8; 28 / 4
+// heads, one row of 8192 15.3 / 12.7 / 13.4 / 12.8. Windows go the other way by up to 2.5 us: 8 rows through 4096
+// 20.3 / 20.1 / 15.0 / 17.4, 8 through 1024 10.3 / 11.2 / 11.3 / 11.3, 32 through 256 10.2 / 11.6 / 11.4 / 11.5.
+// Device and host use the same rule: the host's tiles are a bound of the device's.
 __host__ __device__ inline int64_t cache_units(int64_t tiles, int D) {
   const int64_t most = kAttnCUs * (D == 128 ? 4 : 8);
   const int64_t u = tiles <= kAttnCUs ? tiles : (tiles / 4 > kAttnCUs ? tiles / 4 : kAttnCUs);
@@ -630,7 +634,8 @@ __device__ __forceinline__ void store_rows_t(T* row, const f32x16 (&acc)[D / 32]
     }
 }
 
-// What the rounding of o = acc * mul to T drops, stored in T as o is: its own rounding is 2^-8 (bf16) of a half step.
+// What the rounding of o = acc * mul to T drops, stored in T as o is: its own rounding is half a step of T's (bf16
+// 2^-8, fp16 2^-11) of what is at most half a step of o.
 template <typename T, int D>
 __device__ __forceinline__ void store_low_t(T* row, f32x16 (&acc)[D / 32], int hi, float mul) {
 #pragma unroll

@@ -49,6 +49,8 @@ __device__ __forceinline__ void mask_window(f32x16& acc, int kh, int utop, int u
 // the first V^T ones before the softmax, whose VALU work hides their latency), pinned by
 // scheduling barriers: the compiler sinks each read to just before its use (config 5 forward
 // 2.03 -> 1.93 ms).
+// The probabilities are rounded to T, the matrix instructions' operand type, before P V (half a step of each; l
+// adds them up unrounded): with V and the result in T too, o is off by up to about twice its own rounding.
 // mask(acc) sets the scores that the lane's query does not see to -inf.
 template <typename T, int D, class Mask>
 __device__ __forceinline__ void fwd_tile_swz(const char* ks, const char* vs, int lane,
@@ -127,7 +129,7 @@ __device__ __forceinline__ void fwd_tile_swz(const char* ks, const char* vs, int
 // dP^T = V dO^T with the wave's Q and dO as B operands, dS^T = P^T * (dP^T - delta), then
 // dQ^T += K^T dS^T with K^T read transposed out of ks and dS^T in the permuted key order. K and V
 // operands are read three ahead of their MFMAs and the first two K^T ones before the exponentials
-// (config 5 bwd 7.11 -> 6.97 ms).
+// (config 5 bwd 7.11 -> 6.97 ms). dS is rounded to T, the matrix instructions' operand type.
 template <typename T, int D, class Mask>
 __device__ __forceinline__ void dq_tile_swz(const char* ks, const char* vs, int lane,
                                             float scale_log2, float lse2, float delta,

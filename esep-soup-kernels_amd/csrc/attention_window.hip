@@ -17,8 +17,11 @@
 // delta = rowsum(dO o) of an o rounded to 16 bits is off by half a step of it, which shows in dQ and dK where a
 // query sees few keys (o is then as large as v). The forward can store what o's rounding dropped (o_low), and the
 // backward adds it. Errors of dQ and dK in bf16 in the 2-norm against float64: 2.42e-3 instead of 2.57e-3 at a
-// window of 16, 2.38e-3 instead of 2.47e-3 at 256 (1.66e-3 is the rounding of the results alone). That costs 3%
-// of both passes (65536 tokens, 28 / 4 heads, window 1024: 4.14 ms against 4.01), o_low's bytes.
+// window of 16, 2.38e-3 instead of 2.47e-3 at 256 (1.66e-3 is the rounding of the results alone; P and dS, rounded
+// to 16 bits for the matrix instructions, make the rest). That costs o_low's bytes: as much memory as o until the
+// backward, and 1 to 4% of both passes (forward + backward in us without and with: 65536 tokens, 28 / 4 heads,
+// window 1024, bf16 858 + 2990 and 931 + 3053, fp16 898 + 3102 and 964 + 3187; 32768 tokens, 12 / 2 heads, window
+// 4096 791 + 2745 and 804 + 2755; 5933 tokens in 8 sequences, window 256 23.0 + 99.4 and 25.6 + 102).
 //
 // All blocks of a launch do near-equal work, so no order by length is needed: the (sequence, tile,
 // head) triples are numbered with the heads innermost and cut into 8 contiguous runs, one to an XCD,
@@ -337,7 +340,8 @@ __global__ __launch_bounds__(kAttnThreads, kDqPerCU<D>) void k_attn_win_dq(const
 // 32 queries of the dK / dV walk for a wavefront's 32 keys: the query rows at qrow / drow (Q and dO,
 // 32 rows of the swizzled LDS tiles), their lse and delta words, the keys' K operands in registers and
 // their V rows at vlds. s[i] is S[q][key] for query row 8 (i / 4) + 4 hi + i % 4; mask(s) sets what the
-// lane's key is not seen by to -inf. rop is the lane's row operand offset (swz_row_base).
+// lane's key is not seen by to -inf. rop is the lane's row operand offset (swz_row_base). P and dS are rounded to
+// T, the matrix instructions' operand type.
 template <typename T, int D, class Mask>
 __device__ __forceinline__ void dkdv_tile_swz(const char* qrow, const char* drow, const char* vlds,
                                               const float* lse_s, const float* del_s, int hi,

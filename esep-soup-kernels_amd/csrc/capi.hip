@@ -132,8 +132,10 @@ struct WinLayout {
 // Blocks per (kv head, key tile) of the windowed dK / dV kernel: of 1 .. HQ / HK the number with the least
 // estimated time; its blocks take G / s of the G query heads, rounded down or up. They do near-equal work, so
 // what counts beside the partials' bytes is how they fill the 512 that are resident: half of them or fewer run a
-// quarter faster each, and a round that is begun costs about a third of one more. A 32-query item of two blocks
-// to a CU takes 2.6 us (D = 64: 1.3), the partials are written and read at 5 TB/s. Backward in us with 1 / 2 / 3 /
+// quarter faster each, and a round that is begun costs about a third of one more. (512 is two to a CU, D = 128's; at
+// D = 64 three are resident, and the times below stand for the rule with 512 there too.) A 32-query item of two
+// blocks to a CU takes 2.6 us (D = 64: 1.3), the partials are written and read at 5 TB/s. The constants were fitted
+// to these five sizes. Backward in us with 1 / 2 / 3 /
 // 4 / 5 / 6 (/ 7) blocks, bf16 (* what it picks): 12 / 2 heads, D = 128, 5933 tokens in 8 sequences, window 256,
 // 136 / 104 / 102* / 102 / 113 / 110; 8192, 512: 220 / 180 / 159* / 204 / 188 / 177; 32768, 4096: 3396 / 2981 / 2849 /
 // 3004 / 2788 / 2780*; 28 / 4 heads, 8192, 512: 344 / 383 / 335* / 357 / 352 / 371 / 380; 14 / 2 heads, D = 64, 12011

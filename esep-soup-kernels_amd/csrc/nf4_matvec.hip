@@ -12,16 +12,17 @@
 //     one block and (n, q = 2, 3) the next. A's 16 rows are 8 rows of x twice, the first with zeros against
 //     q = 2, 3, the second against q = 0, 1, so that each of D's values belongs to one block, whose scale is
 //     that of the lane that holds it. Four products of 128 k are then added with one fma per value.
-// The codes are rounded to x's type (fp16 2^-12, bf16 2^-9 relative at most on average half of that), as
-// dequantize_nf4 rounds the whole weight to it; scales, products and sums stay in fp32.
+// The codes are rounded to x's type, the matrix instructions' operand type, as dequantize_nf4 rounds the whole weight
+// to it: by up to 2^-11.6 of a code in fp16 and 2^-8.3 in bf16 (2^-12.5 and 2^-9.5 in the root mean square), the same
+// for each of the 16 wherever it stands. Scales, products and sums stay in fp32.
 //
 // A block takes a run of tiles of 16 W rows; the tiles' 128-k steps, laid end to end, are cut into equal runs,
 // one to each of its 16 wavefronts, which streams its run four steps ahead with no barrier; parts of a tile
 // meet in LDS at the end and are added in the wavefronts' order. x lies in LDS where it fits.
 //
 // Kernel trace, one row of x in fp16: 2 x 18944 rows of W of 3584 in 20.6 us (70 MB, 3.4 TB/s; 14.0 is the copy
-// rate's time), q / k / v of 1536 in 7.0; 7 rows in bf16, 1536 of 8960 in 11.4 (96 blocks for 256 CUs: a finer
-// cut would add parts of a tile across blocks in a second launch). Parts left out in a copy for timing, 20.3 us
+// rate's time), q / k / v of 1536 in 7.0; 7 rows in bf16, 1536 of 8960 in 11.4 (96 blocks for 256 CUs; a finer
+// cut, parts of a tile added across blocks, was not tried). Parts left out in a copy for timing, 20.3 us
 // with all: without the table reads 19.2, without the loads of W 16.9, so loads and decode overlap. Slower: six or
 // eight steps ahead (21.0, 22.8), x in registers (20.8), loads of 128 bytes of a row (21.0), W past the caches
 // (22.4).

@@ -128,13 +128,19 @@ _ROUND = 1024  # the launches round it up to a block's tokens
 def varlen_attention(q, k, v, cu_seqlens, max_seqlen, scale=None, window=None, sinks=0):
     """Causal attention within each sequence of the packed tokens. q [T, HQ, D] (or
     [1, T, HQ, D]), k, v [T, HK, D]; cu_seqlens int32 [n_seq + 1] on q's device; max_seqlen an
-    int >= every sequence length. Returns o [T, HQ, D] in q's dtype.
+    int >= every sequence length, cu_seqlens from 0 on and not falling. Returns o [T, HQ, D] in q's dtype.
+
+    Scores, softmax sums and the gradients' sums are fp32; the probabilities and, in the backward, the scores'
+    gradients are rounded to q's dtype before the products with v, dO, k and q. An infinity or a NaN reaches queries
+    of its own sequence only, but there also some that do not see its token.
 
     window (None: no bound): query i of a sequence sees key j <= i only if i - j < window (the last
     `window` tokens, its own among them, as HF's sliding_window) or j < sinks (the sequence's
     first tokens, which stay visible; without a window they always are). With a window, tokens behind the
-    last sequence get an output and gradients of 0, and dq and dk do not carry the rounding of o. Where
-    window + sinks reach max_seqlen it is the causal kernels that run."""
+    last sequence get an output and gradients of 0, and dq and dk do not carry the rounding of o (which keeps one
+    more tensor of o's size until the backward). Where window + sinks reach max_seqlen it is the causal kernels
+    that run. The backward's scratch memory grows with the sinks (esep_attn_win_bwd); what it would refuse, a forward
+    with gradients refuses."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if q.dim() == 4:  # [1, T, H, D] views: the Function works on [T, H, D]
@@ -171,14 +177,17 @@ class CacheAttention(torch.autograd.Function):
 def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks=0):
     """Attention of each row's newest tokens over its cache: decoding (one new token a row), or a few new
     tokens at once. q [B, n, HQ, D] (or [B, HQ, D]: n = 1), the queries of the n newest tokens; k_cache, v_cache
-    [B, S, HK, D] views of any batch, token and head strides (HF's [B, HK, S, D] cache transposed, say)
-    in which the new tokens are stored already; lengths int32 [B] on the same device: the tokens in each
+    [B, S, HK, D] views (HF's [B, HK, S, D] cache transposed, say) at 16-byte addresses, with a dense head dim and
+    batch, token and head strides of any multiples of 8 elements (tokens up to 2^22 apart), in which the new tokens
+    are stored already; lengths int32 [B] on the same device: the tokens in each
     row's cache, the new ones the last of them. Query head h reads kv head h // (HQ // HK). fp16 and bf16, D
     in {64, 128}.
 
     Query t of a row sits at position p = lengths - n + t and sees key j <= p, through a window only if p - j <
     window or j < sinks, as in varlen_attention. What a cache holds past a row's length is never read; a query
-    at a position below 0 (a row shorter than n) gets 0. Lengths past S count as S.
+    at a position below 0 (a row shorter than n) gets 0. Lengths past S count as S. Scores and sums are fp32, the
+    probabilities are rounded to q's dtype before the product with v. An infinity or a NaN reaches queries of its
+    own row only, but with several new tokens also some that do not see it.
 
     For answering only: there is no gradient, so inputs that record one in grad mode, or carry a forward-mode
     tangent, are refused. The scratch memory is of the caller's stream and, under capture, of the graph. A

@@ -289,7 +289,8 @@ int esep_attn_win_fwd(const void* q, int64_t q_rs, const void* k, int64_t k_rs, 
 /*
  * Its backward, deterministic (esep_attn_bwd's arguments; o_low as the forward wrote it, or NULL). workspace:
  * fp32, 16-byte aligned, esep_attn_win_bwd_workspace floats, a function of the sizes only; max_seqlen >= every
- * sequence length, as the forward's. dq, dk and dv are 0 for the tokens behind the last sequence.
+ * sequence length, as the forward's. dq, dk and dv are 0 for the tokens behind the last sequence (with no sequence
+ * or a max_seqlen of 0 nothing is written, by either direction).
  * The workspace holds delta (HQ T floats), up to HQ / HK partials of dK and dV (2 HK T D each) and, where max_seqlen
  * passes window + 512, the sink rows': up to HQ / HK times 2 HK sinks D for each of min(n_seq, T / (window + 512) + 1)
  * sequences, and as much again for each of them and for every 512 tokens (where that makes more than 4096 blocks
