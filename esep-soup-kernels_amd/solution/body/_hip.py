@@ -219,11 +219,10 @@ def recorded(*tensors):
     a LoRA term's forward and backward.)"""
     if torch.compiler.is_compiling() or _tracing() or _dispatch_modes() or _transforms():
         return True
+    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (type(t) not in _PLAIN_TYPES or not _has_storage(t)):
+        if t is not None and (type(t) not in _PLAIN_TYPES or not _has_storage(t) or (grad and t.requires_grad)):
             return True
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
     return forward_ad._current_level >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 

@@ -197,7 +197,7 @@ def cache_attention(q, k_cache, v_cache, lengths, scale=None, window=None, sinks
         window = _whole("window", window, 1)
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    if _hip.recorded(q, k_cache, v_cache, lengths):
+    if _hip.recorded(q, k_cache, v_cache):  # (lengths are whole numbers)
         if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
             raise _hip.EsepError(_NO_GRADIENT)
         _hip.refuse_proxies("cache_attention")
