@@ -79,7 +79,9 @@ class WindowAttention(torch.autograd.Function):
         o = new((T, HQ, D), device=q.device, dtype=q.dtype)
         low = lse = None
         if any(ctx.needs_input_grad):
-            if sinks:  # more sink rows than the backward takes are refused here already
+            # what the backward would refuse is refused here already: 2^24 sink rows or 2^36 floats of their partials
+            # (esep_attn_win_bwd), which no smaller product reaches
+            if sinks * HQ * T >= 1 << 31:
                 _hip.attn_win_bwd_workspace(T, HQ, k.shape[1], D, max_seqlen, window, sinks,
                                             cu_seqlens.numel() - 1)
             low = torch.empty_like(o)
@@ -104,6 +106,8 @@ class WindowAttention(torch.autograd.Function):
 
 
 def _whole(name, value, least):
+    if type(value) is int and least <= value <= 0x7FFFFFFF:
+        return value
     try:
         n = int(value)
         whole = not isinstance(value, bool) and bool(n == value) and least <= n <= 0x7FFFFFFF
