@@ -578,13 +578,13 @@ def attn_win_bwd(q, k, v, o, dout, lse, dq, dk, dv, cu_seqlens, max_seqlen, scal
     _record(name)
 
 
-def _bth_strides(t, name):
-    """(batch, token, head) strides of a [B, n, H, D] tensor with a dense head dim, as the kernel takes
-    them: multiples of 8 (a dimension of one element has any)."""
+def _bth_strides(t, shape, name):
+    """(batch, token, head) strides of a [B, n, H, D] tensor of this shape with a dense head dim, as the kernel
+    takes them: multiples of 8 (a dimension of one element has any)."""
     b, n, h, d = t.stride()
     if d != 1:
         raise EsepError(f"{name} needs a unit stride on the head dim")
-    B, N, H, _ = t.shape
+    B, N, H, _ = shape
     return b if B > 1 else 0, n if N > 1 else 0, h if H > 1 else 0
 
 
@@ -593,9 +593,9 @@ def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None,
     lengths (int32 [B], the new tokens among them) (esep_attn_cache). o [B, n, HQ, D] dense. `workspace` is
     a contiguous fp32 tensor of >= attn_cache_workspace's elements (allocated here when not given)."""
     dev = _dev(q, k, v, o, lengths, workspace)
-    if q.dim() != 4 or k.dim() != 4:
-        raise EsepError("attn_cache: q [B, n, HQ, D] and k, v [B, S, HK, D]")
     shape, kshape = q.shape, k.shape
+    if len(shape) != 4 or len(kshape) != 4:
+        raise EsepError("attn_cache: q [B, n, HQ, D] and k, v [B, S, HK, D]")
     B, n, HQ, D = shape
     S, HK = kshape[1], kshape[2]
     if kshape != (B, S, HK, D) or v.shape != kshape or o.shape != shape or not o.is_contiguous():
@@ -614,7 +614,8 @@ def attn_cache(q, k, v, o, lengths, scale, window=None, sinks=0, workspace=None,
     elif (workspace.dtype != torch.float32 or not workspace.is_contiguous()
           or workspace.numel() < need):
         raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
-    strides = array("q", (*_bth_strides(q, "q"), *_bth_strides(k, "k"), *_bth_strides(v, "v")))
+    strides = array("q", (*_bth_strides(q, shape, "q"), *_bth_strides(k, kshape, "k"),
+                          *_bth_strides(v, kshape, "v")))
     at = strides.buffer_info()[0]
     with _on(dev):
         rc = lib().esep_attn_cache(
