@@ -23,7 +23,7 @@ import torch
 from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().with_name("libesep_body.so")
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
 _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,

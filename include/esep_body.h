@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define ESEP_ABI_VERSION 1
+#define ESEP_ABI_VERSION 2
 
 /* Element type codes. */
 enum esep_dtype {
