@@ -18,6 +18,7 @@
 // + 3.9; one row of 700 tokens 6.0 + 3.8; 16 new tokens over 4 rows of up to 4001, 14 / 2 heads of 64 14.2 + 4.2.
 #include <cmath>
 
+#include "attention_cache.hpp"
 #include "attention_tiles.hpp"
 
 namespace esep {
@@ -38,30 +39,6 @@ __device__ __forceinline__ CacheRow cache_row(const AttnCacheArgs& a, int b) {
   r.ns = r.lo > 0 ? (r.sink_hi + 31) / 32 : 0;
   r.tiles = r.ns + (r.len - r.lo + 31) / 32;
   return r;
-}
-
-// The walk's geometry, found by every wavefront from the lengths: the tiles of all groups, dealt to `units`
-// wavefronts, the first `extra` of them one more than `each`.
-struct CachePlan {
-  int total, units, each, extra;
-  __device__ __forceinline__ int cut(int u) const { return u * each + (u < extra ? u : extra); }
-  __device__ __forceinline__ int unit_of(int x) const {
-    const int split = extra * (each + 1);
-    return x < split ? x / (each + 1) : extra + (x - split) / each;
-  }
-};
-__device__ __forceinline__ int lane_sum(int v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ CachePlan cache_plan(int tiles, int D) {
-  CachePlan p;
-  p.total = tiles;
-  p.units = (int)cache_units(tiles, D);
-  p.each = p.units > 0 ? tiles / p.units : 0;
-  p.extra = tiles - p.each * p.units;
-  return p;
 }
 
 // The plan, and (found with the same reads where the rows are at most 64) the row whose tiles hold the first
@@ -132,10 +109,6 @@ struct CacheFill {
     }
   }
 };
-
-// s_waitcnt vmcnt(N) and lgkmcnt(0) (the other counters at their maxima).
-constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
-constexpr int kWaitLgkm0 = 0xC07F;
 
 // NT: K and V past the caches, where one query tile alone reads them, in rows of 256 bytes (32 rows of up to
 // 8192 tokens, 28 / 4 heads: 69 -> 63 us; at D = 64 24 -> 25 for 64 rows of up to 4096, 14 / 2 heads).
@@ -231,26 +204,10 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
       store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
                          l > 0.f ? 1.f / l : 0.f);
     } else if (rok) {
-      if (hi == 0) {
-        part[lq] = m;
-        part[live + lq] = l;
-      }
-      float* po = part + 2 * live + lq * D + 4 * hi;
-#pragma unroll
-      for (int md = 0; md < D / 32; ++md)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2)
-            *reinterpret_cast<float2*>(po + 32 * md + 8 * j + e) =
-                make_float2(oacc[md][4 * j + e], oacc[md][4 * j + e + 1]);
+      store_part<D>(part, live, lq, hi, m, l, oacc);
     }
   }
 }
-
-// Parts of a group from which its rows, where there are no more than CUs, are joined by blocks of 1024 threads
-// instead of 256 (12 rows of 512 parts each 17 -> 5.5 us; 896 rows of 27 4.9 -> 8.7).
-constexpr int64_t kCacheManyParts = 24;
 
 // The groups that were cut, and zeros for the rows without tokens: one block per query row. A lane adds two
 // columns over every GROUPS-th part with a running maximum, so that the parts are read once.

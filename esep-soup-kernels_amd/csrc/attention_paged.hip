@@ -1,0 +1,415 @@
+// Attention of a row's n newest tokens over its pages (decoding: n = 1), with an optional window and sinks: the walk
+// of attention_cache.hip with the tokens' addresses found through a block table.
+//
+// Token j of row b lies in page tables[b, j / P] at place j % P. A tile of 32 keys begins at a multiple of 32, so
+// that each half of it lies in one page (P is a power of two of at least 16). A wavefront reads the pages of 32 tiles
+// at once, a half to a lane, and takes each tile's two from there. Keys before a window or past the length repeat the
+// nearest one that is seen and are masked; what a page outside the pool should hold is not read: its keys are
+// masked and its values count as 0.
+//
+// Rows whose first tokens lie in the same pages (the beams of a request) are walked together over those, their query
+// rows in common tiles of 32: K and V of the shared tokens are read once for all of them. Each row's own tokens
+// come in a walk of its own, and the join adds both.
+//
+// Bound by the bytes of K and V, and below a few MB by the launches' latency.
+#include <cmath>
+
+#include "attention_cache.hpp"
+#include "attention_paged.hpp"
+#include "attention_tiles.hpp"
+
+namespace esep {
+namespace {
+
+__device__ __forceinline__ int paged_len(const AttnPagedArgs& a, int b) {
+  const int len = a.len[b], S = a.tokens();
+  return len < 0 ? 0 : (len > S ? S : len);
+}
+// Tokens of the W rows from r W on that are walked together: whole tiles, all of them seen by every new token.
+__device__ __forceinline__ int shared_len(const AttnPagedArgs& a, int r) {
+  int s = a.shared[r];
+  for (int w = 0; w < a.W; ++w) {
+    const int most = paged_len(a, r * a.W + w) - a.n;
+    s = s < most ? s : most;
+  }
+  return s > 0 ? s & ~31 : 0;
+}
+
+// Rows that are walked together: keys lo .. len in tiles from a multiple of 32 on, before them `ns` tiles of the sinks.
+struct PagedRow {
+  int b, len, lo, sink_hi, ns, tiles;
+  bool common;  // W rows from b on, over what they share
+  int shared;   // tokens of the row's keys that a common walk takes
+};
+template <bool SHARED>
+__device__ __forceinline__ PagedRow paged_row(const AttnPagedArgs& a, int e) {
+  PagedRow r{};
+  if constexpr (SHARED) {
+    const int R = a.B / a.W;
+    if (e < R) {
+      r.common = true;
+      r.b = e * a.W;
+      r.len = shared_len(a, e);
+      r.tiles = r.len / 32;
+      return r;
+    }
+    r.b = e - R;
+    r.shared = r.lo = shared_len(a, r.b / a.W);
+    r.len = paged_len(a, r.b);
+  } else {
+    r.b = e;
+    r.len = paged_len(a, e);
+    const int first = r.len > a.n ? r.len - a.n : 0;  // the first query's position
+    r.sink_hi = a.sinks < r.len ? a.sinks : r.len;
+    r.lo = first - a.window + 1;  // window >= 1
+    if (r.lo <= r.sink_hi) r.lo = 0;
+    r.ns = r.lo > 0 ? (r.sink_hi + 31) / 32 : 0;
+  }
+  r.tiles = r.ns + (r.len - (r.lo & ~31) + 31) / 32;
+  return r;
+}
+
+// The plan, and the place (rows e) whose tiles hold the first of wavefront u, with the number of that place's first
+// tile; place -1: no work.
+template <int D, bool SHARED>
+__device__ __forceinline__ CachePlan paged_find(const AttnPagedArgs& a, int per, int per_common, int u, int* place,
+                                                int* first) {
+  const int lane = threadIdx.x & 63, R = SHARED ? a.B / a.W : 0, E = a.B + R;
+  auto tiles_of = [&](int e) {
+    return e < E ? paged_row<SHARED>(a, e).tiles * (e < R ? per_common : per) : 0;
+  };
+  const int mine0 = tiles_of(lane);
+  int sum = mine0;
+  for (int e = lane + 64; e < E; e += 64) sum += tiles_of(e);
+  const CachePlan p = cache_plan(lane_sum(sum), D);
+  *place = -1;
+  *first = 0;
+  if (u >= p.units) return p;
+  const int x = p.cut(u);
+  int before = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const int mine = e0 == 0 ? mine0 : tiles_of(e0 + lane);
+    int run = mine;  // inclusive sums
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(run, d);
+      if (lane >= d) run += o;
+    }
+    const uint64_t past = __ballot(before + run > x);
+    if (past != 0) {
+      const int l = (int)__builtin_ctzll(past);
+      *place = e0 + l;
+      *first = before + __builtin_amdgcn_readlane(run - mine, l);
+      break;
+    }
+    before += __builtin_amdgcn_readlane(run, 63);
+  }
+  return p;
+}
+
+// One wavefront's fill of a 32-row swizzled tile from two runs of 16 tokens.
+template <int RB, bool NT>
+struct PagedFill {
+  static constexpr int GR = 1024 / RB, CH = RB / 16, N = 32 / GR, V = RB == 256 ? 4 : 2;
+  int lrow, chunk;
+  int64_t ps, ts;  // bytes between pages, tokens
+  int mask;        // P - 1
+  uint32_t voff[V];
+  __device__ __forceinline__ PagedFill(int lane, int64_t ps_, int64_t ts_, int mask_) : ps(ps_), ts(ts_), mask(mask_) {
+    lrow = lane / CH;
+    chunk = (lane % CH) ^ swz<RB>(lrow);
+#pragma unroll
+    for (int i = 0; i < V; ++i) voff[i] = (uint32_t)(lrow * ts) + 16u * (uint32_t)(chunk ^ i);
+  }
+  // keys k0 .. k0 + 31, all of them there: the halves in pages g0 and g1
+  __device__ __forceinline__ void whole(char* dst, const char* base, int k0, int g0, int g1) const {
+    const char* h[2] = {base + g0 * ps + (k0 & mask) * ts, base + g1 * ps + ((k0 + 16) & mask) * ts};
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const char* at = h[q / (N / 2)] + GR * (q % (N / 2)) * ts;
+      if constexpr (NT)
+        lds_dma_x4_s_nt(at, voff[q % V], dst + 1024 * q);
+      else
+        lds_dma_x4_s(at, voff[q % V], dst + 1024 * q);
+    }
+  }
+  // the lane's key of row group q, within lo .. hi - 1, and where it lies
+  __device__ __forceinline__ const char* at(const char* base, int q, int k0, int lo, int hi, int g0, int g1,
+                                            int* page) const {
+    int k = k0 + GR * q + lrow;
+    k = k < lo ? lo : (k < hi ? k : hi - 1);
+    *page = k - k0 < 16 ? g0 : g1;
+    return base + *page * ps + (k & mask) * ts + 16 * (chunk ^ (q % V));
+  }
+  __device__ __forceinline__ void partial(char* dst, const char* base, int k0, int lo, int hi, int g0, int g1) const {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      int page;
+      lds_dma_x4(at(base, q, k0, lo, hi, g0, g1, &page), dst + 1024 * q);
+    }
+  }
+  // the same where a page may be none of the n: zeros for its keys
+  __device__ __forceinline__ void checked(char* dst, const char* base, int k0, int lo, int hi, int g0, int g1, int n,
+                                          int lane) const {
+    for (int q = 0; q < N; ++q) {
+      int page;
+      const char* p = at(base, q, k0, lo, hi, g0, g1, &page);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if ((unsigned)page < (unsigned)n) x = *reinterpret_cast<const uint4*>(p);
+      *reinterpret_cast<uint4*>(dst + 1024 * q + 16 * lane) = x;
+    }
+  }
+};
+
+template <typename T, int D, bool NT, bool SHARED>
+__global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnPagedArgs a) {
+  constexpr int RB = 2 * D, TILE = 32 * RB;
+  using V8 = typename Mfma<T>::v8;
+  using Fill = PagedFill<RB, NT>;
+  __shared__ __align__(1024) char kv[2][2][TILE];  // [buffer][K, V]
+
+  const int lane = threadIdx.x, lq = lane & 31, hi = lane >> 5;
+  const int G = a.HQ / a.HK, own_rows = G * a.n, all_rows = SHARED ? a.W * own_rows : own_rows;
+  const int per = a.HK * ((own_rows + 31) / 32), per_common = a.HK * ((all_rows + 31) / 32);
+  const int R = SHARED ? a.B / a.W : 0;
+  const int u = blockIdx.x;
+  int first, e;
+  const CachePlan plan = paged_find<D, SHARED>(a, per, per_common, u, &e, &first);
+  if (e < 0) return;
+  int x = plan.cut(u);
+  const int x1 = plan.cut(u + 1);
+  PagedRow row = paged_row<SHARED>(a, e);
+  const int mask = (1 << a.page_shift) - 1;
+  const Fill fk(lane, a.k_ps * (int64_t)sizeof(T), a.k_ts * (int64_t)sizeof(T), mask);
+  const Fill fv(lane, a.v_ps * (int64_t)sizeof(T), a.v_ts * (int64_t)sizeof(T), mask);
+  const int live = all_rows < 32 ? all_rows : 32;  // rows of a partial
+
+  while (x < x1) {
+    int here = e < R ? per_common : per;
+    while (x >= first + row.tiles * here) {
+      first += row.tiles * here;
+      row = paged_row<SHARED>(a, ++e);
+      here = e < R ? per_common : per;
+    }
+    const int rows = row.common ? all_rows : own_rows, RT = here / a.HK;
+    const int gi = (x - first) / row.tiles;  // kv head and query tile
+    const int g0 = first + gi * row.tiles;
+    const int t0 = x - g0, t1 = x1 - g0 < row.tiles ? x1 - g0 : row.tiles;
+    const int kvh = gi / RT, rt = gi % RT;
+    const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (int64_t)kvh * a.k_hs);
+    const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (int64_t)kvh * a.v_hs);
+    const int32_t* table = a.tables + (int64_t)row.b * a.t_bs;
+    const int lo0 = row.lo & ~31;
+    auto start_of = [&](int t) { return t < row.ns ? 32 * t : lo0 + 32 * (t - row.ns); };
+    int ids = -1, ids0 = 0;  // lane l: the page of half l % 2 of tile ids0 + l / 2
+    auto load_ids = [&](int t) {
+      ids0 = t;
+      const int tl = t + lane / 2;
+      ids = -1;
+      if (tl < t1) {
+        const int from = tl < row.ns ? 0 : row.lo, to = tl < row.ns ? row.sink_hi : row.len;
+        int k = start_of(tl) + 16 * (lane & 1);
+        k = k < from ? from : (k < to ? k : to - 1);
+        ids = table[k >> a.page_shift];
+      }
+      asm volatile("" : "+v"(ids));  // here now: a wait for it in the loop would wait for the tiles in flight too
+    };
+    uint32_t bad = 0;  // bits 2 buffer + half: the page is none
+    // asks for tile t; false: it is there already, without a DMA
+    auto issue = [&](int t) {
+      if (t - ids0 >= 32) load_ids(t);
+      const int p0 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0));
+      const int p1 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0) + 1);
+      const int k0 = start_of(t), from = t < row.ns ? 0 : row.lo, to = t < row.ns ? row.sink_hi : row.len;
+      char* kd = kv[t & 1][0];
+      char* vd = kv[t & 1][1];
+      const uint32_t none = ((unsigned)p0 >= (unsigned)a.N ? 1u : 0u) | ((unsigned)p1 >= (unsigned)a.N ? 2u : 0u);
+      bad = (bad & ~(3u << (2 * (t & 1)))) | none << (2 * (t & 1));
+      if (none) {
+        fk.checked(kd, kbase, k0, from, to, p0, p1, a.N, lane);
+        fv.checked(vd, vbase, k0, from, to, p0, p1, a.N, lane);
+        return false;
+      }
+      if (k0 >= from && k0 + 32 <= to) {
+        fk.whole(kd, kbase, k0, p0, p1);
+        fv.whole(vd, vbase, k0, p0, p1);
+      } else {
+        fk.partial(kd, kbase, k0, from, to, p0, p1);
+        fv.partial(vd, vbase, k0, from, to, p0, p1);
+      }
+      return true;
+    };
+    // every read of the ring by the group before is done
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    load_ids(t0);
+    issue(t0);
+    if (t0 + 1 < t1) issue(t0 + 1);
+
+    const int r = 32 * rt + lq;
+    const bool rok = r < rows;
+    const int rb = rok ? r : 0;  // its row, token and head
+    const int b = row.b + rb / own_rows, tok = rb % own_rows / G, h = kvh * G + rb % G;
+    V8 qb[D / 16];
+    {
+      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_bs + (int64_t)tok * a.q_ts +
+                      (int64_t)h * a.q_hs + 8 * hi;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) qb[c] = rok ? ld16<V8>(qrow + 16 * c) : V8{};
+    }
+    // positions: the lane's, and the tile's first and last
+    const int p0 = row.len - a.n, pos = rok ? p0 + tok : p0 + a.n - 1;
+    const int ufirst = p0 + 32 * rt / G;
+    const int ulast = 32 * rt + 31 < rows ? p0 + (32 * rt + 31) / G : p0 + a.n - 1;
+    f32x16 oacc[D / 32];
+#pragma unroll
+    for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+    // q and the first tiles are here (through the builtin: the compiler then waits for no load of its own
+    // within the loop, which would wait for the tile in flight too)
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    for (int t = t0; t < t1; ++t) {
+      // a window's tiles have no sinks (the first of them may begin among those)
+      const int kh = start_of(t), cap = t < row.ns ? row.sink_hi - 1 : 0x7fffffff;
+      const int sinks = t < row.ns || row.lo == 0 ? row.sink_hi : 0;
+      const char* ks = kv[t & 1][0];
+      const char* vs = kv[t & 1][1];
+      const uint32_t none = bad >> (2 * (t & 1)) & 3;
+      fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
+                         [&](f32x16& acc) __attribute__((always_inline)) {
+                           if (!SHARED || !row.common)
+                             mask_window(acc, kh, ufirst < cap ? ufirst : cap, ulast - a.window,
+                                         pos < cap ? pos : cap, pos - a.window, sinks, hi);
+                           if (none) {
+#pragma unroll
+                             for (int i = 0; i < 16; ++i)
+                               if (none >> (i / 8) & 1) acc[i] = -INFINITY;
+                           }
+                         });
+      // this tile's reads are done: its buffer takes tile t + 2; then tile t + 1 is waited for
+      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 2 < t1 && issue(t + 2))
+        __builtin_amdgcn_s_waitcnt(wait_vm(2 * Fill::N));
+      else
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    x += t1 - t0;
+    const int group = (e < R ? e * per_common : R * per_common + (e - R) * per) + gi;
+    float* part = a.part + (int64_t)(u + group) * live * (D + 2);
+    // the wavefront with a group's first tile says for the join which others have some
+    if (t0 == 0 && lane == 0) a.ends[group] = make_int2(u, plan.unit_of(g0 + row.tiles - 1));
+    if (rok && t0 == 0 && t1 == row.tiles && !(SHARED && (row.common || row.shared > 0))) {  // all of the row's keys
+      store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
+                         l > 0.f ? 1.f / l : 0.f);
+    } else if (rok) {
+      store_part<D>(part, live, lq, hi, m, l, oacc);
+    }
+  }
+}
+
+// The groups that were cut or share keys, and zeros for the rows without tokens: one block per query row. A lane adds two
+// columns over every GROUPS-th part with a running maximum, so that the parts are read once.
+template <typename T, int D, int THREADS, bool SHARED>
+__global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs a) {
+  constexpr int PAIRS = D / 2, GROUPS = THREADS / PAIRS;
+  __shared__ float2 sums[GROUPS][PAIRS];
+  __shared__ float2 stat[GROUPS];  // maximum, sum
+  const int G = a.HQ / a.HK, rows = G * a.n, all_rows = SHARED ? a.W * rows : rows;
+  const int RT = (rows + 31) / 32, CT = (all_rows + 31) / 32, live = all_rows < 32 ? all_rows : 32;
+  const int rg = (int)(blockIdx.x % rows);
+  const int kvh = (int)(blockIdx.x / rows % a.HK), b = (int)(blockIdx.x / rows / a.HK);
+  const int g = threadIdx.x / PAIRS, c = threadIdx.x % PAIRS;
+  T* out = static_cast<T*>(a.o) + (((int64_t)b * a.n + rg / G) * a.HQ + kvh * G + rg % G) * D + 2 * c;
+  if (paged_len(a, b) <= 0) {
+    if (g == 0) out[0] = out[1] = (T)0.f;
+    return;
+  }
+  const int R = SHARED ? a.B / a.W : 0;
+  const int own = R * a.HK * CT + (b * a.HK + kvh) * RT + rg / 32;
+  const int2 ends = a.ends[own];
+  int n = ends.y - ends.x + 1, common = 0, rc = 0;
+  int2 more = make_int2(0, -1);
+  if (SHARED && shared_len(a, b / a.W) > 0) {
+    rc = b % a.W * rows + rg;
+    common = (b / a.W * a.HK + kvh) * CT + rc / 32;
+    more = a.ends[common];
+  } else if (n == 1) {
+    return;  // stored by its wavefront
+  }
+  const int own_parts = n;
+  n += more.y - more.x + 1;
+  const int64_t size = (int64_t)live * (D + 2);
+  float m = -INFINITY, l = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int i = g; i < n; i += GROUPS) {
+    const bool mine = i < own_parts;
+    const int slot = mine ? ends.x + i + own : more.x + (i - own_parts) + common;
+    const int lq = mine ? rg % 32 : rc % 32;
+    const float* p = a.part + slot * size;
+    const float pm = p[lq], pl = p[live + lq];
+    const float2 v = *reinterpret_cast<const float2*>(p + 2 * live + lq * D + 2 * c);
+    const float top = fmaxf(m, pm), ref = top == -INFINITY ? 0.f : top;
+    const float w0 = exp2_fast(m - ref), w1 = exp2_fast(pm - ref);
+    l = fmaf(w1, pl, w0 * l);
+    acc.x = fmaf(w1, v.x, w0 * acc.x);
+    acc.y = fmaf(w1, v.y, w0 * acc.y);
+    m = top;
+  }
+  sums[g][c] = acc;
+  if (c == 0) stat[g] = make_float2(m, l);
+  __syncthreads();
+  if (g != 0) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, stat[i].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float den = 0.f;
+  acc = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float w = exp2_fast(stat[i].x - ref);
+    den = fmaf(w, stat[i].y, den);
+    acc.x = fmaf(w, sums[i][c].x, acc.x);
+    acc.y = fmaf(w, sums[i][c].y, acc.y);
+  }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  out[0] = (T)(acc.x * inv);
+  out[1] = (T)(acc.y * inv);
+}
+
+template <typename T, int D, bool SHARED>
+hipError_t run(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
+  const dim3 grid((unsigned)(z.units > 0 ? z.units : 1)), rows((unsigned)(a.B * a.HQ * a.n));
+  if (D == 128 && z.all_tiles == 1)
+    hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED>), grid, dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attn_paged<T, D, false, SHARED>), grid, dim3(64), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (z.units > kCacheManyParts * z.groups && rows.x <= 256)
+    hipLaunchKernelGGL((k_attn_paged_join<T, D, 1024, SHARED>), rows, dim3(1024), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attn_paged_join<T, D, 256, SHARED>), rows, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_d(const AttnPagedArgs& a, const PagedSizes& z, int D, hipStream_t s, bool* sup) {
+  *sup = D == 128 || D == 64;
+  if (D == 128) return a.shared ? run<T, 128, true>(a, z, s) : run<T, 128, false>(a, z, s);
+  if (D == 64) return a.shared ? run<T, 64, true>(a, z, s) : run<T, 64, false>(a, z, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_attn_paged(const AttnPagedArgs& a, const PagedSizes& z, int dt, int D, hipStream_t s, bool* sup) {
+  if (dt == 1) return run_d<_Float16>(a, z, D, s, sup);
+  if (dt == 2) return run_d<__bf16>(a, z, D, s, sup);
+  *sup = false;
+  return hipErrorInvalidValue;
+}
+
+}  // namespace esep

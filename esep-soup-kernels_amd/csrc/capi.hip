@@ -7,12 +7,15 @@
 #include <mutex>
 
 #include "attention.hpp"
+#include "attention_paged.hpp"
+#include "beam.hpp"
 #include "dropout.hpp"
 #include "esep_body.h"
 #include "gemm.hpp"
 #include "head.hpp"
 #include "lora.hpp"
 #include "nf4.hpp"
+#include "paged.hpp"
 #include "rmsnorm.hpp"
 #include "rope.hpp"
 #include "swiglu.hpp"
@@ -924,6 +927,277 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
   const hipError_t e = esep::launch_attn_cache(a, dt, D, static_cast<hipStream_t>(stream), &sup);
   if (!sup) return fail(ESEP_EINVAL, "attn_cache: unsupported dtype / D");
   return e == hipSuccess ? 0 : hip_fail(e, "attn_cache launch");
+}
+
+int esep_page_tables(int32_t* tables, int64_t tables_bs, const int32_t* lengths, const int32_t* add,
+                     const int32_t* free_pages, const int32_t* taken, int32_t* slots, int32_t* positions,
+                     int32_t* cu_seqlens, int32_t* lengths_out, int32_t* taken_out, int B, int M, int F,
+                     int page, int total, void* stream) {
+  g_err[0] = 0;
+  if (B < 0 || M < 0 || F < 0 || page < 1 || total < 0 || (int64_t)M * page > (1 << 30))
+    return fail(ESEP_ESHAPE, "page_tables: bad sizes B=%d M=%d F=%d page=%d total=%d", B, M, F, page, total);
+  if (B > 1 && tables_bs < M)
+    return fail(ESEP_ESHAPE, "page_tables: rows of the tables overlap (stride %lld)", (long long)tables_bs);
+  if (taken == nullptr || taken_out == nullptr || cu_seqlens == nullptr ||
+      (B > 0 && (lengths == nullptr || add == nullptr || lengths_out == nullptr)) ||
+      (B > 0 && M > 0 && tables == nullptr) || (F > 0 && free_pages == nullptr) ||
+      (total > 0 && (slots == nullptr || positions == nullptr)))
+    return fail(ESEP_EINVAL, "page_tables: tables, lengths, add, the free list and the outputs are required");
+  esep::PageTablesArgs a{};
+  a.tables = tables;
+  a.lengths = lengths;
+  a.add = add;
+  a.free = free_pages;
+  a.taken = taken;
+  a.slots = slots;
+  a.positions = positions;
+  a.cu = cu_seqlens;
+  a.lengths_out = lengths_out;
+  a.taken_out = taken_out;
+  a.t_bs = tables_bs;
+  a.B = B;
+  a.M = M;
+  a.F = F;
+  a.P = page;
+  a.total = total;
+  const hipError_t e = esep::launch_page_tables(a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "page_tables launch");
+}
+
+namespace {
+// The checks that k and v pages share: sizes, 16-byte addresses, strides of whole 16 bytes; 0, or the failure's code.
+int pages_ok(const char* what, const void* k, const int64_t* ks, const void* v, const int64_t* vs, int n, int N,
+             int P, int HK, int D) {
+  if (N < 0 || P < 1 || HK < 1 || D < 8 || D % 8 != 0 || (int64_t)N * P > 0x7fffffff || (int64_t)HK * D > (1 << 24))
+    return fail(ESEP_ESHAPE, "%s: bad sizes N=%d P=%d HK=%d D=%d", what, N, P, HK, D);
+  if (ks == nullptr || vs == nullptr || (N > 0 && (k == nullptr || v == nullptr)))
+    return fail(ESEP_EINVAL, "%s: the pages and their strides are required", what);
+  if (!aligned16(k) || !aligned16(v)) return fail(ESEP_EALIGN, "%s: the pages need 16-byte alignment", what);
+  for (const int64_t* st : {ks, vs})
+    for (int i = 0; i < n; ++i)
+      if (st[i] < 0 || (st[i] & 7)) return fail(ESEP_EALIGN, "%s: strides need to be multiples of 8 elements", what);
+  return 0;
+}
+}  // namespace
+
+int esep_page_store(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                    void* k_pages, const int64_t* kp_strides, void* v_pages, const int64_t* vp_strides,
+                    const int32_t* slots, int64_t T, int N, int page, int HK, int D, void* stream) {
+  g_err[0] = 0;
+  if (T < 0 || T > 0x7fffffff) return fail(ESEP_ESHAPE, "page_store: bad number of tokens %lld", (long long)T);
+  const int rc = pages_ok("page_store", k_pages, kp_strides, v_pages, vp_strides, 3, N, page, HK, D);
+  if (rc != 0) return rc;
+  if (T == 0 || N == 0) return 0;
+  if (k == nullptr || v == nullptr || slots == nullptr || k_strides == nullptr || v_strides == nullptr)
+    return fail(ESEP_EINVAL, "page_store: k, v, their strides and the slots are required");
+  if (!aligned16(k) || !aligned16(v)) return fail(ESEP_EALIGN, "page_store: k and v need 16-byte alignment");
+  for (const int64_t* st : {k_strides, v_strides})
+    for (int i = 0; i < 2; ++i)
+      if (st[i] < 0 || (st[i] & 7))
+        return fail(ESEP_EALIGN, "page_store: strides need to be multiples of 8 elements");
+  esep::PageStoreArgs a{};
+  a.src[0] = k;
+  a.src[1] = v;
+  a.s_ts[0] = k_strides[0];
+  a.s_hs[0] = k_strides[1];
+  a.s_ts[1] = v_strides[0];
+  a.s_hs[1] = v_strides[1];
+  a.dst[0] = esep::Pages{k_pages, 0, kp_strides[0], kp_strides[1], kp_strides[2]};
+  a.dst[1] = esep::Pages{v_pages, 0, vp_strides[0], vp_strides[1], vp_strides[2]};
+  a.slots = slots;
+  a.T = T;
+  a.N = N;
+  a.P = page;
+  a.HK = HK;
+  a.D = D;
+  const hipError_t e = esep::launch_page_store(a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "page_store launch");
+}
+
+int esep_beam_reorder(const int32_t* parents, void* k_pages, const int64_t* kp_strides, void* v_pages,
+                      const int64_t* vp_strides, const int32_t* tables, int64_t tables_bs,
+                      const int32_t* lengths, const int32_t* start, int R, int W, int M, int L, int N,
+                      int page, int HK, int D, void* stream) {
+  g_err[0] = 0;
+  if (R < 0 || R > 65535 || W < 1 || W > esep::kMostBeams || M < 0 || L < 0 || L > 32767 ||
+      (int64_t)R * 2 * L >= (1 << 24))
+    return fail(ESEP_ESHAPE, "beam_reorder: bad sizes R=%d W=%d M=%d L=%d", R, W, M, L);
+  const int rc = pages_ok("beam_reorder", k_pages, kp_strides, v_pages, vp_strides, 4, N, page, HK, D);
+  if (rc != 0) return rc;
+  if ((int64_t)M * page > (1 << 30))
+    return fail(ESEP_ESHAPE, "beam_reorder: rows of %d pages of %d tokens are too long", M, page);
+  if (R * (int64_t)W > 1 && tables_bs < M)
+    return fail(ESEP_ESHAPE, "beam_reorder: rows of the tables overlap (stride %lld)", (long long)tables_bs);
+  if (R == 0 || M == 0 || L == 0 || N == 0) return 0;
+  if (parents == nullptr || tables == nullptr || lengths == nullptr)
+    return fail(ESEP_EINVAL, "beam_reorder: parents, tables and lengths are required");
+  esep::BeamReorderArgs a{};
+  a.parents = parents;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.start = start;
+  a.pages[0] = esep::Pages{k_pages, kp_strides[0], kp_strides[1], kp_strides[2], kp_strides[3]};
+  a.pages[1] = esep::Pages{v_pages, vp_strides[0], vp_strides[1], vp_strides[2], vp_strides[3]};
+  a.t_bs = tables_bs;
+  a.R = R;
+  a.W = W;
+  a.M = M;
+  a.N = N;
+  a.P = page;
+  a.L = L;
+  a.HK = HK;
+  a.D = D;
+  const hipError_t e = esep::launch_beam_reorder(a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "beam_reorder launch");
+}
+
+namespace {
+// The sizes of attention over pages, whether the library takes them.
+bool paged_sizes_of(int B, int n, int M, int page, int HQ, int HK, int D, int window, int sinks, int beams,
+                    bool shared, esep::PagedSizes* z) {
+  if (B < 1 || n < 1 || M < 0 || page < 16 || (page & (page - 1)) != 0 || (int64_t)M * page > (1 << 30) || HQ < 1 ||
+      HK < 1 || HQ % HK != 0 || D < 1 || window < 0 || sinks < 0 || beams < 1 || B % beams != 0 || n > (1 << 24) ||
+      (int64_t)B * HQ * n >= int64_t{1} << 24)
+    return false;
+  const int S = M * page, w = window == 0 || window > S ? S : window;
+  *z = esep::paged_sizes(B, n, beams, S, HQ, HK, D, w, sinks, shared);
+  return z->tiles <= 0x7fffffff;
+}
+}  // namespace
+
+int64_t esep_attn_paged_workspace(int B, int n, int M, int page, int HQ, int HK, int D, int window, int sinks,
+                                  int beams, int shared) {
+  esep::PagedSizes z;
+  return paged_sizes_of(B, n, M, page, HQ, HK, D, window, sinks, beams, shared != 0, &z) ? z.floats : 0;
+}
+
+int esep_attn_paged(const void* q, const int64_t* q_strides, const void* k_pages, const int64_t* kp_strides,
+                    const void* v_pages, const int64_t* vp_strides, void* o, const int32_t* tables,
+                    int64_t tables_bs, const int32_t* lengths, const int32_t* shared, float* workspace, int dt,
+                    int B, int n, int M, int N, int page, int HQ, int HK, int D, float scale, int window,
+                    int sinks, int beams, void* stream) {
+  g_err[0] = 0;
+  if (dt != ESEP_F16 && dt != ESEP_BF16)
+    return fail(ESEP_EINVAL, "attn_paged: dtype %d is not fp16 / bf16", dt);
+  if (D != 64 && D != 128) return fail(ESEP_ESHAPE, "attn_paged: D=%d not in {64, 128}", D);
+  if (page < 16 || (page & (page - 1)) != 0)
+    return fail(ESEP_ESHAPE, "attn_paged: %d tokens to a page: not a power of two of at least 16", page);
+  if (window < 0 || sinks < 0)
+    return fail(ESEP_ESHAPE, "attn_paged: window=%d sinks=%d", window, sinks);
+  if (!(scale > 0.f)) return fail(ESEP_EINVAL, "attn_paged: scale must be positive");
+  if (shared != nullptr && window != 0)
+    return fail(ESEP_EINVAL, "attn_paged: shared tokens and a window do not go together");
+  esep::PagedSizes z{};
+  if (B < 0 || n < 0 || M < 0 || N < 0 ||
+      (B > 0 && n > 0 &&
+       !paged_sizes_of(B, n, M, page, HQ, HK, D, window, sinks, beams, shared != nullptr, &z)))
+    return fail(ESEP_ESHAPE, "attn_paged: bad sizes B=%d n=%d M=%d N=%d HQ=%d HK=%d beams=%d", B, n, M, N, HQ, HK,
+                beams);
+  if (B == 0 || n == 0) return 0;
+  const int rc = pages_ok("attn_paged", k_pages, kp_strides, v_pages, vp_strides, 3, N, page, HK, D);
+  if (rc != 0) return rc;
+  if (q == nullptr || o == nullptr || lengths == nullptr || workspace == nullptr || q_strides == nullptr ||
+      (M > 0 && tables == nullptr))
+    return fail(ESEP_EINVAL, "attn_paged: q, o, tables, lengths, the workspace and strides are required");
+  if (!aligned16(q) || !aligned16(o) || !aligned16(workspace))
+    return fail(ESEP_EALIGN, "attn_paged: q, o and the workspace need 16-byte alignment");
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] < 0 || (q_strides[i] & 7))
+      return fail(ESEP_EALIGN, "attn_paged: strides need to be multiples of 8 elements");
+  if (kp_strides[1] > kAttnMaxStride || vp_strides[1] > kAttnMaxStride)
+    return fail(ESEP_ESHAPE, "attn_paged: token stride above %lld elements", (long long)kAttnMaxStride);
+  if (B > 1 && tables_bs < M)
+    return fail(ESEP_ESHAPE, "attn_paged: rows of the tables overlap (stride %lld)", (long long)tables_bs);
+  esep::AttnPagedArgs a{};
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.o = o;
+  a.tables = tables;
+  a.len = lengths;
+  a.shared = shared;
+  a.ends = reinterpret_cast<int2*>(workspace);
+  a.part = workspace + esep::cache_ends_floats(z.groups);
+  a.q_bs = q_strides[0];
+  a.q_ts = q_strides[1];
+  a.q_hs = q_strides[2];
+  a.k_ps = kp_strides[0];
+  a.k_ts = kp_strides[1];
+  a.k_hs = kp_strides[2];
+  a.v_ps = vp_strides[0];
+  a.v_ts = vp_strides[1];
+  a.v_hs = vp_strides[2];
+  a.t_bs = tables_bs;
+  a.B = B;
+  a.n = n;
+  a.W = beams;
+  a.M = M;
+  a.N = N;
+  a.HQ = HQ;
+  a.HK = HK;
+  while ((1 << a.page_shift) < page) ++a.page_shift;
+  const int S = M * page;
+  a.window = window == 0 || window > S ? (S > 0 ? S : 1) : window;  // none: a row's longest
+  a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  bool sup = false;
+  const hipError_t e = esep::launch_attn_paged(a, z, dt, D, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "attn_paged: unsupported dtype / D");
+  return e == hipSuccess ? 0 : hip_fail(e, "attn_paged launch");
+}
+
+namespace {
+bool beam_sizes_ok(int R, int W, int64_t V, int keep) {
+  return R >= 0 && W >= 1 && W <= 64 && V >= 1 && V <= (1 << 24) && keep >= 1 && keep <= esep::kBeamMostKeep &&
+         keep <= W * V && (int64_t)R * W <= 65535;
+}
+}  // namespace
+
+int64_t esep_beam_select_workspace(int R, int W, int64_t V, int keep) {
+  if (!beam_sizes_ok(R, W, V, keep)) return 0;
+  const int64_t parts = (int64_t)R * W * esep::beam_splits((int64_t)R * W, V);
+  return 8 * parts * (1 + keep);
+}
+
+int esep_beam_select(const void* logits, int64_t ld_r, int64_t ld_w, const float* scores, void* workspace,
+                     float* out_scores, int32_t* out_parents, int32_t* out_tokens, int dt, int R, int W, int64_t V,
+                     int keep, void* stream) {
+  g_err[0] = 0;
+  if (!float_dt(dt)) return fail(ESEP_EINVAL, "beam_select: bad dtype code %d", dt);
+  if (!beam_sizes_ok(R, W, V, keep))
+    return fail(ESEP_ESHAPE, "beam_select: bad sizes R=%d W=%d V=%lld keep=%d", R, W, (long long)V, keep);
+  if (ld_r < 0 || ld_w < 0) return fail(ESEP_ESHAPE, "beam_select: negative strides");
+  if (R == 0) return 0;
+  if (logits == nullptr || scores == nullptr || workspace == nullptr || out_scores == nullptr ||
+      out_parents == nullptr || out_tokens == nullptr)
+    return fail(ESEP_EINVAL, "beam_select: logits, scores, the workspace and the outputs are required");
+  if (reinterpret_cast<uintptr_t>(workspace) & 7)
+    return fail(ESEP_EALIGN, "beam_select: the workspace needs 8-byte alignment");
+  const int64_t rows = (int64_t)R * W, splits = esep::beam_splits(rows, V);
+  esep::BeamArgs a{};
+  a.logits = logits;
+  a.scores = scores;
+  a.stat = static_cast<float2*>(workspace);
+  a.cand = static_cast<uint64_t*>(workspace) + rows * splits;
+  a.out_scores = out_scores;
+  a.out_parents = out_parents;
+  a.out_tokens = out_tokens;
+  a.r_bs = ld_r;
+  a.w_bs = ld_w;
+  a.R = R;
+  a.W = W;
+  a.V = (int)V;
+  a.keep = keep;
+  a.splits = (int)splits;
+  a.piece = esep::beam_piece(rows, V);
+  if (rows * splits * esep::kBeamThreads >= int64_t{1} << 32)
+    return fail(ESEP_ESHAPE, "beam_select: %lld rows of %lld are too many for one launch", (long long)rows,
+                (long long)V);
+  const bool vec = aligned16(logits) && V % 8 == 0 && (R == 1 || ld_ok(ld_r, dt)) && (W == 1 || ld_ok(ld_w, dt));
+  bool sup = false;
+  const hipError_t e = esep::launch_beam_select(a, dt, vec, static_cast<hipStream_t>(stream), &sup);
+  if (!sup) return fail(ESEP_EINVAL, "beam_select: unsupported dtype");
+  return e == hipSuccess ? 0 : hip_fail(e, "beam_select launch");
 }
 
 int esep_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, int dt,

@@ -1,0 +1,266 @@
+// The upkeep of paged caches: which page and place each new token gets (k_page_tables), the store of its key and
+// value there (k_page_store), and the beams' states following their parents (k_beam_reorder).
+#include "paged.hpp"
+
+#include "common.hpp"
+
+namespace esep {
+namespace {
+
+// ---------------------------------------------------------------------------------------
+// Block tables and slots. Row b holds L_b tokens in ceil(L_b / P) pages and gets n_b more. Of its pages each begins
+// with a token t, t % P = 0, so that a new page belongs to exactly one new token: page j of row b is entry
+// taken + sum over the rows before of their new pages + j - ceil(L_b / P) of the free list. The work is laid out
+// by tokens: a block takes kTableTokens of them, finds its rows by prefix sums over the rows (of n and of the new
+// pages), 256 rows at a time, and a token its row by a binary search of those. Block 0 goes through all rows
+// and writes the offsets and the new lengths.
+// ---------------------------------------------------------------------------------------
+constexpr int kTableTokens = 1024;
+
+__device__ __forceinline__ int pages_of(int64_t tokens, int P) { return (int)((tokens + P - 1) / P); }
+
+// Inclusive sums of (x, y) over the block's 256 threads; *tx, *ty: the block's sums. Two barriers.
+__device__ __forceinline__ void block_scan2(int64_t& x, int& y, int64_t* tx, int* ty, int64_t (&wx)[4], int (&wy)[4]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t ox = __shfl_up(x, d);
+    const int oy = __shfl_up(y, d);
+    if (lane >= d) x += ox, y += oy;
+  }
+  __syncthreads();
+  if (lane == 63) wx[w] = x, wy[w] = y;
+  __syncthreads();
+  *tx = 0;
+  *ty = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < w) x += wx[i], y += wy[i];
+    *tx += wx[i];
+    *ty += wy[i];
+  }
+}
+
+// The block's tokens i0 .. i1; with `last` all rows are gone through and their offsets written, with `state` also
+// the new lengths and the pages taken. Tokens past `total` are not added: the row that reaches it gets fewer, the rows
+// behind it none.
+__device__ void page_tables(const PageTablesArgs& a, int64_t i0, int64_t i1, bool last, bool state) {
+  __shared__ int64_t wx[4];
+  __shared__ int wy[4];
+  __shared__ int r_end[256], r_len[256], r_held[256], r_first[256];  // r_end: tokens up to the row's last
+  const int tid = threadIdx.x;
+  const int64_t cap = (int64_t)a.M * a.P;
+  const int64_t taken = *a.taken < 0 ? 0 : *a.taken;
+  int64_t before = 0, pages = 0;  // tokens and new pages of the rows before these 256
+  for (int b0 = 0; b0 < a.B; b0 += 256) {
+    const int b = b0 + tid;
+    int len = 0, add = 0;
+    if (b < a.B) {
+      len = a.lengths[b];
+      len = len < 0 ? 0 : (len > cap ? (int)cap : len);
+      add = a.add[b] < 0 ? 0 : a.add[b];
+    }
+    auto after = [&](int64_t n) { return len + n < cap ? len + n : cap; };
+    const int held = pages_of(len, a.P), take = pages_of(after(add), a.P) - held;
+    int64_t end = add, all;
+    int upto = take, took;
+    block_scan2(end, upto, &all, &took, wx, wy);
+    end += before;
+    const int64_t lo = end - add < a.total ? end - add : a.total, hi = end < a.total ? end : a.total;
+    const int64_t first = taken + pages + (upto - take);  // the row's first new page in the free list
+    r_end[tid] = (int)hi;
+    r_len[tid] = len;
+    r_held[tid] = held;
+    r_first[tid] = first > 0x7fffffff ? 0x7fffffff : (int)first;
+    if (last && b < a.B) {
+      a.cu[b + 1] = (int)hi;
+      if (state) {
+        a.lengths_out[b] = (int)after(hi - lo);
+        // the row that reaches `total` says what is taken
+        if (lo < a.total && end >= a.total) {
+          const int64_t now = first + pages_of(after(hi - lo), a.P) - held;
+          *a.taken_out = now > 0x7fffffff ? 0x7fffffff : (int)now;
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t here0 = before < a.total ? before : a.total;
+    before += all;
+    pages += took;
+    const int64_t here1 = before < a.total ? before : a.total;
+    const int64_t t0 = here0 > i0 ? here0 : i0, t1 = here1 < i1 ? here1 : i1;
+    for (int64_t i = t0 + tid; i < t1; i += 256) {
+      int r = 0;  // the first row whose end lies past i
+#pragma unroll
+      for (int step = 128; step > 0; step >>= 1)
+        if (r_end[r + step - 1] <= i) r += step;
+      const int64_t t = r_len[r] + (i - (r > 0 ? r_end[r - 1] : here0));
+      int64_t slot = -1;
+      if (t < cap) {
+        const int page = (int)t / a.P, place = (int)t - page * a.P;
+        int32_t* entry = a.tables + (int64_t)(b0 + r) * a.t_bs + page;
+        int id = -1;
+        if (page < r_held[r]) {
+          id = *entry;
+        } else {
+          const int64_t at = (int64_t)r_first[r] + page - r_held[r];
+          if (at < a.F) id = a.free[at];
+          if (place == 0) *entry = id < 0 ? -1 : id;
+        }
+        slot = (int64_t)id * a.P + place;
+        if (id < 0 || slot > 0x7fffffff) slot = -1;
+      }
+      a.slots[i] = (int)slot;
+      a.positions[i] = t > 0x7fffffff ? 0x7fffffff : (int)t;
+    }
+    if (!last && before >= i1) return;
+  }
+  // slots behind the last token
+  for (int64_t i = (before > i0 ? before : i0) + tid; i < i1; i += 256) {
+    a.slots[i] = -1;
+    a.positions[i] = 0;
+  }
+  if (last && tid == 0) {
+    a.cu[0] = 0;
+    if (state && (before < a.total || a.total == 0)) {
+      const int64_t now = taken + (a.total == 0 ? 0 : pages);
+      *a.taken_out = now > 0x7fffffff ? 0x7fffffff : (int)now;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void k_page_tables(const PageTablesArgs a, int state) {
+  const int64_t i0 = (int64_t)blockIdx.x * kTableTokens;
+  const int64_t i1 = i0 + kTableTokens < a.total ? i0 + kTableTokens : a.total;
+  page_tables(a, i0, i1, blockIdx.x == 0, state);
+}
+// The new lengths and pages taken alone: where they replace the old ones, which the blocks before read.
+__global__ __launch_bounds__(256) void k_page_state(const PageTablesArgs a) { page_tables(a, 0, 0, true, true); }
+
+// ---------------------------------------------------------------------------------------
+// The store of new keys and values: 16 bytes of K and of V to a thread.
+// ---------------------------------------------------------------------------------------
+
+// A block's threads over the 16-byte pieces of a token's heads: `tokens` tokens at once, each thread one piece of one
+// (or, where a token has more pieces than threads, every 256th).
+struct Pieces {
+  int chunks, all, tokens, tok, first;
+  __device__ __forceinline__ Pieces(int HK, int D) {
+    chunks = D / 8;
+    all = HK * chunks;
+    tokens = all < 256 ? 256 / all : 1;
+    tok = all < 256 ? (int)threadIdx.x / all : 0;
+    first = (int)threadIdx.x - tok * all;
+  }
+  __device__ __forceinline__ bool idle() const { return tok >= tokens; }
+};
+
+__global__ __launch_bounds__(256) void k_page_store(const PageStoreArgs a) {
+  const Pieces p(a.HK, a.D);
+  if (p.idle()) return;
+  for (int64_t t = (int64_t)blockIdx.x * p.tokens + p.tok; t < a.T; t += (int64_t)gridDim.x * p.tokens) {
+    const int slot = a.slots[t], page = slot / a.P, place = slot - page * a.P;
+    if (slot < 0 || page >= a.N) continue;
+    for (int c = p.first; c < p.all; c += 256) {
+      const int h = c / p.chunks, d = 8 * (c - h * p.chunks);
+      u32x4 x[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        x[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.src[i]) + t * a.s_ts[i] +
+                                               h * a.s_hs[i] + d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.dst[i].p) + page * a.dst[i].ps + place * a.dst[i].ts +
+                                  h * a.dst[i].hs + d) = x[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// The beams' states follow their parents, in place: a thread owns 16 bytes of one token, layer and cache of all beams
+// of a request, reads what moves from each parent's page and then writes it to the beams' own, so that no place
+// is overwritten before it is read, whatever permutation or choice the parents are. Beams that stay are neither
+// read nor written, nor are pages that a beam shares with its parent.
+// ---------------------------------------------------------------------------------------
+template <int MOST>
+__global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a) {
+  const int r = blockIdx.y, layer = blockIdx.z >> 1, cache = blockIdx.z & 1;
+  const Pieces p(a.HK, a.D);
+  const int64_t cap = (int64_t)a.M * a.P;
+  const int64_t end = a.lengths[r] < cap ? a.lengths[r] : cap;
+  const int start = a.start == nullptr || a.start[r] < 0 ? 0 : a.start[r];
+  int from[MOST];  // the parent of each beam that moves, else -1
+  bool any = false;
+#pragma unroll
+  for (int w = 0; w < MOST; ++w) {
+    from[w] = -1;
+    if (w < a.W) {
+      const int parent = a.parents[(int64_t)r * a.W + w];
+      if (parent != w && parent >= 0 && parent < a.W) from[w] = parent, any = true;
+    }
+  }
+  if (!any || p.idle()) return;
+  const int32_t* tables = a.tables + (int64_t)r * a.W * a.t_bs;
+  const Pages pg = cache ? a.pages[1] : a.pages[0];
+  uint16_t* const pages = static_cast<uint16_t*>(pg.p) + layer * pg.ls;
+  for (int64_t t = start + (int64_t)blockIdx.x * p.tokens + p.tok; t < end; t += (int64_t)gridDim.x * p.tokens) {
+    const int page = (int)t / a.P, place = (int)t - page * a.P;
+    int src[MOST], dst[MOST];
+#pragma unroll
+    for (int w = 0; w < MOST; ++w) {
+      dst[w] = -1;
+      if (from[w] < 0) continue;
+      src[w] = tables[(int64_t)from[w] * a.t_bs + page];
+      const int to = tables[(int64_t)w * a.t_bs + page];
+      if (src[w] != to && (unsigned)src[w] < (unsigned)a.N && (unsigned)to < (unsigned)a.N) dst[w] = to;
+    }
+    for (int c = p.first; c < p.all; c += 256) {
+      const int h = c / p.chunks, d = 8 * (c - h * p.chunks);
+      uint16_t* const at = pages + place * pg.ts + h * pg.hs + d;
+      u32x4 v[MOST];
+#pragma unroll
+      for (int w = 0; w < MOST; ++w)
+        if (dst[w] >= 0) v[w] = *reinterpret_cast<const u32x4*>(at + src[w] * pg.ps);
+#pragma unroll
+      for (int w = 0; w < MOST; ++w)
+        if (dst[w] >= 0) *reinterpret_cast<u32x4*>(at + dst[w] * pg.ps) = v[w];
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_page_tables(const PageTablesArgs& a, hipStream_t s) {
+  const int64_t blocks = ((int64_t)a.total + kTableTokens - 1) / kTableTokens;
+  const bool in_place = a.lengths_out == a.lengths || a.taken_out == a.taken;
+  const bool later = in_place && blocks > 1;
+  hipLaunchKernelGGL(k_page_tables, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(256), 0, s, a, later ? 0 : 1);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !later) return e;
+  hipLaunchKernelGGL(k_page_state, dim3(1), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_store(const PageStoreArgs& a, hipStream_t s) {
+  const int all = a.HK * (a.D / 8), tokens = all < 256 ? 256 / all : 1;
+  const int64_t blocks = (a.T + tokens - 1) / tokens;
+  hipLaunchKernelGGL(k_page_store, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_beam_reorder(const BeamReorderArgs& a, hipStream_t s) {
+  // the numbers of tokens are known on the device only: blocks for 8 to a CU, each going on through its request's
+  const int64_t groups = (int64_t)a.R * a.L * 2, x = groups >= 2048 ? 1 : 2048 / groups;
+  const dim3 grid((unsigned)x, (unsigned)a.R, (unsigned)(2 * a.L));
+  if (a.W <= 4)
+    hipLaunchKernelGGL(k_beam_reorder<4>, grid, dim3(256), 0, s, a);
+  else if (a.W <= 8)
+    hipLaunchKernelGGL(k_beam_reorder<8>, grid, dim3(256), 0, s, a);
+  else if (a.W <= 16)
+    hipLaunchKernelGGL(k_beam_reorder<16>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_beam_reorder<kMostBeams>, grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace esep

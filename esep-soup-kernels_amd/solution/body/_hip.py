@@ -88,6 +88,13 @@ SIGNATURES = {
     "esep_attn_cache_workspace": (_i64, [_i32] * 8),
     "esep_attn_cache": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i32] * 7
                         + [_f32, _i32, _i32, _vp]),
+    "esep_page_tables": (_i32, [_vp, _i64] + [_vp] * 9 + [_i32] * 5 + [_vp]),
+    "esep_page_store": (_i32, [_vp] * 9 + [_i64] + [_i32] * 4 + [_vp]),
+    "esep_attn_paged_workspace": (_i64, [_i32] * 11),
+    "esep_attn_paged": (_i32, [_vp] * 8 + [_i64] + [_vp] * 3 + [_i32] * 9 + [_f32] + [_i32] * 3 + [_vp]),
+    "esep_beam_select_workspace": (_i64, [_i32, _i32, _i64, _i32]),
+    "esep_beam_select": (_i32, [_vp, _i64, _i64] + [_vp] * 5 + [_i32] * 3 + [_i64, _i32, _vp]),
+    "esep_beam_reorder": (_i32, [_vp] * 6 + [_i64] + [_vp] * 2 + [_i32] * 8 + [_vp]),
     "esep_nf4_matvec": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
     "esep_rope": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64,
                          _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _f32, _vp]),
@@ -235,6 +242,23 @@ def refuse_proxies(what):
 
         if get_proxy_mode() is not None:
             raise EsepError(f"{what} runs a kernel that proxy tensors cannot put into a graph")
+
+
+def refuse_recorded(what, *tensors):
+    """For operators without a gradient that fill or change their tensors behind torch's back: inputs that record a
+    gradient or carry a tangent, traces, compilers, transforms and tensors of other classes are refused. (Modes
+    that only look on change nothing.)"""
+    if not recorded(*tensors):
+        return
+    refuse_proxies(what)
+    if torch.compiler.is_compiling() or _tracing() or _transforms():
+        raise EsepError(f"{what} runs a kernel that traces, compilers and function transforms cannot record")
+    given = [t for t in tensors if t is not None]
+    if any(type(t) not in _PLAIN_TYPES or not _has_storage(t) for t in given):
+        raise EsepError(f"{what} takes plain tensors only")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given) or (
+            forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given)):
+        raise EsepError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
 
 
 def dense16(*tensors):
@@ -629,6 +653,212 @@ def attn_cache_workspace(B, n, S, HQ, HK, D, window=None, sinks=0):
     """Floats of fp32 workspace esep_attn_cache needs for these sizes."""
     return int(lib().esep_attn_cache_workspace(B, n, S, HQ, HK, D, 0 if window is None else int(window),
                                                int(sinks)))
+
+
+def _int32(name, t, *shape):
+    """t, an int32 tensor of this shape, contiguous."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise EsepError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} "
+                        f"{list(t.shape)}")
+    return t
+
+
+def _table_ld(tables, rows=None):
+    """(rows, M, row stride) of a block table [rows, M] with a unit column stride."""
+    if tables.dtype != torch.int32 or tables.dim() != 2 or (rows is not None and tables.shape[0] != rows):
+        raise EsepError(f"tables must be int32 [{'B' if rows is None else rows}, M], got {tables.dtype} "
+                        f"{list(tables.shape)}")
+    B, M = tables.shape
+    ld, col = tables.stride()
+    if M > 1 and col != 1:
+        raise EsepError("tables need a unit stride along a row")
+    return B, M, max(ld, M) if B <= 1 else ld
+
+
+def _page_strides(name, t, dims, written):
+    """The strides of pages [..., N, P, HK, D] with a dense head dim (a dimension of one element has any); those
+    that are written must not overlap."""
+    if t.dim() != dims:
+        raise EsepError(f"{name} must be {'[L, N, P, HK, D]' if dims == 5 else '[N, P, HK, D]'}, got {list(t.shape)}")
+    *strides, last = t.stride()
+    if last != 1:
+        raise EsepError(f"{name} needs a unit stride on the head dim")
+    out = [st if n > 1 else 0 for st, n in zip(strides, t.shape)]
+    if written:
+        at = t.shape[-1]
+        for st, n in sorted((st, n) for st, n in zip(out, t.shape) if n > 1):
+            if st < at:
+                raise EsepError(f"elements of {name} overlap (strides {t.stride()})")
+            at = st * n
+    return out
+
+
+def _pages_pair(k_pages, v_pages, dims, written):
+    shape = k_pages.shape
+    if v_pages.shape != shape or v_pages.dtype != k_pages.dtype or k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise EsepError(f"k_pages and v_pages must be fp16 or bf16 of one shape, got {k_pages.dtype} {list(shape)} "
+                        f"and {v_pages.dtype} {list(v_pages.shape)}")
+    if max(shape, default=0) > 0x7FFFFFFF:
+        raise EsepError(f"pages of {list(shape)}: the library counts in 32 bits")
+    return array("q", _page_strides("k_pages", k_pages, dims, written)
+                 + _page_strides("v_pages", v_pages, dims, written))
+
+
+def page_tables(tables, lengths, new, free, taken, slots, positions, cu, lengths_out, taken_out, page,
+                name="_page_tables"):
+    """Places of `new` more tokens a row (esep_page_tables): tables int32 [B, M] extended in place; slots and
+    positions int32 [total], cu int32 [B + 1]; lengths_out and taken_out may be lengths and taken."""
+    dev = _dev(tables, lengths, new, free, taken, slots, positions, cu, lengths_out, taken_out)
+    B, M, ld = _table_ld(tables)
+    total = slots.numel()
+    if M > 0x7FFFFFFF or B > 0x7FFFFFFF or free.numel() > 0x7FFFFFFF or total > 0x7FFFFFFF or page > 0x7FFFFFFF:
+        raise EsepError(f"page_tables: bad sizes B={B} M={M} F={free.numel()} page={page} total={total}")
+    _int32("lengths", lengths, B), _int32("new", new, B), _int32("taken", taken, 1)
+    _int32("free", free, free.numel())
+    _int32("slots", slots, total), _int32("positions", positions, total), _int32("cu_seqlens", cu, B + 1)
+    _int32("lengths_out", lengths_out, B), _int32("taken_out", taken_out, 1)
+    with _on(dev):
+        rc = lib().esep_page_tables(
+            tables.data_ptr(), ld, lengths.data_ptr(), new.data_ptr(), free.data_ptr(), taken.data_ptr(),
+            slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lengths_out.data_ptr(), taken_out.data_ptr(), B, M,
+            free.numel(), page, total, _stream(dev))
+    _check(rc, "esep_page_tables")
+    _record(name)
+
+
+def page_store(k, v, k_pages, v_pages, slots, name="_page_store"):
+    """k, v [T, HK, D] to slots int32 [T] of the pages [N, P, HK, D] (esep_page_store)."""
+    dev = _dev(k, v, k_pages, v_pages, slots)
+    strides = _pages_pair(k_pages, v_pages, 4, True)
+    N, P, HK, D = k_pages.shape
+    T = slots.numel()
+    if k.shape != (T, HK, D) or v.shape != (T, HK, D) or k.dtype != k_pages.dtype or v.dtype != k.dtype:
+        raise EsepError(f"page_store: k and v must be {k_pages.dtype} [{T}, {HK}, {D}], got {k.dtype} "
+                        f"{list(k.shape)} and {v.dtype} {list(v.shape)}")
+    _int32("slots", slots, T)
+    if D > 1 and (k.stride(2) != 1 or v.stride(2) != 1):
+        raise EsepError("k and v need a unit stride on the head dim")
+    for t in (k, v):
+        ts, hs, _ = t.stride()
+        strides.extend((ts if T > 1 else 0, hs if HK > 1 else 0))
+    at = strides.buffer_info()[0]
+    with _on(dev):
+        rc = lib().esep_page_store(k.data_ptr(), at + 48, v.data_ptr(), at + 64, k_pages.data_ptr(), at,
+                                   v_pages.data_ptr(), at + 24, slots.data_ptr(), T, N, P, HK, D, _stream(dev))
+    _check(rc, "esep_page_store")
+    _record(name)
+
+
+def attn_paged(q, k_pages, v_pages, o, tables, lengths, scale, window=None, sinks=0, beams=1, shared=None,
+               workspace=None, name="_attn_paged"):
+    """Attention of q [B, n, HQ, D], each row's n newest tokens, over pages [N, P, HK, D] that tables int32 [B, M] name,
+    filled to lengths (int32 [B]) (esep_attn_paged). o [B, n, HQ, D] dense; shared int32 [B / beams]: tokens in
+    pages that `beams` rows in turn have in common. `workspace` is a contiguous fp32 tensor of >=
+    attn_paged_workspace's elements (allocated here when not given)."""
+    dev = _dev(q, k_pages, v_pages, o, tables, lengths, shared, workspace)
+    shape = q.shape
+    if len(shape) != 4 or o.shape != shape or not o.is_contiguous():
+        raise EsepError("attn_paged: q, o [B, n, HQ, D] (o dense)")
+    B, n, HQ, D = shape
+    strides = _pages_pair(k_pages, v_pages, 4, False)
+    N, P, HK, dim = k_pages.shape
+    _, M, ld = _table_ld(tables, B)
+    if dim != D or q.dtype != k_pages.dtype or o.dtype != q.dtype:
+        raise EsepError(f"attn_paged: q and o must be {k_pages.dtype} with heads of {dim}, got {q.dtype} {list(shape)}")
+    if B > 0x7FFFFFFF or n > 0x7FFFFFFF or HQ > 0x7FFFFFFF or M > 0x7FFFFFFF:
+        raise EsepError(f"attn_paged: bad sizes B={B} n={n} HQ={HQ} M={M}")
+    _int32("lengths", lengths, B)
+    if beams < 1 or B % beams != 0:
+        raise EsepError(f"attn_paged: {B} rows are no multiple of {beams} beams")
+    if shared is not None:
+        _int32("shared", shared, B // beams)
+    w, sinks, share = 0 if window is None else int(window), int(sinks), int(shared is not None)
+    need = lib().esep_attn_paged_workspace(B, n, M, P, HQ, HK, D, w, sinks, beams, share)
+    if workspace is None:
+        workspace = torch.empty(max(need, 1), device=dev, dtype=torch.float32)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
+    strides.extend(_bth_strides(q, shape, "q"))
+    at = strides.buffer_info()[0]
+    with _on(dev):
+        rc = lib().esep_attn_paged(
+            q.data_ptr(), at + 48, k_pages.data_ptr(), at, v_pages.data_ptr(), at + 24, o.data_ptr(),
+            tables.data_ptr(), ld, lengths.data_ptr(), None if shared is None else shared.data_ptr(),
+            workspace.data_ptr(), dtype_code(q.dtype), B, n, M, N, P, HQ, HK, D, float(scale), w, sinks, beams,
+            _stream(dev))
+    _check(rc, "esep_attn_paged")
+    _record(name)
+
+
+def attn_paged_workspace(B, n, M, page, HQ, HK, D, window=None, sinks=0, beams=1, shared=False):
+    """Floats of fp32 workspace esep_attn_paged needs for these sizes."""
+    return int(lib().esep_attn_paged_workspace(B, n, M, page, HQ, HK, D, 0 if window is None else int(window),
+                                               int(sinks), beams, int(shared)))
+
+
+def beam_select(logits, scores, out_scores, parents, tokens, workspace=None, name="_beam_select"):
+    """The greatest of scores [R, W] fp32 + log softmax of logits [R, W, V] of each request, as many as the outputs
+    [R, keep] (fp32, int32, int32) hold (esep_beam_select). `workspace` is a contiguous uint8 tensor of >=
+    beam_select_workspace's bytes (allocated here when not given)."""
+    dev = _dev(logits, scores, out_scores, parents, tokens, workspace)
+    if logits.dim() != 3:
+        raise EsepError(f"logits must be [R, W, V], got {list(logits.shape)}")
+    R, W, V = logits.shape
+    if V > 1 and logits.stride(2) != 1:
+        raise EsepError("logits need a unit stride along the vocabulary")
+    if scores.dtype != torch.float32 or scores.shape != (R, W) or not scores.is_contiguous():
+        raise EsepError(f"scores must be a contiguous fp32 tensor of shape {[R, W]}")
+    if R > 0x7FFFFFFF or W > 0x7FFFFFFF:
+        raise EsepError(f"beam_select: bad sizes R={R} W={W}")
+    keep = out_scores.shape[-1]
+    if out_scores.dtype != torch.float32 or out_scores.shape != (R, keep) or not out_scores.is_contiguous():
+        raise EsepError("out_scores must be a contiguous fp32 tensor [R, keep]")
+    _int32("parents", parents, R, keep), _int32("tokens", tokens, R, keep)
+    if keep > 0x7FFFFFFF:
+        raise EsepError(f"beam_select: bad sizes keep={keep}")
+    need = beam_select_workspace(R, W, V, keep)
+    if workspace is None:
+        workspace = torch.empty(max(need, 8), device=dev, dtype=torch.uint8)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise EsepError(f"workspace must be a contiguous uint8 tensor of >= {need} elements")
+    with _on(dev):
+        rc = lib().esep_beam_select(
+            logits.data_ptr(), logits.stride(0) if R > 1 else 0, logits.stride(1) if W > 1 else 0, scores.data_ptr(),
+            workspace.data_ptr(), out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+            dtype_code(logits.dtype), R, W, V, keep, _stream(dev))
+    _check(rc, "esep_beam_select")
+    _record(name)
+
+
+def beam_select_workspace(R, W, V, keep):
+    """Bytes of workspace esep_beam_select needs for these sizes."""
+    return int(lib().esep_beam_select_workspace(R, W, V, keep))
+
+
+def beam_reorder(parents, k_pages, v_pages, tables, lengths, start=None, name="_beam_reorder"):
+    """Tokens start .. lengths (int32 [R]) of each beam's pages [L, N, P, HK, D] become its parent's, in place
+    (esep_beam_reorder); parents int32 [R, W], tables int32 [R * W, M]."""
+    dev = _dev(parents, k_pages, v_pages, tables, lengths, start)
+    strides = _pages_pair(k_pages, v_pages, 5, True)
+    L, N, P, HK, D = k_pages.shape
+    if parents.dim() != 2:
+        raise EsepError(f"parents must be int32 [R, W], got {list(parents.shape)}")
+    R, W = parents.shape
+    if W < 1:
+        raise EsepError("beam_reorder: no beams")
+    _int32("parents", parents, R, W), _int32("lengths", lengths, R)
+    if start is not None:
+        _int32("start", start, R)
+    _, M, ld = _table_ld(tables, R * W)
+    if max(R, W, M) > 0x7FFFFFFF:
+        raise EsepError(f"beam_reorder: bad sizes R={R} W={W} M={M}")
+    at = strides.buffer_info()[0]
+    with _on(dev):
+        rc = lib().esep_beam_reorder(
+            parents.data_ptr(), k_pages.data_ptr(), at, v_pages.data_ptr(), at + 32, tables.data_ptr(), ld,
+            lengths.data_ptr(), None if start is None else start.data_ptr(), R, W, M, L, N, P, HK, D, _stream(dev))
+    _check(rc, "esep_beam_reorder")
+    _record(name)
 
 
 def _flat(t, name):

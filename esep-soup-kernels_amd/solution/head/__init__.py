@@ -6,6 +6,7 @@ Soup wiring) is not provided: TRL and Soup are not part of this build, and the i
 outside the kernel path.
 """
 
+from .beam import beam_select
 from .op import CHUNK_ROWS, G_SCALE, VOCAB, FusedLinearCE, fused_linear_ce, warmup
 
-__all__ = ["fused_linear_ce", "FusedLinearCE", "warmup", "CHUNK_ROWS", "G_SCALE", "VOCAB"]
+__all__ = ["beam_select", "fused_linear_ce", "FusedLinearCE", "warmup", "CHUNK_ROWS", "G_SCALE", "VOCAB"]

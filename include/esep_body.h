@@ -329,6 +329,79 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
                     int window, int sinks, void* stream);
 
 /*
+ * Paged caches, for answering. No reference counterpart. Tokens of a row lie in pages of `page` tokens; row b's token t
+ * is in page tables[b, t / page] at place t % page. Pages [N, page, HK, D] of fp16 or bf16: strides of page, token
+ * and head (int64 [3], elements, multiples of 8), 16-byte addresses.
+ *
+ * esep_page_tables: rows of `lengths` tokens (int32 [B]) get `add` more (int32 [B]; negative: 0).
+ *   tables int32 [B, M]       by row stride tables_bs; entries of the pages that are begun now are written
+ *   free_pages int32 [F]      page numbers; taken from entry *taken on, row by row
+ *   slots, positions [total]  of each new token, the rows' one behind another: tables[b, t / page] * page + t % page, and
+ *                             t. -1 where the row's table or the free list has no page for it (the entry becomes -1),
+ *                             and behind the last token (position 0)
+ *   cu_seqlens [B + 1]        the offsets of the rows' new tokens
+ *   lengths_out, taken_out    the new lengths (at most M * page) and *taken + the pages that were needed; they may be
+ *                             lengths and taken themselves
+ * Tokens past `total` are not added. lengths count as clamped into [0, M * page], a negative *taken as 0. M * page
+ * <= 2^30.
+ */
+int esep_page_tables(int32_t* tables, int64_t tables_bs, const int32_t* lengths, const int32_t* add,
+                     const int32_t* free_pages, const int32_t* taken, int32_t* slots, int32_t* positions,
+                     int32_t* cu_seqlens, int32_t* lengths_out, int32_t* taken_out, int B, int M, int F,
+                     int page, int total, void* stream);
+
+/*
+ * Stores k, v [T, HK, D] (strides of token and head, int64 [2], multiples of 8; 16-byte addresses) at slots int32 [T]
+ * of the pages: slot s is place s % page of page s / page. Slots below 0 or past the N pages are left out. Tokens that
+ * name one slot leave it with pieces of either. D a multiple of 8, N * page < 2^31.
+ */
+int esep_page_store(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                    void* k_pages, const int64_t* kp_strides, void* v_pages, const int64_t* vp_strides,
+                    const int32_t* slots, int64_t T, int N, int page, int HK, int D, void* stream);
+
+/*
+ * esep_attn_cache over pages: page a power of two of at least 16, D in {64, 128}, token strides at most 2^22. lengths
+ * count as clamped into [0, M * page]; keys in a page outside [0, N) are not seen. shared (int32 [B / beams], or
+ * NULL; not with a window): the first shared[r] tokens of the rows r * beams .. + beams - 1 lie in the same pages; their
+ * K and V are then read once for all of these rows, from the first one's table (whole tiles of 32, and no further than each
+ * row's new tokens). workspace: fp32, 16-byte aligned, esep_attn_paged_workspace floats, a function of the sizes.
+ * Deterministic (no atomics). B * HQ * n < 2^24, M * page <= 2^30.
+ */
+int64_t esep_attn_paged_workspace(int B, int n, int M, int page, int HQ, int HK, int D, int window, int sinks,
+                                  int beams, int shared);
+int esep_attn_paged(const void* q, const int64_t* q_strides, const void* k_pages, const int64_t* kp_strides,
+                    const void* v_pages, const int64_t* vp_strides, void* o, const int32_t* tables,
+                    int64_t tables_bs, const int32_t* lengths, const int32_t* shared, float* workspace, int dt,
+                    int B, int n, int M, int N, int page, int HQ, int HK, int D, float scale, int window,
+                    int sinks, int beams, void* stream);
+
+/*
+ * Beam search's selection: of score[r, w] + logits[r, w, t] - lse[r, w] over a request's W beams and V tokens the `keep`
+ * greatest, the greatest first, ties to the lowest w * V + t. logits [R, W, V] of fp32 / fp16 / bf16 by (ld_r, ld_w);
+ * scores fp32 [R, W]. A beam whose score or lse is not finite (no finite logit, a NaN, +inf) is out: its values count as
+ * -inf, as a logit of -inf does; where fewer than `keep` are left, -inf fills up at the lowest places that are not
+ * chosen. Exponentials' sums in fp32, lse and the comparison of beams in 64 bits. Outputs [R, keep]. workspace: 8-byte
+ * aligned, esep_beam_select_workspace BYTES. W <= 64, keep <= min(64, W V), V <= 2^24, R * W <= 65535. The outputs do not
+ * depend on the order of the blocks.
+ */
+int64_t esep_beam_select_workspace(int R, int W, int64_t V, int keep);
+int esep_beam_select(const void* logits, int64_t ld_r, int64_t ld_w, const float* scores, void* workspace,
+                     float* out_scores, int32_t* out_parents, int32_t* out_tokens, int dt, int R, int W, int64_t V,
+                     int keep, void* stream);
+
+/*
+ * The beams' paged states follow their parents, in place: tokens start[r] .. lengths[r] - 1 (start NULL: 0) of row r * W + w
+ * become what row r * W + parents[r, w] held. parents int32 [R, W] (outside [0, W): the beam stays); tables int32
+ * [R * W, M]; pages [L, N, page, HK, D], strides of layer, page, token and head (int64 [4]). Pages that a beam shares with its
+ * parent are left alone, as are tokens for which either has a page outside [0, N). Other pages belong to one beam. W <= 32,
+ * L <= 32767, R <= 65535, 2 L R < 2^24.
+ */
+int esep_beam_reorder(const int32_t* parents, void* k_pages, const int64_t* kp_strides, void* v_pages,
+                      const int64_t* vp_strides, const int32_t* tables, int64_t tables_bs,
+                      const int32_t* lengths, const int32_t* start, int R, int W, int M, int L, int N,
+                      int page, int HK, int D, void* stream);
+
+/*
  * SwiGLU of the Qwen2 MLP, element-wise over n elements of one dtype (fp32 / fp16 / bf16),
  * contiguous, 16-byte aligned. Replaces the example kernels the reference decoder calls,
  * solution/swiglu.py:15-37 (example_swiglu_fwd_kernel / example_swiglu_bwd_kernel, launched at
