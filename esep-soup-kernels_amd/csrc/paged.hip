@@ -15,7 +15,7 @@ namespace {
 // pages), 256 rows at a time, and a token its row by a binary search of those. Block 0 goes through all rows
 // and writes the offsets and the new lengths.
 // ---------------------------------------------------------------------------------------
-constexpr int kTableTokens = 1024;
+constexpr int kTableTokens = 1024, kTableEach = kTableTokens / 256;
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int P) { return (int)((tokens + P - 1) / P); }
 
@@ -89,29 +89,46 @@ __device__ void page_tables(const PageTablesArgs& a, int64_t i0, int64_t i1, boo
     pages += took;
     const int64_t here1 = before < a.total ? before : a.total;
     const int64_t t0 = here0 > i0 ? here0 : i0, t1 = here1 < i1 ? here1 : i1;
-    for (int64_t i = t0 + tid; i < t1; i += 256) {
-      int r = 0;  // the first row whose end lies past i
+    for (int64_t i0k = t0 + tid; i0k < t1; i0k += 256 * kTableEach) {
+      // the pages of all of the thread's tokens are asked for before any is used
+      int64_t t[kTableEach];
+      int page[kTableEach], id[kTableEach];
+      int32_t* entry[kTableEach];
+      bool fresh[kTableEach];
 #pragma unroll
-      for (int step = 128; step > 0; step >>= 1)
-        if (r_end[r + step - 1] <= i) r += step;
-      const int64_t t = r_len[r] + (i - (r > 0 ? r_end[r - 1] : here0));
-      int64_t slot = -1;
-      if (t < cap) {
-        const int page = (int)t / a.P, place = (int)t - page * a.P;
-        int32_t* entry = a.tables + (int64_t)(b0 + r) * a.t_bs + page;
-        int id = -1;
-        if (page < r_held[r]) {
-          id = *entry;
+      for (int k = 0; k < kTableEach; ++k) {
+        const int64_t i = i0k + 256 * k;
+        id[k] = -1;
+        fresh[k] = false;
+        entry[k] = nullptr;
+        t[k] = 0;
+        if (i >= t1) continue;
+        int r = 0;  // the first row whose end lies past i
+#pragma unroll
+        for (int step = 128; step > 0; step >>= 1)
+          if (r_end[r + step - 1] <= i) r += step;
+        t[k] = r_len[r] + (i - (r > 0 ? r_end[r - 1] : here0));
+        if (t[k] >= cap) continue;
+        page[k] = (int)t[k] / a.P;
+        entry[k] = a.tables + (int64_t)(b0 + r) * a.t_bs + page[k];
+        if (page[k] < r_held[r]) {
+          id[k] = *entry[k];
         } else {
-          const int64_t at = (int64_t)r_first[r] + page - r_held[r];
-          if (at < a.F) id = a.free[at];
-          if (place == 0) *entry = id < 0 ? -1 : id;
+          const int64_t at = (int64_t)r_first[r] + page[k] - r_held[r];
+          if (at < a.F) id[k] = a.free[at];
+          fresh[k] = page[k] * a.P == (int)t[k];  // the page's first token
         }
-        slot = (int64_t)id * a.P + place;
-        if (id < 0 || slot > 0x7fffffff) slot = -1;
       }
-      a.slots[i] = (int)slot;
-      a.positions[i] = t > 0x7fffffff ? 0x7fffffff : (int)t;
+#pragma unroll
+      for (int k = 0; k < kTableEach; ++k) {
+        const int64_t i = i0k + 256 * k;
+        if (i >= t1) continue;
+        if (fresh[k]) *entry[k] = id[k] < 0 ? -1 : id[k];
+        int64_t slot = -1;
+        if (id[k] >= 0) slot = (int64_t)id[k] * a.P + ((int)t[k] - page[k] * a.P);
+        a.slots[i] = slot > 0x7fffffff ? -1 : (int)slot;
+        a.positions[i] = t[k] > 0x7fffffff ? 0x7fffffff : (int)t[k];
+      }
     }
     if (!last && before >= i1) return;
   }
@@ -177,53 +194,68 @@ __global__ __launch_bounds__(256) void k_page_store(const PageStoreArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------
-// The beams' states follow their parents, in place: a thread owns 16 bytes of one token, layer and cache of all beams
-// of a request, reads what moves from each parent's page and then writes it to the beams' own, so that no place
-// is overwritten before it is read, whatever permutation or choice the parents are. Beams that stay are neither
-// read nor written, nor are pages that a beam shares with its parent.
+// The beams' states follow their parents, in place: a thread owns 16 bytes of a token of all beams of a request (of
+// one layer's K or V), reads what moves from each parent's page and then writes it to the beams' own, so that no
+// place is overwritten before it is read, whatever permutation or choice the parents are. Beams that stay are neither
+// read nor written, nor are pages that a beam shares with its parent. A block goes through a request's pages, whose
+// numbers are read once a page.
 // ---------------------------------------------------------------------------------------
-template <int MOST>
+template <int MOST, int UNROLL>
 __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a) {
-  const int r = blockIdx.y, layer = blockIdx.z >> 1, cache = blockIdx.z & 1;
-  const Pieces p(a.HK, a.D);
+  const int r = blockIdx.y, layer = blockIdx.z >> 1, cache = blockIdx.z & 1, lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.M * a.P;
-  const int64_t end = a.lengths[r] < cap ? a.lengths[r] : cap;
+  const int end = a.lengths[r] < cap ? a.lengths[r] : (int)cap;
   const int start = a.start == nullptr || a.start[r] < 0 ? 0 : a.start[r];
-  int from[MOST];  // the parent of each beam that moves, else -1
-  bool any = false;
-#pragma unroll
-  for (int w = 0; w < MOST; ++w) {
-    from[w] = -1;
-    if (w < a.W) {
-      const int parent = a.parents[(int64_t)r * a.W + w];
-      if (parent != w && parent >= 0 && parent < a.W) from[w] = parent, any = true;
-    }
+  if (start >= end) return;
+  // lane w: the parent of beam w where it moves, else w
+  int from = lane;
+  if (lane < a.W) {
+    const int parent = a.parents[(int64_t)r * a.W + lane];
+    if (parent >= 0 && parent < a.W) from = parent;
   }
-  if (!any || p.idle()) return;
+  if (__ballot(from != lane) == 0) return;
+  const Pieces p(a.HK, a.D);
   const int32_t* tables = a.tables + (int64_t)r * a.W * a.t_bs;
   const Pages pg = cache ? a.pages[1] : a.pages[0];
   uint16_t* const pages = static_cast<uint16_t*>(pg.p) + layer * pg.ls;
-  for (int64_t t = start + (int64_t)blockIdx.x * p.tokens + p.tok; t < end; t += (int64_t)gridDim.x * p.tokens) {
-    const int page = (int)t / a.P, place = (int)t - page * a.P;
-    int src[MOST], dst[MOST];
+  const int last = (end - 1) / a.P;
+  for (int page = start / a.P + blockIdx.x; page <= last; page += gridDim.x) {
+    const int mine = lane < a.W ? tables[(int64_t)lane * a.t_bs + page] : -1;
+    const int theirs = __shfl(mine, from);
+    const bool moves = theirs != mine && (unsigned)theirs < (unsigned)a.N && (unsigned)mine < (unsigned)a.N;
+    const uint64_t go = __ballot(moves);
+    if (go == 0 || p.idle()) continue;
+    int64_t src[MOST], dst[MOST];
 #pragma unroll
     for (int w = 0; w < MOST; ++w) {
-      dst[w] = -1;
-      if (from[w] < 0) continue;
-      src[w] = tables[(int64_t)from[w] * a.t_bs + page];
-      const int to = tables[(int64_t)w * a.t_bs + page];
-      if (src[w] != to && (unsigned)src[w] < (unsigned)a.N && (unsigned)to < (unsigned)a.N) dst[w] = to;
+      src[w] = __builtin_amdgcn_readlane(theirs, w) * pg.ps;
+      dst[w] = __builtin_amdgcn_readlane(mine, w) * pg.ps;
     }
+    const int p0 = page * a.P > start ? 0 : start - page * a.P;
+    const int p1 = (int64_t)(page + 1) * a.P < end ? a.P : end - page * a.P;
     for (int c = p.first; c < p.all; c += 256) {
       const int h = c / p.chunks, d = 8 * (c - h * p.chunks);
-      uint16_t* const at = pages + place * pg.ts + h * pg.hs + d;
-      u32x4 v[MOST];
+      uint16_t* const head = pages + h * pg.hs + d;
+      for (int t = p0 + p.tok; t < p1; t += UNROLL * p.tokens) {
+        u32x4 v[UNROLL][MOST];
 #pragma unroll
-      for (int w = 0; w < MOST; ++w)
-        if (dst[w] >= 0) v[w] = *reinterpret_cast<const u32x4*>(at + src[w] * pg.ps);
+        for (int k = 0; k < UNROLL; ++k) {
+          const int tk = t + k * p.tokens;
+          uint16_t* const at = head + (tk < p1 ? tk : t) * pg.ts;
 #pragma unroll
-      for (int w = 0; w < MOST; ++w)
-        if (dst[w] >= 0) *reinterpret_cast<u32x4*>(at + dst[w] * pg.ps) = v[w];
+          for (int w = 0; w < MOST; ++w)
+            if (go >> w & 1) v[k][w] = *reinterpret_cast<const u32x4*>(at + src[w]);
+        }
+#pragma unroll
+        for (int k = 0; k < UNROLL; ++k) {
+          const int tk = t + k * p.tokens;
+          if (tk >= p1) break;
+          uint16_t* const at = head + tk * pg.ts;
+#pragma unroll
+          for (int w = 0; w < MOST; ++w)
+            if (go >> w & 1) *reinterpret_cast<u32x4*>(at + dst[w]) = v[k][w];
+        }
+      }
     }
   }
 }
@@ -249,17 +281,17 @@ hipError_t launch_page_store(const PageStoreArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_beam_reorder(const BeamReorderArgs& a, hipStream_t s) {
-  // the numbers of tokens are known on the device only: blocks for 8 to a CU, each going on through its request's
-  const int64_t groups = (int64_t)a.R * a.L * 2, x = groups >= 2048 ? 1 : 2048 / groups;
-  const dim3 grid((unsigned)x, (unsigned)a.R, (unsigned)(2 * a.L));
+  // a request's own pages are known on the device only: blocks for 16 of a CU's, up to one to a page of the table
+  const int64_t groups = (int64_t)a.R * a.L * 2, most = groups >= 16384 ? 1 : 16384 / groups;
+  const dim3 grid((unsigned)(most < a.M ? most : a.M), (unsigned)a.R, (unsigned)(2 * a.L));
   if (a.W <= 4)
-    hipLaunchKernelGGL(k_beam_reorder<4>, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<4, 4>), grid, dim3(256), 0, s, a);
   else if (a.W <= 8)
-    hipLaunchKernelGGL(k_beam_reorder<8>, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<8, 2>), grid, dim3(256), 0, s, a);
   else if (a.W <= 16)
-    hipLaunchKernelGGL(k_beam_reorder<16>, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<16, 1>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL(k_beam_reorder<kMostBeams>, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<kMostBeams, 1>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
