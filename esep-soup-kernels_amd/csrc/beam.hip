@@ -55,6 +55,14 @@ __device__ __forceinline__ float wave_bound(float v, int keep) {
   return bound;
 }
 
+// Lanes that count a listed candidate's betters together, and their sum, in each of them.
+constexpr int kRankLanes = 8;
+__device__ __forceinline__ int rank_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);   // lane ^ 1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);   // lane ^ 2
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);  // the other quad of each 8
+}
+
 // The piece's elements of thread i: i * 8 .. + 7 of each run of 2048, whatever the row's alignment, so that equal
 // rows give equal sums.
 template <typename T, int U, bool VEC>
@@ -133,11 +141,12 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   uint64_t* out = a.cand + part * a.keep;
   const int n = count;
   if (n <= kList) {
-    for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+    for (int i = threadIdx.x / kRankLanes; i < n; i += kBeamThreads / kRankLanes) {
       const uint64_t k = list[i];
       int place = 0;
-      for (int j = 0; j < n; ++j) place += list[j] > k;
-      if (place < a.keep) out[place] = k;
+      for (int j = threadIdx.x % kRankLanes; j < n; j += kRankLanes) place += list[j] > k;
+      place = rank_sum(place);
+      if (place < a.keep && threadIdx.x % kRankLanes == 0) out[place] = k;
     }
     for (int i = n + threadIdx.x; i < a.keep; i += kBeamThreads) out[i] = 0;
     return;
@@ -167,16 +176,18 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   }
 }
 
-// A candidate of the join: its value and its place w V + t; the greater value first, then the lower place.
+// A candidate of the join: its value and its place w V + t; the greater value first, then the lower place. None: -inf
+// at a place that no candidate has.
 struct Cand {
   double value;
-  int64_t at;
+  int at;
 };
+constexpr int kNoPlace = 0x7fffffff;
 __device__ __forceinline__ bool before(const Cand& x, const Cand& y) {
   return x.value > y.value || (x.value == y.value && x.at < y.at);
 }
 
-constexpr int kJoinThreads = 1024, kJoinMostBeams = 64;
+constexpr int kJoinThreads = 1024, kJoinFirst = 4, kJoinMostBeams = 64;
 
 __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   constexpr int NW = kJoinThreads / 64;
@@ -185,25 +196,40 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   __shared__ float tops[kJoinMostBeams];
   __shared__ Cand list[kList], w_best[NW];
   __shared__ float w_bound[NW];
-  __shared__ int64_t chosen[kBeamMostKeep];
-  __shared__ int count, found;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = wave_id();
-  if (threadIdx.x == 0) count = 0, found = 0;
+  __shared__ int chosen[kBeamMostKeep];
+  __shared__ int count;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = wave_id();
+  const int per = a.splits * a.keep, all = a.W * per;
+  const uint64_t* keys = a.cand + (int64_t)r * all;
+  // everything is asked for at once: the thread's first candidates, the pieces' parts (those of a beam that is out hold
+  // nothing, and are not used)
+  uint64_t key[kJoinFirst];
+#pragma unroll
+  for (int j = 0; j < kJoinFirst; ++j) {
+    const int i = tid + j * kJoinThreads;
+    key[j] = i < all ? keys[i] : 0;
+  }
+  if (tid == 0) count = 0;
+#pragma unroll 1
   for (int b = w; b < a.W; b += NW) {
-    const int64_t row = (int64_t)r * a.W + b;
+    const int row = r * a.W + b;
     const float sc = a.scores[row];
+    const float2* st = a.stat + (int64_t)row * a.splits;
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 p0 = lane < a.splits ? st[lane] : none, p1 = lane + 64 < a.splits ? st[lane + 64] : none;
     double l = 0.0;
-    float top = -INFINITY;
+    float top = fmaxf(p0.x, p1.x);
     const bool in = fabsf(sc) < INFINITY;
     if (in) {
-      const float2* st = a.stat + row * a.splits;
-      for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, st[i].x);
+#pragma unroll 1
+      for (int i = lane + 128; i < a.splits; i += 64) top = fmaxf(top, st[i].x);
       top = wave_max(top);
-      double sum = 0.0;
-      for (int i = lane; i < a.splits; i += 64) {
-        const float2 p = st[i];
-        sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)top);
-      }
+      auto part = [&](const float2& p) {  // a piece without a finite logit has 0, or a NaN
+        return p.x == -INFINITY ? p.y : p.y * __builtin_amdgcn_exp2f((p.x - top) * kLog2e);
+      };
+      double sum = (double)part(p0) + (double)part(p1);
+#pragma unroll 1
+      for (int i = lane + 128; i < a.splits; i += 64) sum += (double)part(st[i]);
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
       l = log(sum);
@@ -215,61 +241,57 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
     }
   }
   __syncthreads();
-  const int per = a.splits * a.keep, all = a.W * per;
-  const uint64_t* keys = a.cand + (int64_t)r * all;
-  auto get = [&](int i, Cand& c) {  // whether there is one
+  auto value = [&](int i, uint64_t k) {  // of candidate i
     const int b = i / per;
-    if (!(score[b] == score[b])) return false;
-    const uint64_t k = keys[i];
-    if (k == 0) return false;
-    c.value = (((double)unordered((uint32_t)(k >> 32)) - (double)tops[b]) - rest[b]) + score[b];
-    c.at = (int64_t)b * a.V + (int64_t)(uint32_t)~(uint32_t)k;
-    return true;
+    if (k == 0 || !(score[b] == score[b])) return Cand{-(double)INFINITY, kNoPlace};
+    return Cand{(((double)unordered((uint32_t)(k >> 32)) - (double)tops[b]) - rest[b]) + score[b],
+                b * a.V + (int)~(uint32_t)k};
   };
-  float mine = -INFINITY;
-  for (int i = threadIdx.x; i < all; i += kJoinThreads) {
-    Cand c;
-    if (get(i, c)) mine = fmaxf(mine, (float)c.value);
+  Cand mine[kJoinFirst];
+  float best32 = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kJoinFirst; ++j) {
+    const int i = tid + j * kJoinThreads;
+    mine[j] = value(i < all ? i : 0, key[j]);
+    best32 = fmaxf(best32, (float)mine[j].value);
   }
-  const float wb = wave_bound(mine, a.keep);
+  constexpr int kRest = kJoinFirst * kJoinThreads;
+#pragma unroll 1
+  for (int i = tid + kRest; i < all; i += kJoinThreads) best32 = fmaxf(best32, (float)value(i, keys[i]).value);
+  const float wb = wave_bound(best32, a.keep);
   if (lane == 0) w_bound[w] = wb;
   __syncthreads();
-  float bound = w_bound[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) bound = fmaxf(bound, w_bound[i]);
+  float bound = w_bound[lane < NW ? lane : 0];
+  bound = wave_max(bound);
   // by value in 32 bits (rounding keeps the order): what reaches the bound
-  for (int i = threadIdx.x; i < all; i += kJoinThreads) {
-    Cand c;
-    if (get(i, c) && (float)c.value >= bound) {
+  auto enter = [&](const Cand& c) {
+    if (c.at != kNoPlace && (float)c.value >= bound) {
       const int at = atomicAdd(&count, 1);
       if (at < kList) list[at] = c;
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kJoinFirst; ++j) enter(mine[j]);
+#pragma unroll 1
+  for (int i = tid + kRest; i < all; i += kJoinThreads) enter(value(i, keys[i]));
   __syncthreads();
   auto put = [&](int place, const Cand& c) {
-    const int64_t o = (int64_t)r * a.keep + place;
-    const int b = (int)(c.at / a.V);
+    const int o = r * a.keep + place, b = c.at / a.V;
     a.out_scores[o] = (float)c.value;
     a.out_parents[o] = b;
-    a.out_tokens[o] = (int)(c.at - (int64_t)b * a.V);
+    a.out_tokens[o] = c.at - b * a.V;
     chosen[place] = c.at;
   };
   const int n = count;
-  if (n <= kList) {
-    for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-      const Cand c = list[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += before(list[j], c);
-      if (place < a.keep) put(place, c);
-    }
-    if (threadIdx.x == 0) found = n < a.keep ? n : a.keep;
-  } else {
+  if (n > kList) {  // ties: the greatest, `keep` times
     Cand last{(double)INFINITY, -1};
+#pragma unroll 1
     for (int k = 0; k < a.keep; ++k) {
-      Cand best{-(double)INFINITY, INT64_MAX};
-      for (int i = threadIdx.x; i < all; i += kJoinThreads) {
-        Cand c;
-        if (get(i, c) && before(last, c) && before(c, best)) best = c;
+      Cand best{-(double)INFINITY, kNoPlace};
+#pragma unroll 1
+      for (int i = tid; i < all; i += kJoinThreads) {
+        const Cand c = value(i, keys[i]);
+        if (before(last, c) && before(c, best)) best = c;
       }
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) {
@@ -278,27 +300,33 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
       }
       if (lane == 0) w_best[w] = best;
       __syncthreads();
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < NW; ++i)
         if (before(w_best[i], best)) best = w_best[i];
-      if (threadIdx.x == 0) put(k, best);
+      if (tid == 0) put(k, best);
       last = best;
       __syncthreads();
     }
-    if (threadIdx.x == 0) found = a.keep;
+    return;
   }
+  for (int i = tid / kRankLanes; i < n; i += kJoinThreads / kRankLanes) {
+    const Cand c = list[i];
+    int place = 0;
+    for (int j = tid % kRankLanes; j < n; j += kRankLanes) place += before(list[j], c);
+    place = rank_sum(place);
+    if (place < a.keep && tid % kRankLanes == 0) put(place, c);
+  }
+  if (n >= a.keep) return;
+  // the others are -inf, at the lowest places that are not among the chosen
   __syncthreads();
-  // fewer than `keep`: the others are -inf, the lowest places that are not among the chosen
-  const int f = found;
-  if (f < a.keep && threadIdx.x == 0) {
-    int64_t at = 0;
-    for (int k = f; k < a.keep; ++at) {
-      bool taken = false;
-      for (int j = 0; j < f; ++j) taken |= chosen[j] == at;
-      if (taken) continue;
-      put(k, Cand{-(double)INFINITY, at});
-      ++k;
-    }
+  if (tid != 0) return;
+  int at = 0;
+#pragma unroll 1
+  for (int k = n; k < a.keep; ++at) {
+    bool taken = false;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) taken |= chosen[j] == at;
+    if (!taken) put(k++, Cand{-(double)INFINITY, at});
   }
 }
 
