@@ -204,12 +204,14 @@ def _stream(dev):
 
 
 _NO_GUARD = contextlib.nullcontext()
+# (torch.cuda.current_device looks first whether torch has initialized the GPU: 0.3 us of a call)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _on(dev):
     """The launch's device made current where it is not (a kernel goes to the current device's queue of
     modules, whatever stream it is given)."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _NO_GUARD if _current_device() == dev.index else torch.cuda.device(dev)
 
 
 _has_storage, _transforms = torch._C._has_storage, torch._C._are_functorch_transforms_active
@@ -678,52 +680,64 @@ def _table_ld(tables, rows=None):
 def _page_strides(name, t, dims, written):
     """The strides of pages [..., N, P, HK, D] with a dense head dim (a dimension of one element has any); those
     that are written must not overlap."""
-    if t.dim() != dims:
-        raise EsepError(f"{name} must be {'[L, N, P, HK, D]' if dims == 5 else '[N, P, HK, D]'}, got {list(t.shape)}")
-    *strides, last = t.stride()
-    if last != 1:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != dims:
+        raise EsepError(f"{name} must be {'[L, N, P, HK, D]' if dims == 5 else '[N, P, HK, D]'}, got {list(shape)}")
+    if 1 not in shape:
+        if t.is_contiguous():
+            return strides[:-1]
+        if not written and strides[-1] == 1:
+            return strides[:-1]
+    if strides[-1] != 1:
         raise EsepError(f"{name} needs a unit stride on the head dim")
-    out = [st if n > 1 else 0 for st, n in zip(strides, t.shape)]
+    out = [st if n > 1 else 0 for st, n in zip(strides, shape[:-1])]
     if written:
-        at = t.shape[-1]
-        for st, n in sorted((st, n) for st, n in zip(out, t.shape) if n > 1):
+        at = shape[-1]
+        for st, n in sorted((st, n) for st, n in zip(out, shape) if n > 1):
             if st < at:
-                raise EsepError(f"elements of {name} overlap (strides {t.stride()})")
+                raise EsepError(f"elements of {name} overlap (strides {strides})")
             at = st * n
     return out
 
 
+_HALVES = (torch.float16, torch.bfloat16)
+
+
 def _pages_pair(k_pages, v_pages, dims, written):
-    shape = k_pages.shape
-    if v_pages.shape != shape or v_pages.dtype != k_pages.dtype or k_pages.dtype not in (torch.float16, torch.bfloat16):
-        raise EsepError(f"k_pages and v_pages must be fp16 or bf16 of one shape, got {k_pages.dtype} {list(shape)} "
+    """Both pages' strides, one array of C integers."""
+    shape, dt = k_pages.shape, k_pages.dtype
+    if v_pages.shape != shape or v_pages.dtype != dt or dt not in _HALVES:
+        raise EsepError(f"k_pages and v_pages must be fp16 or bf16 of one shape, got {dt} {list(shape)} "
                         f"and {v_pages.dtype} {list(v_pages.shape)}")
-    if max(shape, default=0) > 0x7FFFFFFF:
+    strides = array("q", (*_page_strides("k_pages", k_pages, dims, written),
+                          *_page_strides("v_pages", v_pages, dims, written)))
+    if shape[-4] * shape[-3] > 0x7FFFFFFF or shape[-2] * shape[-1] > 0x7FFFFFFF or shape[0] > 0x7FFFFFFF:
         raise EsepError(f"pages of {list(shape)}: the library counts in 32 bits")
-    return array("q", _page_strides("k_pages", k_pages, dims, written)
-                 + _page_strides("v_pages", v_pages, dims, written))
+    return strides
 
 
-def page_tables(tables, lengths, new, free, taken, slots, positions, cu, lengths_out, taken_out, page,
-                name="_page_tables"):
-    """Places of `new` more tokens a row (esep_page_tables): tables int32 [B, M] extended in place; slots and
-    positions int32 [total], cu int32 [B + 1]; lengths_out and taken_out may be lengths and taken."""
-    dev = _dev(tables, lengths, new, free, taken, slots, positions, cu, lengths_out, taken_out)
+def page_tables(tables, lengths, new, free, taken, page, total, update, name="_page_tables"):
+    """Places of `new` more tokens a row (esep_page_tables): tables int32 [B, M] extended in place, with update lengths
+    and taken too. Returns (slots [total], positions [total], cu [B + 1], lengths, taken)."""
+    dev = _dev(tables, lengths, new, free, taken)
     B, M, ld = _table_ld(tables)
-    total = slots.numel()
-    if M > 0x7FFFFFFF or B > 0x7FFFFFFF or free.numel() > 0x7FFFFFFF or total > 0x7FFFFFFF or page > 0x7FFFFFFF:
-        raise EsepError(f"page_tables: bad sizes B={B} M={M} F={free.numel()} page={page} total={total}")
-    _int32("lengths", lengths, B), _int32("new", new, B), _int32("taken", taken, 1)
-    _int32("free", free, free.numel())
-    _int32("slots", slots, total), _int32("positions", positions, total), _int32("cu_seqlens", cu, B + 1)
-    _int32("lengths_out", lengths_out, B), _int32("taken_out", taken_out, 1)
+    F = free.numel()
+    if M > 0x7FFFFFFF or B > 0x7FFFFFFF or F > 0x7FFFFFFF:
+        raise EsepError(f"page_tables: bad sizes B={B} M={M} F={F}")
+    _int32("lengths", lengths, B), _int32("new", new, B), _int32("taken", taken, 1), _int32("free", free, F)
+    sizes = [total, total, B + 1] if update else [total, total, B + 1, B, 1]
+    out = torch.empty(sum(sizes), device=dev, dtype=torch.int32)
+    at = out.data_ptr()
+    cu = at + 8 * total
+    lens, took = (lengths.data_ptr(), taken.data_ptr()) if update else (cu + 4 * (B + 1), cu + 4 * (2 * B + 1))
     with _on(dev):
         rc = lib().esep_page_tables(
-            tables.data_ptr(), ld, lengths.data_ptr(), new.data_ptr(), free.data_ptr(), taken.data_ptr(),
-            slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lengths_out.data_ptr(), taken_out.data_ptr(), B, M,
-            free.numel(), page, total, _stream(dev))
+            tables.data_ptr(), ld, lengths.data_ptr(), new.data_ptr(), free.data_ptr(), taken.data_ptr(), at,
+            at + 4 * total, cu, lens, took, B, M, F, page, total, _stream(dev))
     _check(rc, "esep_page_tables")
     _record(name)
+    out = out.split_with_sizes(sizes)
+    return (*out, lengths, taken) if update else out
 
 
 def page_store(k, v, k_pages, v_pages, slots, name="_page_store"):

@@ -47,15 +47,8 @@ def block_tables(tables, lengths, new, free, taken, page, total, update=False):
     new `taken` is more than F. With update, lengths and taken are changed in place, else they are left
     and the same call can be made again."""
     page, total = _whole("page", page, 1), _whole("total", total, 0)
-    _hip.refuse_recorded("block_tables", tables, lengths, new, free, taken)
-    B = lengths.shape[0] if lengths.dim() == 1 else -1
-    if B < 0:
-        raise _hip.EsepError(f"lengths must be int32 [B], got {list(lengths.shape)}")
-    sizes = [total, total, B + 1] if update else [total, total, B + 1, B, 1]
-    out = torch.empty(sum(sizes), device=lengths.device, dtype=torch.int32).split_with_sizes(sizes)
-    plan = PagePlan(*out, lengths, taken) if update else PagePlan(*out)
-    _hip.page_tables(tables, lengths, new, free, taken, *plan, page)
-    return plan
+    _hip.refuse_recorded("block_tables", tables)
+    return PagePlan(*_hip.page_tables(tables, lengths, new, free, taken, page, total, update))
 
 
 def paged_store(k, v, k_pages, v_pages, slots):

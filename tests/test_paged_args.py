@@ -228,6 +228,10 @@ def test_shapes_and_types_are_refused(monkeypatch):
         tables(torch.zeros(1, 4, dtype=torch.int32)[:, ::2], I1, I1, I1, I1)
     with pytest.raises(E, match="lengths"):
         tables(TAB, I1.long(), I1, I1, I1)
+    with pytest.raises(E, match="lengths"):
+        tables(TAB, I1[0], I1, I1, I1)
+    with pytest.raises(E, match="lengths"):
+        tables(TAB, two, two, I1, I1)
     with pytest.raises(E, match="new"):
         tables(TAB, I1, two, I1, I1)
     with pytest.raises(E, match="taken"):
