@@ -657,9 +657,12 @@ def attn_cache_workspace(B, n, S, HQ, HK, D, window=None, sinks=0):
                                                int(sinks)))
 
 
+_INT32, _HALVES = torch.int32, (torch.float16, torch.bfloat16)
+
+
 def _int32(name, t, *shape):
     """t, an int32 tensor of this shape, contiguous."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype != _INT32 or t.shape != shape or not t.is_contiguous():
         raise EsepError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} "
                         f"{list(t.shape)}")
     return t
@@ -667,14 +670,15 @@ def _int32(name, t, *shape):
 
 def _table_ld(tables, rows=None):
     """(rows, M, row stride) of a block table [rows, M] with a unit column stride."""
-    if tables.dtype != torch.int32 or tables.dim() != 2 or (rows is not None and tables.shape[0] != rows):
+    shape = tables.shape
+    if tables.dtype != _INT32 or len(shape) != 2 or (rows is not None and shape[0] != rows):
         raise EsepError(f"tables must be int32 [{'B' if rows is None else rows}, M], got {tables.dtype} "
-                        f"{list(tables.shape)}")
-    B, M = tables.shape
+                        f"{list(shape)}")
+    B, M = shape
     ld, col = tables.stride()
-    if M > 1 and col != 1:
+    if col != 1 and M > 1:
         raise EsepError("tables need a unit stride along a row")
-    return B, M, max(ld, M) if B <= 1 else ld
+    return B, M, ld if B > 1 else max(ld, M)
 
 
 def _page_strides(name, t, dims, written):
@@ -700,9 +704,6 @@ def _page_strides(name, t, dims, written):
     return out
 
 
-_HALVES = (torch.float16, torch.bfloat16)
-
-
 def _pages_pair(k_pages, v_pages, dims, written):
     """Both pages' strides, one array of C integers."""
     shape, dt = k_pages.shape, k_pages.dtype
@@ -711,8 +712,9 @@ def _pages_pair(k_pages, v_pages, dims, written):
                         f"and {v_pages.dtype} {list(v_pages.shape)}")
     strides = array("q", (*_page_strides("k_pages", k_pages, dims, written),
                           *_page_strides("v_pages", v_pages, dims, written)))
-    if shape[-4] * shape[-3] > 0x7FFFFFFF or shape[-2] * shape[-1] > 0x7FFFFFFF or shape[0] > 0x7FFFFFFF:
-        raise EsepError(f"pages of {list(shape)}: the library counts in 32 bits")
+    for n in shape:
+        if n > 0x7FFFFFFF:
+            raise EsepError(f"pages of {list(shape)}: the library counts in 32 bits")
     return strides
 
 

@@ -98,7 +98,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, scale=None, window=Non
     q4 = q.unsqueeze(1) if q.dim() == 3 else q
     if q4.dim() == 4 and _unaligned(q4):
         q4 = _copy(q4)
-    o = torch.empty(q4.shape, device=q.device, dtype=q.dtype)
+    o = torch.empty_like(q4, memory_format=torch.contiguous_format)
     _hip.attn_paged(q4, k_pages, v_pages, o, tables, lengths, scale, window, sinks, beams, shared)
     return o.squeeze(1) if q.dim() == 3 else o
 

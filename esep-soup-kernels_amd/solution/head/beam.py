@@ -32,7 +32,7 @@ def beam_select(logits, scores, keep=None):
     _hip.refuse_recorded("beam_select", logits, scores)
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
-    out = torch.empty((R, keep), device=logits.device, dtype=torch.float32)
-    parents, tokens = torch.empty((2, R, keep), device=logits.device, dtype=torch.int32).unbind(0)
+    parents, tokens, out = torch.empty((3, R, keep), device=logits.device, dtype=torch.int32).unbind(0)
+    out = out.view(torch.float32)
     _hip.beam_select(logits, scores.contiguous(), out, parents, tokens)
     return out, parents, tokens
