@@ -308,18 +308,21 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnP
   }
 }
 
-// The groups that were cut or share keys, and zeros for the rows without tokens: one block per query row. A lane adds two
-// columns over every GROUPS-th part with a running maximum, so that the parts are read once.
-template <typename T, int D, int THREADS, bool SHARED>
+// The groups that were cut or share keys, and zeros for the rows without tokens. A lane adds two columns of a query row
+// over every GROUPS-th part with a running maximum, so that the parts are read once; a block has as many rows as
+// its threads hold.
+template <typename T, int D, int THREADS, int GROUPS, bool SHARED>
 __global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs a) {
-  constexpr int PAIRS = D / 2, GROUPS = THREADS / PAIRS;
+  constexpr int PAIRS = D / 2, ROWS = THREADS / PAIRS / GROUPS;
+  static_assert(ROWS == 1 || GROUPS == 1, "rows of a block do not wait for each other");
   __shared__ float2 sums[GROUPS][PAIRS];
   __shared__ float2 stat[GROUPS];  // maximum, sum
   const int G = a.HQ / a.HK, rows = G * a.n, all_rows = SHARED ? a.W * rows : rows;
   const int RT = (rows + 31) / 32, CT = (all_rows + 31) / 32, live = all_rows < 32 ? all_rows : 32;
-  const int rg = (int)(blockIdx.x % rows);
-  const int kvh = (int)(blockIdx.x / rows % a.HK), b = (int)(blockIdx.x / rows / a.HK);
-  const int g = threadIdx.x / PAIRS, c = threadIdx.x % PAIRS;
+  const int g = ROWS > 1 ? 0 : threadIdx.x / PAIRS, c = threadIdx.x % PAIRS;
+  const int row = ROWS > 1 ? (int)(blockIdx.x * ROWS + threadIdx.x / PAIRS) : (int)blockIdx.x;
+  if (ROWS > 1 && row >= a.B * a.HK * rows) return;
+  const int rg = row % rows, kvh = row / rows % a.HK, b = row / rows / a.HK;
   T* out = static_cast<T*>(a.o) + (((int64_t)b * a.n + rg / G) * a.HQ + kvh * G + rg % G) * D + 2 * c;
   if (paged_len(a, b) <= 0) {
     if (g == 0) out[0] = out[1] = (T)0.f;
@@ -357,41 +360,52 @@ __global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs
     acc.y = fmaf(w1, v.y, w0 * acc.y);
     m = top;
   }
-  sums[g][c] = acc;
-  if (c == 0) stat[g] = make_float2(m, l);
-  __syncthreads();
-  if (g != 0) return;
-  float top = -INFINITY;
+  if constexpr (GROUPS > 1) {
+    sums[g][c] = acc;
+    if (c == 0) stat[g] = make_float2(m, l);
+    __syncthreads();
+    if (g != 0) return;
+    m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, stat[i].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float den = 0.f;
-  acc = make_float2(0.f, 0.f);
+    for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, stat[i].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    acc = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const float w = exp2_fast(stat[i].x - ref);
-    den = fmaf(w, stat[i].y, den);
-    acc.x = fmaf(w, sums[i][c].x, acc.x);
-    acc.y = fmaf(w, sums[i][c].y, acc.y);
+    for (int i = 0; i < GROUPS; ++i) {
+      const float w = exp2_fast(stat[i].x - ref);
+      l = fmaf(w, stat[i].y, l);
+      acc.x = fmaf(w, sums[i][c].x, acc.x);
+      acc.y = fmaf(w, sums[i][c].y, acc.y);
+    }
   }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
   out[0] = (T)(acc.x * inv);
   out[1] = (T)(acc.y * inv);
 }
 
+// Wavefronts to a group up to which a row's few parts are added by one lane each, so that a block joins 256 / (D / 2)
+// rows (256 rows of up to 300 tokens, 28 / 4 heads of 128: 38 -> 32 us in all; with it up to 8 wavefronts to a group
+// 32 rows of 4 beams over up to 8000 shared tokens 35.3 -> 38.5).
+constexpr int64_t kPagedFewParts = 2;
+
 template <typename T, int D, bool SHARED>
 hipError_t run(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
-  const dim3 grid((unsigned)(z.units > 0 ? z.units : 1)), rows((unsigned)(a.B * a.HQ * a.n));
+  const dim3 grid((unsigned)(z.units > 0 ? z.units : 1));
   if (D == 128 && z.all_tiles == 1)
     hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED>), grid, dim3(64), 0, s, a);
   else
     hipLaunchKernelGGL((k_attn_paged<T, D, false, SHARED>), grid, dim3(64), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (z.units > kCacheManyParts * z.groups && rows.x <= 256)
-    hipLaunchKernelGGL((k_attn_paged_join<T, D, 1024, SHARED>), rows, dim3(1024), 0, s, a);
+  const unsigned rows = (unsigned)(a.B * a.HQ * a.n);
+  constexpr unsigned per = 256 / (D / 2);
+  if (z.units > kCacheManyParts * z.groups && rows <= 256)
+    hipLaunchKernelGGL((k_attn_paged_join<T, D, 1024, 2048 / D, SHARED>), dim3(rows), dim3(1024), 0, s, a);
+  else if (z.units > kPagedFewParts * z.groups)
+    hipLaunchKernelGGL((k_attn_paged_join<T, D, 256, 512 / D, SHARED>), dim3(rows), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((k_attn_paged_join<T, D, 256, SHARED>), rows, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_attn_paged_join<T, D, 256, 1, SHARED>), dim3((rows + per - 1) / per), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

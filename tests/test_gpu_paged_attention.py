@@ -164,6 +164,26 @@ def test_more_groups_than_wavefronts():
     _check(paged_attention(q, kp, vp, tables, _i(lengths)), ref, tol, "groups")
 
 
+@pytest.mark.parametrize("beams", [1, 3])
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_rows_than_wavefronts(D, beams):
+    """Rows of one or two parts, joined several to a block, their number no multiple of those."""
+    from solution.body.paged import paged_attention
+
+    rng = random.Random(D)
+    rows, HQ, HK = 699, 3, 3
+    lengths = [rng.choice([0, 1, 31, 65, 40 + rng.randrange(200)]) for _ in range(rows // beams) for _ in range(beams)]
+    shared = [rng.choice([0, n // 16 * 16]) for n in lengths[::beams]]
+    q, k, v = _inputs(rows, 1, 240, HQ, HK, D, torch.float16, 6)
+    for b in range(rows):
+        s = shared[b // beams]
+        k[b, :s], v[b, :s] = k[b // beams * beams, :s].clone(), v[b // beams * beams, :s].clone()
+    kp, vp, tables = _scatter(k, v, lengths, 16, rng, shared=shared if beams > 1 else None, beams=beams)
+    ref, tol = _reference(q, k, v, lengths, D ** -0.5, None, 0, 2.0 ** -11, 2.0 ** -25)
+    o = paged_attention(q, kp, vp, tables, _i(lengths), beams=beams, shared=_i(shared))
+    _check(o, ref, tol, "rows")
+
+
 def test_long_runs():
     """A wavefront's run is longer than the 32 tiles whose pages it reads at once."""
     from solution.body.paged import paged_attention
