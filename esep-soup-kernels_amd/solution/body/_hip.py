@@ -812,38 +812,37 @@ def attn_paged_workspace(B, n, M, page, HQ, HK, D, window=None, sinks=0, beams=1
                                                int(sinks), beams, int(shared)))
 
 
-def beam_select(logits, scores, out_scores, parents, tokens, workspace=None, name="_beam_select"):
-    """The greatest of scores [R, W] fp32 + log softmax of logits [R, W, V] of each request, as many as the outputs
-    [R, keep] (fp32, int32, int32) hold (esep_beam_select). `workspace` is a contiguous uint8 tensor of >=
+def beam_select(logits, scores, keep, workspace=None, name="_beam_select"):
+    """The `keep` greatest of scores [R, W] fp32 + log softmax of logits [R, W, V] of each request (esep_beam_select):
+    (scores fp32, parents int32, tokens int32) [R, keep]. `workspace` is a contiguous uint8 tensor of >=
     beam_select_workspace's bytes (allocated here when not given)."""
-    dev = _dev(logits, scores, out_scores, parents, tokens, workspace)
-    if logits.dim() != 3:
-        raise EsepError(f"logits must be [R, W, V], got {list(logits.shape)}")
-    R, W, V = logits.shape
-    if V > 1 and logits.stride(2) != 1:
+    dev = _dev(logits, scores, workspace)
+    shape = logits.shape
+    if len(shape) != 3:
+        raise EsepError(f"logits must be [R, W, V], got {list(shape)}")
+    R, W, V = shape
+    ld_r, ld_w, col = logits.stride()
+    if V > 1 and col != 1:
         raise EsepError("logits need a unit stride along the vocabulary")
     if scores.dtype != torch.float32 or scores.shape != (R, W) or not scores.is_contiguous():
         raise EsepError(f"scores must be a contiguous fp32 tensor of shape {[R, W]}")
-    if R > 0x7FFFFFFF or W > 0x7FFFFFFF:
-        raise EsepError(f"beam_select: bad sizes R={R} W={W}")
-    keep = out_scores.shape[-1]
-    if out_scores.dtype != torch.float32 or out_scores.shape != (R, keep) or not out_scores.is_contiguous():
-        raise EsepError("out_scores must be a contiguous fp32 tensor [R, keep]")
-    _int32("parents", parents, R, keep), _int32("tokens", tokens, R, keep)
-    if keep > 0x7FFFFFFF:
-        raise EsepError(f"beam_select: bad sizes keep={keep}")
-    need = beam_select_workspace(R, W, V, keep)
+    if R > 0x7FFFFFFF or W > 0x7FFFFFFF or keep > 0x7FFFFFFF:
+        raise EsepError(f"beam_select: bad sizes R={R} W={W} keep={keep}")
+    need = lib().esep_beam_select_workspace(R, W, V, keep)
     if workspace is None:
         workspace = torch.empty(max(need, 8), device=dev, dtype=torch.uint8)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
         raise EsepError(f"workspace must be a contiguous uint8 tensor of >= {need} elements")
+    out = torch.empty((3, R, keep), device=dev, dtype=torch.int32)
+    at, step = out.data_ptr(), 4 * R * keep
     with _on(dev):
         rc = lib().esep_beam_select(
-            logits.data_ptr(), logits.stride(0) if R > 1 else 0, logits.stride(1) if W > 1 else 0, scores.data_ptr(),
-            workspace.data_ptr(), out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-            dtype_code(logits.dtype), R, W, V, keep, _stream(dev))
+            logits.data_ptr(), ld_r if R > 1 else 0, ld_w if W > 1 else 0, scores.data_ptr(), workspace.data_ptr(), at,
+            at + step, at + 2 * step, dtype_code(logits.dtype), R, W, V, keep, _stream(dev))
     _check(rc, "esep_beam_select")
     _record(name)
+    best, parents, tokens = out.unbind(0)
+    return best.view(torch.float32), parents, tokens
 
 
 def beam_select_workspace(R, W, V, keep):

@@ -1,8 +1,6 @@
 """Beam search's selection over the vocabulary, on the HIP kernels (esep_beam_select): what answering with several
 beams does with the head's logits. No reference counterpart (the reference trains)."""
 
-import torch
-
 from ..body import _hip
 from ..body.attention import _whole
 
@@ -32,7 +30,4 @@ def beam_select(logits, scores, keep=None):
     _hip.refuse_recorded("beam_select", logits, scores)
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
-    parents, tokens, out = torch.empty((3, R, keep), device=logits.device, dtype=torch.int32).unbind(0)
-    out = out.view(torch.float32)
-    _hip.beam_select(logits, scores.contiguous(), out, parents, tokens)
-    return out, parents, tokens
+    return _hip.beam_select(logits, scores.contiguous(), keep)
