@@ -21,9 +21,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kList = 512;
 
-// A float's bits in the order of the floats (-inf lowest but for NaN, which does not come here).
+// A float's bits in the order of the floats, -0 as 0 (-inf lowest but for NaN, which does not come here).
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t k) {
@@ -41,18 +41,25 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
 }
 
-// A bound that at least `keep` of the wavefront's lanes reach with v; -inf where fewer have more than that.
-__device__ __forceinline__ float wave_bound(float v, int keep) {
-  int n = 0;
-  float bound = -INFINITY;
-  while (n < keep) {
-    bound = wave_max(v);
-    if (bound == -INFINITY) break;
-    const uint64_t at = __ballot(v == bound);
-    n += (int)__popcll(at);
-    if (v == bound) v = -INFINITY;
+// A bound that at least `keep` of the wavefront's lanes reach with their keys, and of the values with these first 20 bits the
+// greatest: bit by bit, the lanes at or above it counted. 0 where fewer lanes have a finite value.
+constexpr int kBoundBits = 20;
+__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int keep) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 32 - kBoundBits; --bit) {
+    const uint32_t t = bound | 1u << bit;
+    if (__popcll(__ballot(key >= t)) >= keep) bound = t;
   }
   return bound;
+}
+// The greatest of what lane l of each wavefront has put into v (after a barrier): 64 groups of the block's threads.
+template <int NW>
+__device__ __forceinline__ float group_max(const float (&v)[NW * 64], int lane) {
+  float m = v[lane];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, v[64 * i + lane]);
+  return m;
 }
 
 // Lanes that count a listed candidate's betters together, and their sum, in each of them.
@@ -68,7 +75,7 @@ __device__ __forceinline__ int rank_sum(int v) {
 template <typename T, int U, bool VEC>
 __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   constexpr int NW = kBeamThreads / 64;
-  __shared__ float w_max[NW], w_sum[NW], w_bound[NW];
+  __shared__ float w_sum[NW], best[kBeamThreads];
   __shared__ uint64_t list[kList];
   __shared__ uint64_t w_best[NW];
   __shared__ int count;
@@ -100,16 +107,10 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < 8; ++e) mine = fmaxf(mine, v[u][e]);  // NaN is passed over
-  const float wm = wave_max(mine);
-  const float wb = wave_bound(mine, a.keep);
-  if (lane == 0) {
-    w_max[w] = wm;
-    w_bound[w] = wb;
-  }
+  best[threadIdx.x] = mine;
   __syncthreads();
-  float top = w_max[0], bound = w_bound[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) top = fmaxf(top, w_max[i]), bound = fmaxf(bound, w_bound[i]);
+  const float group = group_max<NW>(best, lane), top = wave_max(group);
+  const uint32_t bound = wave_bound(ordered(group), a.keep);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
@@ -118,15 +119,14 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
     for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f((v[u][e] - ref) * kLog2e);
   sum = wave_sum(sum);
   if (lane == 0) w_sum[w] = sum;
-  auto key = [&](int u, int e) {  // -0 counts as 0
-    const float f = v[u][e] == 0.f ? 0.f : v[u][e];
-    return (uint64_t)ordered(f) << 32 | (uint32_t)~(base + 2048 * u + e);
+  auto key = [&](int u, int e) {
+    return (uint64_t)ordered(v[u][e]) << 32 | (uint32_t)~(base + 2048 * u + e);
   };
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (v[u][e] >= bound && v[u][e] > -INFINITY) {
+      if (ordered(v[u][e]) >= bound && v[u][e] > -INFINITY) {
         const int at = atomicAdd(&count, 1);
         if (at < kList) list[at] = key(u, e);
       }
@@ -195,20 +195,23 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   __shared__ double rest[kJoinMostBeams], score[kJoinMostBeams];
   __shared__ float tops[kJoinMostBeams];
   __shared__ Cand list[kList], w_best[NW];
-  __shared__ float w_bound[NW];
+  __shared__ float group[kJoinThreads];
   __shared__ int chosen[kBeamMostKeep];
   __shared__ int count;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = wave_id();
   const int per = a.splits * a.keep, all = a.W * per;
   const uint64_t* keys = a.cand + (int64_t)r * all;
+  // Candidate j of the thread: each 64 of them turned by one lane more, as a piece's lie there in their order, and 64 groups
+  // of lanes of which some hold the pieces' first and others their last would bound nothing.
+  auto index = [&](int j) {
+    const int chunk = j * NW + w;
+    return 64 * chunk + ((lane + chunk) & 63);
+  };
   // everything is asked for at once: the thread's first candidates, the pieces' parts (those of a beam that is out hold
   // nothing, and are not used)
   uint64_t key[kJoinFirst];
 #pragma unroll
-  for (int j = 0; j < kJoinFirst; ++j) {
-    const int i = tid + j * kJoinThreads;
-    key[j] = i < all ? keys[i] : 0;
-  }
+  for (int j = 0; j < kJoinFirst; ++j) key[j] = index(j) < all ? keys[index(j)] : 0;
   if (tid == 0) count = 0;
 #pragma unroll 1
   for (int b = w; b < a.W; b += NW) {
@@ -251,21 +254,19 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   float best32 = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kJoinFirst; ++j) {
-    const int i = tid + j * kJoinThreads;
-    mine[j] = value(i < all ? i : 0, key[j]);
+    mine[j] = value(index(j) < all ? index(j) : 0, key[j]);
     best32 = fmaxf(best32, (float)mine[j].value);
   }
-  constexpr int kRest = kJoinFirst * kJoinThreads;
+  const int rounds = (all + kJoinThreads - 1) / kJoinThreads;
+  auto later = [&](int j) { return index(j) < all ? value(index(j), keys[index(j)]) : Cand{-(double)INFINITY, kNoPlace}; };
 #pragma unroll 1
-  for (int i = tid + kRest; i < all; i += kJoinThreads) best32 = fmaxf(best32, (float)value(i, keys[i]).value);
-  const float wb = wave_bound(best32, a.keep);
-  if (lane == 0) w_bound[w] = wb;
+  for (int j = kJoinFirst; j < rounds; ++j) best32 = fmaxf(best32, (float)later(j).value);
+  group[tid] = best32;
   __syncthreads();
-  float bound = w_bound[lane < NW ? lane : 0];
-  bound = wave_max(bound);
+  const uint32_t bound = wave_bound(ordered(group_max<NW>(group, lane)), a.keep);
   // by value in 32 bits (rounding keeps the order): what reaches the bound
   auto enter = [&](const Cand& c) {
-    if (c.at != kNoPlace && (float)c.value >= bound) {
+    if (c.at != kNoPlace && ordered((float)c.value) >= bound) {
       const int at = atomicAdd(&count, 1);
       if (at < kList) list[at] = c;
     }
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
 #pragma unroll
   for (int j = 0; j < kJoinFirst; ++j) enter(mine[j]);
 #pragma unroll 1
-  for (int i = tid + kRest; i < all; i += kJoinThreads) enter(value(i, keys[i]));
+  for (int j = kJoinFirst; j < rounds; ++j) enter(later(j));
   __syncthreads();
   auto put = [&](int place, const Cand& c) {
     const int o = r * a.keep + place, b = c.at / a.V;
@@ -289,8 +290,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
     for (int k = 0; k < a.keep; ++k) {
       Cand best{-(double)INFINITY, kNoPlace};
 #pragma unroll 1
-      for (int i = tid; i < all; i += kJoinThreads) {
-        const Cand c = value(i, keys[i]);
+      for (int j = 0; j < rounds; ++j) {
+        const Cand c = later(j);
         if (before(last, c) && before(c, best)) best = c;
       }
 #pragma unroll
