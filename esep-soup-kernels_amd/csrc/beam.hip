@@ -53,6 +53,8 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int keep) {
   }
   return bound;
 }
+// It as a float, at least the lowest finite one.
+__device__ __forceinline__ float bound_of(uint32_t key) { return unordered(key < 0x00800000u ? 0x00800000u : key); }
 // The greatest of what lane l of each wavefront has put into v (after a barrier): 64 groups of the block's threads.
 template <int NW>
 __device__ __forceinline__ float group_max(const float (&v)[NW * 64], int lane) {
@@ -87,30 +89,43 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   const int base = split * a.piece + 8 * (int)threadIdx.x;
   float v[U][8];
   if (threadIdx.x == 0) count = 0;
+  // all of it is asked for at once: what lies past the row is read at its begin and replaced
+  if constexpr (VEC) {
+    Raw<T> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const u32x4* at = reinterpret_cast<const u32x4*>(x + (base + 2048 * u < a.V ? base + 2048 * u : 0));
+      raw[u].a = at[0];
+      if constexpr (sizeof(T) == 4) raw[u].b = at[1];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Buf<T>::unpack(raw[u], v[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] = base + 2048 * u < a.V ? v[u][e] : -INFINITY;  // V is a multiple of 8
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = base + 2048 * u + e;
+        const float f = (float)x[i < a.V ? i : 0];
+        v[u][e] = i < a.V ? f : -INFINITY;
+      }
+  }
+  float mine = -INFINITY, run[U];  // the greatest of all, of each eight; NaN is passed over
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = base + 2048 * u;
-    if constexpr (VEC) {
-      if (i < a.V) {  // whole: V is a multiple of 8
-        Chunk<T>::load(x + i, v[u]);
-      } else {
+    run[u] = v[u][0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] = -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[u][e] = i + e < a.V ? (float)x[i + e] : -INFINITY;
-    }
+    for (int e = 1; e < 8; ++e) run[u] = fmaxf(run[u], v[u][e]);
+    mine = fmaxf(mine, run[u]);
   }
-  float mine = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, v[u][e]);  // NaN is passed over
   best[threadIdx.x] = mine;
   __syncthreads();
   const float group = group_max<NW>(best, lane), top = wave_max(group);
-  const uint32_t bound = wave_bound(ordered(group), a.keep);
+  const float bound = bound_of(wave_bound(ordered(group), a.keep));
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
@@ -122,14 +137,26 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   auto key = [&](int u, int e) {
     return (uint64_t)ordered(v[u][e]) << 32 | (uint32_t)~(base + 2048 * u + e);
   };
+  if (mine >= bound) {
+    int n = 0;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
+      if (run[u] >= bound) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (ordered(v[u][e]) >= bound && v[u][e] > -INFINITY) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kList) list[at] = key(u, e);
+        for (int e = 0; e < 8; ++e) n += v[u][e] >= bound;
       }
+    int at = atomicAdd(&count, n);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (run[u] >= bound) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (v[u][e] >= bound) {
+            if (at < kList) list[at] = key(u, e);
+            ++at;
+          }
+      }
+  }
   __syncthreads();
   const int64_t part = (int64_t)row * a.splits + split;
   if (threadIdx.x == 0) {
@@ -263,10 +290,10 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   for (int j = kJoinFirst; j < rounds; ++j) best32 = fmaxf(best32, (float)later(j).value);
   group[tid] = best32;
   __syncthreads();
-  const uint32_t bound = wave_bound(ordered(group_max<NW>(group, lane)), a.keep);
+  const float bound = bound_of(wave_bound(ordered(group_max<NW>(group, lane)), a.keep));
   // by value in 32 bits (rounding keeps the order): what reaches the bound
   auto enter = [&](const Cand& c) {
-    if (c.at != kNoPlace && ordered((float)c.value) >= bound) {
+    if ((float)c.value >= bound) {
       const int at = atomicAdd(&count, 1);
       if (at < kList) list[at] = c;
     }
