@@ -11,7 +11,17 @@
 // rows in common tiles of 32: K and V of the shared tokens are read once for all of them. Each row's own tokens
 // come in a walk of its own, and the join adds both.
 //
-// Bound by the bytes of K and V, and below a few MB by the launches' latency.
+// Bound by the bytes of K and V, and below a few MB by latency: where rows are short, one launch (k_attn_paged_solo) takes
+// the walk's and the join's place (the rule and both sides' times: attention_paged.hpp).
+//
+// Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.5 + 4.7 us (497 MB, 5.5
+// TB/s; a copy reaches 5.0, half of it writes); 8 requests of 4 beams over up to 8000 shared tokens and 130 each, pages of 16
+// 30.3 + 6.2 (96 MB; each beam on its own 4 times the bytes of the prompt); 5 new tokens over 7 rows through a window of
+// 1500, 14 / 2 heads of 64 13.1 + 3.9; one row of 700 tokens, 12 / 2 heads 9.0 in one launch (7.0 + 3.9 in two).
+// Without its products the walk of the beams takes 27.4 us, without its partials' stores 25.5; tried in vain: four wavefronts
+// to a block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us there, but 10.2 instead of 7.0 for the one row),
+// rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to three tiles to a
+// wavefront (-7% to +7% over twenty shapes), partials eight columns at a time (the join reads 32 bytes of a line).
 #include <cmath>
 
 #include "attention_cache.hpp"
@@ -161,10 +171,131 @@ struct PagedFill {
   }
 };
 
+// The query row of lane lq (of both halves) in tile rt of a kv head's `rows`: its batch row, token and head.
+struct PagedQuery {
+  int G, rows, b, tok, h;
+  bool ok;
+  __device__ __forceinline__ PagedQuery(const AttnPagedArgs& a, const PagedRow& row, int kvh, int rt, int lq) {
+    G = a.HQ / a.HK;
+    const int own = G * a.n, r = 32 * rt + lq;
+    rows = row.common ? a.W * own : own;
+    ok = r < rows;
+    const int q = ok ? r : 0;
+    b = row.b + q / own;
+    tok = q % own / G;
+    h = kvh * G + q % G;
+  }
+};
+
+// A wavefront's tiles t0 .. t1 - 1 of one group through its own ring: the lane's query row's maximum, sum and weighted
+// sums.
+template <typename T, int D, bool NT>
+__device__ __forceinline__ void paged_walk(const AttnPagedArgs& a, const PagedRow& row, const PagedQuery& at, int kvh,
+                                           int rt, int t0, int t1, const PagedFill<2 * D, NT>& fk,
+                                           const PagedFill<2 * D, NT>& fv, char (&kv)[2][2][32 * 2 * D], int lane,
+                                           float& m, float& l, f32x16 (&oacc)[D / 32]) {
+  using V8 = typename Mfma<T>::v8;
+  using Fill = PagedFill<2 * D, NT>;
+  const int hi = lane >> 5;
+  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (int64_t)kvh * a.k_hs);
+  const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (int64_t)kvh * a.v_hs);
+  const int32_t* table = a.tables + (int64_t)row.b * a.t_bs;
+  const int lo0 = row.lo & ~31;
+  auto start_of = [&](int t) { return t < row.ns ? 32 * t : lo0 + 32 * (t - row.ns); };
+  int ids = -1, ids0 = 0;  // lane l: the page of half l % 2 of tile ids0 + l / 2
+  auto load_ids = [&](int t) {
+    ids0 = t;
+    const int tl = t + lane / 2;
+    ids = -1;
+    if (tl < t1) {
+      const int from = tl < row.ns ? 0 : row.lo, to = tl < row.ns ? row.sink_hi : row.len;
+      int k = start_of(tl) + 16 * (lane & 1);
+      k = k < from ? from : (k < to ? k : to - 1);
+      ids = table[k >> a.page_shift];
+    }
+    asm volatile("" : "+v"(ids));  // here now: a wait for it in the loop would wait for the tiles in flight too
+  };
+  uint32_t bad = 0;  // bits 2 buffer + half: the page is none
+  // asks for tile t; false: it is there already, without a DMA
+  auto issue = [&](int t) {
+    if (t - ids0 >= 32) load_ids(t);
+    const int p0 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0));
+    const int p1 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0) + 1);
+    const int k0 = start_of(t), from = t < row.ns ? 0 : row.lo, to = t < row.ns ? row.sink_hi : row.len;
+    char* kd = kv[t & 1][0];
+    char* vd = kv[t & 1][1];
+    const uint32_t none = ((unsigned)p0 >= (unsigned)a.N ? 1u : 0u) | ((unsigned)p1 >= (unsigned)a.N ? 2u : 0u);
+    bad = (bad & ~(3u << (2 * (t & 1)))) | none << (2 * (t & 1));
+    if (none) {
+      fk.checked(kd, kbase, k0, from, to, p0, p1, a.N, lane);
+      fv.checked(vd, vbase, k0, from, to, p0, p1, a.N, lane);
+      return false;
+    }
+    if (k0 >= from && k0 + 32 <= to) {
+      fk.whole(kd, kbase, k0, p0, p1);
+      fv.whole(vd, vbase, k0, p0, p1);
+    } else {
+      fk.partial(kd, kbase, k0, from, to, p0, p1);
+      fv.partial(vd, vbase, k0, from, to, p0, p1);
+    }
+    return true;
+  };
+  // every read of the ring by the group before is done
+  __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+  load_ids(t0);
+  issue(t0);
+  if (t0 + 1 < t1) issue(t0 + 1);
+
+  V8 qb[D / 16];
+  {
+    const T* qrow = static_cast<const T*>(a.q) + (int64_t)at.b * a.q_bs + (int64_t)at.tok * a.q_ts +
+                    (int64_t)at.h * a.q_hs + 8 * hi;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) qb[c] = at.ok ? ld16<V8>(qrow + 16 * c) : V8{};
+  }
+  // positions: the lane's, and the tile's first and last
+  const int p0 = row.len - a.n, pos = at.ok ? p0 + at.tok : p0 + a.n - 1;
+  const int ufirst = p0 + 32 * rt / at.G;
+  const int ulast = 32 * rt + 31 < at.rows ? p0 + (32 * rt + 31) / at.G : p0 + a.n - 1;
+#pragma unroll
+  for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
+  m = -INFINITY;
+  l = 0.f;
+  // q and the first tiles are here (through the builtin: the compiler then waits for no load of its own
+  // within the loop, which would wait for the tile in flight too)
+  __builtin_amdgcn_s_waitcnt(kWaitVm0);
+  for (int t = t0; t < t1; ++t) {
+    // a window's tiles have no sinks (the first of them may begin among those)
+    const int kh = start_of(t), cap = t < row.ns ? row.sink_hi - 1 : 0x7fffffff;
+    const int sinks = t < row.ns || row.lo == 0 ? row.sink_hi : 0;
+    const char* ks = kv[t & 1][0];
+    const char* vs = kv[t & 1][1];
+    const uint32_t none = bad >> (2 * (t & 1)) & 3;
+    fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
+                       [&](f32x16& acc) __attribute__((always_inline)) {
+                         if (!row.common)
+                           mask_window(acc, kh, ufirst < cap ? ufirst : cap, ulast - a.window,
+                                       pos < cap ? pos : cap, pos - a.window, sinks, hi);
+                         if (none) {
+#pragma unroll
+                           for (int i = 0; i < 16; ++i)
+                             if (none >> (i / 8) & 1) acc[i] = -INFINITY;
+                         }
+                       });
+    // this tile's reads are done: its buffer takes tile t + 2; then tile t + 1 is waited for
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 2 < t1 && issue(t + 2))
+      __builtin_amdgcn_s_waitcnt(wait_vm(2 * Fill::N));
+    else
+      __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 template <typename T, int D, bool NT, bool SHARED>
 __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnPagedArgs a) {
   constexpr int RB = 2 * D, TILE = 32 * RB;
-  using V8 = typename Mfma<T>::v8;
   using Fill = PagedFill<RB, NT>;
   __shared__ __align__(1024) char kv[2][2][TILE];  // [buffer][K, V]
 
@@ -191,119 +322,108 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnP
       row = paged_row<SHARED>(a, ++e);
       here = e < R ? per_common : per;
     }
-    const int rows = row.common ? all_rows : own_rows, RT = here / a.HK;
+    const int RT = here / a.HK;
     const int gi = (x - first) / row.tiles;  // kv head and query tile
     const int g0 = first + gi * row.tiles;
     const int t0 = x - g0, t1 = x1 - g0 < row.tiles ? x1 - g0 : row.tiles;
     const int kvh = gi / RT, rt = gi % RT;
-    const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (int64_t)kvh * a.k_hs);
-    const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (int64_t)kvh * a.v_hs);
-    const int32_t* table = a.tables + (int64_t)row.b * a.t_bs;
-    const int lo0 = row.lo & ~31;
-    auto start_of = [&](int t) { return t < row.ns ? 32 * t : lo0 + 32 * (t - row.ns); };
-    int ids = -1, ids0 = 0;  // lane l: the page of half l % 2 of tile ids0 + l / 2
-    auto load_ids = [&](int t) {
-      ids0 = t;
-      const int tl = t + lane / 2;
-      ids = -1;
-      if (tl < t1) {
-        const int from = tl < row.ns ? 0 : row.lo, to = tl < row.ns ? row.sink_hi : row.len;
-        int k = start_of(tl) + 16 * (lane & 1);
-        k = k < from ? from : (k < to ? k : to - 1);
-        ids = table[k >> a.page_shift];
-      }
-      asm volatile("" : "+v"(ids));  // here now: a wait for it in the loop would wait for the tiles in flight too
-    };
-    uint32_t bad = 0;  // bits 2 buffer + half: the page is none
-    // asks for tile t; false: it is there already, without a DMA
-    auto issue = [&](int t) {
-      if (t - ids0 >= 32) load_ids(t);
-      const int p0 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0));
-      const int p1 = __builtin_amdgcn_readlane(ids, 2 * (t - ids0) + 1);
-      const int k0 = start_of(t), from = t < row.ns ? 0 : row.lo, to = t < row.ns ? row.sink_hi : row.len;
-      char* kd = kv[t & 1][0];
-      char* vd = kv[t & 1][1];
-      const uint32_t none = ((unsigned)p0 >= (unsigned)a.N ? 1u : 0u) | ((unsigned)p1 >= (unsigned)a.N ? 2u : 0u);
-      bad = (bad & ~(3u << (2 * (t & 1)))) | none << (2 * (t & 1));
-      if (none) {
-        fk.checked(kd, kbase, k0, from, to, p0, p1, a.N, lane);
-        fv.checked(vd, vbase, k0, from, to, p0, p1, a.N, lane);
-        return false;
-      }
-      if (k0 >= from && k0 + 32 <= to) {
-        fk.whole(kd, kbase, k0, p0, p1);
-        fv.whole(vd, vbase, k0, p0, p1);
-      } else {
-        fk.partial(kd, kbase, k0, from, to, p0, p1);
-        fv.partial(vd, vbase, k0, from, to, p0, p1);
-      }
-      return true;
-    };
-    // every read of the ring by the group before is done
-    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-    load_ids(t0);
-    issue(t0);
-    if (t0 + 1 < t1) issue(t0 + 1);
-
-    const int r = 32 * rt + lq;
-    const bool rok = r < rows;
-    const int rb = rok ? r : 0;  // its row, token and head
-    const int b = row.b + rb / own_rows, tok = rb % own_rows / G, h = kvh * G + rb % G;
-    V8 qb[D / 16];
-    {
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_bs + (int64_t)tok * a.q_ts +
-                      (int64_t)h * a.q_hs + 8 * hi;
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) qb[c] = rok ? ld16<V8>(qrow + 16 * c) : V8{};
-    }
-    // positions: the lane's, and the tile's first and last
-    const int p0 = row.len - a.n, pos = rok ? p0 + tok : p0 + a.n - 1;
-    const int ufirst = p0 + 32 * rt / G;
-    const int ulast = 32 * rt + 31 < rows ? p0 + (32 * rt + 31) / G : p0 + a.n - 1;
+    const PagedQuery at(a, row, kvh, rt, lq);
     f32x16 oacc[D / 32];
-#pragma unroll
-    for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
-    float m = -INFINITY, l = 0.f;
-    // q and the first tiles are here (through the builtin: the compiler then waits for no load of its own
-    // within the loop, which would wait for the tile in flight too)
-    __builtin_amdgcn_s_waitcnt(kWaitVm0);
-    for (int t = t0; t < t1; ++t) {
-      // a window's tiles have no sinks (the first of them may begin among those)
-      const int kh = start_of(t), cap = t < row.ns ? row.sink_hi - 1 : 0x7fffffff;
-      const int sinks = t < row.ns || row.lo == 0 ? row.sink_hi : 0;
-      const char* ks = kv[t & 1][0];
-      const char* vs = kv[t & 1][1];
-      const uint32_t none = bad >> (2 * (t & 1)) & 3;
-      fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
-                         [&](f32x16& acc) __attribute__((always_inline)) {
-                           if (!SHARED || !row.common)
-                             mask_window(acc, kh, ufirst < cap ? ufirst : cap, ulast - a.window,
-                                         pos < cap ? pos : cap, pos - a.window, sinks, hi);
-                           if (none) {
-#pragma unroll
-                             for (int i = 0; i < 16; ++i)
-                               if (none >> (i / 8) & 1) acc[i] = -INFINITY;
-                           }
-                         });
-      // this tile's reads are done: its buffer takes tile t + 2; then tile t + 1 is waited for
-      __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-      __builtin_amdgcn_sched_barrier(0);
-      if (t + 2 < t1 && issue(t + 2))
-        __builtin_amdgcn_s_waitcnt(wait_vm(2 * Fill::N));
-      else
-        __builtin_amdgcn_s_waitcnt(kWaitVm0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    float m, l;
+    paged_walk<T, D, NT>(a, row, at, kvh, rt, t0, t1, fk, fv, kv, lane, m, l, oacc);
     x += t1 - t0;
     const int group = (e < R ? e * per_common : R * per_common + (e - R) * per) + gi;
     float* part = a.part + (int64_t)(u + group) * live * (D + 2);
     // the wavefront with a group's first tile says for the join which others have some
     if (t0 == 0 && lane == 0) a.ends[group] = make_int2(u, plan.unit_of(g0 + row.tiles - 1));
-    if (rok && t0 == 0 && t1 == row.tiles && !(SHARED && (row.common || row.shared > 0))) {  // all of the row's keys
-      store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
+    if (at.ok && t0 == 0 && t1 == row.tiles && !(SHARED && (row.common || row.shared > 0))) {  // all of the row's keys
+      store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)at.b * a.n + at.tok) * a.HQ + at.h) * D, oacc, hi,
                          l > 0.f ? 1.f / l : 0.f);
-    } else if (rok) {
+    } else if (at.ok) {
       store_part<D>(part, live, lq, hi, m, l, oacc);
+    }
+  }
+}
+
+// One launch for short rows: a block of four wavefronts to a group, a quarter of its tiles to each, whose sums meet in LDS.
+template <typename T, int D, bool NT>
+__global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn_paged_solo(const AttnPagedArgs a) {
+  constexpr int RB = 2 * D, TILE = 32 * RB, NW = kPagedSoloWaves;
+  constexpr int LD = D + 4;  // floats of a row of sums: the 16-byte pieces of 32 rows on different banks
+  static_assert(4 * TILE >= 32 * LD * 4, "the sums fit a ring");
+  // [wavefront][buffer][K, V]. (Of a size known at launch only: told that a wavefront has a SIMD for itself, the compiler
+  // keeps the accumulators in the other half of the registers and moves them back and forth.)
+  extern __shared__ __align__(1024) char lds[];
+  auto& rings = *reinterpret_cast<char (*)[NW][2][2][TILE]>(lds);
+  __shared__ float stat[NW][2][32];  // maximum, sum
+  const int lane = threadIdx.x & 63, lq = lane & 31, hi = lane >> 5, w = wave_id();
+  const int G = a.HQ / a.HK, RT = (G * a.n + 31) / 32;
+  const int rt = (int)(blockIdx.x % RT), kvh = (int)(blockIdx.x / RT % a.HK), b = (int)(blockIdx.x / RT / a.HK);
+  const PagedRow row = paged_row<false>(a, b);
+  const int each = (row.tiles + NW - 1) / NW, busy = each > 0 ? (row.tiles + each - 1) / each : 0;
+  const PagedQuery at(a, row, kvh, rt, lq);
+  if (w < busy) {
+    const int mask = (1 << a.page_shift) - 1;
+    const PagedFill<RB, NT> fk(lane, a.k_ps * (int64_t)sizeof(T), a.k_ts * (int64_t)sizeof(T), mask);
+    const PagedFill<RB, NT> fv(lane, a.v_ps * (int64_t)sizeof(T), a.v_ts * (int64_t)sizeof(T), mask);
+    f32x16 oacc[D / 32];
+    float m, l;
+    const int t0 = w * each, t1 = t0 + each < row.tiles ? t0 + each : row.tiles;
+    paged_walk<T, D, NT>(a, row, at, kvh, rt, t0, t1, fk, fv, rings[w], lane, m, l, oacc);
+    float* sums = reinterpret_cast<float*>(rings[w]) + lq * LD + 4 * hi;
+#pragma unroll
+    for (int md = 0; md < D / 32; ++md)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(sums + 32 * md + 8 * j) =
+            make_float4(oacc[md][4 * j], oacc[md][4 * j + 1], oacc[md][4 * j + 2], oacc[md][4 * j + 3]);
+    if (hi == 0) {
+      stat[w][0][lq] = m;
+      stat[w][1][lq] = l;
+    }
+  }
+  __syncthreads();
+  // lane q: the weights of row q's sums
+  float top = -INFINITY, den = 0.f, f[NW];
+#pragma unroll
+  for (int c = 0; c < NW; ++c) {
+    f[c] = c < busy ? stat[c][0][lq] : -INFINITY;
+    top = fmaxf(top, f[c]);
+  }
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int c = 0; c < NW; ++c) {
+    f[c] = exp2_fast(f[c] - ref);
+    if (c < busy) den = fmaf(f[c], stat[c][1][lq], den);
+  }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  constexpr int C = D / 64, Q = 2;  // columns of a lane, rows at once
+  typedef T Out __attribute__((ext_vector_type(C)));
+  const int most = at.rows - 32 * rt < 32 ? at.rows - 32 * rt : 32;
+  for (int q0 = w; q0 < most; q0 += Q * NW) {
+    float acc[Q][C] = {};
+#pragma unroll
+    for (int c = 0; c < NW; ++c) {
+      if (c >= busy) break;
+      const float* v = reinterpret_cast<const float*>(rings[c]) + C * lane;
+#pragma unroll
+      for (int k = 0; k < Q; ++k) {
+        const int q = q0 + k * NW < 31 ? q0 + k * NW : 31;
+        const float fq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[c]), q));
+#pragma unroll
+        for (int i = 0; i < C; ++i) acc[k][i] = fmaf(fq, v[q * LD + i], acc[k][i]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+      const int q = q0 + k * NW, r = 32 * rt + q;
+      if (q >= most) break;
+      const float iq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), q));
+      Out out;
+#pragma unroll
+      for (int i = 0; i < C; ++i) out[i] = (T)(acc[k][i] * iq);
+      *reinterpret_cast<Out*>(static_cast<T*>(a.o) +
+                              (((int64_t)b * a.n + r / G) * a.HQ + kvh * G + r % G) * D + C * lane) = out;
     }
   }
 }
@@ -391,6 +511,16 @@ constexpr int64_t kPagedFewParts = 2;
 
 template <typename T, int D, bool SHARED>
 hipError_t run(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
+  if constexpr (!SHARED)
+    if (z.solo) {
+      const dim3 grid((unsigned)z.groups), block(64 * kPagedSoloWaves);
+      constexpr unsigned lds = kPagedSoloWaves * 4 * 32 * 2 * D;
+      if (D == 128 && z.row_tiles == 1)
+        hipLaunchKernelGGL((k_attn_paged_solo<T, D, D == 128>), grid, block, lds, s, a);
+      else
+        hipLaunchKernelGGL((k_attn_paged_solo<T, D, false>), grid, block, lds, s, a);
+      return hipGetLastError();
+    }
   const dim3 grid((unsigned)(z.units > 0 ? z.units : 1));
   if (D == 128 && z.all_tiles == 1)
     hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED>), grid, dim3(64), 0, s, a);

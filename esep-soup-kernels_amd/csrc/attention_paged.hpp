@@ -29,22 +29,41 @@ struct PagedSizes {
   int64_t rows, row_tiles;      // query rows of a kv head on their own, tiles of 32 of them
   int64_t all_rows, all_tiles;  // of W rows together
   int64_t shared_groups, groups, tiles, units, floats;
+  bool shared, solo;
 };
+// One launch, a block of four wavefronts to a group, instead of the cut walk with its partials and their join: where one
+// round of blocks takes all groups, and a block's wavefronts have only so many tiles more than the walk's would (up to
+// four of few tiles; of many, 5 / 8 of an equal share, as rows are ragged) that its launch and, with many groups, their
+// partials cost more. Both launches / one in us (graph replays), D = 128, 28 / 4 heads: 64 rows of up to 500 tokens 20.8 /
+// 13.9, 1000 27.9 / 21.2, 2500 47.8 / 43.5, 4000 66.7 / 66.9*; 32 of 2000 26.5* / 29.4, 5 of 900 13.4 / 14.2; 12 / 2 heads, one
+// row of 60 9.3 / 5.9, 700 10.3 / 11.0 (the launch saved takes the host 3 us), 1000 10.5* / 13.8; 64 of up to 200 14.2 / 7.9; D =
+// 64, 14 / 2 heads, 128 of up to 1500 23.3 / 17.4, 64 of 4096 26.5* / 32.5. (*: taken; else the one launch.)
+constexpr int kPagedSoloWaves = 4;
+inline bool paged_solo(int64_t groups, int64_t tiles, int D) {
+  const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles;
+  const int64_t few = total / kAttnCUs < 4 ? total / kAttnCUs : 4, many = total * 5 / 8 / waves;
+  const int64_t more = 6 + groups / 40;
+  return groups <= waves / kPagedSoloWaves && (tiles + 3) / kPagedSoloWaves <= (few > many ? few : many) + more;
+}
 inline PagedSizes paged_sizes(int B, int n, int W, int S, int HQ, int HK, int D, int window, int sinks,
                               bool shared) {
   PagedSizes z{};
   z.rows = (int64_t)n * (HQ / HK);
   z.row_tiles = (z.rows + 31) / 32;
-  z.all_rows = shared ? z.rows * W : z.rows;
-  z.all_tiles = (z.all_rows + 31) / 32;
-  z.shared_groups = shared ? (int64_t)(B / W) * HK * z.all_tiles : 0;
-  z.groups = z.shared_groups + (int64_t)B * HK * z.row_tiles;
+  const int64_t own = (int64_t)B * HK * z.row_tiles;
   const int64_t all = ((int64_t)S + 31) / 32 + 1;  // the sinks' end and the window's begin may share one
   const int64_t seen = ((int64_t)sinks + 31) / 32 + ((int64_t)window + n + 61) / 32;
-  z.tiles = z.shared_groups * (S / 32) + (z.groups - z.shared_groups) * (seen < all ? seen : all);
+  const int64_t each = seen < all ? seen : all;
+  z.solo = paged_solo(own, each, D);
+  z.shared = shared && !z.solo;
+  z.all_rows = z.shared ? z.rows * W : z.rows;
+  z.all_tiles = (z.all_rows + 31) / 32;
+  z.shared_groups = z.shared ? (int64_t)(B / W) * HK * z.all_tiles : 0;
+  z.groups = z.shared_groups + own;
+  z.tiles = z.shared_groups * (S / 32) + own * each;
   z.units = cache_units(z.tiles, D);
   const int64_t live = z.all_rows < 32 ? z.all_rows : 32;
-  z.floats = cache_ends_floats(z.groups) + (z.units + z.groups) * live * (D + 2);
+  z.floats = z.solo ? 0 : cache_ends_floats(z.groups) + (z.units + z.groups) * live * (D + 2);
   return z;
 }
 

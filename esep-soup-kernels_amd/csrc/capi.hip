@@ -1096,8 +1096,8 @@ int esep_attn_paged(const void* q, const int64_t* q_strides, const void* k_pages
   if (B == 0 || n == 0) return 0;
   const int rc = pages_ok("attn_paged", k_pages, kp_strides, v_pages, vp_strides, 3, N, page, HK, D);
   if (rc != 0) return rc;
-  if (q == nullptr || o == nullptr || lengths == nullptr || workspace == nullptr || q_strides == nullptr ||
-      (M > 0 && tables == nullptr))
+  if (q == nullptr || o == nullptr || lengths == nullptr || (workspace == nullptr && z.floats > 0) ||
+      q_strides == nullptr || (M > 0 && tables == nullptr))
     return fail(ESEP_EINVAL, "attn_paged: q, o, tables, lengths, the workspace and strides are required");
   if (!aligned16(q) || !aligned16(o) || !aligned16(workspace))
     return fail(ESEP_EALIGN, "attn_paged: q, o and the workspace need 16-byte alignment");
@@ -1115,9 +1115,9 @@ int esep_attn_paged(const void* q, const int64_t* q_strides, const void* k_pages
   a.o = o;
   a.tables = tables;
   a.len = lengths;
-  a.shared = shared;
+  a.shared = z.shared ? shared : nullptr;
   a.ends = reinterpret_cast<int2*>(workspace);
-  a.part = workspace + esep::cache_ends_floats(z.groups);
+  a.part = z.floats > 0 ? workspace + esep::cache_ends_floats(z.groups) : nullptr;
   a.q_bs = q_strides[0];
   a.q_ts = q_strides[1];
   a.q_hs = q_strides[2];

@@ -791,7 +791,8 @@ def attn_paged(q, k_pages, v_pages, o, tables, lengths, scale, window=None, sink
     w, sinks, share = 0 if window is None else int(window), int(sinks), int(shared is not None)
     need = lib().esep_attn_paged_workspace(B, n, M, P, HQ, HK, D, w, sinks, beams, share)
     if workspace is None:
-        workspace = torch.empty(max(need, 1), device=dev, dtype=torch.float32)
+        if need > 0:
+            workspace = torch.empty(need, device=dev, dtype=torch.float32)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() < need:
         raise EsepError(f"workspace must be a contiguous fp32 tensor of >= {need} elements")
     strides.extend(_bth_strides(q, shape, "q"))
@@ -800,7 +801,7 @@ def attn_paged(q, k_pages, v_pages, o, tables, lengths, scale, window=None, sink
         rc = lib().esep_attn_paged(
             q.data_ptr(), at + 48, k_pages.data_ptr(), at, v_pages.data_ptr(), at + 24, o.data_ptr(),
             tables.data_ptr(), ld, lengths.data_ptr(), None if shared is None else shared.data_ptr(),
-            workspace.data_ptr(), dtype_code(q.dtype), B, n, M, N, P, HQ, HK, D, float(scale), w, sinks, beams,
+            _p(workspace), dtype_code(q.dtype), B, n, M, N, P, HQ, HK, D, float(scale), w, sinks, beams,
             _stream(dev))
     _check(rc, "esep_attn_paged")
     _record(name)

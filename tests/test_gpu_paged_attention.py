@@ -44,6 +44,14 @@ def _scatter(k, v, lengths, P, rng, layout="nphd", shared=None, beams=1, fill=fl
     return *pages, _i(tables)
 
 
+def _wide(tables, page, tokens=1 << 15):
+    """The same tables with room for `tokens`: rows that may be long are walked in cut runs and joined, where short ones
+    take one launch."""
+    out = torch.full((tables.shape[0], max(tokens // page, tables.shape[1])), -1, dtype=torch.int32, device=DEV)
+    out[:, :tables.shape[1]] = tables
+    return out
+
+
 def _inputs(B, n, S, HQ, HK, D, dtype, seed):
     g = gen(seed)
     q = torch.randn(B, n, HQ, D, generator=g).to(dtype).to(DEV)
@@ -91,11 +99,14 @@ def test_paged_vs_float64(case, dtype):
     clean = [t.nan_to_num(0.0, 0.0, 0.0) for t in (k, v)]
     ref, tol = _reference(q, *clean, lengths, D ** -0.5, window, sinks, torch.finfo(dtype).eps / 2, _sub(dtype))
     _check(o, ref, tol, CASES[case])
-    # the same bits twice, and from a table with room behind the rows
-    wide = torch.full((len(lengths), tables.shape[1] + 3), -1, dtype=torch.int32, device=DEV)
-    wide[:, :tables.shape[1]] = tables
+    # the same bits twice, from a table whose rows are further apart
+    wide = _wide(tables, page)
     part = wide[:, :tables.shape[1]]
     assert torch.equal(o, paged_attention(q, kp, vp, part, _i(lengths), window=window, sinks=sinks))
+    # rows that may be long
+    o = paged_attention(q, kp, vp, wide, _i(lengths), window=window, sinks=sinks)
+    _check(o, ref, tol, ("wide", CASES[case]))
+    assert torch.equal(o, paged_attention(q, kp, vp, wide, _i(lengths), window=window, sinks=sinks))
 
 
 # (lengths of each request's beams, beams, shared, n, HQ, HK, D, page)
@@ -125,11 +136,12 @@ def test_shared_pages(case, dtype):
         k[b, :s], v[b, :s] = k[b // W * W, :s].clone(), v[b // W * W, :s].clone()
     kp, vp, tables = _scatter(k, v, lengths, page, random.Random(case), shared=shared, beams=W)
     ref, tol = _reference(q, k, v, lengths, D ** -0.5, None, 0, torch.finfo(dtype).eps / 2, _sub(dtype))
-    o = paged_attention(q, kp, vp, tables, _i(lengths), beams=W, shared=_i(shared))
-    _check(o, ref, tol, ("shared", SHARED[case]))
-    assert torch.equal(o, paged_attention(q, kp, vp, tables, _i(lengths), beams=W, shared=_i(shared)))
-    own = paged_attention(q, kp, vp, tables, _i(lengths))
-    _check(own, ref, tol, ("own", SHARED[case]))
+    for t in (tables, _wide(tables, page)):
+        o = paged_attention(q, kp, vp, t, _i(lengths), beams=W, shared=_i(shared))
+        _check(o, ref, tol, ("shared", SHARED[case]))
+        assert torch.equal(o, paged_attention(q, kp, vp, t, _i(lengths), beams=W, shared=_i(shared)))
+        own = paged_attention(q, kp, vp, t, _i(lengths))
+        _check(own, ref, tol, ("own", SHARED[case]))
     # through a window the pages are read row by row
     assert torch.equal(paged_attention(q, kp, vp, tables, _i(lengths), window=50, beams=W, shared=_i(shared)),
                        paged_attention(q, kp, vp, tables, _i(lengths), window=50))
@@ -196,9 +208,10 @@ def test_long_runs():
     _check(o, ref, tol, "long runs")
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("page", [16, 32, 64])
-@pytest.mark.parametrize("n,window", [(1, None), (3, None), (2, 70)])
-def test_missing_pages_are_not_seen(page, n, window):
+@pytest.mark.parametrize("n,window", [(1, None), (3, None), (2, 70), (60, None)])
+def test_missing_pages_are_not_seen(page, n, window, wide):
     """Entries of -1 and past the pool: as if their keys were masked; a row of nothing else gets 0."""
     from solution.body.paged import paged_attention
 
@@ -211,7 +224,7 @@ def test_missing_pages_are_not_seen(page, n, window):
     for b, j, bad in holes:
         tables[b, j] = bad
         hidden[b, j * page:(j + 1) * page] = True
-    o = paged_attention(q, kp, vp, tables, _i(lengths), window=window)
+    o = paged_attention(q, kp, vp, _wide(tables, page) if wide else tables, _i(lengths), window=window)
     for b, length in enumerate(lengths):
         pos = torch.arange(length - n, length, device=DEV)[:, None]
         j = torch.arange(length, device=DEV)[None]
@@ -236,6 +249,7 @@ def test_missing_shared_pages_are_not_seen():
     lengths = _i([250] * 4)
     kp, vp, tables = _scatter(k, v, [250] * 4, 32, random.Random(0), shared=[224], beams=4)
     tables[:, 3] = -1
+    tables = _wide(tables, 32)
     ref = paged_attention(q, kp, vp, tables, lengths)
     o = paged_attention(q, kp, vp, tables, lengths, beams=4, shared=_i([224]))
     keep = torch.cat([torch.arange(96), torch.arange(128, 250)]).to(DEV)
@@ -259,7 +273,9 @@ def test_no_pages_and_no_rows():
     q, k, v = _inputs(2, 1, 16, 4, 2, 64, torch.float16, 9)
     kp, vp, tables = _scatter(k, v, [16, 16], 16, random.Random(4))
     assert not paged_attention(q, kp, vp, tables[:, :0], _i([5, 5])).any()  # no room at all
-    assert not paged_attention(q, kp[:0], vp[:0], tables, _i([5, 5])).any()  # an empty pool
+    for t in (tables, _wide(tables, 16)):
+        assert not paged_attention(q, kp[:0], vp[:0], t, _i([5, 5])).any()  # an empty pool
+        assert not paged_attention(q, kp, vp, t, _i([0, -3])).any()
     assert paged_attention(q[:0], kp, vp, tables[:0], _i([])).shape == (0, 1, 4, 64)
 
 
@@ -272,7 +288,8 @@ def test_agrees_with_the_contiguous_form():
     q, k, v = _inputs(3, 1, 3008, 12, 2, 128, torch.bfloat16, 10)
     kp, vp, tables = _scatter(k, v, lengths, 16, random.Random(5))
     ref, tol = _reference(q, k, v, lengths, 128 ** -0.5, 200, 4, 2.0 ** -8, 0.0)
-    _check(paged_attention(q, kp, vp, tables, _i(lengths), window=200, sinks=4), ref, tol, "pages")
+    for t in (tables, _wide(tables, 16)):
+        _check(paged_attention(q, kp, vp, t, _i(lengths), window=200, sinks=4), ref, tol, "pages")
     _check(cache_attention(q, k, v, _i(lengths), window=200, sinks=4), ref, tol, "cache")
 
 
@@ -312,13 +329,15 @@ def test_pages_past_32_bit_offsets():
     _check(o, ref, tol, "far pages")
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("beams", [1, 2])
-def test_graph_replays_follow_the_lengths(beams):
+def test_graph_replays_follow_the_lengths(beams, wide):
     """A captured step replayed while the rows grow: lengths and tables are read on the device."""
     from solution.body.paged import paged_attention
 
     q, k, v = _inputs(4, 1, 640, 12, 2, 128, torch.bfloat16, 12)
     kp, vp, tables = _scatter(k, v, [640] * 4, 16, random.Random(7))
+    tables = _wide(tables, 16) if wide else tables
     shared = _i([0, 0]) if beams == 2 else None
     lens = _i([10, 300, 1, 64])
 
@@ -350,6 +369,7 @@ def test_two_streams_at_once():
         if shared:
             k[1], v[1] = k[0], v[0]
         kp, vp, tables = _scatter(k, v, lengths, 16, random.Random(i), shared=shared, beams=beams)
+        tables = _wide(tables, 16)
         sets.append((q, kp, vp, tables, _i(lengths), None, None, 0, beams, shared and _i(shared)))
     want = [paged_attention(*s) for s in sets]
     torch.cuda.synchronize()

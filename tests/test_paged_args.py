@@ -73,7 +73,7 @@ def test_reorder_refusals():
 
 def _attn(**kw):
     a = dict(q=16, qs=_S3(256, 256, 64), k=16, ks=_S3(2048, 128, 64), v=16, vs=_S3(2048, 128, 64), o=16, tables=16,
-             ld=4, lengths=16, shared=None, ws=16, dt=1, B=2, n=1, M=4, N=9, page=16, HQ=4, HK=2, D=64, scale=0.1,
+             ld=4000, lengths=16, shared=None, ws=16, dt=1, B=2, n=1, M=4000, N=9, page=16, HQ=4, HK=2, D=64, scale=0.1,
              window=0, sinks=0, beams=1, stream=None)
     a.update(kw)
     return _hip.lib().esep_attn_paged(*a.values())
@@ -94,18 +94,23 @@ def test_attention_refusals():
         assert _attn(**{name: 8}) == -3, name
     assert _attn(ks=_S3(2048, 129, 64)) == -3 and _attn(qs=_S3(-8, 256, 64)) == -3
     assert _attn(vs=_S3(2048, (1 << 22) + 8, 64)) == -2 and b"token stride" in _err()
-    assert _attn(ld=3) == -2 and b"overlap" in _err()
+    assert _attn(ld=3999) == -2 and b"overlap" in _err()
     assert _attn(B=0) == 0 and _attn(n=0) == 0
 
 
 def test_attention_workspace():
     ws = _hip.attn_paged_workspace
-    # two numbers per group, then a partial per wavefront (one to a tile up to 256) and per group, of each query row a
-    # maximum, a sum and D values; a row of 64 tokens has up to 3 tiles
-    assert ws(1, 1, 4, 16, 4, 2, 64) == 4 + (6 + 2) * 2 * 66
-    # two beams: their 4 rows together over up to 2 tiles of shared tokens
-    assert ws(2, 1, 4, 16, 4, 2, 64, beams=2, shared=True) == 12 + (2 * 2 + 4 * 3 + 6) * 4 * 66
-    assert ws(1, 1, 2048, 16, 12, 2, 128, 64, 4) < ws(1, 1, 2048, 16, 12, 2, 128)
+    # two numbers per group, then a partial per wavefront and per group, of each query row a maximum, a sum and D values:
+    # 1025 tiles, four to a wavefront, of each of two kv heads
+    assert ws(1, 1, 2048, 16, 4, 2, 64) == 4 + (512 + 2) * 2 * 66
+    # two beams: their 4 rows together over up to 1024 tiles of shared tokens, and each on its own
+    assert ws(2, 1, 2048, 16, 4, 2, 64, beams=2, shared=True) == 12 + (1537 + 6) * 4 * 66
+    # short rows in one launch: none
+    assert ws(1, 1, 44, 16, 12, 2, 128) == 0 and ws(1, 1, 64, 16, 12, 2, 128) > 0
+    assert ws(64, 1, 64, 16, 28, 4, 128) == 0 and ws(65, 1, 64, 16, 28, 4, 128) > 0  # one round of blocks
+    assert ws(128, 1, 64, 16, 28, 4, 64) == 0 and ws(129, 1, 64, 16, 28, 4, 64) > 0
+    assert ws(8, 1, 2048, 16, 12, 2, 128) > 0 and ws(8, 1, 2048, 16, 12, 2, 128, 300, 4) == 0  # a window keeps them short
+    assert ws(8, 1, 16, 16, 12, 2, 128, beams=4, shared=True) == 0
     assert ws(0, 1, 1, 16, 1, 1, 64) == 0 and ws(1, 1, 1, 24, 1, 1, 64) == 0
 
 
