@@ -17,7 +17,7 @@
 // Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.5 + 4.7 us (497 MB, 5.5
 // TB/s; a copy reaches 5.0, half of it writes); 8 requests of 4 beams over up to 8000 shared tokens and 130 each, pages of 16
 // 30.3 + 6.2 (96 MB; each beam on its own 4 times the bytes of the prompt); 5 new tokens over 7 rows through a window of
-// 1500, 14 / 2 heads of 64 13.1 + 3.9; one row of 700 tokens, 12 / 2 heads 9.0 in one launch (7.0 + 3.9 in two).
+// 1500, 14 / 2 heads of 64 12.5 + 3.9; one row of 700 tokens, 12 / 2 heads 10.8 in one launch (7.0 + 3.9 in two).
 // Without its products the walk of the beams takes 27.4 us, without its partials' stores 25.5; tried in vain: four wavefronts
 // to a block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us there, but 10.2 instead of 7.0 for the one row),
 // rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to three tiles to a

@@ -1026,8 +1026,7 @@ int esep_beam_reorder(const int32_t* parents, void* k_pages, const int64_t* kp_s
   if (rc != 0) return rc;
   if ((int64_t)M * page > (1 << 30))
     return fail(ESEP_ESHAPE, "beam_reorder: rows of %d pages of %d tokens are too long", M, page);
-  if (R * (int64_t)W > 1 && tables_bs < M)
-    return fail(ESEP_ESHAPE, "beam_reorder: rows of the tables overlap (stride %lld)", (long long)tables_bs);
+  if (tables_bs < 0) return fail(ESEP_ESHAPE, "beam_reorder: negative stride of the tables");
   if (R == 0 || M == 0 || L == 0 || N == 0) return 0;
   if (parents == nullptr || tables == nullptr || lengths == nullptr)
     return fail(ESEP_EINVAL, "beam_reorder: parents, tables and lengths are required");
@@ -1106,8 +1105,7 @@ int esep_attn_paged(const void* q, const int64_t* q_strides, const void* k_pages
       return fail(ESEP_EALIGN, "attn_paged: strides need to be multiples of 8 elements");
   if (kp_strides[1] > kAttnMaxStride || vp_strides[1] > kAttnMaxStride)
     return fail(ESEP_ESHAPE, "attn_paged: token stride above %lld elements", (long long)kAttnMaxStride);
-  if (B > 1 && tables_bs < M)
-    return fail(ESEP_ESHAPE, "attn_paged: rows of the tables overlap (stride %lld)", (long long)tables_bs);
+  if (tables_bs < 0) return fail(ESEP_ESHAPE, "attn_paged: negative stride of the tables");
   esep::AttnPagedArgs a{};
   a.q = q;
   a.k = k_pages;

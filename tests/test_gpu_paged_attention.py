@@ -293,6 +293,24 @@ def test_agrees_with_the_contiguous_form():
     _check(cache_attention(q, k, v, _i(lengths), window=200, sinks=4), ref, tol, "cache")
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_one_table_for_all_rows(wide):
+    """Rows over the same pages, their table expanded."""
+    from solution.body.paged import paged_attention
+
+    q, k, v = _inputs(5, 1, 96, 6, 2, 64, torch.bfloat16, 10)
+    kp, vp, tables = _scatter(k[:1], v[:1], [96], 16, random.Random(8))
+    tables = _wide(tables, 16) if wide else tables
+    lens = _i([96, 1, 0, 50, 64])
+    got = paged_attention(q, kp, vp, tables.expand(5, -1), lens)
+    assert torch.equal(got, paged_attention(q, kp, vp, tables.expand(5, -1).contiguous(), lens))
+    shared = paged_attention(q, kp, vp, tables.expand(5, -1), lens, beams=5, shared=_i([96]))
+    ref, tol = _reference(q, k[:1].expand(5, -1, -1, -1), v[:1].expand(5, -1, -1, -1), lens.tolist(), 0.125, None, 0,
+                          2.0 ** -8, 0.0)
+    _check(got, ref, tol, "expanded")
+    _check(shared, ref, tol, "expanded, shared")
+
+
 def test_strides_and_three_dims():
     """q as a slice of the fused q / k / v output and at an odd address, k and v pages of one allocation; [B, HQ, D]."""
     from solution.body.paged import paged_attention

@@ -64,7 +64,7 @@ def test_reorder_refusals():
                dict(R=60000, L=200)):
         assert _reorder(**kw) == -2 and b"bad sizes R" in _err(), kw
     assert _reorder(M=1 << 28) == -2 and b"too long" in _err()
-    assert _reorder(ld=3) == -2 and b"overlap" in _err()
+    assert _reorder(ld=-1) == -2 and b"negative" in _err()
     for name in ("parents", "kp", "vp", "kps", "vps", "tables", "lengths"):
         assert _reorder(**{name: None}) == -1, name
     assert _reorder(kp=8) == -3 and _reorder(vps=_S4(0, 2048, 128, 66)) == -3
@@ -94,7 +94,7 @@ def test_attention_refusals():
         assert _attn(**{name: 8}) == -3, name
     assert _attn(ks=_S3(2048, 129, 64)) == -3 and _attn(qs=_S3(-8, 256, 64)) == -3
     assert _attn(vs=_S3(2048, (1 << 22) + 8, 64)) == -2 and b"token stride" in _err()
-    assert _attn(ld=3999) == -2 and b"overlap" in _err()
+    assert _attn(ld=-1) == -2 and b"negative" in _err()
     assert _attn(B=0) == 0 and _attn(n=0) == 0
 
 
