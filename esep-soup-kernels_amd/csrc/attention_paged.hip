@@ -14,10 +14,10 @@
 // Bound by the bytes of K and V, and below a few MB by latency: where rows are short, one launch (k_attn_paged_solo) takes
 // the walk's and the join's place (the rule and both sides' times: attention_paged.hpp).
 //
-// Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.5 + 4.7 us (497 MB, 5.5
+// Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.4 + 4.8 us (497 MB, 5.5
 // TB/s; a copy reaches 5.0, half of it writes); 8 requests of 4 beams over up to 8000 shared tokens and 130 each, pages of 16
-// 30.3 + 6.2 (96 MB; each beam on its own 4 times the bytes of the prompt); 5 new tokens over 7 rows through a window of
-// 1500, 14 / 2 heads of 64 12.5 + 3.9; one row of 700 tokens, 12 / 2 heads 10.8 in one launch (7.0 + 3.9 in two).
+// 29.9 + 6.4 (96 MB; each beam on its own 4 times the bytes of the prompt); 5 new tokens over 7 rows through a window of
+// 1500, 14 / 2 heads of 64 12.6 + 4.0; one row of 700 tokens, 12 / 2 heads 9.9 in one launch (6.6 + 3.8 in two).
 // Without its products the walk of the beams takes 27.4 us, without its partials' stores 25.5; tried in vain: four wavefronts
 // to a block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us there, but 10.2 instead of 7.0 for the one row),
 // rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to three tiles to a
@@ -26,7 +26,7 @@
 
 #include "attention_cache.hpp"
 #include "attention_paged.hpp"
-#include "attention_tiles.hpp"
+#include "attention_paged_tiles.hpp"
 
 namespace esep {
 namespace {
@@ -171,13 +171,13 @@ struct PagedFill {
   }
 };
 
-// The query row of lane lq (of both halves) in tile rt of a kv head's `rows`: its batch row, token and head.
+// Query row r of a kv head's `rows`: its batch row, token and head.
 struct PagedQuery {
   int G, rows, b, tok, h;
   bool ok;
-  __device__ __forceinline__ PagedQuery(const AttnPagedArgs& a, const PagedRow& row, int kvh, int rt, int lq) {
+  __device__ __forceinline__ PagedQuery(const AttnPagedArgs& a, const PagedRow& row, int kvh, int r) {
     G = a.HQ / a.HK;
-    const int own = G * a.n, r = 32 * rt + lq;
+    const int own = G * a.n;
     rows = row.common ? a.W * own : own;
     ok = r < rows;
     const int q = ok ? r : 0;
@@ -187,16 +187,13 @@ struct PagedQuery {
   }
 };
 
-// A wavefront's tiles t0 .. t1 - 1 of one group through its own ring: the lane's query row's maximum, sum and weighted
-// sums.
-template <typename T, int D, bool NT>
+// A wavefront's tiles t0 .. t1 - 1 of one group through its own ring into `x`, its query rows (tile rt of the kv head's).
+template <typename T, int D, bool NT, int ROWS>
 __device__ __forceinline__ void paged_walk(const AttnPagedArgs& a, const PagedRow& row, const PagedQuery& at, int kvh,
                                            int rt, int t0, int t1, const PagedFill<2 * D, NT>& fk,
                                            const PagedFill<2 * D, NT>& fv, char (&kv)[2][2][32 * 2 * D], int lane,
-                                           float& m, float& l, f32x16 (&oacc)[D / 32]) {
-  using V8 = typename Mfma<T>::v8;
+                                           PagedTile<T, D, ROWS>& x) {
   using Fill = PagedFill<2 * D, NT>;
-  const int hi = lane >> 5;
   const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (int64_t)kvh * a.k_hs);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (int64_t)kvh * a.v_hs);
   const int32_t* table = a.tables + (int64_t)row.b * a.t_bs;
@@ -246,21 +243,11 @@ __device__ __forceinline__ void paged_walk(const AttnPagedArgs& a, const PagedRo
   issue(t0);
   if (t0 + 1 < t1) issue(t0 + 1);
 
-  V8 qb[D / 16];
-  {
-    const T* qrow = static_cast<const T*>(a.q) + (int64_t)at.b * a.q_bs + (int64_t)at.tok * a.q_ts +
-                    (int64_t)at.h * a.q_hs + 8 * hi;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) qb[c] = at.ok ? ld16<V8>(qrow + 16 * c) : V8{};
-  }
+  x.load(static_cast<const T*>(a.q) + (int64_t)at.b * a.q_bs + (int64_t)at.tok * a.q_ts + (int64_t)at.h * a.q_hs, at.ok);
   // positions: the lane's, and the tile's first and last
   const int p0 = row.len - a.n, pos = at.ok ? p0 + at.tok : p0 + a.n - 1;
-  const int ufirst = p0 + 32 * rt / at.G;
-  const int ulast = 32 * rt + 31 < at.rows ? p0 + (32 * rt + 31) / at.G : p0 + a.n - 1;
-#pragma unroll
-  for (int md = 0; md < D / 32; ++md) oacc[md] = f32x16{};
-  m = -INFINITY;
-  l = 0.f;
+  const int ufirst = p0 + ROWS * rt / at.G;
+  const int ulast = ROWS * (rt + 1) <= at.rows ? p0 + (ROWS * (rt + 1) - 1) / at.G : p0 + a.n - 1;
   // q and the first tiles are here (through the builtin: the compiler then waits for no load of its own
   // within the loop, which would wait for the tile in flight too)
   __builtin_amdgcn_s_waitcnt(kWaitVm0);
@@ -268,20 +255,10 @@ __device__ __forceinline__ void paged_walk(const AttnPagedArgs& a, const PagedRo
     // a window's tiles have no sinks (the first of them may begin among those)
     const int kh = start_of(t), cap = t < row.ns ? row.sink_hi - 1 : 0x7fffffff;
     const int sinks = t < row.ns || row.lo == 0 ? row.sink_hi : 0;
-    const char* ks = kv[t & 1][0];
-    const char* vs = kv[t & 1][1];
-    const uint32_t none = bad >> (2 * (t & 1)) & 3;
-    fwd_tile_swz<T, D>(ks, vs, lane, a.scale_log2, qb, oacc, m, l,
-                       [&](f32x16& acc) __attribute__((always_inline)) {
-                         if (!row.common)
-                           mask_window(acc, kh, ufirst < cap ? ufirst : cap, ulast - a.window,
-                                       pos < cap ? pos : cap, pos - a.window, sinks, hi);
-                         if (none) {
-#pragma unroll
-                           for (int i = 0; i < 16; ++i)
-                             if (none >> (i / 8) & 1) acc[i] = -INFINITY;
-                         }
-                       });
+    const int top = pos < cap ? pos : cap, low = pos - a.window;
+    const bool some = !row.common && (kh + 31 > (ufirst < cap ? ufirst : cap) || kh <= ulast - a.window);
+    x.step(kv[t & 1][0], kv[t & 1][1], a.scale_log2, kh, some, bad >> (2 * (t & 1)) & 3,
+           [&](int key) { return key > top || (key <= low && key >= sinks); });
     // this tile's reads are done: its buffer takes tile t + 2; then tile t + 1 is waited for
     __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
     __builtin_amdgcn_sched_barrier(0);
@@ -291,15 +268,16 @@ __device__ __forceinline__ void paged_walk(const AttnPagedArgs& a, const PagedRo
       __builtin_amdgcn_s_waitcnt(kWaitVm0);
     __builtin_amdgcn_sched_barrier(0);
   }
+  x.finish();
 }
 
-template <typename T, int D, bool NT, bool SHARED>
+template <typename T, int D, bool NT, bool SHARED, int ROWS>
 __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnPagedArgs a) {
   constexpr int RB = 2 * D, TILE = 32 * RB;
   using Fill = PagedFill<RB, NT>;
   __shared__ __align__(1024) char kv[2][2][TILE];  // [buffer][K, V]
 
-  const int lane = threadIdx.x, lq = lane & 31, hi = lane >> 5;
+  const int lane = threadIdx.x;
   const int G = a.HQ / a.HK, own_rows = G * a.n, all_rows = SHARED ? a.W * own_rows : own_rows;
   const int per = a.HK * ((own_rows + 31) / 32), per_common = a.HK * ((all_rows + 31) / 32);
   const int R = SHARED ? a.B / a.W : 0;
@@ -327,26 +305,33 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnP
     const int g0 = first + gi * row.tiles;
     const int t0 = x - g0, t1 = x1 - g0 < row.tiles ? x1 - g0 : row.tiles;
     const int kvh = gi / RT, rt = gi % RT;
-    const PagedQuery at(a, row, kvh, rt, lq);
-    f32x16 oacc[D / 32];
-    float m, l;
-    paged_walk<T, D, NT>(a, row, at, kvh, rt, t0, t1, fk, fv, kv, lane, m, l, oacc);
+    PagedTile<T, D, ROWS> tile(lane);
+    const PagedQuery at(a, row, kvh, ROWS * rt + tile.row());
+    paged_walk<T, D, NT, ROWS>(a, row, at, kvh, rt, t0, t1, fk, fv, kv, lane, tile);
     x += t1 - t0;
     const int group = (e < R ? e * per_common : R * per_common + (e - R) * per) + gi;
     float* part = a.part + (int64_t)(u + group) * live * (D + 2);
     // the wavefront with a group's first tile says for the join which others have some
     if (t0 == 0 && lane == 0) a.ends[group] = make_int2(u, plan.unit_of(g0 + row.tiles - 1));
     if (at.ok && t0 == 0 && t1 == row.tiles && !(SHARED && (row.common || row.shared > 0))) {  // all of the row's keys
-      store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)at.b * a.n + at.tok) * a.HQ + at.h) * D, oacc, hi,
-                         l > 0.f ? 1.f / l : 0.f);
+      tile.store(static_cast<T*>(a.o) + (((int64_t)at.b * a.n + at.tok) * a.HQ + at.h) * D);
     } else if (at.ok) {
-      store_part<D>(part, live, lq, hi, m, l, oacc);
+      const int q = tile.row();
+      if (tile.first()) {
+        part[q] = tile.m;
+        part[live + q] = tile.l;
+      }
+      float* sums = part + 2 * live + q * D;  // at even addresses
+      tile.each4([&](int column, f32x4 v) {
+        *reinterpret_cast<float2*>(sums + column) = make_float2(v[0], v[1]);
+        *reinterpret_cast<float2*>(sums + column + 2) = make_float2(v[2], v[3]);
+      });
     }
   }
 }
 
 // One launch for short rows: a block of four wavefronts to a group, a quarter of its tiles to each, whose sums meet in LDS.
-template <typename T, int D, bool NT>
+template <typename T, int D, bool NT, int ROWS>
 __global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn_paged_solo(const AttnPagedArgs a) {
   constexpr int RB = 2 * D, TILE = 32 * RB, NW = kPagedSoloWaves;
   constexpr int LD = D + 4;  // floats of a row of sums: the 16-byte pieces of 32 rows on different banks
@@ -356,30 +341,24 @@ __global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn
   extern __shared__ __align__(1024) char lds[];
   auto& rings = *reinterpret_cast<char (*)[NW][2][2][TILE]>(lds);
   __shared__ float stat[NW][2][32];  // maximum, sum
-  const int lane = threadIdx.x & 63, lq = lane & 31, hi = lane >> 5, w = wave_id();
+  const int lane = threadIdx.x & 63, w = wave_id();
   const int G = a.HQ / a.HK, RT = (G * a.n + 31) / 32;
   const int rt = (int)(blockIdx.x % RT), kvh = (int)(blockIdx.x / RT % a.HK), b = (int)(blockIdx.x / RT / a.HK);
   const PagedRow row = paged_row<false>(a, b);
   const int each = (row.tiles + NW - 1) / NW, busy = each > 0 ? (row.tiles + each - 1) / each : 0;
-  const PagedQuery at(a, row, kvh, rt, lq);
   if (w < busy) {
     const int mask = (1 << a.page_shift) - 1;
     const PagedFill<RB, NT> fk(lane, a.k_ps * (int64_t)sizeof(T), a.k_ts * (int64_t)sizeof(T), mask);
     const PagedFill<RB, NT> fv(lane, a.v_ps * (int64_t)sizeof(T), a.v_ts * (int64_t)sizeof(T), mask);
-    f32x16 oacc[D / 32];
-    float m, l;
+    PagedTile<T, D, ROWS> tile(lane);
+    const PagedQuery at(a, row, kvh, ROWS * rt + tile.row());
     const int t0 = w * each, t1 = t0 + each < row.tiles ? t0 + each : row.tiles;
-    paged_walk<T, D, NT>(a, row, at, kvh, rt, t0, t1, fk, fv, rings[w], lane, m, l, oacc);
-    float* sums = reinterpret_cast<float*>(rings[w]) + lq * LD + 4 * hi;
-#pragma unroll
-    for (int md = 0; md < D / 32; ++md)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<float4*>(sums + 32 * md + 8 * j) =
-            make_float4(oacc[md][4 * j], oacc[md][4 * j + 1], oacc[md][4 * j + 2], oacc[md][4 * j + 3]);
-    if (hi == 0) {
-      stat[w][0][lq] = m;
-      stat[w][1][lq] = l;
+    paged_walk<T, D, NT, ROWS>(a, row, at, kvh, rt, t0, t1, fk, fv, rings[w], lane, tile);
+    float* sums = reinterpret_cast<float*>(rings[w]) + tile.row() * LD;
+    tile.each4([&](int column, f32x4 v) { *reinterpret_cast<f32x4*>(sums + column) = v; });
+    if (tile.first()) {
+      stat[w][0][tile.row()] = tile.m;
+      stat[w][1][tile.row()] = tile.l;
     }
   }
   __syncthreads();
@@ -387,19 +366,19 @@ __global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn
   float top = -INFINITY, den = 0.f, f[NW];
 #pragma unroll
   for (int c = 0; c < NW; ++c) {
-    f[c] = c < busy ? stat[c][0][lq] : -INFINITY;
+    f[c] = c < busy ? stat[c][0][lane % ROWS] : -INFINITY;
     top = fmaxf(top, f[c]);
   }
   const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
   for (int c = 0; c < NW; ++c) {
     f[c] = exp2_fast(f[c] - ref);
-    if (c < busy) den = fmaf(f[c], stat[c][1][lq], den);
+    if (c < busy) den = fmaf(f[c], stat[c][1][lane % ROWS], den);
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
   constexpr int C = D / 64, Q = 2;  // columns of a lane, rows at once
   typedef T Out __attribute__((ext_vector_type(C)));
-  const int most = at.rows - 32 * rt < 32 ? at.rows - 32 * rt : 32;
+  const int rows = G * a.n - ROWS * rt, most = rows < ROWS ? rows : ROWS;
   for (int q0 = w; q0 < most; q0 += Q * NW) {
     float acc[Q][C] = {};
 #pragma unroll
@@ -408,7 +387,7 @@ __global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn
       const float* v = reinterpret_cast<const float*>(rings[c]) + C * lane;
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
-        const int q = q0 + k * NW < 31 ? q0 + k * NW : 31;
+        const int q = q0 + k * NW < ROWS ? q0 + k * NW : ROWS - 1;
         const float fq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[c]), q));
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[k][i] = fmaf(fq, v[q * LD + i], acc[k][i]);
@@ -416,7 +395,7 @@ __global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn
     }
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
-      const int q = q0 + k * NW, r = 32 * rt + q;
+      const int q = q0 + k * NW, r = ROWS * rt + q;
       if (q >= most) break;
       const float iq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), q));
       Out out;
@@ -509,25 +488,33 @@ __global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs
 // 32 rows of 4 beams over up to 8000 shared tokens 35.3 -> 38.5).
 constexpr int64_t kPagedFewParts = 2;
 
-template <typename T, int D, bool SHARED>
-hipError_t run(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
+template <typename T, int D, bool SHARED, int ROWS>
+void walk(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
   if constexpr (!SHARED)
     if (z.solo) {
       const dim3 grid((unsigned)z.groups), block(64 * kPagedSoloWaves);
       constexpr unsigned lds = kPagedSoloWaves * 4 * 32 * 2 * D;
       if (D == 128 && z.row_tiles == 1)
-        hipLaunchKernelGGL((k_attn_paged_solo<T, D, D == 128>), grid, block, lds, s, a);
+        hipLaunchKernelGGL((k_attn_paged_solo<T, D, D == 128, ROWS>), grid, block, lds, s, a);
       else
-        hipLaunchKernelGGL((k_attn_paged_solo<T, D, false>), grid, block, lds, s, a);
-      return hipGetLastError();
+        hipLaunchKernelGGL((k_attn_paged_solo<T, D, false, ROWS>), grid, block, lds, s, a);
+      return;
     }
   const dim3 grid((unsigned)(z.units > 0 ? z.units : 1));
   if (D == 128 && z.all_tiles == 1)
-    hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED, ROWS>), grid, dim3(64), 0, s, a);
   else
-    hipLaunchKernelGGL((k_attn_paged<T, D, false, SHARED>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((k_attn_paged<T, D, false, SHARED, ROWS>), grid, dim3(64), 0, s, a);
+}
+
+template <typename T, int D, bool SHARED>
+hipError_t run(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
+  if (z.all_rows <= 16)
+    walk<T, D, SHARED, 16>(a, z, s);
+  else
+    walk<T, D, SHARED, 32>(a, z, s);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || z.solo) return e;
   const unsigned rows = (unsigned)(a.B * a.HQ * a.n);
   constexpr unsigned per = 256 / (D / 2);
   if (z.units > kCacheManyParts * z.groups && rows <= 256)

@@ -34,10 +34,10 @@ struct PagedSizes {
 // One launch, a block of four wavefronts to a group, instead of the cut walk with its partials and their join: where one
 // round of blocks takes all groups, and a block's wavefronts have only so many tiles more than the walk's would (up to
 // four of few tiles; of many, 5 / 8 of an equal share, as rows are ragged) that its launch and, with many groups, their
-// partials cost more. Both launches / one in us (graph replays), D = 128, 28 / 4 heads: 64 rows of up to 500 tokens 20.8 /
-// 13.9, 1000 27.9 / 21.2, 2500 47.8 / 43.5, 4000 66.7 / 66.9*; 32 of 2000 26.5* / 29.4, 5 of 900 13.4 / 14.2; 12 / 2 heads, one
-// row of 60 9.3 / 5.9, 700 10.3 / 11.0 (the launch saved takes the host 3 us), 1000 10.5* / 13.8; 64 of up to 200 14.2 / 7.9; D =
-// 64, 14 / 2 heads, 128 of up to 1500 23.3 / 17.4, 64 of 4096 26.5* / 32.5. (*: taken; else the one launch.)
+// partials cost more. Both launches / one in us (graph replays), D = 128, 28 / 4 heads: 64 rows of up to 500 tokens 20.2 /
+// 12.9, 1000 27.3 / 20.4, 2500 47.4 / 42.8, 4000 65.9* / 66.1; 32 of 2000 25.8* / 28.8, 5 of 900 12.8 / 13.3; 12 / 2 heads, one
+// row of 60 8.8 / 5.3, 700 9.8 / 10.1 (the launch saved takes the host 3 us), 1000 10.1* / 12.6; 64 of up to 200 13.8 / 7.3;
+// D = 64, 14 / 2 heads, 128 of up to 1500 23.1 / 17.1, 64 of 4096 26.0* / 29.2. (*: taken; else the one launch.)
 constexpr int kPagedSoloWaves = 4;
 inline bool paged_solo(int64_t groups, int64_t tiles, int D) {
   const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles;
