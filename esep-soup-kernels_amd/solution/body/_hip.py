@@ -658,6 +658,9 @@ def attn_cache_workspace(B, n, S, HQ, HK, D, window=None, sinks=0):
 
 
 _INT32, _HALVES = torch.int32, (torch.float16, torch.bfloat16)
+# Of tensors that a kernel changes in place: a backward pass that saved one fails then, as after torch's own writes
+# (0.5 us a call).
+_changed = torch.autograd.graph.increment_version
 
 
 def _int32(name, t, *shape):
@@ -737,6 +740,7 @@ def page_tables(tables, lengths, new, free, taken, page, total, update, name="_p
             tables.data_ptr(), ld, lengths.data_ptr(), new.data_ptr(), free.data_ptr(), taken.data_ptr(), at,
             at + 4 * total, cu, lens, took, B, M, F, page, total, _stream(dev))
     _check(rc, "esep_page_tables")
+    _changed((tables, lengths, taken) if update else (tables,))
     _record(name)
     out = out.split_with_sizes(sizes)
     return (*out, lengths, taken) if update else out
@@ -762,6 +766,7 @@ def page_store(k, v, k_pages, v_pages, slots, name="_page_store"):
         rc = lib().esep_page_store(k.data_ptr(), at + 48, v.data_ptr(), at + 64, k_pages.data_ptr(), at,
                                    v_pages.data_ptr(), at + 24, slots.data_ptr(), T, N, P, HK, D, _stream(dev))
     _check(rc, "esep_page_store")
+    _changed((k_pages, v_pages))
     _record(name)
 
 
@@ -874,6 +879,7 @@ def beam_reorder(parents, k_pages, v_pages, tables, lengths, start=None, name="_
             parents.data_ptr(), k_pages.data_ptr(), at, v_pages.data_ptr(), at + 32, tables.data_ptr(), ld,
             lengths.data_ptr(), None if start is None else start.data_ptr(), R, W, M, L, N, P, HK, D, _stream(dev))
     _check(rc, "esep_beam_reorder")
+    _changed((k_pages, v_pages))
     _record(name)
 
 

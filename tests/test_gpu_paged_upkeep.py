@@ -284,3 +284,32 @@ def test_reorder_nothing():
     beam_reorder(_i([[1, 0]]), kp, vp, _i([[0], [1]]), _i([9]), _i([9]))
     beam_reorder(_i([[1, 0]]), kp, vp, _i([[0], [1]]), _i([-5]), _i([-9]))
     assert torch.equal(kp, want) and torch.equal(vp, want)
+
+
+# ----------------------------------------------------------------------------------------
+# what is changed behind torch's back
+# ----------------------------------------------------------------------------------------
+def test_saved_tensors_that_change_are_noticed():
+    """A backward pass that saved the pages, tables or lengths does not run over what took their place."""
+    from solution.body.paged import beam_reorder, block_tables, paged_store
+
+    dt = torch.bfloat16
+    tables, lengths, taken = _i([[0, 1], [2, 3]]), _i([16, 16]), _i([0])
+
+    def refuses(t, change):
+        out = (torch.ones(t.shape, device=DEV, dtype=dt, requires_grad=True) * t).sum()
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+
+    pages = [_pages((4, 16, 1, 64), dt, i) for i in range(2)]
+    k = torch.zeros(1, 1, 64, device=DEV, dtype=dt)
+    parents = _i([[1, 0]])
+    for t in pages:
+        refuses(t, lambda: paged_store(k, k, *pages, _i([3])))
+        refuses(t, lambda: beam_reorder(parents, *pages, tables, _i([20])))
+    versions = [t._version for t in (tables, lengths, taken)]
+    block_tables(tables, lengths, _i([1, 1]), _i([5, 6]), taken, 16, 2)
+    assert [t._version for t in (tables, lengths, taken)] == [versions[0] + 1, *versions[1:]]
+    block_tables(tables, lengths, _i([1, 1]), _i([5, 6]), taken, 16, 2, update=True)
+    assert [t._version for t in (tables, lengths, taken)] == [versions[0] + 2, versions[1] + 1, versions[2] + 1]
