@@ -137,6 +137,16 @@ def test_beams_that_are_out(V, dtype):
         _check(_go(logits, scores, keep), logits, scores, keep)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("W,V,keep", [(16, 151936, 32), (8, 100003, 64), (1, 2048, 64)])
+def test_rows_in_order(W, V, keep, dtype):
+    """Rows that rise or fall all along (a piece's greatest lie with a few of its threads), beside ones in no order."""
+    logits, scores = _inputs(3, W, V, dtype, V + keep)
+    logits[1] = logits[1].float().sort(-1).values.to(dtype)
+    logits[2] = logits[2].float().sort(-1, descending=True).values.to(dtype)
+    _check(_go(logits, scores, keep), logits, scores, keep)
+
+
 def test_extremes():
     """The largest values of each type, differences that the exponentials flush, far apart scores."""
     for dtype in DTYPES:
