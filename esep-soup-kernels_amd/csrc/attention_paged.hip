@@ -17,7 +17,8 @@
 // Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.4 + 4.8 us (497 MB, 5.5
 // TB/s; a copy reaches 5.0, half of it writes); 8 requests of 4 beams over up to 8000 shared tokens and 130 each, pages of 16
 // 29.9 + 6.4 (96 MB; each beam on its own 4 times the bytes of the prompt); 5 new tokens over 7 rows through a window of
-// 1500, 14 / 2 heads of 64 12.6 + 4.0; one row of 700 tokens, 12 / 2 heads 9.9 in one launch (6.6 + 3.8 in two).
+// 1500, 14 / 2 heads of 64 14.3 in one launch (12.6 + 4.0 in two); one row of 700 tokens, 12 / 2 heads 9.9 (6.6 + 3.8).
+// A CU of its own takes in up to 70 GB/s; a wavefront's products of a tile take 0.3 (D = 64) and 0.44 us (128).
 // Without its products the walk of the beams takes 27.4 us, without its partials' stores 25.5; tried in vain: four wavefronts
 // to a block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us there, but 10.2 instead of 7.0 for the one row),
 // rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to three tiles to a
@@ -330,10 +331,11 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_paged(const AttnP
   }
 }
 
-// One launch for short rows: a block of four wavefronts to a group, a quarter of its tiles to each, whose sums meet in LDS.
-template <typename T, int D, bool NT, int ROWS>
-__global__ __launch_bounds__(64 * kPagedSoloWaves, D == 128 ? 2 : 3) void k_attn_paged_solo(const AttnPagedArgs a) {
-  constexpr int RB = 2 * D, TILE = 32 * RB, NW = kPagedSoloWaves;
+// One launch for short rows: a block of NW wavefronts to a group, an equal share of its tiles to each, whose sums meet in
+// LDS.
+template <typename T, int D, int NW, bool NT, int ROWS>
+__global__ __launch_bounds__(64 * NW, D == 128 ? 2 : 3) void k_attn_paged_solo(const AttnPagedArgs a) {
+  constexpr int RB = 2 * D, TILE = 32 * RB;
   constexpr int LD = D + 4;  // floats of a row of sums: the 16-byte pieces of 32 rows on different banks
   static_assert(4 * TILE >= 32 * LD * 4, "the sums fit a ring");
   // [wavefront][buffer][K, V]. (Of a size known at launch only: told that a wavefront has a SIMD for itself, the compiler
@@ -488,18 +490,23 @@ __global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs
 // 32 rows of 4 beams over up to 8000 shared tokens 35.3 -> 38.5).
 constexpr int64_t kPagedFewParts = 2;
 
+template <typename T, int D, int NW, int ROWS>
+void solo(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
+  const dim3 grid((unsigned)z.groups), block(64 * NW);
+  constexpr unsigned lds = NW * 4 * 32 * 2 * D;
+  if (D == 128 && z.row_tiles == 1)
+    hipLaunchKernelGGL((k_attn_paged_solo<T, D, NW, D == 128, ROWS>), grid, block, lds, s, a);
+  else
+    hipLaunchKernelGGL((k_attn_paged_solo<T, D, NW, false, ROWS>), grid, block, lds, s, a);
+}
+
 template <typename T, int D, bool SHARED, int ROWS>
 void walk(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
-  if constexpr (!SHARED)
-    if (z.solo) {
-      const dim3 grid((unsigned)z.groups), block(64 * kPagedSoloWaves);
-      constexpr unsigned lds = kPagedSoloWaves * 4 * 32 * 2 * D;
-      if (D == 128 && z.row_tiles == 1)
-        hipLaunchKernelGGL((k_attn_paged_solo<T, D, D == 128, ROWS>), grid, block, lds, s, a);
-      else
-        hipLaunchKernelGGL((k_attn_paged_solo<T, D, false, ROWS>), grid, block, lds, s, a);
-      return;
-    }
+  if constexpr (!SHARED) {
+    if constexpr (D == 64)
+      if (z.solo == 8) return solo<T, D, 8, ROWS>(a, z, s);
+    if (z.solo) return solo<T, D, 4, ROWS>(a, z, s);
+  }
   const dim3 grid((unsigned)(z.units > 0 ? z.units : 1));
   if (D == 128 && z.all_tiles == 1)
     hipLaunchKernelGGL((k_attn_paged<T, D, D == 128, SHARED, ROWS>), grid, dim3(64), 0, s, a);

@@ -29,21 +29,29 @@ struct PagedSizes {
   int64_t rows, row_tiles;      // query rows of a kv head on their own, tiles of 32 of them
   int64_t all_rows, all_tiles;  // of W rows together
   int64_t shared_groups, groups, tiles, units, floats;
-  bool shared, solo;
+  bool shared;
+  int solo;  // one launch: wavefronts to a block, else 0
 };
-// One launch, a block of four wavefronts to a group, instead of the cut walk with its partials and their join: where one
-// round of blocks takes all groups, and a block's wavefronts have only so many tiles more than the walk's would (up to
-// four of few tiles; of many, 5 / 8 of an equal share, as rows are ragged) that its launch and, with many groups, their
-// partials cost more. Both launches / one in us (graph replays), D = 128, 28 / 4 heads: 64 rows of up to 500 tokens 20.2 /
-// 12.9, 1000 27.3 / 20.4, 2500 47.4 / 42.8, 4000 65.9* / 66.1; 32 of 2000 25.8* / 28.8, 5 of 900 12.8 / 13.3; 12 / 2 heads, one
-// row of 60 8.8 / 5.3, 700 9.8 / 10.1 (the launch saved takes the host 3 us), 1000 10.1* / 12.6; 64 of up to 200 13.8 / 7.3;
-// D = 64, 14 / 2 heads, 128 of up to 1500 23.1 / 17.1, 64 of 4096 26.0* / 29.2. (*: taken; else the one launch.)
-constexpr int kPagedSoloWaves = 4;
-inline bool paged_solo(int64_t groups, int64_t tiles, int D) {
+// One launch, a block of four or eight wavefronts to a group, instead of the cut walk with its partials and their
+// join: where one round of blocks takes all groups, and a block's wavefronts have only so many tiles more than the
+// walk's would (up to four of few tiles; of many, 5 / 8 of an equal share, as rows are ragged) that its launch and,
+// with many groups, their partials cost more. As many wavefronts as the rings of a CU's LDS allow: at D = 64 eight,
+// while a CU has one block.
+//
+// Both launches / one in us (graph replays over caches that no cache of the card holds; *: taken, else the one
+// launch). D = 128, 28 / 4 heads: 64 rows of up to 300 tokens 17.9 / 10.5, 1500 35.3 / 29.5, 2500 55.5 / 52.9, 4000
+// 77.9* / 79.9; 32 of 700 17.5 / 14.0, 2000 26.5* / 29.5; 5 of 900 13.1 / 14.5 (the launch saved takes the host 3
+// us); 12 / 2 heads, one row of 60 8.3 / 4.8, 700 9.3 / 11.6 (the same), 1000 9.5* / 14.6. D = 64, 14 / 2 heads, both
+// / four wavefronts / eight: one row of 300 8.4 / 5.8 / 6.1, 700 9.1 / 8.2 / 7.2, 1500 9.5* / 12.6 / 10.1; 32 of 1000
+// 14.1 / 11.5 / 10.7, 2500 17.2* / 20.6 / 19.1; 7 of 5 new tokens and a window of 1500 14.4 / 16.5 / 13.7; 120 of
+// 4000 43.7 / 40.7 / 40.9; 130 (260 groups) of 1200 23.0 / 19.1, 2000 29.2* / 31.9; 8 / 8 heads, 40 of 1200 22.6 /
+// 21.5, 2000 28.4* / 36.6.
+inline int paged_solo(int64_t groups, int64_t tiles, int D) {
   const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles;
+  const int each = D == 64 && groups <= kAttnCUs ? 8 : 4;
   const int64_t few = total / kAttnCUs < 4 ? total / kAttnCUs : 4, many = total * 5 / 8 / waves;
-  const int64_t more = 6 + groups / 40;
-  return groups <= waves / kPagedSoloWaves && (tiles + 3) / kPagedSoloWaves <= (few > many ? few : many) + more;
+  const int64_t more = D == 64 ? 4 + groups / 64 : 6 + groups / 40;
+  return groups <= waves / each && (tiles + each - 1) / each <= (few > many ? few : many) + more ? each : 0;
 }
 inline PagedSizes paged_sizes(int B, int n, int W, int S, int HQ, int HK, int D, int window, int sinks,
                               bool shared) {
@@ -55,7 +63,7 @@ inline PagedSizes paged_sizes(int B, int n, int W, int S, int HQ, int HK, int D,
   const int64_t seen = ((int64_t)sinks + 31) / 32 + ((int64_t)window + n + 61) / 32;
   const int64_t each = seen < all ? seen : all;
   z.solo = paged_solo(own, each, D);
-  z.shared = shared && !z.solo;
+  z.shared = shared && z.solo == 0;
   z.all_rows = z.shared ? z.rows * W : z.rows;
   z.all_tiles = (z.all_rows + 31) / 32;
   z.shared_groups = z.shared ? (int64_t)(B / W) * HK * z.all_tiles : 0;

@@ -147,7 +147,7 @@ def test_shared_pages(case, dtype):
                        paged_attention(q, kp, vp, tables, _i(lengths), window=50))
 
 
-@pytest.mark.parametrize("rows", [64, 65, 300])
+@pytest.mark.parametrize("rows", [64, 65, 200, 300])
 def test_many_rows(rows):
     """More rows than a wavefront has lanes, of all lengths, empty ones among them; also as beams of nothing in common."""
     from solution.body.paged import paged_attention
