@@ -9,6 +9,14 @@
 // 2 keep), and a listed key's place is the number of greater ones. k_beam_join: lse of each beam from the pieces'
 // parts, the same selection among the pieces' candidates by value, in 64 bits (two beams' values lie closer than 32 bits
 // tell apart once in about 10^4 choices). Where ties fill the list the greatest is taken `keep` times instead.
+//
+// Bound by two launches' latency (one request of 4 beams over 151936 in bf16, keep 8: 4.4 + 4.4 us, where its bytes
+// take 0.2), with many rows by the logits and a block's chain from its loads to its list. Both launches, graph
+// replays, cold caches, us (the bytes' time): 24 x 5 x 151936 fp32, keep 5 22.6 (14.5), with one beam of five alive
+// 13.2 (2.9); 128 x 4 x 151936 bf16, keep 8 44.9 (30.9), without the lists 40; 16 x 8 x 50001 fp32, keep 16 15.9
+// (5.1; read an element at a time, as its rows begin anywhere, 25.8); 1 x 8 x 151936 bf16, keep 64 21.9; 64 x 4 x
+// 151936 bf16, keep 64 47 (with 64 groups to bound it 517: one list in 50 overflows); 1 x 64 x 151936, keep 64 79:
+// 78000 candidates for the join's one block. Loads past the caches change none of it by more than 3%.
 #include "beam.hpp"
 
 #include <cmath>
@@ -41,27 +49,43 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
 }
 
-// A bound that at least `keep` of the wavefront's lanes reach with their keys, and of the values with these first 20 bits the
-// greatest: bit by bit, the lanes at or above it counted. 0 where fewer lanes have a finite value.
+// A bound that at least `keep` of the wavefront's 64 G keys reach, and of the values with these first 20 bits the
+// greatest: bit by bit, the keys at or above it counted. 0 where fewer are finite.
 constexpr int kBoundBits = 20;
-__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int keep) {
+template <int G>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[G], int keep) {
   uint32_t bound = 0;
 #pragma unroll
   for (int bit = 31; bit >= 32 - kBoundBits; --bit) {
     const uint32_t t = bound | 1u << bit;
-    if (__popcll(__ballot(key >= t)) >= keep) bound = t;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < G; ++i) n += __popcll(__ballot(key[i] >= t));
+    if (n >= keep) bound = t;
   }
   return bound;
 }
 // It as a float, at least the lowest finite one.
 __device__ __forceinline__ float bound_of(uint32_t key) { return unordered(key < 0x00800000u ? 0x00800000u : key); }
-// The greatest of what lane l of each wavefront has put into v (after a barrier): 64 groups of the block's threads.
+// A bound that the `keep` greatest of what the block's threads have put into v (after a barrier) reach, and the
+// greatest of all. The threads make 64 groups, for a large `keep` 256: of 64 the least one's maximum would bound 64
+// of them, which 300 values of random rows reach (and more than the list holds in one row of 50), of 256 74 do.
+constexpr int kFewKeep = 32;
 template <int NW>
-__device__ __forceinline__ float group_max(const float (&v)[NW * 64], int lane) {
-  float m = v[lane];
+__device__ __forceinline__ float block_bound(const float (&v)[NW * 64], int lane, int keep, float* top) {
+  float m[4];
 #pragma unroll
-  for (int i = 1; i < NW; ++i) m = fmaxf(m, v[64 * i + lane]);
-  return m;
+  for (int i = 0; i < 4; ++i) m[i] = v[64 * i + lane];
+#pragma unroll
+  for (int i = 4; i < NW; ++i) m[i % 4] = fmaxf(m[i % 4], v[64 * i + lane]);
+  const float all = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  *top = wave_max(all);
+  if (keep <= kFewKeep) {
+    const uint32_t key[1] = {ordered(all)};
+    return bound_of(wave_bound(key, keep));
+  }
+  const uint32_t key[4] = {ordered(m[0]), ordered(m[1]), ordered(m[2]), ordered(m[3])};
+  return bound_of(wave_bound(key, keep));
 }
 
 // Lanes that count a listed candidate's betters together, and their sum, in each of them.
@@ -72,10 +96,14 @@ __device__ __forceinline__ int rank_sum(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);  // the other quad of each 8
 }
 
+// 16 bytes of logits, wherever they lie (a row of an odd vocabulary begins anywhere).
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2)));
+
 // The piece's elements of thread i: i * 8 .. + 7 of each run of 2048, whatever the row's alignment, so that equal
-// rows give equal sums.
-template <typename T, int U, bool VEC>
-__global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
+// rows give equal sums. (Registers for six wavefronts to a SIMD: 128 requests of 4 beams over 151936 in bf16 47.7 ->
+// 44.9 us, where the compiler's own choice leaves five and eight spill: 48.5.)
+template <typename T, int U>
+__global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a) {
   constexpr int NW = kBeamThreads / 64;
   __shared__ float w_sum[NW], best[kBeamThreads];
   __shared__ uint64_t list[kList];
@@ -89,30 +117,30 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   const int base = split * a.piece + 8 * (int)threadIdx.x;
   float v[U][8];
   if (threadIdx.x == 0) count = 0;
-  // all of it is asked for at once: what lies past the row is read at its begin and replaced
-  if constexpr (VEC) {
-    Raw<T> raw[U];
+  // all of it is asked for at once, in pieces of 16 bytes at any address; eights that the row does not fill are read at its
+  // begin (or not: it has fewer) and replaced
+  Raw<T> raw[U];
+  if (a.V >= 8) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const u32x4* at = reinterpret_cast<const u32x4*>(x + (base + 2048 * u < a.V ? base + 2048 * u : 0));
+      const Any16* at = reinterpret_cast<const Any16*>(x + (base + 2048 * u + 7 < a.V ? base + 2048 * u : 0));
       raw[u].a = at[0];
       if constexpr (sizeof(T) == 4) raw[u].b = at[1];
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      Buf<T>::unpack(raw[u], v[u]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[u][e] = base + 2048 * u < a.V ? v[u][e] : -INFINITY;  // V is a multiple of 8
-    }
   } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) raw[u] = Raw<T>{};
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    Buf<T>::unpack(raw[u], v[u]);
+    if (base + 2048 * u + 7 >= a.V) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int i = base + 2048 * u + e;
-        const float f = (float)x[i < a.V ? i : 0];
-        v[u][e] = i < a.V ? f : -INFINITY;
+        v[u][e] = i < a.V ? (float)x[i] : -INFINITY;
       }
+    }
   }
   float mine = -INFINITY, run[U];  // the greatest of all, of each eight; NaN is passed over
 #pragma unroll
@@ -124,8 +152,8 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const BeamArgs a) {
   }
   best[threadIdx.x] = mine;
   __syncthreads();
-  const float group = group_max<NW>(best, lane), top = wave_max(group);
-  const float bound = bound_of(wave_bound(ordered(group), a.keep));
+  float top;
+  const float bound = block_bound<NW>(best, lane, a.keep, &top);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
@@ -214,7 +242,7 @@ __device__ __forceinline__ bool before(const Cand& x, const Cand& y) {
   return x.value > y.value || (x.value == y.value && x.at < y.at);
 }
 
-constexpr int kJoinThreads = 1024, kJoinFirst = 4, kJoinMostBeams = 64;
+constexpr int kJoinThreads = 1024, kJoinFirst = kBeamJoinFirst, kJoinMore = 8, kJoinMostBeams = 64;
 
 __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   constexpr int NW = kJoinThreads / 64;
@@ -285,12 +313,22 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
     best32 = fmaxf(best32, (float)mine[j].value);
   }
   const int rounds = (all + kJoinThreads - 1) / kJoinThreads;
-  auto later = [&](int j) { return index(j) < all ? value(index(j), keys[index(j)]) : Cand{-(double)INFINITY, kNoPlace}; };
+  // f of the thread's candidates from j0 on, kJoinMore asked for at once
+  auto each_from = [&](int j0, auto&& f) {
 #pragma unroll 1
-  for (int j = kJoinFirst; j < rounds; ++j) best32 = fmaxf(best32, (float)later(j).value);
+    for (int j = j0; j < rounds; j += kJoinMore) {
+      uint64_t more[kJoinMore];
+#pragma unroll
+      for (int i = 0; i < kJoinMore; ++i) more[i] = index(j + i) < all ? keys[index(j + i)] : 0;
+#pragma unroll
+      for (int i = 0; i < kJoinMore; ++i) f(value(index(j + i) < all ? index(j + i) : 0, more[i]));
+    }
+  };
+  each_from(kJoinFirst, [&](const Cand& c) { best32 = fmaxf(best32, (float)c.value); });
   group[tid] = best32;
   __syncthreads();
-  const float bound = bound_of(wave_bound(ordered(group_max<NW>(group, lane)), a.keep));
+  float highest;
+  const float bound = block_bound<NW>(group, lane, a.keep, &highest);
   // by value in 32 bits (rounding keeps the order): what reaches the bound
   auto enter = [&](const Cand& c) {
     if ((float)c.value >= bound) {
@@ -300,8 +338,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   };
 #pragma unroll
   for (int j = 0; j < kJoinFirst; ++j) enter(mine[j]);
-#pragma unroll 1
-  for (int j = kJoinFirst; j < rounds; ++j) enter(later(j));
+  if (best32 >= bound) each_from(kJoinFirst, enter);
   __syncthreads();
   auto put = [&](int place, const Cand& c) {
     const int o = r * a.keep + place, b = c.at / a.V;
@@ -316,11 +353,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
 #pragma unroll 1
     for (int k = 0; k < a.keep; ++k) {
       Cand best{-(double)INFINITY, kNoPlace};
-#pragma unroll 1
-      for (int j = 0; j < rounds; ++j) {
-        const Cand c = later(j);
+      each_from(0, [&](const Cand& c) {
         if (before(last, c) && before(c, best)) best = c;
-      }
+      });
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) {
         const Cand o{__shfl_xor(best.value, d), __shfl_xor(best.at, d)};
@@ -358,23 +393,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
   }
 }
 
-template <typename T, int U>
-void rows(const BeamArgs& a, bool vec, hipStream_t s) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.R * a.W));
-  if (vec)
-    hipLaunchKernelGGL((k_beam_rows<T, U, true>), grid, dim3(kBeamThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_beam_rows<T, U, false>), grid, dim3(kBeamThreads), 0, s, a);
-}
-
 template <typename T>
-hipError_t run(const BeamArgs& a, bool vec, hipStream_t s) {
+hipError_t run(const BeamArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)a.splits, (unsigned)(a.R * a.W));
   if (a.piece == 2048)
-    rows<T, 1>(a, vec, s);
+    hipLaunchKernelGGL((k_beam_rows<T, 1>), grid, dim3(kBeamThreads), 0, s, a);
   else if (a.piece == 4096)
-    rows<T, 2>(a, vec, s);
+    hipLaunchKernelGGL((k_beam_rows<T, 2>), grid, dim3(kBeamThreads), 0, s, a);
   else
-    rows<T, 4>(a, vec, s);
+    hipLaunchKernelGGL((k_beam_rows<T, 4>), grid, dim3(kBeamThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.R), dim3(kJoinThreads), 0, s, a);
@@ -383,11 +410,11 @@ hipError_t run(const BeamArgs& a, bool vec, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_beam_select(const BeamArgs& a, int dt, bool vec, hipStream_t s, bool* sup) {
+hipError_t launch_beam_select(const BeamArgs& a, int dt, hipStream_t s, bool* sup) {
   *sup = true;
-  if (dt == 0) return run<float>(a, vec, s);
-  if (dt == 1) return run<_Float16>(a, vec, s);
-  if (dt == 2) return run<__bf16>(a, vec, s);
+  if (dt == 0) return run<float>(a, s);
+  if (dt == 1) return run<_Float16>(a, s);
+  if (dt == 2) return run<__bf16>(a, s);
   *sup = false;
   return hipErrorInvalidValue;
 }

@@ -1153,7 +1153,7 @@ bool beam_sizes_ok(int R, int W, int64_t V, int keep) {
 
 int64_t esep_beam_select_workspace(int R, int W, int64_t V, int keep) {
   if (!beam_sizes_ok(R, W, V, keep)) return 0;
-  const int64_t parts = (int64_t)R * W * esep::beam_splits((int64_t)R * W, V);
+  const int64_t parts = (int64_t)R * W * esep::beam_splits(R, W, V, keep);
   return 8 * parts * (1 + keep);
 }
 
@@ -1171,7 +1171,7 @@ int esep_beam_select(const void* logits, int64_t ld_r, int64_t ld_w, const float
     return fail(ESEP_EINVAL, "beam_select: logits, scores, the workspace and the outputs are required");
   if (reinterpret_cast<uintptr_t>(workspace) & 7)
     return fail(ESEP_EALIGN, "beam_select: the workspace needs 8-byte alignment");
-  const int64_t rows = (int64_t)R * W, splits = esep::beam_splits(rows, V);
+  const int64_t rows = (int64_t)R * W, splits = esep::beam_splits(R, W, V, keep);
   esep::BeamArgs a{};
   a.logits = logits;
   a.scores = scores;
@@ -1187,13 +1187,12 @@ int esep_beam_select(const void* logits, int64_t ld_r, int64_t ld_w, const float
   a.V = (int)V;
   a.keep = keep;
   a.splits = (int)splits;
-  a.piece = esep::beam_piece(rows, V);
+  a.piece = esep::beam_piece(R, W, V, keep);
   if (rows * splits * esep::kBeamThreads >= int64_t{1} << 32)
     return fail(ESEP_ESHAPE, "beam_select: %lld rows of %lld are too many for one launch", (long long)rows,
                 (long long)V);
-  const bool vec = aligned16(logits) && V % 8 == 0 && (R == 1 || ld_ok(ld_r, dt)) && (W == 1 || ld_ok(ld_w, dt));
   bool sup = false;
-  const hipError_t e = esep::launch_beam_select(a, dt, vec, static_cast<hipStream_t>(stream), &sup);
+  const hipError_t e = esep::launch_beam_select(a, dt, static_cast<hipStream_t>(stream), &sup);
   if (!sup) return fail(ESEP_EINVAL, "beam_select: unsupported dtype");
   return e == hipSuccess ? 0 : hip_fail(e, "beam_select launch");
 }
