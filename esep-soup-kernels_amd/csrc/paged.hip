@@ -200,16 +200,18 @@ __global__ __launch_bounds__(256) void k_page_store(const PageStoreArgs a) {
 // The beams' states follow their parents, in place: a thread owns 16 bytes of a token of all beams of a request (of
 // one layer's K or V), reads what moves from each parent's page and then writes it to the beams' own, so that no
 // place is overwritten before it is read, whatever permutation or choice the parents are. Beams that stay are neither
-// read nor written, nor are pages that a beam shares with its parent. A block goes through a request's pages, whose
-// numbers are read once a page.
+// read nor written, nor are pages that a beam shares with its parent. A block goes through runs of a request's pages, whose
+// numbers are read once a run.
 //
 // Bound by the bytes that move. 12 requests of 8 beams, 358 to 391 tokens, 28 layers, 4 heads of 128 (1.45 GB moved): tokens
 // dealt to the threads one at a time, each with its own look at the tables, 472 us; a page to a block and two tokens at
 // once 325, four 318, stores past the caches 313 (4.6 TB/s; a copy reaches 5.0); half as many blocks 358, loads past the
-// caches 370.
+// caches 370. Runs of 16 tokens, of twice as many as a block copies at once where that is more: whole pages / 64 / 32 / 16 tokens,
+// one layer of 4 x 4 x 700 tokens in pages of 64 - / 10.4 / 7.9 / 7.4, contiguous caches (a page a row) of 4 beams of 8000
+// 828 / 14.2 / 13.5 / 12.0, 8 x 4 x 4000 801 / 87 / 88 / 84; 4 x 5 x 1800 with 2 heads of 64 - / 17.1 / 17.4 / 21.0.
 // ---------------------------------------------------------------------------------------
 template <int MOST, int UNROLL>
-__global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a) {
+__global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a, int each) {
   const int r = blockIdx.y, layer = blockIdx.z >> 1, cache = blockIdx.z & 1, lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.M * a.P;
   const int end = a.lengths[r] < cap ? a.lengths[r] : (int)cap;
@@ -226,8 +228,10 @@ __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a) {
   const int32_t* tables = a.tables + (int64_t)r * a.W * a.t_bs;
   const Pages pg = cache ? a.pages[1] : a.pages[0];
   uint16_t* const pages = static_cast<uint16_t*>(pg.p) + layer * pg.ls;
-  const int last = (end - 1) / a.P;
-  for (int page = start / a.P + blockIdx.x; page <= last; page += gridDim.x) {
+  const int runs = (a.P + each - 1) / each;  // of `each` tokens, the last of a page perhaps of fewer
+  const int last = (end - 1) / a.P * runs + (end - 1) % a.P / each;
+  for (int run = start / a.P * runs + start % a.P / each + blockIdx.x; run <= last; run += gridDim.x) {
+    const int page = run / runs;
     const int mine = lane < a.W ? tables[(int64_t)lane * a.t_bs + page] : -1;
     const int theirs = __shfl(mine, from);
     const bool moves = theirs != mine && (unsigned)theirs < (unsigned)a.N && (unsigned)mine < (unsigned)a.N;
@@ -239,8 +243,9 @@ __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a) {
       src[w] = __builtin_amdgcn_readlane(theirs, w) * pg.ps;
       dst[w] = __builtin_amdgcn_readlane(mine, w) * pg.ps;
     }
-    const int p0 = page * a.P > start ? 0 : start - page * a.P;
-    const int p1 = (int64_t)(page + 1) * a.P < end ? a.P : end - page * a.P;
+    const int at0 = page * a.P, run0 = (run - page * runs) * each, run1 = run0 + each < a.P ? run0 + each : a.P;
+    const int p0 = at0 + run0 > start ? run0 : start - at0;
+    const int p1 = run1 < end - at0 ? run1 : end - at0;
     for (int c = p.first; c < p.all; c += 256) {
       const int h = c / p.chunks, d = 8 * (c - h * p.chunks);
       uint16_t* const head = pages + h * pg.hs + d;
@@ -289,17 +294,20 @@ hipError_t launch_page_store(const PageStoreArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_beam_reorder(const BeamReorderArgs& a, hipStream_t s) {
-  // a request's own pages are known on the device only: blocks for 16 of a CU's, up to one to a page of the table
+  const int all = a.HK * (a.D / 8), at_once = all < 256 ? 256 / all : 1, run = at_once > 8 ? 2 * at_once : 16;
+  const int each = a.P < run ? a.P : run;
+  // a request's own pages are known on the device only: blocks for 16 of a CU's, up to one to a run of the table's pages
   const int64_t groups = (int64_t)a.R * a.L * 2, most = groups >= 16384 ? 1 : 16384 / groups;
-  const dim3 grid((unsigned)(most < a.M ? most : a.M), (unsigned)a.R, (unsigned)(2 * a.L));
+  const int64_t runs = (int64_t)a.M * ((a.P + each - 1) / each);
+  const dim3 grid((unsigned)(most < runs ? most : runs), (unsigned)a.R, (unsigned)(2 * a.L));
   if (a.W <= 4)
-    hipLaunchKernelGGL((k_beam_reorder<4, 4>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<4, 4>), grid, dim3(256), 0, s, a, each);
   else if (a.W <= 8)
-    hipLaunchKernelGGL((k_beam_reorder<8, 4>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<8, 4>), grid, dim3(256), 0, s, a, each);
   else if (a.W <= 16)
-    hipLaunchKernelGGL((k_beam_reorder<16, 2>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<16, 2>), grid, dim3(256), 0, s, a, each);
   else
-    hipLaunchKernelGGL((k_beam_reorder<kMostBeams, 1>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_beam_reorder<kMostBeams, 1>), grid, dim3(256), 0, s, a, each);
   return hipGetLastError();
 }
 

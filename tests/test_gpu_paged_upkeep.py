@@ -224,7 +224,8 @@ def _parents(rng, R, W, how):
     (1, 2, 1, 16, 1, 64, 1, torch.float16), (3, 4, 2, 16, 2, 128, 90, torch.bfloat16),
     (2, 5, 3, 7, 3, 64, 40, torch.float16), (4, 8, 1, 32, 4, 128, 100, torch.bfloat16),
     (2, 16, 2, 16, 2, 64, 50, torch.float16), (1, 32, 1, 16, 5, 64, 33, torch.bfloat16),
-    (2, 3, 1, 64, 20, 256, 70, torch.float16), (1, 1, 1, 16, 1, 64, 20, torch.float16)])
+    (2, 3, 1, 64, 20, 256, 70, torch.float16), (1, 1, 1, 16, 1, 64, 20, torch.float16),
+    (2, 3, 1, 100, 4, 128, 270, torch.bfloat16), (1, 4, 2, 333, 1, 64, 600, torch.float16)])
 def test_reorder(R, W, L, P, HK, D, top, dtype, how):
     from solution.body.paged import beam_reorder
 
