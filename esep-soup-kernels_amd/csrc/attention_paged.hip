@@ -347,6 +347,19 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 2 : 3) void k_attn_paged_solo(c
   const int G = a.HQ / a.HK, RT = (G * a.n + 31) / 32;
   const int rt = (int)(blockIdx.x % RT), kvh = (int)(blockIdx.x / RT % a.HK), b = (int)(blockIdx.x / RT / a.HK);
   const PagedRow row = paged_row<false>(a, b);
+  if constexpr (NW == 1) {
+    const int mask = (1 << a.page_shift) - 1;
+    const PagedFill<RB, NT> fk(lane, a.k_ps * (int64_t)sizeof(T), a.k_ts * (int64_t)sizeof(T), mask);
+    const PagedFill<RB, NT> fv(lane, a.v_ps * (int64_t)sizeof(T), a.v_ts * (int64_t)sizeof(T), mask);
+    PagedTile<T, D, ROWS> tile(lane);
+    const PagedQuery at(a, row, kvh, ROWS * rt + tile.row());
+    if (row.tiles > 0)
+      paged_walk<T, D, NT, ROWS>(a, row, at, kvh, rt, 0, row.tiles, fk, fv, rings[0], lane, tile);
+    else
+      tile.load(nullptr, false);
+    if (at.ok) tile.store(static_cast<T*>(a.o) + (((int64_t)at.b * a.n + at.tok) * a.HQ + at.h) * D);
+    return;
+  }
   const int each = (row.tiles + NW - 1) / NW, busy = each > 0 ? (row.tiles + each - 1) / each : 0;
   if (w < busy) {
     const int mask = (1 << a.page_shift) - 1;
@@ -486,7 +499,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_paged_join(const AttnPagedArgs
 }
 
 // Wavefronts to a group up to which a row's few parts are added by one lane each, so that a block joins 256 / (D / 2)
-// rows (256 rows of up to 300 tokens, 28 / 4 heads of 128: 38 -> 32 us in all; with it up to 8 wavefronts to a group
+// rows (256 rows of up to 300 tokens in wider tables, 28 / 4 heads of 128: 38 -> 32 us in all; with it up to 8 wavefronts to a group
 // 32 rows of 4 beams over up to 8000 shared tokens 35.3 -> 38.5).
 constexpr int64_t kPagedFewParts = 2;
 
@@ -505,7 +518,9 @@ void walk(const AttnPagedArgs& a, const PagedSizes& z, hipStream_t s) {
   if constexpr (!SHARED) {
     if constexpr (D == 64)
       if (z.solo == 8) return solo<T, D, 8, ROWS>(a, z, s);
-    if (z.solo) return solo<T, D, 4, ROWS>(a, z, s);
+    if (z.solo == 4) return solo<T, D, 4, ROWS>(a, z, s);
+    if (z.solo == 2) return solo<T, D, 2, ROWS>(a, z, s);
+    if (z.solo == 1) return solo<T, D, 1, ROWS>(a, z, s);
   }
   const dim3 grid((unsigned)(z.units > 0 ? z.units : 1));
   if (D == 128 && z.all_tiles == 1)

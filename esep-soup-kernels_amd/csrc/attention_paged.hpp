@@ -32,26 +32,34 @@ struct PagedSizes {
   bool shared;
   int solo;  // one launch: wavefronts to a block, else 0
 };
-// One launch, a block of four or eight wavefronts to a group, instead of the cut walk with its partials and their
-// join: where one round of blocks takes all groups, and a block's wavefronts have only so many tiles more than the
-// walk's would (up to four of few tiles; of many, 5 / 8 of an equal share, as rows are ragged) that its launch and,
-// with many groups, their partials cost more. As many wavefronts as the rings of a CU's LDS allow: at D = 64 eight,
-// while a CU has one block.
+// One launch, a block of one to eight wavefronts to a group, instead of the cut walk with its partials and their
+// join: where a block's wavefronts have only so many tiles more than the walk's would that its launch, its search for
+// a wavefront's first group and, with many groups, their partials and starts cost more. That is up to four of few
+// tiles; of many, 5 / 8 of an equal share, as rows are ragged (all of it for a single row's), in one round of blocks;
+// then a few, more with more groups. As many wavefronts to a block as the rings of the CUs' LDS allow, so that one
+// round takes all groups where it can. Shared tokens count once: the one launch reads them for each row.
 //
 // Both launches / one in us (graph replays over caches that no cache of the card holds; *: taken, else the one
 // launch). D = 128, 28 / 4 heads: 64 rows of up to 300 tokens 17.9 / 10.5, 1500 35.3 / 29.5, 2500 55.5 / 52.9, 4000
 // 77.9* / 79.9; 32 of 700 17.5 / 14.0, 2000 26.5* / 29.5; 5 of 900 13.1 / 14.5 (the launch saved takes the host 3
-// us); 12 / 2 heads, one row of 60 8.3 / 4.8, 700 9.3 / 11.6 (the same), 1000 9.5* / 14.6. D = 64, 14 / 2 heads, both
-// / four wavefronts / eight: one row of 300 8.4 / 5.8 / 6.1, 700 9.1 / 8.2 / 7.2, 1500 9.5* / 12.6 / 10.1; 32 of 1000
-// 14.1 / 11.5 / 10.7, 2500 17.2* / 20.6 / 19.1; 7 of 5 new tokens and a window of 1500 14.4 / 16.5 / 13.7; 120 of
-// 4000 43.7 / 40.7 / 40.9; 130 (260 groups) of 1200 23.0 / 19.1, 2000 29.2* / 31.9; 8 / 8 heads, 40 of 1200 22.6 /
-// 21.5, 2000 28.4* / 36.6.
-inline int paged_solo(int64_t groups, int64_t tiles, int D) {
-  const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles;
-  const int each = D == 64 && groups <= kAttnCUs ? 8 : 4;
-  const int64_t few = total / kAttnCUs < 4 ? total / kAttnCUs : 4, many = total * 5 / 8 / waves;
-  const int64_t more = D == 64 ? 4 + groups / 64 : 6 + groups / 40;
-  return groups <= waves / each && (tiles + each - 1) / each <= (few > many ? few : many) + more ? each : 0;
+// us); 256 of 300 31.8 / 25.0, 3000 203* / 212; 600 of 300 68.0 / 55.2, 1500 226* / 226; 4 of 128 new tokens and 2000
+// 62.9 / 45.9, one of 512 and 4000 135 / 92; 4 beams each, 64 of 500 24.9 / 13.0, 2000 32.6* / 34.6, 256 of 300 35.2
+// / 24.2. 12 / 2 heads: one row of 60 8.3 / 4.8, 700 9.3 / 11.6 (as before), 1000 9.5* / 14.6; 300 of 60 22.1 / 7.5;
+// 3000 of 60 80.5 / 37.9. 32 / 32 heads: 64 of 500 75.5 / 74.7, 1500 180* / 209.
+//
+// D = 64, 14 / 2 heads: one row of 300 8.4 / 6.1, 700 9.1 / 7.2, 1500 9.5* / 10.1; 32 of 1000 14.1 / 10.7, 2500 17.2*
+// / 19.1; 7 of 5 new tokens and a window of 1500 14.4 / 13.7; 120 of 4000 43.7 / 40.9; 130 of 1200 23.0 / 19.1, 2000
+// 29.2* / 31.9; 700 of 60 24.7 / 7.7, 1500 81.7* / 79.4; 8 beams each, 2000 of 100 116 / 20. (With four wavefronts
+// where eight fit: one row of 700 8.2, 32 of 1000 11.5.)
+inline int paged_solo(int B, int64_t groups, int64_t tiles, int W, int D) {
+  const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles / W;
+  int each = D == 128 ? 4 : 8;
+  while (each > 1 && groups * each > waves) each /= 2;
+  const int64_t few = total / kAttnCUs < 4 ? total / kAttnCUs : 4;
+  const int64_t many = groups > waves ? 0 : (B == 1 ? total : total * 5 / 8) / waves;
+  const int64_t starts = groups < waves ? groups : waves;
+  const int64_t more = D == 64 || W > 1 ? 4 + starts / 64 : 6 + starts / 40;
+  return (tiles + each - 1) / each <= (few > many ? few : many) + more ? each : 0;
 }
 inline PagedSizes paged_sizes(int B, int n, int W, int S, int HQ, int HK, int D, int window, int sinks,
                               bool shared) {
@@ -62,7 +70,7 @@ inline PagedSizes paged_sizes(int B, int n, int W, int S, int HQ, int HK, int D,
   const int64_t all = ((int64_t)S + 31) / 32 + 1;  // the sinks' end and the window's begin may share one
   const int64_t seen = ((int64_t)sinks + 31) / 32 + ((int64_t)window + n + 61) / 32;
   const int64_t each = seen < all ? seen : all;
-  z.solo = paged_solo(own, each, D);
+  z.solo = paged_solo(B, own, each, shared ? W : 1, D);
   z.shared = shared && z.solo == 0;
   z.all_rows = z.shared ? z.rows * W : z.rows;
   z.all_tiles = (z.all_rows + 31) / 32;

@@ -78,7 +78,9 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, scale=None, window=Non
     Query t of a row sits at position p = lengths - n + t and sees key j <= p, through a window only if p - j < window or
     j < sinks. What lies in the pages past a row's length, before its window or in pages of other rows is never
     read. Keys of a page outside the pool (an entry of -1) are not seen. A query that sees none gets 0, as one at a
-    position below 0 does. Lengths past M * P count as that. Rounding and infinities are cache_attention's.
+    position below 0 does. Lengths past M * P count as that. Rounding and infinities are cache_attention's. The tables' width is
+    all that the host knows of the lengths: where rows are short, tables[:, :m] that just holds them takes one
+    launch that suits them (300 rows of 60 tokens 7 us instead of 22).
 
     beams, shared (int32 [B // beams]): rows r * beams .. + beams - 1 hold their first shared[r] tokens in the same
     pages (a request's beams over its prompt). The pages are then read once for all of them instead of once for

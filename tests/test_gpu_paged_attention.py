@@ -147,8 +147,9 @@ def test_shared_pages(case, dtype):
                        paged_attention(q, kp, vp, tables, _i(lengths), window=50))
 
 
-@pytest.mark.parametrize("rows", [64, 65, 200, 300])
-def test_many_rows(rows):
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("rows", [64, 65, 200, 300, 1100])
+def test_many_rows(rows, wide):
     """More rows than a wavefront has lanes, of all lengths, empty ones among them; also as beams of nothing in common."""
     from solution.body.paged import paged_attention
 
@@ -157,6 +158,7 @@ def test_many_rows(rows):
     lengths[rows // 3] = 600
     q, k, v = _inputs(rows, 1, 608, 4, 2, 64, torch.float16, 5)
     kp, vp, tables = _scatter(k, v, lengths, 16, rng)
+    tables = _wide(tables, 16) if wide else tables
     ref, tol = _reference(q, k, v, lengths, 0.125, None, 0, 2.0 ** -11, 2.0 ** -25)
     _check(paged_attention(q, kp, vp, tables, _i(lengths)), ref, tol, rows)
     if rows % 5 == 0:
@@ -164,7 +166,8 @@ def test_many_rows(rows):
         _check(paged_attention(q, kp, vp, tables, _i(lengths), beams=5, shared=none), ref, tol, rows)
 
 
-def test_more_groups_than_wavefronts():
+@pytest.mark.parametrize("wide", [False, True])
+def test_more_groups_than_wavefronts(wide):
     """9600 (row, kv head) groups of one to three tiles: a wavefront walks several."""
     from solution.body.paged import paged_attention
 
@@ -172,13 +175,15 @@ def test_more_groups_than_wavefronts():
     lengths = [rng.randrange(96) for _ in range(1200)]
     q, k, v = _inputs(1200, 1, 96, 8, 8, 64, torch.bfloat16, 6)
     kp, vp, tables = _scatter(k, v, lengths, 32, rng)
+    tables = _wide(tables, 32) if wide else tables
     ref, tol = _reference(q, k, v, lengths, 0.125, None, 0, 2.0 ** -8, 0.0)
     _check(paged_attention(q, kp, vp, tables, _i(lengths)), ref, tol, "groups")
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("beams", [1, 3])
 @pytest.mark.parametrize("D", [64, 128])
-def test_more_rows_than_wavefronts(D, beams):
+def test_more_rows_than_wavefronts(D, beams, wide):
     """Rows of one or two parts, joined several to a block, their number no multiple of those."""
     from solution.body.paged import paged_attention
 
@@ -191,6 +196,7 @@ def test_more_rows_than_wavefronts(D, beams):
         s = shared[b // beams]
         k[b, :s], v[b, :s] = k[b // beams * beams, :s].clone(), v[b // beams * beams, :s].clone()
     kp, vp, tables = _scatter(k, v, lengths, 16, rng, shared=shared if beams > 1 else None, beams=beams)
+    tables = _wide(tables, 16) if wide else tables
     ref, tol = _reference(q, k, v, lengths, D ** -0.5, None, 0, 2.0 ** -11, 2.0 ** -25)
     o = paged_attention(q, kp, vp, tables, _i(lengths), beams=beams, shared=_i(shared))
     _check(o, ref, tol, "rows")
