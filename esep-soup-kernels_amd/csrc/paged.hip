@@ -14,6 +14,9 @@ namespace {
 // by tokens: a block takes kTableTokens of them, finds its rows by prefix sums over the rows (of n and of the new
 // pages), 256 rows at a time, and a token its row by a binary search of those. Block 0 goes through all rows
 // and writes the offsets and the new lengths.
+//
+// Bound by latency: lengths, a scan's two barriers, a page's number, the slot. 64 rows of one new token 3.5 us, 300 rows of up
+// to 2047 (300000 tokens) 7.8, 4000 rows of one 22.6; a thread's four tokens ask for their pages together.
 // ---------------------------------------------------------------------------------------
 constexpr int kTableTokens = 1024, kTableEach = kTableTokens / 256;
 
@@ -203,12 +206,14 @@ __global__ __launch_bounds__(256) void k_page_store(const PageStoreArgs a) {
 // read nor written, nor are pages that a beam shares with its parent. A block goes through runs of a request's pages, whose
 // numbers are read once a run.
 //
-// Bound by the bytes that move. 12 requests of 8 beams, 358 to 391 tokens, 28 layers, 4 heads of 128 (1.45 GB moved): tokens
-// dealt to the threads one at a time, each with its own look at the tables, 472 us; a page to a block and two tokens at
-// once 325, four 318, stores past the caches 313 (4.6 TB/s; a copy reaches 5.0); half as many blocks 358, loads past the
-// caches 370. Runs of 16 tokens, of twice as many as a block copies at once where that is more: whole pages / 64 / 32 / 16 tokens,
-// one layer of 4 x 4 x 700 tokens in pages of 64 - / 10.4 / 7.9 / 7.4, contiguous caches (a page a row) of 4 beams of 8000
-// 828 / 14.2 / 13.5 / 12.0, 8 x 4 x 4000 801 / 87 / 88 / 84; 4 x 5 x 1800 with 2 heads of 64 - / 17.1 / 17.4 / 21.0.
+// Bound by the bytes that move. 12 requests of 8 beams, 358 to 391 tokens, 28 layers, 4 heads of 128, pages of 64 (1.45 GB
+// moved): tokens dealt to the threads one at a time, each with its own look at the tables, 472 us; a page to a block and two
+// tokens at once 325, four 318, stores past the caches 313; in runs of 16 tokens, whatever the page, 286 (5.1 TB/s, what
+// a copy reaches). With whole pages, half as many blocks took 358, loads past the caches 370.
+//
+// A run is 16 tokens, or twice what a block copies at once where that is more. Whole pages / 64 / 32 / 16 tokens: one layer of
+// 4 x 8 x 700 tokens in pages of 64 - / 35.7 / 25.4 / 21.3, contiguous caches (a page a row) of 4 beams of 8000 tokens 828 /
+// 14.2 / 13.5 / 12.0, 8 x 4 x 4000 801 / 87 / 88 / 84; 4 x 5 x 1800 with 2 heads of 64 - / 17.1 / 17.4 / 21.0.
 // ---------------------------------------------------------------------------------------
 template <int MOST, int UNROLL>
 __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a, int each) {

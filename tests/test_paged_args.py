@@ -107,8 +107,9 @@ def test_attention_workspace():
     assert ws(2, 1, 2048, 16, 4, 2, 64, beams=2, shared=True) == 12 + (1537 + 6) * 4 * 66
     # short rows in one launch: none
     assert ws(1, 1, 44, 16, 12, 2, 128) == 0 and ws(1, 1, 64, 16, 12, 2, 128) > 0
-    assert ws(64, 1, 64, 16, 28, 4, 128) == 0 and ws(65, 1, 64, 16, 28, 4, 128) > 0  # one round of blocks
-    assert ws(128, 1, 64, 16, 28, 4, 64) == 0 and ws(129, 1, 64, 16, 28, 4, 64) > 0
+    assert ws(64, 1, 64, 16, 28, 4, 128) == 0  # one round of large blocks, or
+    assert ws(65, 1, 64, 16, 28, 4, 128) == 0 and ws(129, 1, 64, 16, 28, 4, 64) == 0  # of smaller ones
+    assert ws(1000, 1, 20, 16, 28, 4, 64) == 0 and ws(1000, 1, 256, 16, 28, 4, 64) > 0  # several rounds
     assert ws(8, 1, 2048, 16, 12, 2, 128) > 0 and ws(8, 1, 2048, 16, 12, 2, 128, 300, 4) == 0  # a window keeps them short
     assert ws(8, 1, 16, 16, 12, 2, 128, beams=4, shared=True) == 0
     assert ws(0, 1, 1, 16, 1, 1, 64) == 0 and ws(1, 1, 1, 24, 1, 1, 64) == 0
