@@ -204,7 +204,19 @@ __global__ __launch_bounds__(64, D == 128 ? 2 : 3) void k_attn_cache(const AttnC
       store_rows_t<T, D>(static_cast<T*>(a.o) + (((int64_t)b * a.n + tok) * a.HQ + h) * D, oacc, hi,
                          l > 0.f ? 1.f / l : 0.f);
     } else if (rok) {
-      store_part<D>(part, live, lq, hi, m, l, oacc);
+      if (hi == 0) {
+        part[lq] = m;
+        part[live + lq] = l;
+      }
+      float* po = part + 2 * live + lq * D + 4 * hi;
+#pragma unroll
+      for (int md = 0; md < D / 32; ++md)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+            *reinterpret_cast<float2*>(po + 32 * md + 8 * j + e) =
+                make_float2(oacc[md][4 * j + e], oacc[md][4 * j + e + 1]);
     }
   }
 }

@@ -1,6 +1,6 @@
 // What the walks over a cache (attention_cache.hip) and over pages (attention_paged.hip) share: the tiles of all
-// groups laid end to end and cut into one run to a wavefront, the waits of a wavefront's own ring, the
-// partials of the groups that are cut.
+// groups laid end to end and cut into one run to a wavefront, the waits of a wavefront's own ring, the join's
+// large blocks.
 #pragma once
 
 #include "attention.hpp"
@@ -34,25 +34,6 @@ __device__ __forceinline__ CachePlan cache_plan(int tiles, int D) {
 // s_waitcnt vmcnt(N) and lgkmcnt(0) (the other counters at their maxima).
 constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 constexpr int kWaitLgkm0 = 0xC07F;
-
-// A cut group's partial of `live` query rows: maxima, sums, weighted sums.
-template <int D>
-__device__ __forceinline__ void store_part(float* part, int live, int lq, int hi, float m, float l,
-                                           const f32x16 (&oacc)[D / 32]) {
-  if (hi == 0) {
-    part[lq] = m;
-    part[live + lq] = l;
-  }
-  float* po = part + 2 * live + lq * D + 4 * hi;
-#pragma unroll
-  for (int md = 0; md < D / 32; ++md)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2)
-        *reinterpret_cast<float2*>(po + 32 * md + 8 * j + e) =
-            make_float2(oacc[md][4 * j + e], oacc[md][4 * j + e + 1]);
-}
 
 // Parts of a group from which its rows, where there are no more than CUs, are joined by blocks of 1024 threads
 // instead of 256 (12 rows of 512 parts each 17 -> 5.5 us; 896 rows of 27 4.9 -> 8.7).
