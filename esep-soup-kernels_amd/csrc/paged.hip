@@ -208,8 +208,8 @@ __global__ __launch_bounds__(256) void k_page_store(const PageStoreArgs a) {
 //
 // Bound by the bytes that move. 12 requests of 8 beams, 358 to 391 tokens, 28 layers, 4 heads of 128, pages of 64 (1.45 GB
 // moved): tokens dealt to the threads one at a time, each with its own look at the tables, 472 us; a page to a block and two
-// tokens at once 325, four 318, stores past the caches 313; in runs of 16 tokens, whatever the page, 286 (5.1 TB/s, what
-// a copy reaches). With whole pages, half as many blocks took 358, loads past the caches 370.
+// tokens at once 325, four 318, stores past the caches 313; in runs of 16 tokens, whatever the page, 286, an odd
+// number of blocks to a request 283 (5.1 TB/s, what a copy reaches). With whole pages, half as many blocks took 358, loads past the caches 370.
 //
 // A run is 16 tokens, or twice what a block copies at once where that is more. Whole pages / 64 / 32 / 16 tokens: one layer of
 // 4 x 8 x 700 tokens in pages of 64 - / 35.7 / 25.4 / 21.3, contiguous caches (a page a row) of 4 beams of 8000 tokens 828 /
@@ -222,6 +222,10 @@ __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a, i
   const int end = a.lengths[r] < cap ? a.lengths[r] : (int)cap;
   const int start = a.start == nullptr || a.start[r] < 0 ? 0 : a.start[r];
   if (start >= end) return;
+  const int runs = (a.P + each - 1) / each;  // of `each` tokens, the last of a page perhaps of fewer
+  const int first = start / a.P * runs + start % a.P / each + blockIdx.x;
+  const int last = (end - 1) / a.P * runs + (end - 1) % a.P / each;
+  if (first > last) return;
   // lane w: the parent of beam w where it moves, else w
   int from = lane;
   if (lane < a.W) {
@@ -233,9 +237,7 @@ __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a, i
   const int32_t* tables = a.tables + (int64_t)r * a.W * a.t_bs;
   const Pages pg = cache ? a.pages[1] : a.pages[0];
   uint16_t* const pages = static_cast<uint16_t*>(pg.p) + layer * pg.ls;
-  const int runs = (a.P + each - 1) / each;  // of `each` tokens, the last of a page perhaps of fewer
-  const int last = (end - 1) / a.P * runs + (end - 1) % a.P / each;
-  for (int run = start / a.P * runs + start % a.P / each + blockIdx.x; run <= last; run += gridDim.x) {
+  for (int run = first; run <= last; run += gridDim.x) {
     const int page = run / runs;
     const int mine = lane < a.W ? tables[(int64_t)lane * a.t_bs + page] : -1;
     const int theirs = __shfl(mine, from);
@@ -304,7 +306,9 @@ hipError_t launch_beam_reorder(const BeamReorderArgs& a, hipStream_t s) {
   // a request's own pages are known on the device only: blocks for 16 of a CU's, up to one to a run of the table's pages
   const int64_t groups = (int64_t)a.R * a.L * 2, most = groups >= 16384 ? 1 : 16384 / groups;
   const int64_t runs = (int64_t)a.M * ((a.P + each - 1) / each);
-  const dim3 grid((unsigned)(most < runs ? most : runs), (unsigned)a.R, (unsigned)(2 * a.L));
+  // an odd number, so that the requests' first runs, of wide tables all that has work, are not all the same XCDs' (2 x 8
+  // beams of 21 tokens in tables of 32 pages, 24 layers, 4 heads of 128: 41.8 -> 15.0 us; 12 x 8 of 390 892 -> 840)
+  const dim3 grid((unsigned)(most < runs ? most : runs) | 1u, (unsigned)a.R, (unsigned)(2 * a.L));
   if (a.W <= 4)
     hipLaunchKernelGGL((k_beam_reorder<4, 4>), grid, dim3(256), 0, s, a, each);
   else if (a.W <= 8)
