@@ -23,7 +23,8 @@
 // block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us at the beams, but 10.2 instead of 7.0 for the
 // one row), rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to
 // three tiles to a wavefront (-7% to +7% over twenty shapes), partials eight columns at a time (the join reads 32
-// bytes of a line) or through LDS in whole lines (no change over twenty shapes), joins by 512 threads (+1 to 4%).
+// bytes of a line) or through LDS in whole lines (no change over twenty shapes), joins by 512 threads (+1 to 4%) or of
+// half the columns (-4 to +24%).
 #include <cmath>
 
 #include "attention_cache.hpp"

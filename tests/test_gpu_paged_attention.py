@@ -202,6 +202,21 @@ def test_more_rows_than_wavefronts(D, beams, wide):
     _check(o, ref, tol, "rows")
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3)])
+@pytest.mark.parametrize("B,n,HQ,HK,D", [(100, 20, 12, 2, 128), (60, 11, 12, 2, 128), (150, 9, 14, 2, 64),
+                                         (300, 9, 14, 2, 64)])
+def test_many_rows_of_several_query_tiles(B, n, HQ, HK, D, window, sinks):
+    """Blocks of one and two wavefronts, a query tile of a kv head each; empty rows and rows shorter than n among them."""
+    from solution.body.paged import paged_attention
+
+    rng = random.Random(B)
+    lengths = [rng.choice([0, 1, n - 1, n, 33, 40 + rng.randrange(110)]) for _ in range(B)]
+    q, k, v = _inputs(B, n, 160, HQ, HK, D, torch.float16, 8)
+    kp, vp, tables = _scatter(k, v, lengths, 16, rng)
+    ref, tol = _reference(q, k, v, lengths, D ** -0.5, window, sinks, 2.0 ** -11, 2.0 ** -25)
+    _check(paged_attention(q, kp, vp, tables, _i(lengths), window=window, sinks=sinks), ref, tol, "tiles")
+
+
 def test_long_runs():
     """A wavefront's run is longer than the 32 tiles whose pages it reads at once."""
     from solution.body.paged import paged_attention
