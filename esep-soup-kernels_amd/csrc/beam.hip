@@ -96,6 +96,25 @@ __device__ __forceinline__ int rank_sum(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);  // the other quad of each 8
 }
 
+// How many of a lane's share of the n listed are better; of a long list four looked at at once (384 in one piece 34 -> 13 us;
+// of ten that takes 0.3 us more).
+template <class F>
+__device__ __forceinline__ int betters(int n, int first, F&& better) {
+  int count = 0;
+  if (n <= 64) {
+    for (int j = first; j < n; j += kRankLanes) count += better(j);
+    return count;
+  }
+  for (int j0 = first; j0 < n; j0 += 4 * kRankLanes) {
+    bool b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = better(j0 + i * kRankLanes < n ? j0 + i * kRankLanes : j0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) count += b[i] && j0 + i * kRankLanes < n;
+  }
+  return count;
+}
+
 // 16 bytes of logits, wherever they lie (a row of an odd vocabulary begins anywhere).
 typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -114,7 +133,8 @@ __global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a)
   if (!(fabsf(score) < INFINITY)) return;  // the beam is out: the join does not look at its pieces
   const int r = row / a.W;
   const T* x = static_cast<const T*>(a.logits) + r * a.r_bs + (row - r * a.W) * a.w_bs;
-  const int base = split * a.piece + 8 * (int)threadIdx.x;
+  const int base = split * a.each + 8 * (int)threadIdx.x;
+  const int end = base - 8 * (int)threadIdx.x + a.each < a.V ? base - 8 * (int)threadIdx.x + a.each : a.V;
   float v[U][8];
   if (threadIdx.x == 0) count = 0;
   // all of it is asked for at once, in pieces of 16 bytes at any address; eights that the row does not fill are read at its
@@ -123,7 +143,7 @@ __global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a)
   if (a.V >= 8) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Any16* at = reinterpret_cast<const Any16*>(x + (base + 2048 * u + 7 < a.V ? base + 2048 * u : 0));
+      const Any16* at = reinterpret_cast<const Any16*>(x + (base + 2048 * u + 7 < end ? base + 2048 * u : 0));
       raw[u].a = at[0];
       if constexpr (sizeof(T) == 4) raw[u].b = at[1];
     }
@@ -134,11 +154,14 @@ __global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     Buf<T>::unpack(raw[u], v[u]);
-    if (base + 2048 * u + 7 >= a.V) {
+    const int at = base + 2048 * u;
+    if (at + 7 >= end) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = base + 2048 * u + e;
-        v[u][e] = i < a.V ? (float)x[i] : -INFINITY;
+      for (int e = 0; e < 8; ++e) v[u][e] = -INFINITY;
+      if (at < end) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (at + e < end) v[u][e] = (float)x[at + e];
       }
     }
   }
@@ -198,9 +221,7 @@ __global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a)
   if (n <= kList) {
     for (int i = threadIdx.x / kRankLanes; i < n; i += kBeamThreads / kRankLanes) {
       const uint64_t k = list[i];
-      int place = 0;
-      for (int j = threadIdx.x % kRankLanes; j < n; j += kRankLanes) place += list[j] > k;
-      place = rank_sum(place);
+      const int place = rank_sum(betters(n, (int)threadIdx.x % kRankLanes, [&](int j) { return list[j] > k; }));
       if (place < a.keep && threadIdx.x % kRankLanes == 0) out[place] = k;
     }
     for (int i = n + threadIdx.x; i < a.keep; i += kBeamThreads) out[i] = 0;
@@ -242,15 +263,16 @@ __device__ __forceinline__ bool before(const Cand& x, const Cand& y) {
   return x.value > y.value || (x.value == y.value && x.at < y.at);
 }
 
-constexpr int kJoinThreads = 1024, kJoinFirst = kBeamJoinFirst, kJoinMore = 8, kJoinMostBeams = 64;
+constexpr int kJoinFirst = kBeamJoinFirst, kJoinMore = 8, kJoinMostBeams = 64;
 
-__global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
-  constexpr int NW = kJoinThreads / 64;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_beam_join(const BeamArgs a) {
+  constexpr int NW = THREADS / 64;
   // lse = top + rest, apart, so that large logits do not swallow the rest; score: NaN where the beam is out
   __shared__ double rest[kJoinMostBeams], score[kJoinMostBeams];
   __shared__ float tops[kJoinMostBeams];
   __shared__ Cand list[kList], w_best[NW];
-  __shared__ float group[kJoinThreads];
+  __shared__ float group[THREADS];
   __shared__ int chosen[kBeamMostKeep];
   __shared__ int count;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = wave_id();
@@ -312,7 +334,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
     mine[j] = value(index(j) < all ? index(j) : 0, key[j]);
     best32 = fmaxf(best32, (float)mine[j].value);
   }
-  const int rounds = (all + kJoinThreads - 1) / kJoinThreads;
+  const int rounds = (all + THREADS - 1) / THREADS;
   // f of the thread's candidates from j0 on, kJoinMore asked for at once
   auto each_from = [&](int j0, auto&& f) {
 #pragma unroll 1
@@ -372,11 +394,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const BeamArgs a) {
     }
     return;
   }
-  for (int i = tid / kRankLanes; i < n; i += kJoinThreads / kRankLanes) {
+  for (int i = tid / kRankLanes; i < n; i += THREADS / kRankLanes) {
     const Cand c = list[i];
-    int place = 0;
-    for (int j = tid % kRankLanes; j < n; j += kRankLanes) place += before(list[j], c);
-    place = rank_sum(place);
+    const int place = rank_sum(betters(n, tid % kRankLanes, [&](int j) { return before(list[j], c); }));
     if (place < a.keep && tid % kRankLanes == 0) put(place, c);
   }
   if (n >= a.keep) return;
@@ -404,7 +424,12 @@ hipError_t run(const BeamArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_beam_rows<T, 4>), grid, dim3(kBeamThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.R), dim3(kJoinThreads), 0, s, a);
+  // small blocks for many requests' few candidates (2000 of 24 candidates 41.5 -> 32.5 us in all, 4000 of 32 90 -> 72; 24 of
+  // 475 13.2 -> 13.6)
+  if (a.R > 256 && (int64_t)a.W * a.splits * a.keep <= 256 * kJoinFirst)
+    hipLaunchKernelGGL((k_beam_join<256>), dim3((unsigned)a.R), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_beam_join<1024>), dim3((unsigned)a.R), dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 

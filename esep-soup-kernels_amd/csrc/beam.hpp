@@ -19,7 +19,8 @@ struct BeamArgs {
   int32_t* out_parents;
   int32_t* out_tokens;
   int64_t r_bs, w_bs;
-  int R, W, V, keep, splits, piece;
+  int R, W, V, keep, splits;
+  int piece, each;  // elements that a block has room for, and that it takes: pieces of one size, as few values bound nothing
 };
 
 // Candidates that a thread of the join (of 1024) asks for at once.

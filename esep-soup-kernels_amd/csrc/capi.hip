@@ -1188,6 +1188,7 @@ int esep_beam_select(const void* logits, int64_t ld_r, int64_t ld_w, const float
   a.keep = keep;
   a.splits = (int)splits;
   a.piece = esep::beam_piece(R, W, V, keep);
+  a.each = (int)((V + splits - 1) / splits + 7) & ~7;
   if (rows * splits * esep::kBeamThreads >= int64_t{1} << 32)
     return fail(ESEP_ESHAPE, "beam_select: %lld rows of %lld are too many for one launch", (long long)rows,
                 (long long)V);

@@ -74,7 +74,8 @@ def _inputs(R, W, V, dtype, seed, scale=2.5):
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("R,W,V,keep", [(1, 1, 1, 1), (1, 2, 5, 10), (2, 64, 100, 64), (1, 4, 151936, 8),
                                         (3, 5, 50001, 10), (70, 3, 1000, 6), (24, 5, 50000, 5), (2, 3, 2049, 64),
-                                        (30, 8, 32000, 16), (1, 1, 70000, 1)])
+                                        (30, 8, 32000, 16), (1, 1, 70000, 1), (1, 1, 151936, 64),
+                                        (300, 3, 1000, 8), (260, 2, 4099, 20)])
 def test_select(R, W, V, keep, dtype):
     logits, scores = _inputs(R, W, V, dtype, R * 7 + V % 13)
     got = _go(logits, scores, keep)
