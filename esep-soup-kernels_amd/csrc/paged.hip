@@ -243,13 +243,16 @@ __global__ __launch_bounds__(256) void k_beam_reorder(const BeamReorderArgs a, i
     const int theirs = __shfl(mine, from);
     const bool moves = theirs != mine && (unsigned)theirs < (unsigned)a.N && (unsigned)mine < (unsigned)a.N;
     const uint64_t go = __ballot(moves);
-    if (go == 0 || p.idle()) continue;
+    if (go == 0) continue;
+    // read before the idle threads go on: a wavefront's idle lanes (HK D / 8 = 136 pieces leave 56 in the third) may hold
+    // pages of beams, and what the compiler moves or spills behind that branch it moves in the others' lanes only
     int64_t src[MOST], dst[MOST];
 #pragma unroll
     for (int w = 0; w < MOST; ++w) {
       src[w] = __builtin_amdgcn_readlane(theirs, w) * pg.ps;
       dst[w] = __builtin_amdgcn_readlane(mine, w) * pg.ps;
     }
+    if (p.idle()) continue;
     const int at0 = page * a.P, run0 = (run - page * runs) * each, run1 = run0 + each < a.P ? run0 + each : a.P;
     const int p0 = at0 + run0 > start ? run0 : start - at0;
     const int p1 = run1 < end - at0 ? run1 : end - at0;
