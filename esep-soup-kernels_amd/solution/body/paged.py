@@ -13,7 +13,15 @@ of which the first `taken` are in use. A step, all of it on the device and fit f
     paged_store(k, v, k_pages, v_pages, plan.slots)
     o = paged_attention(q, k_pages, v_pages, tables, plan.lengths)
 
-Pages of a row that is done go back by the host: their numbers to free[taken - n:taken], taken -= n.
+Pages go back by the host, between steps. Of the list, used = min(taken, F) entries are in use (taken also counts the
+pages that were not there). A row that is done: its n numbers of 0 or more among tables[b, :ceil(lengths[b] / P)] to
+free[used - n:used], taken = used - n, lengths[b] = 0; pages that rows share go back once, with the last of them.
+
+Where taken was more than F, rows have gone short: one that did has -1 among those entries, and holds its tokens before
+the first such page, j, only. A page is taken for its first token and for no later one (what lies in it for the
+earlier ones would be another row's). So the row goes on once its numbers behind j have gone back as well and lengths[b] =
+j * P: its tokens from there on are given anew. Left as it is, it gets slots again from its next page on, and
+nothing sees the keys of the page that is missing.
 """
 
 from typing import NamedTuple
@@ -44,8 +52,9 @@ def block_tables(tables, lengths, new, free, taken, page, total, update=False):
 
     A token whose row is full (M * page tokens, which the new lengths never pass) or for which no free page is left
     gets slot -1; in the latter case the table's entry is -1 (paged_attention sees none of that page's keys) and the
-    new `taken` is more than F. With update, lengths and taken are changed in place, else they are left
-    and the same call can be made again."""
+    new `taken` is more than F: the pages that were not there count, as do the tokens in the new lengths, and the
+    module's text says how rows go on. With update, lengths and taken are changed in place, else they are left
+    and the same call can be made again, with more pages in the list, say."""
     page, total = _whole("page", page, 1), _whole("total", total, 0)
     _hip.refuse_recorded("block_tables", tables)
     return PagePlan(*_hip.page_tables(tables, lengths, new, free, taken, page, total, update))

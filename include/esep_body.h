@@ -343,7 +343,8 @@ int esep_attn_cache(const void* q, const int64_t* q_strides, const void* k, cons
  *   lengths_out, taken_out    the new lengths (at most M * page) and *taken + the pages that were needed; they may be
  *                             lengths and taken themselves
  * Tokens past `total` are not added. lengths count as clamped into [0, M * page], a negative *taken as 0. M * page
- * <= 2^30.
+ * <= 2^30. A page is taken with its first token and for no later one: a row that got none for page j holds its tokens
+ * before j * page, and goes on from there where its length is set to that; of the list min(*taken, F) entries are in use.
  */
 int esep_page_tables(int32_t* tables, int64_t tables_bs, const int32_t* lengths, const int32_t* add,
                      const int32_t* free_pages, const int32_t* taken, int32_t* slots, int32_t* positions,
