@@ -327,12 +327,15 @@ __global__ __launch_bounds__(THREADS) void k_beam_join(const BeamArgs a) {
     return Cand{(((double)unordered((uint32_t)(k >> 32)) - (double)tops[b]) - rest[b]) + score[b],
                 b * a.V + (int)~(uint32_t)k};
   };
+  // A value in 32 bits, in the values' order: a quarter of it, as three of fp32's greatest may be taken from 0 (score, and a
+  // logit far below its row's greatest), and what rounds to -inf would count as none.
+  auto in32 = [](const Cand& c) { return (float)(0.25 * c.value); };
   Cand mine[kJoinFirst];
   float best32 = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kJoinFirst; ++j) {
     mine[j] = value(index(j) < all ? index(j) : 0, key[j]);
-    best32 = fmaxf(best32, (float)mine[j].value);
+    best32 = fmaxf(best32, in32(mine[j]));
   }
   const int rounds = (all + THREADS - 1) / THREADS;
   // f of the thread's candidates from j0 on, kJoinMore asked for at once
@@ -346,14 +349,14 @@ __global__ __launch_bounds__(THREADS) void k_beam_join(const BeamArgs a) {
       for (int i = 0; i < kJoinMore; ++i) f(value(index(j + i) < all ? index(j + i) : 0, more[i]));
     }
   };
-  each_from(kJoinFirst, [&](const Cand& c) { best32 = fmaxf(best32, (float)c.value); });
+  each_from(kJoinFirst, [&](const Cand& c) { best32 = fmaxf(best32, in32(c)); });
   group[tid] = best32;
   __syncthreads();
   float highest;
   const float bound = block_bound<NW>(group, lane, a.keep, &highest);
-  // by value in 32 bits (rounding keeps the order): what reaches the bound
+  // what reaches the bound
   auto enter = [&](const Cand& c) {
-    if ((float)c.value >= bound) {
+    if (in32(c) >= bound) {
       const int at = atomicAdd(&count, 1);
       if (at < kList) list[at] = c;
     }

@@ -20,7 +20,8 @@ def beam_select(logits, scores, keep=None):
     are left. keep up to 64 and W * V, W up to 64.
 
     Sums of exponentials are fp32; log softmax, the sum with the score and the comparison of beams are in 64 bits,
-    rounded once. No gradient: logits that record one, traces and transforms are refused."""
+    rounded once (to -inf below fp32's range, in their order still). No gradient: logits that record one, traces and
+    transforms are refused."""
     if logits.dim() != 3:
         raise _hip.EsepError(f"logits must be [R, W, V], got {list(logits.shape)}")
     R, W, V = logits.shape
