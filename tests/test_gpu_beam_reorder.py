@@ -29,3 +29,20 @@ def test_lanes_without_a_piece(W, HK, D, how):
     want = [_reorder_ref(parents, t, tables, lengths, start) for t in (kp, vp)]
     beam_reorder(_i(parents), kp, vp, _i(tables), _i(lengths), _i(start))
     assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+def test_pages_past_32_bit_offsets():
+    """Layers of more than 2^32 bytes, pages at both ends of each: every offset's part needs 64 bits."""
+    from solution.body.paged import beam_reorder
+
+    L, N, P, HK, D = 2, 4100, 1024, 4, 128  # 4.3 GB a layer
+    tables = [[5, N - 1], [5, 0], [5, 2050], [5, N - 2]]
+    parents, lengths, start = [[1, 0, 0, 2]], [P + 60], [P - 9]  # the first page is shared
+    kp, vp = (torch.zeros(L, N, P, HK, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    for i, t in enumerate((kp, vp)):
+        for page in (0, 5, 2050, N - 2, N - 1):
+            t[:, page] = _pages((L, P, HK, D), torch.float16, 10 * i + page)
+    want = [_reorder_ref(parents, t, tables, lengths, start) for t in (kp, vp)]
+    assert not torch.equal(want[0], kp)
+    beam_reorder(_i(parents), kp, vp, _i(tables), _i(lengths), _i(start))
+    assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
