@@ -16,15 +16,16 @@
 //
 // Kernel trace, walk + join: 48 rows of up to 8192 tokens, 28 / 4 heads of 128, bf16, pages of 64 85.8 + 4.8 us (497
 // MB, 5.8 TB/s in the walk; a copy reaches 5.0, half of it writes); 8 requests of 4 beams over up to 8000 shared
-// tokens and 130 each, pages of 16 29.8 + 7.0 (96 MB; each beam on its own 4 times the bytes of the prompt; 27.4
-// without the walk's products). In one launch: 5 new tokens over 7 rows through a window of 1500, 14 / 2 heads of 64
-// 14.4 (in two 12.6 + 4.0); one row of 700 tokens, 12 / 2 heads 9.7 (6.6 + 3.8). A CU of its own takes in up to 70
-// GB/s; a wavefront's products of a tile take 0.3 (D = 64) and 0.44 us (128). Tried in vain: four wavefronts to a
-// block whose tails meet in LDS (one partial for four: 29.6 + 5.1 us at the beams, but 10.2 instead of 7.0 for the
-// one row), rings of three and four tiles with fewer wavefronts (beams -4%, 256 rows of 300 tokens +20%), one to
-// three tiles to a wavefront (-7% to +7% over twenty shapes), partials eight columns at a time (the join reads 32
-// bytes of a line) or through LDS in whole lines (no change over twenty shapes), joins by 512 threads (+1 to 4%) or of
-// half the columns (-4 to +24%).
+// tokens and 130 each, pages of 16 29.8 + 7.0 (96 MB, and 13.9 MB of partials written, by the counter; each beam on its
+// own 4 times the bytes of the prompt; 27.4 without the walk's products, 25.5 without its partials' stores). In one
+// launch: 5 new tokens over 7 rows through a window of 1500, 14 / 2 heads of 64 14.4 (in two 12.6 + 4.0); one row of
+// 700 tokens, 12 / 2 heads 9.7 (6.6 + 3.8). A CU of its own takes in up to 70 GB/s; a wavefront's products of a tile
+// take 0.3 (D = 64) and 0.44 us (128). Tried in vain: rings of three and four tiles with fewer wavefronts (beams -4%,
+// 256 rows of 300 tokens +20%), one to three tiles to a wavefront (-7% to +7% over twenty shapes), partials eight
+// columns at a time (the join reads 32 bytes of a line) or through LDS in whole lines (no change over twenty shapes),
+// joins by 512 threads (+1 to 4%) or of half the columns (-4 to +24%). Four wavefronts to a block whose tails meet in
+// LDS, one partial for four, took 29.6 + 5.1 us at the beams and 10.2 instead of 7.0 in the walk of the one row; that row
+// has had its own launch since, so that for shared pages this is open.
 #include <cmath>
 
 #include "attention_cache.hpp"

@@ -51,6 +51,11 @@ struct PagedSizes {
 // / 19.1; 7 of 5 new tokens and a window of 1500 14.4 / 13.7; 120 of 4000 43.7 / 40.9; 130 of 1200 23.0 / 19.1, 2000
 // 29.2* / 31.9; 700 of 60 24.7 / 7.7, 1500 81.7* / 79.4; 8 beams each, 2000 of 100 116 / 20. (With four wavefronts
 // where eight fit: one row of 700 8.2, 32 of 1000 11.5.)
+//
+// All of these have rows of a quarter to all of the longest, and the 5 / 8 is theirs. The rule sees the tables' width alone:
+// where one row is that long and the others have 20 to 100 tokens, the one launch lasts as long as that row's block. One of 2500
+// among 256, 28 / 4 heads of 128: 86.0 / 25.6 (in tables for 32768, which take the walk); of 2000 among 64 26.6 / 18.5;
+// of 2800 among 1000, 14 / 2 heads of 64 69.8 / 32.8.
 inline int paged_solo(int B, int64_t groups, int64_t tiles, int W, int D) {
   const int64_t waves = kAttnCUs * (D == 128 ? 4 : 8), total = groups * tiles / W;
   int each = D == 128 ? 4 : 8;

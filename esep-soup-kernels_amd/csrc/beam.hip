@@ -120,7 +120,8 @@ typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2)));
 
 // The piece's elements of thread i: i * 8 .. + 7 of each run of 2048, whatever the row's alignment, so that equal
 // rows give equal sums. (Registers for six wavefronts to a SIMD: 128 requests of 4 beams over 151936 in bf16 47.7 ->
-// 44.9 us, where the compiler's own choice leaves five and eight spill: 48.5.)
+// 44.9 us, where the compiler's own choice leaves five, and eight spill: 48.5. With six, at U = 4, three registers go to
+// scratch memory behind the branch of a list that overflows, none before it.)
 template <typename T, int U>
 __global__ __launch_bounds__(kBeamThreads, 6) void k_beam_rows(const BeamArgs a) {
   constexpr int NW = kBeamThreads / 64;

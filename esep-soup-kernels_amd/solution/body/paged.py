@@ -89,7 +89,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, scale=None, window=Non
     read. Keys of a page outside the pool (an entry of -1) are not seen. A query that sees none gets 0, as one at a
     position below 0 does. Lengths past M * P count as that. Rounding and infinities are cache_attention's. The tables' width is
     all that the host knows of the lengths: where rows are short, tables[:, :m] that just holds them takes one
-    launch that suits them (300 rows of 60 tokens 7 us instead of 22).
+    launch that suits them (300 rows of 60 tokens 7 us instead of 22); where few are long and the rest short, wide ones
+    take the launches that share the long rows out (one of 2500 tokens among 256 of up to 100 26 us instead of 86).
 
     beams, shared (int32 [B // beams]): rows r * beams .. + beams - 1 hold their first shared[r] tokens in the same
     pages (a request's beams over its prompt). The pages are then read once for all of them instead of once for
@@ -122,7 +123,8 @@ def beam_reorder(parents, k_pages, v_pages, tables, lengths, start=None):
 
     The beams of a request are equally long. Beams that are their own parent, or name one outside [0, W), are left
     alone, as are pages that a beam shares with its parent (the prompt's) and -1 entries; every other page in that
-    range is one beam's own. Up to 32 beams."""
+    range is one beam's own. Up to 32 beams. (lengths and start at a stride, as block_tables' lengths[::W], are copied
+    first, one more launch.)"""
     _hip.refuse_recorded("beam_reorder", k_pages, v_pages, parents)
     if k_pages.dim() == 4 and v_pages.dim() == 4:
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
